@@ -73,6 +73,20 @@ SIGNATURES = {
     "el_peer_barrier_next": [_vp, _i, _i, _vp, _vp, _vp, C.c_size_t, _vp],
     "el_counter_add": [_vp, _i, _vp],
     "el_peer_put_dma": [_vp, _vp, _i, C.c_size_t, C.c_size_t, _vp],
+    # the operators of a Mamba block take one struct (csrc/host_ops.cpp fills it)
+    "el_causal_conv": [_vp, _vp],
+    "el_causal_conv_backward": [_vp, _vp],
+    "el_causal_conv_backward_workspace_bytes": [_vp],
+    "el_causal_conv_step": [_vp, _vp],
+    "el_selective_scan": [_vp, _vp],
+    "el_selective_scan_checkpoint_bytes": [_vp],
+    "el_selective_scan_workspace_bytes": [_vp],
+    "el_selective_scan_backward": [_vp, _vp],
+    "el_selective_scan_backward_workspace_bytes": [_vp],
+    "el_selective_scan_step": [_vp, _vp],
+    "el_block_norm": [_vp, _vp],
+    "el_block_norm_backward": [_vp, _vp],
+    "el_block_norm_backward_workspace_bytes": [_vp],
 }
 
 
@@ -100,8 +114,7 @@ def lib() -> C.CDLL:
             fn = getattr(handle, name)
             fn.argtypes = argtypes
             fn.restype = (C.c_char_p if name == "el_status_string" else
-                          C.c_size_t if name in ("el_decode_workspace_bytes", "el_rmsnorm_backward_workspace_bytes", "el_swiglu_backward_workspace_bytes",
-                                                "el_gemm_workspace_bytes") else C.c_int)
+                          C.c_size_t if name.endswith("_bytes") else C.c_int)
         _lib = handle
     return _lib
 

@@ -72,6 +72,20 @@ bool gemv_mma_preq_fits(int M, int N, int K);
 int launch_gemv_mma_preq(const int8_t* xq, const float* amax, const uint8_t* Wp, const EpiParams& epi, int M, int N, int K,
                          cudaStream_t st);
 
+size_t causal_conv_backward_workspace_bytes(const el_conv_t& a);
+int launch_causal_conv(const el_conv_t& a, cudaStream_t st);
+int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st);
+int launch_causal_conv_step(const el_conv_t& a, cudaStream_t st);
+size_t selective_scan_checkpoint_bytes(const el_scan_t& a);
+size_t selective_scan_workspace_bytes(const el_scan_t& a);
+size_t selective_scan_backward_workspace_bytes(const el_scan_t& a);
+int launch_selective_scan(const el_scan_t& a, cudaStream_t st);
+int launch_selective_scan_backward(const el_scan_t& a, cudaStream_t st);
+int launch_selective_scan_step(const el_scan_t& a, cudaStream_t st);
+size_t block_norm_backward_workspace_bytes(const el_block_norm_t& a);
+int launch_block_norm(const el_block_norm_t& a, cudaStream_t st);
+int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st);
+
 static thread_local int g_last_cuda_error = 0;
 
 int record_cuda_error(cudaError_t e) {
@@ -178,6 +192,31 @@ int launch_decode_preq(const int8_t* xq, const float* absmax, const uint8_t* Wp,
     if (M <= decode_mma_max_tokens() && gemv_mma_preq_fits(M, N, K) && !decode_tcgen05_wins(M, N, K))
         return launch_gemv_mma_preq(xq, absmax, Wp, epi, M, N, K, st);
     return launch_gemm_wt_decode(xq, absmax, Wp, epi, M, N, K, status, st);
+}
+
+// ---- between the projections of a Mamba block: what every entry point of an operator checks ----------------------------------
+static int check_conv(const el_conv_t* a) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->channels < 0 || a->x_stride_b < 0 || a->x_stride_t < 0 || a->dy_stride_b < 0 ||
+        a->dy_stride_t < 0)
+        return EL_ERR_INVALID_ARG;
+    return a->width >= 2 && a->width <= 4 ? EL_OK : EL_ERR_UNSUPPORTED_SHAPE;
+}
+static int check_scan(const el_scan_t* a) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->channels < 0 || a->groups < 1 || a->states < 1 || a->channels % a->groups != 0)
+        return EL_ERR_INVALID_ARG;
+    const long long strides[] = {a->u_stride_b, a->u_stride_t, a->dt_stride_b, a->dt_stride_t, a->z_stride_b, a->z_stride_t, a->B_stride_b,
+                                 a->B_stride_t, a->B_stride_g, a->C_stride_b, a->C_stride_t, a->C_stride_g, a->dy_stride_b, a->dy_stride_t};
+    for (long long s : strides)
+        if (s < 0) return EL_ERR_INVALID_ARG;
+    return a->states <= 64 ? EL_OK : EL_ERR_UNSUPPORTED_SHAPE;
+}
+static int check_norm(const el_block_norm_t* a) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->rows < 0 || a->width < 0 || a->ld_h < 0 || a->ld_y < 0 || a->ld_gate < 0 || a->ld_dh_out < 0 || a->ld_dnormed < 0)
+        return EL_ERR_INVALID_ARG;
+    return a->width <= 16384 ? EL_OK : EL_ERR_UNSUPPORTED_SHAPE;
 }
 
 // The workspace that the decode calls used to need.  No kernel reads or writes it; callers may size and pass it as before, or none.
@@ -594,6 +633,107 @@ int el_prelinear_decode(const void* x, const void* up, int x_dtype, long long ld
     if (rc != EL_OK) return rc;
     const EpiParams epi{Y, (long long)N, out_dtype, nullptr, 0, gamma};
     return launch_decode_preq(xq_scratch, absmax, W_packed, epi, M, N, K, dev_status, (cudaStream_t)stream);
+}
+
+// ---- between the projections of a Mamba block --------------------------------------------------------------------------------
+
+int el_causal_conv(const el_conv_t* a, el_stream_t stream) {
+    int rc = check_conv(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->channels == 0) return EL_OK;
+    if (!a->weight || (a->length > 0 && (!a->x || !a->y))) return EL_ERR_NULL_PTR;
+    return launch_causal_conv(*a, (cudaStream_t)stream);
+}
+
+size_t el_causal_conv_backward_workspace_bytes(const el_conv_t* a) {
+    if (check_conv(a) != EL_OK || a->batch == 0 || a->channels == 0) return 0;
+    return causal_conv_backward_workspace_bytes(*a);
+}
+
+int el_causal_conv_backward(const el_conv_t* a, el_stream_t stream) {
+    int rc = check_conv(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->channels == 0) return EL_OK;
+    if (!a->weight || (a->length > 0 && a->batch > 0 && !a->x) || ((a->dweight || a->dbias) && a->batch > 0 && !a->workspace)) return EL_ERR_NULL_PTR;
+    if ((a->dweight || a->dbias) && a->batch > 0) {
+        if (a->workspace_bytes < causal_conv_backward_workspace_bytes(*a)) return EL_ERR_INVALID_ARG;
+        if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
+    }
+    return launch_causal_conv_backward(*a, (cudaStream_t)stream);
+}
+
+int el_causal_conv_step(const el_conv_t* a, el_stream_t stream) {
+    int rc = check_conv(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->channels == 0) return EL_OK;
+    if (!a->weight || !a->x || !a->y || !a->initial_state || !a->final_state) return EL_ERR_NULL_PTR;
+    return launch_causal_conv_step(*a, (cudaStream_t)stream);
+}
+
+size_t el_selective_scan_checkpoint_bytes(const el_scan_t* a) { return check_scan(a) == EL_OK ? selective_scan_checkpoint_bytes(*a) : 0; }
+size_t el_selective_scan_workspace_bytes(const el_scan_t* a) { return check_scan(a) == EL_OK ? selective_scan_workspace_bytes(*a) : 0; }
+size_t el_selective_scan_backward_workspace_bytes(const el_scan_t* a) {
+    return check_scan(a) == EL_OK ? selective_scan_backward_workspace_bytes(*a) : 0;
+}
+
+int el_selective_scan(const el_scan_t* a, el_stream_t stream) {
+    int rc = check_scan(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->channels == 0) return EL_OK;
+    const size_t need = selective_scan_workspace_bytes(*a);
+    if (!a->A || (a->length > 0 && (!a->u || !a->dt || !a->B || !a->C || !a->y)) || (need > 0 && !a->workspace)) return EL_ERR_NULL_PTR;
+    if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(a->checkpoints) % 16 != 0) return EL_ERR_ALIGNMENT;
+    return launch_selective_scan(*a, (cudaStream_t)stream);
+}
+
+int el_selective_scan_backward(const el_scan_t* a, el_stream_t stream) {
+    int rc = check_scan(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->channels == 0) return EL_OK;
+    const size_t need = selective_scan_backward_workspace_bytes(*a);
+    if (!a->A || (a->length > 0 && a->batch > 0 && (!a->u || !a->dt || !a->B || !a->C || !a->checkpoints)) || (need > 0 && !a->workspace))
+        return EL_ERR_NULL_PTR;
+    if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(a->checkpoints) % 16 != 0) return EL_ERR_ALIGNMENT;
+    return launch_selective_scan_backward(*a, (cudaStream_t)stream);
+}
+
+int el_selective_scan_step(const el_scan_t* a, el_stream_t stream) {
+    int rc = check_scan(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->channels == 0) return EL_OK;
+    if (!a->A || !a->u || !a->dt || !a->B || !a->C || !a->y || !a->initial_state || !a->final_state) return EL_ERR_NULL_PTR;
+    return launch_selective_scan_step(*a, (cudaStream_t)stream);
+}
+
+int el_block_norm(const el_block_norm_t* a, el_stream_t stream) {
+    int rc = check_norm(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->rows == 0 || a->width == 0) return EL_OK;
+    if (!a->h || !a->y || !a->post_weight || !a->pre_weight || !a->h_out || !a->normed) return EL_ERR_NULL_PTR;
+    return launch_block_norm(*a, (cudaStream_t)stream);
+}
+
+size_t el_block_norm_backward_workspace_bytes(const el_block_norm_t* a) { return check_norm(a) == EL_OK ? block_norm_backward_workspace_bytes(*a) : 0; }
+
+int el_block_norm_backward(const el_block_norm_t* a, el_stream_t stream) {
+    int rc = check_norm(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->width == 0) return EL_OK;
+    const size_t need = block_norm_backward_workspace_bytes(*a);
+    if (a->rows > 0 && (!a->h || !a->y || !a->post_weight || !a->pre_weight || !a->rstd || !a->workspace)) return EL_ERR_NULL_PTR;
+    if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
+    return launch_block_norm_backward(*a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 // No state of its own but the handles that set_hooks hands over: the status word of each device, the function that turns a status
 // into an exception and the one that checks the device's status word.  Scratch that a call needs and leaves is allocated per call.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -17,6 +18,7 @@
 #include <dlfcn.h>
 
 #include <cstdlib>
+#include <vector>
 
 #include "../../include/elleci_int2.h"
 
@@ -33,7 +35,11 @@ PyObject* g_check_status = nullptr;     // int2_tc_ops.check_device_status(devic
     X(el_quantize_rows) X(el_zero) X(el_quantize_grad) X(el_quantize_tensor) X(el_rmsnorm_quantize_rows)                          \
     X(el_rmsnorm_backward) X(el_rmsnorm_backward_workspace_bytes) X(el_swiglu_quantize_rows) X(el_swiglu_backward)     \
     X(el_swiglu_backward_workspace_bytes) X(el_prelinear_rows) X(el_gemm_workspace_bytes) X(el_gemm_fwd_ws)            \
-    X(el_gemm_dx_ws) X(el_dw_hysteresis) X(el_gemm_dw) X(el_hysteresis_from_dw) X(el_linear_decode) X(el_prelinear_decode) X(el_decode_workspace_bytes)
+    X(el_gemm_dx_ws) X(el_dw_hysteresis) X(el_gemm_dw) X(el_hysteresis_from_dw) X(el_linear_decode) X(el_prelinear_decode) X(el_decode_workspace_bytes) \
+    X(el_causal_conv) X(el_causal_conv_backward) X(el_causal_conv_backward_workspace_bytes) X(el_causal_conv_step)        \
+    X(el_selective_scan) X(el_selective_scan_checkpoint_bytes) X(el_selective_scan_workspace_bytes)                       \
+    X(el_selective_scan_backward) X(el_selective_scan_backward_workspace_bytes) X(el_selective_scan_step)                 \
+    X(el_block_norm) X(el_block_norm_backward) X(el_block_norm_backward_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     EL_FUNCTIONS(X)
@@ -601,6 +607,414 @@ PyObject* linear_decode(PyObject* const* a) {
     return wrap(Y);
 }
 
+// ---- between the projections of a Mamba block ----------------------------------------------------------------------------
+// Activations of one dtype, channel-last; a tensor whose channels are contiguous is read in place, whatever its other strides.
+
+// `o` as a tensor on x's device with x's dtype and the given sizes, its last dimension contiguous; empty sizes: any
+Tensor tokens_arg(PyObject* o, const char* name, const Tensor& x, at::IntArrayRef sizes) {
+    const Tensor& t = cuda_arg(o, name);
+    if (t.device() != x.device()) raise(std::string(name) + " is on another device");
+    if (t.scalar_type() != x.scalar_type()) raise(std::string(name) + " has another dtype than the activations");
+    if (t.sizes() != sizes) {
+        std::string want;
+        for (auto s : sizes) want += (want.empty() ? "" : ", ") + std::to_string(s);
+        raise(std::string(name) + " must have shape [" + want + "]");
+    }
+    return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+Tensor dense_arg(PyObject* o, const char* name, const Tensor& x, at::ScalarType dt, at::IntArrayRef sizes) {
+    const Tensor& t = cuda_arg(o, name);
+    if (t.device() != x.device()) raise(std::string(name) + " is on another device");
+    if (t.scalar_type() != dt) raise(std::string(name) + " must be " + c10::toString(dt));
+    if (t.sizes() != sizes) {
+        std::string want;
+        for (auto s : sizes) want += (want.empty() ? "" : ", ") + std::to_string(s);
+        raise(std::string(name) + " must have shape [" + want + "]");
+    }
+    return t.contiguous();
+}
+Tensor maybe_dense(PyObject* o, const char* name, const Tensor& x, at::ScalarType dt, at::IntArrayRef sizes) {
+    return is_none(o) ? Tensor() : dense_arg(o, name, x, dt, sizes);
+}
+Tensor maybe_tokens(PyObject* o, const char* name, const Tensor& x, at::IntArrayRef sizes) { return is_none(o) ? Tensor() : tokens_arg(o, name, x, sizes); }
+Tensor lengths_arg(PyObject* o, const Tensor& x, int64_t batch) {
+    if (is_none(o)) return Tensor();
+    const Tensor& t = cuda_arg(o, "lengths");
+    if (t.device() != x.device()) raise("lengths is on another device");
+    EL_REQUIRE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "lengths must be int32 or int64");
+    EL_REQUIRE(t.dim() == 1 && t.size(0) == batch, "lengths must have one entry per sequence");
+    return t.to(at::kInt).contiguous();
+}
+// the state that a step writes: a dense tensor like `state`, either state itself or one apart from it
+const Tensor& state_out_arg(PyObject* o, const Tensor& state) {
+    EL_REQUIRE(state.is_contiguous(), "state must be contiguous");
+    if (is_none(o)) return state;
+    const Tensor& t = cuda_arg(o, "state_out");
+    EL_REQUIRE(t.device() == state.device() && t.scalar_type() == state.scalar_type() && t.sizes() == state.sizes() && t.is_contiguous(),
+               "state_out must be a contiguous tensor like state");
+    const char *p = static_cast<const char*>(state.data_ptr()), *q = static_cast<const char*>(t.data_ptr());
+    const int64_t bytes = state.numel() * state.element_size();
+    EL_REQUIRE(p == q || q + bytes <= p || p + bytes <= q, "state_out overlaps state");
+    return t;
+}
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+long long stride_of(const Tensor& t, int64_t dim) { return t.defined() && t.size(dim) > 1 ? t.stride(dim) : 0; }
+int int_size(int64_t n) {
+    EL_REQUIRE(n <= INT32_MAX, "a size does not fit 32 bits");
+    return (int)n;
+}
+void* stream_on(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.device().index()).stream(); }
+PyObject* wrap_or_none(const Tensor& t) { return t.defined() ? wrap(t) : none(); }
+Tensor scratch(const Tensor& x, size_t bytes) { return bytes ? new_empty(x, {(int64_t)bytes}, at::kByte) : Tensor(); }
+
+// What the three calls of the convolution share; `keep` holds the tensors that the struct points into.
+struct ConvCall {
+    el_conv_t c = {};
+    std::vector<Tensor> keep;
+    Tensor x;
+};
+void conv_call(ConvCall& k, PyObject* x_arg, PyObject* weight, PyObject* bias, bool silu, bool step) {
+    const Tensor& x = cuda_arg(x_arg, "x");
+    EL_REQUIRE(float_type(x.scalar_type()), "x must be float16, bfloat16 or float32");
+    EL_REQUIRE(x.dim() == (step ? 2 : 3), step ? "x must be [batch, channels]" : "x must be [batch, length, channels]");
+    const Tensor& w = cuda_arg(weight, "weight");
+    const int64_t D = x.size(-1);
+    EL_REQUIRE(w.dim() == 2 && w.size(1) >= 2 && w.size(1) <= 4, "weight must be [channels, width] with a width of 2, 3 or 4");
+    k.x = tokens_arg(x_arg, "x", x, x.sizes());
+    k.keep = {dense_arg(weight, "weight", x, at::kFloat, {D, w.size(1)}), maybe_dense(bias, "bias", x, at::kFloat, {D})};
+    el_conv_t& c = k.c;
+    c.dtype = code_of(x.scalar_type());
+    c.batch = int_size(x.size(0));
+    c.length = step ? 1 : int_size(x.size(1));
+    c.channels = int_size(D);
+    c.width = (int)w.size(1);
+    c.silu = silu;
+    c.x = ptr(k.x);
+    c.x_stride_b = stride_of(k.x, 0);
+    c.x_stride_t = step ? 0 : stride_of(k.x, 1);
+    c.weight = ptr<float>(k.keep[0]);
+    c.bias = ptr<float>(k.keep[1]);
+}
+
+// causal_conv(x, weight, bias, silu, initial_state, lengths, final_state wanted) -> (y, final state or None)
+PyObject* causal_conv(PyObject* const* a) {
+    ConvCall k;
+    conv_call(k, a[0], a[1], a[2], int_arg(a[3]) != 0, false);
+    const Tensor& x = k.x;
+    const c10::cuda::CUDAGuard device(x.device());
+    const int64_t B = x.size(0), H = k.c.width - 1, D = x.size(2);
+    Tensor first = maybe_dense(a[4], "initial_state", x, x.scalar_type(), {B, H, D}), lengths = lengths_arg(a[5], x, B);
+    k.c.initial_state = ptr(first);
+    k.c.lengths = ptr<int32_t>(lengths);
+    Tensor y = new_empty(x, x.sizes(), x.scalar_type()), last;
+    if (int_arg(a[6])) last = new_empty(x, {B, H, D}, x.scalar_type());
+    k.c.y = ptr(y);
+    k.c.final_state = ptr(last);
+    call("el_causal_conv", g_lib.el_causal_conv, &k.c, stream_on(x));
+    return tuple_of(wrap(y), wrap_or_none(last));
+}
+
+// causal_conv_backward(x, weight, bias, silu, initial_state, lengths, dy, d_final_state, wanted) -> (dx, dweight, dbias, d_initial_state),
+// `wanted`: bits 0 .. 3 in this order
+PyObject* causal_conv_backward(PyObject* const* a) {
+    ConvCall k;
+    conv_call(k, a[0], a[1], a[2], int_arg(a[3]) != 0, false);
+    const Tensor& x = k.x;
+    const c10::cuda::CUDAGuard device(x.device());
+    const int64_t B = x.size(0), H = k.c.width - 1, D = x.size(2);
+    const int want = (int)int_arg(a[8]);
+    Tensor first = maybe_dense(a[4], "initial_state", x, x.scalar_type(), {B, H, D}), lengths = lengths_arg(a[5], x, B);
+    Tensor dy = maybe_tokens(a[6], "dy", x, x.sizes()), d_last = maybe_dense(a[7], "d_final_state", x, x.scalar_type(), {B, H, D});
+    Tensor dx, dw, db, d_first;
+    if (want & 1) dx = new_empty(x, x.sizes(), x.scalar_type());
+    if (want & 2) dw = new_empty(x, {D, H + 1}, at::kFloat);
+    if (want & 4) db = new_empty(x, {D}, at::kFloat);
+    if (want & 8) d_first = new_empty(x, {B, H, D}, x.scalar_type());
+    el_conv_t& c = k.c;
+    c.initial_state = ptr(first);
+    c.lengths = ptr<int32_t>(lengths);
+    c.dy = ptr(dy);
+    c.dy_stride_b = dy.defined() ? stride_of(dy, 0) : 0;
+    c.dy_stride_t = dy.defined() ? stride_of(dy, 1) : 0;
+    c.d_final_state = ptr(d_last);
+    c.dx = ptr(dx);
+    c.dweight = ptr<float>(dw);
+    c.dbias = ptr<float>(db);
+    c.d_initial_state = ptr(d_first);
+    c.workspace_bytes = want & 6 ? g_lib.el_causal_conv_backward_workspace_bytes(&c) : 0;
+    Tensor ws = scratch(x, c.workspace_bytes);
+    c.workspace = ptr(ws);
+    call("el_causal_conv_backward", g_lib.el_causal_conv_backward, &c, stream_on(x));
+    return tuple_of(wrap_or_none(dx), wrap_or_none(dw), wrap_or_none(db), wrap_or_none(d_first));
+}
+
+// causal_conv_step(x, state, weight, bias, silu, state_out) -> y
+PyObject* causal_conv_step(PyObject* const* a) {
+    ConvCall k;
+    conv_call(k, a[0], a[2], a[3], int_arg(a[4]) != 0, true);
+    const Tensor& x = k.x;
+    const c10::cuda::CUDAGuard device(x.device());
+    const Tensor& state = cuda_arg(a[1], "state");
+    dense_arg(a[1], "state", x, x.scalar_type(), {x.size(0), k.c.width - 1, x.size(1)});
+    const Tensor& out = state_out_arg(a[5], state);
+    Tensor y = new_empty(x, x.sizes(), x.scalar_type());
+    k.c.initial_state = ptr(state);
+    k.c.final_state = ptr(out);
+    k.c.y = ptr(y);
+    call("el_causal_conv_step", g_lib.el_causal_conv_step, &k.c, stream_on(x));
+    written(out);
+    return wrap(y);
+}
+
+struct ScanCall {
+    el_scan_t c = {};
+    std::vector<Tensor> keep;
+    Tensor u;
+    int64_t B = 0, L = 0, D = 0, G = 0, N = 0;
+};
+// u, dt [batch, length, channels], A [channels, states], B, C [batch, length, groups, states], D, z, dt_bias; a step has no length
+void scan_call(ScanCall& k, PyObject* const* a, bool softplus, bool step) {
+    const Tensor& u = cuda_arg(a[0], "u");
+    EL_REQUIRE(float_type(u.scalar_type()), "u must be float16, bfloat16 or float32");
+    EL_REQUIRE(u.dim() == (step ? 2 : 3), step ? "u must be [batch, channels]" : "u must be [batch, length, channels]");
+    const Tensor &A = cuda_arg(a[2], "A"), &Bm = cuda_arg(a[3], "B");
+    EL_REQUIRE(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, "A must be [channels, states] with 1 to 64 states");
+    EL_REQUIRE(Bm.dim() == u.dim() + 1, step ? "B must be [batch, groups, states]" : "B must be [batch, length, groups, states]");
+    k.B = u.size(0);
+    k.L = step ? 1 : u.size(1);
+    k.D = u.size(-1);
+    k.N = A.size(1);
+    k.G = Bm.size(-2);
+    EL_REQUIRE(k.G >= 1 && k.D % k.G == 0, "the channels must be a multiple of B's groups");
+    k.u = tokens_arg(a[0], "u", u, u.sizes());
+    std::vector<int64_t> shared(u.sizes().begin(), u.sizes().end() - 1);
+    shared.push_back(k.G);
+    shared.push_back(k.N);
+    Tensor dt = tokens_arg(a[1], "dt", u, u.sizes()), B2 = tokens_arg(a[3], "B", u, shared), C2 = tokens_arg(a[4], "C", u, shared);
+    Tensor A2 = dense_arg(a[2], "A", u, at::kFloat, {k.D, k.N}), Dv = maybe_dense(a[5], "D", u, at::kFloat, {k.D});
+    Tensor z = maybe_tokens(a[6], "z", u, u.sizes()), bias = maybe_dense(a[7], "dt_bias", u, at::kFloat, {k.D});
+    el_scan_t& c = k.c;
+    c.dtype = code_of(u.scalar_type());
+    c.batch = int_size(k.B);
+    c.length = int_size(k.L);
+    c.channels = int_size(k.D);
+    c.groups = int_size(k.G);
+    c.states = int_size(k.N);
+    c.softplus = softplus;
+    c.u = ptr(k.u);
+    c.dt = ptr(dt);
+    c.z = ptr(z);
+    c.B = ptr(B2);
+    c.C = ptr(C2);
+    c.u_stride_b = stride_of(k.u, 0);
+    c.dt_stride_b = stride_of(dt, 0);
+    c.z_stride_b = z.defined() ? stride_of(z, 0) : 0;
+    c.B_stride_b = stride_of(B2, 0);
+    c.C_stride_b = stride_of(C2, 0);
+    c.B_stride_g = stride_of(B2, -2);
+    c.C_stride_g = stride_of(C2, -2);
+    if (!step) {
+        c.u_stride_t = stride_of(k.u, 1);
+        c.dt_stride_t = stride_of(dt, 1);
+        c.z_stride_t = z.defined() ? stride_of(z, 1) : 0;
+        c.B_stride_t = stride_of(B2, 1);
+        c.C_stride_t = stride_of(C2, 1);
+    }
+    c.A = ptr<float>(A2);
+    c.D = ptr<float>(Dv);
+    c.dt_bias = ptr<float>(bias);
+    k.keep = {dt, B2, C2, A2, Dv, z, bias};
+}
+
+// selective_scan(u, dt, A, B, C, D, z, dt_bias, softplus, initial_state, lengths, final_state wanted, checkpoints wanted)
+// -> (y, final state or None, checkpoints or None)
+PyObject* selective_scan(PyObject* const* a) {
+    ScanCall k;
+    scan_call(k, a, int_arg(a[8]) != 0, false);
+    const Tensor& u = k.u;
+    const c10::cuda::CUDAGuard device(u.device());
+    Tensor first = maybe_dense(a[9], "initial_state", u, at::kFloat, {k.B, k.D, k.N}), lengths = lengths_arg(a[10], u, k.B);
+    el_scan_t& c = k.c;
+    c.initial_state = ptr<float>(first);
+    c.lengths = ptr<int32_t>(lengths);
+    Tensor y = new_empty(u, u.sizes(), u.scalar_type()), last, kept;
+    if (int_arg(a[11])) last = new_empty(u, {k.B, k.D, k.N}, at::kFloat);
+    if (int_arg(a[12])) kept = new_empty(u, {(int64_t)(g_lib.el_selective_scan_checkpoint_bytes(&c) / sizeof(float))}, at::kFloat);
+    c.y = ptr(y);
+    c.final_state = ptr<float>(last);
+    c.checkpoints = ptr<float>(kept);
+    c.workspace_bytes = g_lib.el_selective_scan_workspace_bytes(&c);
+    Tensor ws = scratch(u, c.workspace_bytes);
+    c.workspace = ptr(ws);
+    call("el_selective_scan", g_lib.el_selective_scan, &c, stream_on(u));
+    return tuple_of(wrap(y), wrap_or_none(last), wrap_or_none(kept));
+}
+
+// selective_scan_backward(u, dt, A, B, C, D, z, dt_bias, softplus, initial_state, lengths, checkpoints, dy, d_final_state, wanted)
+// -> (du, ddt, dA, dB, dC, dD, dz, ddt_bias, d_initial_state), `wanted`: bits 0 .. 8 in this order
+PyObject* selective_scan_backward(PyObject* const* a) {
+    ScanCall k;
+    scan_call(k, a, int_arg(a[8]) != 0, false);
+    const Tensor& u = k.u;
+    const c10::cuda::CUDAGuard device(u.device());
+    Tensor first = maybe_dense(a[9], "initial_state", u, at::kFloat, {k.B, k.D, k.N}), lengths = lengths_arg(a[10], u, k.B);
+    el_scan_t& c = k.c;
+    c.initial_state = ptr<float>(first);
+    c.lengths = ptr<int32_t>(lengths);
+    Tensor kept = dense_arg(a[11], "checkpoints", u, at::kFloat, {(int64_t)(g_lib.el_selective_scan_checkpoint_bytes(&c) / sizeof(float))});
+    Tensor dy = maybe_tokens(a[12], "dy", u, u.sizes()), d_last = maybe_dense(a[13], "d_final_state", u, at::kFloat, {k.B, k.D, k.N});
+    const int want = (int)int_arg(a[14]);
+    const auto io = u.scalar_type();
+    Tensor du, ddt, dA, dB, dC, dD, dz, dbias, d_first;
+    if (want & 1) du = new_empty(u, u.sizes(), io);
+    if (want & 2) ddt = new_empty(u, u.sizes(), io);
+    if (want & 4) dA = new_empty(u, {k.D, k.N}, at::kFloat);
+    if (want & 8) dB = new_empty(u, {k.B, k.L, k.G, k.N}, io);
+    if (want & 16) dC = new_empty(u, {k.B, k.L, k.G, k.N}, io);
+    if (want & 32) dD = new_empty(u, {k.D}, at::kFloat);
+    if ((want & 64) && c.z) dz = new_empty(u, u.sizes(), io);
+    if (want & 128) dbias = new_empty(u, {k.D}, at::kFloat);
+    if (want & 256) d_first = new_empty(u, {k.B, k.D, k.N}, at::kFloat);
+    c.checkpoints = ptr<float>(kept);
+    c.dy = ptr(dy);
+    c.dy_stride_b = dy.defined() ? stride_of(dy, 0) : 0;
+    c.dy_stride_t = dy.defined() ? stride_of(dy, 1) : 0;
+    c.d_final_state = ptr<float>(d_last);
+    c.du = ptr(du);
+    c.ddt = ptr(ddt);
+    c.dz = ptr(dz);
+    c.dB = ptr(dB);
+    c.dC = ptr(dC);
+    c.dA = ptr<float>(dA);
+    c.dD = ptr<float>(dD);
+    c.ddt_bias = ptr<float>(dbias);
+    c.d_initial_state = ptr<float>(d_first);
+    c.workspace_bytes = g_lib.el_selective_scan_backward_workspace_bytes(&c);
+    Tensor ws = scratch(u, c.workspace_bytes);
+    c.workspace = ptr(ws);
+    call("el_selective_scan_backward", g_lib.el_selective_scan_backward, &c, stream_on(u));
+    return tuple_of(wrap_or_none(du), wrap_or_none(ddt), wrap_or_none(dA), wrap_or_none(dB), wrap_or_none(dC), wrap_or_none(dD), wrap_or_none(dz),
+                    wrap_or_none(dbias), wrap_or_none(d_first));
+}
+
+// selective_scan_step(u, dt, A, B, C, D, z, dt_bias, softplus, state, state_out) -> y
+PyObject* selective_scan_step(PyObject* const* a) {
+    ScanCall k;
+    scan_call(k, a, int_arg(a[8]) != 0, true);
+    const Tensor& u = k.u;
+    const c10::cuda::CUDAGuard device(u.device());
+    const Tensor& state = cuda_arg(a[9], "state");
+    dense_arg(a[9], "state", u, at::kFloat, {k.B, k.D, k.N});
+    const Tensor& out = state_out_arg(a[10], state);
+    Tensor y = new_empty(u, u.sizes(), u.scalar_type());
+    k.c.initial_state = ptr<float>(state);
+    k.c.final_state = ptr<float>(out);
+    k.c.y = ptr(y);
+    call("el_selective_scan_step", g_lib.el_selective_scan_step, &k.c, stream_on(u));
+    written(out);
+    return wrap(y);
+}
+
+struct NormCall {
+    el_block_norm_t c = {};
+    Rows h, y, g;
+    Tensor w1, w2, scale;
+};
+Rows norm_rows(PyObject* o, const char* name, const Tensor& h) {
+    const Tensor& t = cuda_arg(o, name);
+    if (t.device() != h.device()) raise(std::string(name) + " is on another device");
+    if (t.scalar_type() != h.scalar_type() || t.sizes() != h.sizes()) raise(std::string(name) + " must have the shape and dtype of h");
+    return rows_view(t);
+}
+// h, y, post_weight, pre_weight, gate, scale, eps
+void norm_call(NormCall& k, PyObject* const* a) {
+    const Tensor& h = cuda_arg(a[0], "h");
+    EL_REQUIRE(float_type(h.scalar_type()), "h must be float16, bfloat16 or float32");
+    EL_REQUIRE(h.dim() >= 1, "h must have at least one dimension");
+    const int64_t K = h.size(-1);
+    EL_REQUIRE(K <= 16384, "rows of up to 16384 columns are supported");
+    k.h = rows_view(h);
+    k.y = norm_rows(a[1], "y", h);
+    if (!is_none(a[4])) k.g = norm_rows(a[4], "gate", h);
+    k.w1 = dense_arg(a[2], "post_weight", h, at::kFloat, {K});
+    k.w2 = dense_arg(a[3], "pre_weight", h, at::kFloat, {K});
+    k.scale = maybe_dense(a[5], "scale", h, at::kFloat, {K});
+    el_block_norm_t& c = k.c;
+    c.dtype = code_of(h.scalar_type());
+    c.rows = int_size(k.h.M);
+    c.width = (int)K;
+    c.eps = (float)float_arg(a[6]);
+    EL_REQUIRE(c.eps >= 0.0f, "eps must not be negative");
+    c.h = ptr(k.h.t);
+    c.ld_h = k.h.ld;
+    c.y = ptr(k.y.t);
+    c.ld_y = k.y.ld;
+    if (k.g.t.defined()) {
+        c.gate = ptr(k.g.t);
+        c.ld_gate = k.g.ld;
+    }
+    c.post_weight = ptr<float>(k.w1);
+    c.pre_weight = ptr<float>(k.w2);
+    c.scale = ptr<float>(k.scale);
+}
+
+// block_norm(h, y, post_weight, pre_weight, gate, scale, eps, rstd wanted) -> (h_out, normed, rstd or None)
+PyObject* block_norm(PyObject* const* a) {
+    NormCall k;
+    norm_call(k, a);
+    const Tensor& h = k.h.t;
+    const c10::cuda::CUDAGuard device(h.device());
+    const Tensor& shaped = THPVariable_Unpack(a[0]);
+    Tensor out = new_empty(h, shaped.sizes(), h.scalar_type()), normed = new_empty(h, shaped.sizes(), h.scalar_type()), rstd;
+    if (int_arg(a[7])) rstd = new_empty(h, {k.h.M, 2}, at::kFloat);
+    k.c.h_out = ptr(out);
+    k.c.normed = ptr(normed);
+    k.c.rstd = ptr<float>(rstd);
+    call("el_block_norm", g_lib.el_block_norm, &k.c, stream_on(h));
+    return tuple_of(wrap(out), wrap(normed), wrap_or_none(rstd));
+}
+
+// block_norm_backward(h, y, post_weight, pre_weight, gate, scale, eps, rstd, dh_out, dnormed) -> (dh, dy, dpost_weight, dpre_weight, dgate, dscale)
+PyObject* block_norm_backward(PyObject* const* a) {
+    NormCall k;
+    norm_call(k, a);
+    const Tensor& h = k.h.t;
+    const c10::cuda::CUDAGuard device(h.device());
+    const Tensor& shaped = THPVariable_Unpack(a[0]);
+    const int64_t K = k.c.width;
+    el_block_norm_t& c = k.c;
+    Tensor rstd = dense_arg(a[7], "rstd", h, at::kFloat, {k.h.M, 2});
+    Rows dh_out, dn;
+    if (!is_none(a[8])) dh_out = norm_rows(a[8], "dh_out", shaped);
+    if (!is_none(a[9])) dn = norm_rows(a[9], "dnormed", shaped);
+    Tensor dh = new_empty(h, shaped.sizes(), h.scalar_type()), dy = new_empty(h, shaped.sizes(), h.scalar_type()), dg, ds;
+    Tensor dw1 = new_empty(h, {K}, at::kFloat), dw2 = new_empty(h, {K}, at::kFloat);
+    if (c.gate) dg = new_empty(h, shaped.sizes(), h.scalar_type());
+    if (c.scale) ds = new_empty(h, {K}, at::kFloat);
+    c.rstd = ptr<float>(rstd);
+    if (dh_out.t.defined()) {
+        c.dh_out = ptr(dh_out.t);
+        c.ld_dh_out = dh_out.ld;
+    }
+    if (dn.t.defined()) {
+        c.dnormed = ptr(dn.t);
+        c.ld_dnormed = dn.ld;
+    }
+    c.dh = ptr(dh);
+    c.dy_in = ptr(dy);
+    c.dgate = ptr(dg);
+    c.dpost_weight = ptr<float>(dw1);
+    c.dpre_weight = ptr<float>(dw2);
+    c.dscale = ptr<float>(ds);
+    c.workspace_bytes = g_lib.el_block_norm_backward_workspace_bytes(&c);
+    Tensor ws = scratch(h, c.workspace_bytes);
+    c.workspace = ptr(ws);
+    call("el_block_norm_backward", g_lib.el_block_norm_backward, &c, stream_on(h));
+    return tuple_of(wrap(dh), wrap(dy), wrap(dw1), wrap(dw2), wrap_or_none(dg), wrap_or_none(ds));
+}
+
 // ---- module -------------------------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int NARGS>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -641,6 +1055,8 @@ PyMethodDef methods[] = {
     EL_ENTRY(quantize_rows, 5), EL_ENTRY(quantize_grad, 3), EL_ENTRY(quantize_tensor, 2), EL_ENTRY(rmsnorm_quantize_rows, 4),
     EL_ENTRY(rmsnorm_backward, 4), EL_ENTRY(swiglu_quantize_rows, 5), EL_ENTRY(swiglu_backward, 6), EL_ENTRY(prelinear_rows, 4),
     EL_ENTRY(gemm_fwd, 7), EL_ENTRY(gemm_dx, 8), EL_ENTRY(dw_hysteresis, 11), EL_ENTRY(weight_update, 13), EL_ENTRY(linear_decode, 8), EL_ENTRY(set_hooks, 4),
+    EL_ENTRY(causal_conv, 7), EL_ENTRY(causal_conv_backward, 9), EL_ENTRY(causal_conv_step, 6), EL_ENTRY(selective_scan, 13),
+    EL_ENTRY(selective_scan_backward, 15), EL_ENTRY(selective_scan_step, 11), EL_ENTRY(block_norm, 8), EL_ENTRY(block_norm_backward, 10),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "elleci_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

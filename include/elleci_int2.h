@@ -402,6 +402,140 @@ EL_API int el_prelinear_decode(const void* x, const void* up, int x_dtype, long 
 EL_API int el_linear_decode_static(const void* x, int x_dtype, const uint8_t* W_packed, void* Y, int out_dtype, float gamma,
                                    int M, int N, int K, int32_t* dev_status, el_stream_t stream);
 
+/* ---- between the projections of a Mamba block --------------------------------------------------------- */
+
+/* The three operators that the block runs between its INT2 projections (in_proj -> convolution -> x_proj, dt_proj -> scan -> out_proj ->
+ * norms and residual): channel-last activations, one dtype (EL_F16 / EL_BF16 / EL_F32) per call for all tensors given as void*, float32
+ * parameters, float32 sums and states.  Arguments come in a struct that the caller zeroes first; what a call does not name may be NULL.
+ * Strides count elements; the channels of a token are contiguous.  Outputs are dense.  No pointer needs more alignment than
+ * its element type; bases and strides of 16 bytes are read faster.
+ * `lengths` [batch] (NULL: all sequences have `length` tokens): tokens from lengths[b] on are padding.  They are not read, their outputs and
+ * gradients are zeros and they leave the state as it is; a sequence of length 0 keeps its initial state.  Values outside
+ * 0 .. length are clamped.
+ * Outside the reference's INT2 path: its block has them as tensor operations (core/mamba/mamba2.py). */
+
+/* Depthwise causal convolution over the last `width` (2 .. 4) tokens of each channel, with bias and SiLU:
+ *   y[b,t,d] = act(bias[d] + sum_j weight[d,j] * x[b, t - (width-1) + j, d]), x at negative t = initial_state[b, width-1+t, d] or 0.
+ * final_state [batch, width-1, channels] receives the last width-1 inputs of each sequence.
+ * el_causal_conv_backward: dx, dweight, dbias (with bias), d_initial_state (each may be NULL) from dy and d_final_state (either may be NULL).
+ * el_causal_conv_step: one token for every sequence (x [batch, channels] by x_stride_b, y dense); initial_state and final_state are
+ * the state before and after, and may be one buffer. */
+typedef struct el_conv_t {
+    int dtype, batch, length, channels, width, silu;
+    const void* x;
+    long long x_stride_b, x_stride_t;
+    const float* weight;                /* [channels, width] */
+    const float* bias;                  /* [channels] or NULL */
+    const void* initial_state;          /* [batch, width-1, channels] or NULL (zeros) */
+    const int32_t* lengths;
+    void* y;                            /* [batch, length, channels] */
+    void* final_state;                  /* [batch, width-1, channels] or NULL */
+    const void* dy;
+    long long dy_stride_b, dy_stride_t;
+    const void* d_final_state;
+    void* dx;
+    float* dweight;
+    float* dbias;
+    void* d_initial_state;
+    void* workspace;                    /* backward with dweight or dbias: el_causal_conv_backward_workspace_bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} el_conv_t;
+EL_API int el_causal_conv(const el_conv_t* args, el_stream_t stream);
+EL_API size_t el_causal_conv_backward_workspace_bytes(const el_conv_t* args);
+EL_API int el_causal_conv_backward(const el_conv_t* args, el_stream_t stream);
+EL_API int el_causal_conv_step(const el_conv_t* args, el_stream_t stream);
+
+/* Selective state space scan.  With delta = softplus(dt + dt_bias) (softplus 0: dt + dt_bias itself) and g = the group of channel d
+ * (channels / groups consecutive channels share B and C):
+ *   h[b,t,d,n] = exp(delta[b,t,d] * A[d,n]) * h[b,t-1,d,n] + delta[b,t,d] * u[b,t,d] * B[b,t,g,n]
+ *   y[b,t,d]   = (sum_n C[b,t,g,n] * h[b,t,d,n] + D[d] * u[b,t,d]) * (z ? z * sigmoid(z) : 1)
+ * from h = initial_state (NULL: zeros); final_state receives h after each sequence's last token.  1 <= states <= 64; groups divides channels.
+ * `checkpoints` (el_selective_scan_checkpoint_bytes; NULL when no gradient is wanted) receives the states that the backward pass
+ * starts from and has to reach it unchanged.
+ * el_selective_scan_backward writes du, ddt, dz (with z), dB, dC [batch, length, groups, states], dA, dD (with D), ddt_bias (with dt_bias) and
+ * d_initial_state (each may be NULL) from dy and d_final_state (either may be NULL).  All sums have a fixed order.
+ * el_selective_scan_step: one token for every sequence, as el_causal_conv_step. */
+typedef struct el_scan_t {
+    int dtype, batch, length, channels, groups, states, softplus;
+    const void* u;
+    long long u_stride_b, u_stride_t;
+    const void* dt;
+    long long dt_stride_b, dt_stride_t;
+    const void* z;
+    long long z_stride_b, z_stride_t;
+    const void* B;
+    long long B_stride_b, B_stride_t, B_stride_g;
+    const void* C;
+    long long C_stride_b, C_stride_t, C_stride_g;
+    const float* A;                     /* [channels, states] */
+    const float* D;                     /* [channels] or NULL */
+    const float* dt_bias;               /* [channels] or NULL */
+    const float* initial_state;         /* [batch, channels, states] or NULL */
+    const int32_t* lengths;
+    void* y;
+    float* final_state;
+    float* checkpoints;
+    const void* dy;
+    long long dy_stride_b, dy_stride_t;
+    const float* d_final_state;
+    void* du;
+    void* ddt;
+    void* dz;
+    void* dB;
+    void* dC;
+    float* dA;
+    float* dD;
+    float* ddt_bias;
+    float* d_initial_state;
+    void* workspace;                    /* el_selective_scan_workspace_bytes (forward) / _backward_workspace_bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} el_scan_t;
+EL_API size_t el_selective_scan_checkpoint_bytes(const el_scan_t* args);
+EL_API size_t el_selective_scan_workspace_bytes(const el_scan_t* args);
+EL_API size_t el_selective_scan_backward_workspace_bytes(const el_scan_t* args);
+EL_API int el_selective_scan(const el_scan_t* args, el_stream_t stream);
+EL_API int el_selective_scan_backward(const el_scan_t* args, el_stream_t stream);
+EL_API int el_selective_scan_step(const el_scan_t* args, el_stream_t stream);
+
+/* The norm after a block, its gate and residual scale, the residual addition and the norm before the next block as one pass over [rows, width]:
+ *   h_out  = h + scale * sigmoid(gate) * (post_weight * y / rms(y))       (gate, scale: NULL for none)
+ *   normed = pre_weight * h_out / rms(h_out)                              (of h_out before it is rounded to the dtype)
+ * with rms(v) = sqrt(mean v^2 + eps).  ld_*: row pitches of the inputs.  rstd [rows, 2] receives 1/rms of y and of h_out (NULL when no
+ * gradient is wanted).  el_block_norm_backward writes dh, dy_in (the gradient of y), dgate, dscale, dpost_weight, dpre_weight
+ * (dgate with gate, dscale with scale) from dh_out and dnormed (either may be NULL), and reads h, y, gate and rstd again.
+ * Width up to 16384. */
+typedef struct el_block_norm_t {
+    int dtype, rows, width;
+    float eps;
+    const void* h;
+    long long ld_h;
+    const void* y;
+    long long ld_y;
+    const void* gate;
+    long long ld_gate;
+    const float* post_weight;           /* [width] */
+    const float* pre_weight;            /* [width] */
+    const float* scale;                 /* [width] or NULL */
+    void* h_out;                        /* [rows, width] */
+    void* normed;                       /* [rows, width] */
+    float* rstd;                        /* [rows, 2] or NULL */
+    const void* dh_out;
+    long long ld_dh_out;
+    const void* dnormed;
+    long long ld_dnormed;
+    void* dh;
+    void* dy_in;
+    void* dgate;
+    float* dpost_weight;
+    float* dpre_weight;
+    float* dscale;
+    void* workspace;                    /* backward: el_block_norm_backward_workspace_bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} el_block_norm_t;
+EL_API int el_block_norm(const el_block_norm_t* args, el_stream_t stream);
+EL_API size_t el_block_norm_backward_workspace_bytes(const el_block_norm_t* args);
+EL_API int el_block_norm_backward(const el_block_norm_t* args, el_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
