@@ -48,6 +48,7 @@ struct Shape {
     static constexpr int BCS = NS / 4 * TILE / 32;                                    // quads of B (and of C) per lane
     static constexpr int GROUP = 2;                   // tokens whose exponentials are in flight together; 4 cost registers and gain nothing
     static constexpr int PER_SM = NS > 32 ? 8 : 16;   // warps of an SM that the registers have to suffice for: what fits in shared memory
+    static constexpr int BACK_PER_SM = NS > 16 ? 8 : 16;                              // the same of the backward kernel
     static_assert(CW % 4 == 0 && 32 % QUADS == 0 && BCS >= 1, "");
 };
 
@@ -395,6 +396,7 @@ struct BackTile {
     float dyg[KEEP][S::CW];
     float4 h[KEEP][2][32];                            // state before the token: a lane's [state 0, 1 or 2, 3][channel]; then the sums [3][SG][CW]
     float bc[2][KEEP][2][S::NS];                      // dB and dC of the warp's channels, of two tiles
+    float bias[S::CW], D[S::CW];
 };
 
 // Sums V values over LANES lanes, STRIDE apart, so that lane s of them keeps one: in each step a lane hands half of its values to the lane
@@ -445,7 +447,7 @@ template <typename S> __device__ __forceinline__ void bc_sums(float (&v)[8], flo
 // LOCAL: the gradient of the state at the chunk's start from zeros at its end, and the sum of delta.
 // partial_bc [blocks of a group][2][batch][length][groups][states]; partial_a [batch][chunks][channels][states + 2]: dA, dD, dbias.
 template <typename T, typename S, bool LOCAL>
-__global__ void __launch_bounds__(32 * BACK_WARPS, S::NS > 16 ? 1 : 2)
+__global__ void __launch_bounds__(32 * BACK_WARPS, S::BACK_PER_SM / BACK_WARPS)
 selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bool aligned_bc, float* __restrict__ partial_bc,
                                float* __restrict__ partial_a) {
     constexpr int BCQ = S::NS / 4 * KEEP, BCS = (BCQ + 31) / 32;              // quads of B (and of C) of a tile, and per lane
@@ -468,13 +470,13 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     const int begin = chunk * split.tokens, end = min(begin + split.tokens, a.length), stop = min(end, n_live);
     const int sg = lane / S::CG, cg = lane % S::CG;
     const int d0 = p.d0 + 2 * cg, channels = p.n - 2 * cg;
-    f32x2 A[4], adj[4], h[4], dA[4], dA_all[4];               // adj: gradient of the state before the token in hand
+    f32x2 A[4], adj[4], h[4], dA[4];                          // adj: gradient of the state before the token in hand
     float dsum[2] = {};
     load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, A);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         A[n] = mul2(A[n], both(LOG2E));
-        adj[n] = dA[n] = dA_all[n] = both(0.0f);
+        adj[n] = dA[n] = both(0.0f);
     }
     if (!LOCAL) {
         if (a.d_final_state) load_states2(a.d_final_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, adj);
@@ -488,12 +490,15 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
         }
     }
     const int quad = lane % S::QUADS * 4, row = lane / S::QUADS, valid = p.n - quad;
-    float bias[4], D[4], dD[4] = {}, dbias[4] = {}, dD_all[4] = {}, dbias_all[4] = {};
+    float dD[4] = {}, dbias[4] = {};
+    if (row == 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        bias[j] = a.dt_bias && j < valid ? a.dt_bias[p.d0 + quad + j] : 0.0f;
-        D[j] = a.D && j < valid ? a.D[p.d0 + quad + j] : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            tile.bias[quad + j] = a.dt_bias && j < valid ? a.dt_bias[p.d0 + quad + j] : 0.0f;
+            tile.D[quad + j] = a.D && j < valid ? a.D[p.d0 + quad + j] : 0.0f;
+        }
     }
+    __syncwarp();
     const T* up = static_cast<const T*>(a.u) + p.b * a.u_stride_b + p.d0 + quad;
     const T* dtp = static_cast<const T*>(a.dt) + p.b * a.dt_stride_b + p.d0 + quad;
     const T* zp = a.z ? static_cast<const T*>(a.z) + p.b * a.z_stride_b + p.d0 + quad : nullptr;
@@ -512,7 +517,6 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     };
 
     Quad<T> u[PAIRS], z[PAIRS], dy[PAIRS], u_next[PAIRS], dt_next[PAIRS], z_next[PAIRS], dy_next[PAIRS], b_next[BCS], c_next[BCS];
-    f32x2 h_next[4];
     const int kept = (a.length + KEEP - 1) / KEEP;
     auto fetch = [&](int t0) {                                // a tile's inputs; zeros behind the sequence's end
 #pragma unroll
@@ -529,7 +533,34 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             if (!LOCAL) b_next[i] = fetch_quad<T>(Bp + t * a.B_stride_t + n, v, aligned_bc);
             c_next[i] = fetch_quad<T>(Cp + t * a.C_stride_t + n, v, aligned_bc);
         }
-        if (!LOCAL) load_states2(a.checkpoints + (((long long)p.b * kept + t0 / KEEP) * a.channels + d0) * N, channels, sg * 4, N, h_next);
+    };
+    // The sums over tokens of the last FLUSH tiles are added to those in memory: in registers alone their rounding errors would grow with the
+    // sequence, and second accumulators there would spill.
+    float* pa = LOCAL ? nullptr : partial_a + ((long long)p.b * split.chunks + chunk) * a.channels * (N + 2);
+    auto flush = [&](bool first) {
+        auto put = [&](int d, int n, float v) {
+            float* to = pa + (long long)d * (N + 2) + n;
+            *to = first ? v : *to + v;
+        };
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (channels > 0 && sg * 4 + n < N) put(d0, sg * 4 + n, lo_of(dA[n]));
+            if (channels > 1 && sg * 4 + n < N) put(d0 + 1, sg * 4 + n, hi_of(dA[n]));
+            dA[n] = both(0.0f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int o = S::QUADS; o < 32; o <<= 1) {         // over the rows
+                dD[j] += __shfl_xor_sync(0xffffffffu, dD[j], o);
+                dbias[j] += __shfl_xor_sync(0xffffffffu, dbias[j], o);
+            }
+            if (row == 0 && j < valid) {
+                put(p.d0 + quad + j, N, dD[j]);
+                put(p.d0 + quad + j, N + 1, dbias[j]);
+            }
+            dD[j] = dbias[j] = 0.0f;
+        }
     };
     const int n_tiles = stop > begin ? (stop - begin + KEEP - 1) / KEEP : 0;
     if (!LOCAL) {                                             // padding
@@ -545,8 +576,11 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     if (n_tiles > 0) fetch(begin + (n_tiles - 1) * KEEP);
     for (int k = n_tiles - 1; k >= 0; --k) {
         const int t0 = begin + k * KEEP;
+        // on its way while the steps are formed: one tile ahead it would take registers from the walk over the tokens
+        if (!LOCAL) load_states2(a.checkpoints + (((long long)p.b * kept + t0 / KEEP) * a.channels + d0) * N, channels, sg * 4, N, h);
         __syncwarp();                                         // the last tile has been read
-        float raw_sig[PAIRS][4], delta[PAIRS][4];
+        float raw_sig[PAIRS][4];
+        const float4 bias = *reinterpret_cast<const float4*>(&tile.bias[quad]);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
             const int r = row + i * ROWS;
@@ -554,8 +588,8 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             if (zp) z[i] = z_next[i];
             dy[i] = dy_next[i];
             const float4 uv = LOCAL ? make_float4(0.f, 0.f, 0.f, 0.f) : widen<T>(u[i]), dv = widen<T>(dt_next[i]), yv = widen<T>(dy[i]);
-            const float raw[4] = {dv.x + bias[0], dv.y + bias[1], dv.z + bias[2], dv.w + bias[3]};
-            float g[4] = {yv.x, yv.y, yv.z, yv.w};
+            const float raw[4] = {dv.x + bias.x, dv.y + bias.y, dv.z + bias.z, dv.w + bias.w};
+            float g[4] = {yv.x, yv.y, yv.z, yv.w}, delta[4];
             if (a.softplus) {
                 float e[4];
 #pragma unroll
@@ -564,10 +598,10 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
                     raw_sig[i][j] = sigmoid_of(raw[j], e[j]);
                 }
                 const f32x2 s0 = softplus2(raw[0], raw[1], e[0], e[1]), s1 = softplus2(raw[2], raw[3], e[2], e[3]);
-                delta[i][0] = lo_of(s0); delta[i][1] = hi_of(s0); delta[i][2] = lo_of(s1); delta[i][3] = hi_of(s1);
+                delta[0] = lo_of(s0); delta[1] = hi_of(s0); delta[2] = lo_of(s1); delta[3] = hi_of(s1);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { delta[i][j] = raw[j]; raw_sig[i][j] = 1.0f; }
+                for (int j = 0; j < 4; ++j) { delta[j] = raw[j]; raw_sig[i][j] = 1.0f; }
             }
             if (zp) {
                 const float4 zv = widen<T>(z[i]);
@@ -575,11 +609,11 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             }
             const uint32_t live = t0 + r < stop ? 0xffffffffu : 0u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) delta[i][j] = __uint_as_float(__float_as_uint(delta[i][j]) & live);
+            for (int j = 0; j < 4; ++j) delta[j] = __uint_as_float(__float_as_uint(delta[j]) & live);
             if (FULL || r < KEEP) {
                 const int at = r * S::QUADS + quad / 4;
-                tile.steps[0][at] = make_float4(delta[i][0], delta[i][1], __fmul_rn(delta[i][0], uv.x), __fmul_rn(delta[i][1], uv.y));
-                tile.steps[1][at] = make_float4(delta[i][2], delta[i][3], __fmul_rn(delta[i][2], uv.z), __fmul_rn(delta[i][3], uv.w));
+                tile.steps[0][at] = make_float4(delta[0], delta[1], __fmul_rn(delta[0], uv.x), __fmul_rn(delta[1], uv.y));
+                tile.steps[1][at] = make_float4(delta[2], delta[3], __fmul_rn(delta[2], uv.z), __fmul_rn(delta[3], uv.w));
                 *reinterpret_cast<float4*>(&tile.dyg[r][quad]) = make_float4(g[0], g[1], g[2], g[3]);
             }
         }
@@ -596,14 +630,10 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             tile.c[0][r][n] = make_float4(cv.x, cv.x, cv.y, cv.y);
             tile.c[1][r][n] = make_float4(cv.z, cv.z, cv.w, cv.w);
         }
-        if (!LOCAL) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) h[n] = h_next[n];
-        }
         __syncwarp();
         if (k > 0) fetch(t0 - KEEP);
         if (!LOCAL) {                                         // the tile's states
-#pragma unroll
+#pragma unroll 2                                              // all eight: 962 us instead of 912, for registers
             for (int t = 0; t < KEEP; ++t) {
                 tile.h[t][0][lane] = make_float4(lo_of(h[0]), hi_of(h[0]), lo_of(h[1]), hi_of(h[1]));
                 tile.h[t][1][lane] = make_float4(lo_of(h[2]), hi_of(h[2]), lo_of(h[3]), hi_of(h[3]));
@@ -614,7 +644,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
                 for (int n = 0; n < 4; ++n) h[n] = fma2(decay_of(A[n], pair(s.x, s.y)), h[n], mul2(pair(s.z, s.w), B[n]));
             }
         }
-#pragma unroll
+#pragma unroll 2
         for (int t = KEEP - 1; t >= 0; --t) {
             f32x2 C[4], g[4];
             load_twice(tile.c, t, sg, C);
@@ -682,6 +712,11 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
                 const float4 zv = widen<T>(z[i]);
                 zz[0] = zv.x; zz[1] = zv.y; zz[2] = zv.z; zz[3] = zv.w;
             }
+            const float2 d01 = *reinterpret_cast<const float2*>(&tile.steps[0][r % KEEP * S::QUADS + quad / 4]);
+            const float2 d23 = *reinterpret_cast<const float2*>(&tile.steps[1][r % KEEP * S::QUADS + quad / 4]);
+            const float delta[4] = {d01.x, d01.y, d23.x, d23.y};
+            const float4 Dv = *reinterpret_cast<const float4*>(&tile.D[quad]);
+            const float D[4] = {Dv.x, Dv.y, Dv.z, Dv.w};
             float o_u[4], o_t[4], o_z[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -691,7 +726,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
                     dyg *= zz[j] * s;
                     o_z[j] = dd[j] * __fmaf_rn(D[j], uu[j], sum[0][j]) * silu_slope(zz[j], s);
                 }
-                o_u[j] = __fmaf_rn(D[j], dyg, delta[i][j] * sum[1][j]);
+                o_u[j] = __fmaf_rn(D[j], dyg, delta[j] * sum[1][j]);
                 o_t[j] = __fmaf_rn(sum[2][j], LN2, uu[j] * sum[1][j]) * raw_sig[i][j];       // A was times log2(e)
                 if (FULL || r < KEEP) {
                     dD[j] = __fmaf_rn(dyg, uu[j], dD[j]);
@@ -706,16 +741,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
                 if (dz) store_quad<T>(dz + (long long)t * a.channels, valid, aligned, on ? make_float4(o_z[0], o_z[1], o_z[2], o_z[3]) : zero);
             }
         }
-        if (k % FLUSH == 0) {                                 // sums of sums: their rounding errors do not grow with the sequence
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                dA_all[n] = add2(dA_all[n], dA[n]);
-                dA[n] = both(0.0f);
-                dD_all[n] += dD[n];
-                dbias_all[n] += dbias[n];
-                dD[n] = dbias[n] = 0.0f;
-            }
-        }
+        if (k % FLUSH == 0) flush(k / FLUSH == (n_tiles - 1) / FLUSH);
     }
     if (LOCAL) {
         const long long at = ((long long)p.b * split.chunks + chunk) * a.channels + d0;
@@ -725,24 +751,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
         return;
     }
     if (a.d_initial_state && chunk == 0) store_states2(a.d_initial_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, adj);
-    float* pa = partial_a + ((long long)p.b * split.chunks + chunk) * a.channels * (N + 2);
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-            if (c < channels && sg * 4 + n < N) pa[(long long)(d0 + c) * (N + 2) + sg * 4 + n] = c ? hi_of(dA_all[n]) : lo_of(dA_all[n]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int o = S::QUADS; o < 32; o <<= 1) {             // over the rows
-            dD_all[j] += __shfl_xor_sync(0xffffffffu, dD_all[j], o);
-            dbias_all[j] += __shfl_xor_sync(0xffffffffu, dbias_all[j], o);
-        }
-        if (row == 0 && j < valid) {
-            pa[(long long)(p.d0 + quad + j) * (N + 2) + N] = dD_all[j];
-            pa[(long long)(p.d0 + quad + j) * (N + 2) + N + 1] = dbias_all[j];
-        }
-    }
+    if (n_tiles == 0) flush(true);
 }
 
 template <typename T>
@@ -830,24 +839,29 @@ static long long parts_of(const el_scan_t& a, int width) {     // pieces of that
     return (long long)a.batch * a.groups * ((a.channels / a.groups + width - 1) / width);
 }
 
-// A sequence is cut into chunks when its channels leave most of the GPU idle: all chunks run side by side, first for the state that
-// each adds on its own (half of the work again), then, from the states that those give, for the outputs.
-static ScanSplit scan_split(const el_scan_t& a, long long warps, float* states) {
+// A sequence is cut into chunks when its channels leave much of the GPU idle: all chunks run side by side, first for the state that each adds on
+// its own (half of a forward pass again, a quarter of a backward pass), then, from the states that those give, for the outputs.  As many chunks as the
+// SMs take at once (`slots` warps each): one more would be a second round.  Below `enough` warps an SM, as measured, 16 states, us:
+//   forward (slots 8, enough 3)    16384 x 2048 channels 0.9 warps an SM: 9 chunks 417, 10 chunks 568;  4096 x 8192 3.5: whole 343, 2 chunks 464
+//   backward (slots 16, enough 12) 4096 x 8192 channels 3.5: whole 3459, 4 chunks 1138;  4 x 1024 x 8192 13.8: whole 915, 2 chunks 1263
+static ScanSplit scan_split(const el_scan_t& a, long long warps, int slots, int enough, float* states) {
     int sms = 148;
     device_sm_count(&sms);
-    const long long slots = (long long)sms * 4;
     ScanSplit s = {1, a.length > 0 ? a.length : 1, states, nullptr};
-    if (warps * 8 < slots * 3) {
-        long long chunks = 2 * slots / warps;
-        if (chunks > 32) chunks = 32;
+    if (warps < (long long)enough * sms) {
+        long long chunks = (long long)slots * sms / warps;
+        if (chunks > 32) chunks = 32;                         // a chunk's first warps go through those before it one by one
         if (chunks > a.length / 64) chunks = a.length / 64;
-        if (chunks >= 3) {
+        if (chunks >= 2) {
             s.tokens = (int)((a.length + chunks - 1) / chunks + TILE - 1) / TILE * TILE;
             s.chunks = (a.length + s.tokens - 1) / s.tokens;
         }
     }
     s.deltas = states + (size_t)a.batch * s.chunks * a.channels * a.states;
     return s;
+}
+template <typename S> static ScanSplit forward_split(const el_scan_t& a, float* states) {
+    return scan_split(a, parts_of(a, S::CW), S::PER_SM / 2, S::PER_SM * 3 / 16, states);
 }
 static size_t split_floats(const el_scan_t& a, const ScanSplit& s) { return s.chunks > 1 ? (size_t)a.batch * s.chunks * a.channels * (a.states + 1) : 0; }
 
@@ -858,7 +872,7 @@ size_t selective_scan_workspace_bytes(const el_scan_t& a) {
     if (a.batch == 0 || a.channels == 0) return 0;
     size_t floats = 0;
     scan_by_shape(a, [&](auto shape) {
-        floats = split_floats(a, scan_split(a, parts_of(a, decltype(shape)::CW), nullptr));
+        floats = split_floats(a, forward_split<decltype(shape)>(a, nullptr));
         return EL_OK;
     });
     return floats * sizeof(float);
@@ -869,7 +883,7 @@ struct ScanBackwardPlan { ScanSplit split; long long blocks; float *bc, *a; size
 template <typename S> static ScanBackwardPlan scan_backward_plan(const el_scan_t& a, float* ws) {
     ScanBackwardPlan p;
     p.blocks = parts_of(a, S::CW * BACK_WARPS);
-    p.split = scan_split(a, parts_of(a, S::CW), nullptr);
+    p.split = scan_split(a, parts_of(a, S::CW), S::BACK_PER_SM, S::BACK_PER_SM * 3 / 4, nullptr);
     const size_t per_group = (a.channels / a.groups + S::CW * BACK_WARPS - 1) / (S::CW * BACK_WARPS);
     const size_t n_bc = 2 * per_group * a.batch * a.length * a.groups * a.states, n_a = (size_t)a.batch * p.split.chunks * a.channels * (a.states + 2);
     p.bc = ws;
@@ -932,7 +946,7 @@ int launch_selective_scan(const el_scan_t& a, cudaStream_t st) {
             using S = decltype(shape);
             const long long warps = parts_of(a, S::CW);
             if (warps > (1ll << 31) - COUPLES) return (int)EL_ERR_TOO_LARGE;
-            const ScanSplit s = scan_split(a, warps, static_cast<float*>(a.workspace));
+            const ScanSplit s = forward_split<S>(a, static_cast<float*>(a.workspace));
             const int rc = s.chunks > 1 ? launch_scan_pass<T, S, true>(a, s, warps, st) : EL_OK;
             return rc != EL_OK ? rc : launch_scan_pass<T, S, false>(a, s, warps, st);
         });
