@@ -4,13 +4,21 @@
 // backward (yn = y r1, hn = h' r2, both formed again from the inputs):
 //   dh = dh' + r2 (dn w2 - hn mean(dn w2 hn));  dw2 = sum dn hn;  ds = sum dh sigmoid(g) p;  dg = dh s p sigmoid'(g)
 //   dp = dh s sigmoid(g);  dw1 = sum dp yn;  dy = r1 (dp w1 - yn mean(dp w1 yn))
-// Row sums in float32: a thread adds 8 or 16 squares, the block adds the threads' in a fixed order.
+// Row sums in float32: a thread adds 8 to 32 squares, the block adds the threads' in a fixed order.
 //
-// A block walks over rows; a thread owns the same one or two vectors of 8 columns in each.
+// Blocks walk over the rows; a thread owns the same vectors of 8 columns in each.  Bound: memory, 5 values read or written per column forward, 8
+// backward, if enough rows are on their way: the next row's values are fetched before this one's two sums over the block.
 #include "mamba_common.cuh"
 
 namespace el {
 using namespace mamba;
+using rowio::add2;
+using rowio::f32x2;
+using rowio::fma2;
+using rowio::hi_of;
+using rowio::lo_of;
+using rowio::mul2;
+using rowio::pair;
 
 constexpr int NORM_MAX_WARPS = 32;
 
@@ -27,180 +35,312 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return v;
 }
 
+// 1 / sqrt(sum / K + eps)
+__device__ __forceinline__ float rms_inverse(float sum, int K, float eps) { return __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)K), eps)); }
+__device__ __forceinline__ float dot(const f32x2 a[4], const f32x2 b[4], float sum) {
+    f32x2 s = mul2(a[0], b[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) s = fma2(a[i], b[i], s);
+    return sum + (lo_of(s) + hi_of(s));
+}
+
+// First column of a thread's vector c, and the distance of its elements: adjacent, or as many apart as the block has threads.
+template <bool ALIGNED> __device__ __forceinline__ int norm_column(int c) { return ALIGNED ? (c * blockDim.x + threadIdx.x) * 8 : c * 8 * blockDim.x + threadIdx.x; }
+
+template <typename T> struct NormRow { Vec<T, 8> h, y, g; };
+
 template <typename T, int VECS, bool ALIGNED>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(512, VECS == 1 ? 2 : 1)
 block_norm_kernel(const el_block_norm_t a) {
     __shared__ float red[2][NORM_MAX_WARPS];
-    const int K = a.width;
-    for (int m = blockIdx.x; m < a.rows; m += gridDim.x) {
-        const T* h = static_cast<const T*>(a.h) + m * a.ld_h;
-        const T* y = static_cast<const T*>(a.y) + m * a.ld_y;
-        const T* g = a.gate ? static_cast<const T*>(a.gate) + m * a.ld_gate : nullptr;
-        float v[VECS][8], ss = 0.0f;
+    const int K = a.width, stride = blockDim.x;
+    NormRow<T> next[VECS];
+    auto fetch_row = [&](int m) {
 #pragma unroll
         for (int c = 0; c < VECS; ++c) {
-            const int k = (c * blockDim.x + threadIdx.x) * 8;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
-            if (k < K) load<T, 8, ALIGNED>(y + k, K - k, v[c]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ss = __fmaf_rn(v[c][j], v[c][j], ss);
+            const int k = norm_column<ALIGNED>(c);
+            next[c].y = next[c].h = next[c].g = zeros<T, 8>();
+            if (k < K) {
+                next[c].y = fetch<T, 8, ALIGNED>(static_cast<const T*>(a.y) + m * a.ld_y + k, K - k, stride);
+                next[c].h = fetch<T, 8, ALIGNED>(static_cast<const T*>(a.h) + m * a.ld_h + k, K - k, stride);
+                if (a.gate) next[c].g = fetch<T, 8, ALIGNED>(static_cast<const T*>(a.gate) + m * a.ld_gate + k, K - k, stride);
+            }
         }
-        const float r1 = __frsqrt_rn(__fadd_rn(__fdiv_rn(block_sum(ss, red[0]), (float)K), a.eps));
+    };
+    int m = blockIdx.x;
+    if (m < a.rows) fetch_row(m);
+    for (; m < a.rows; m += gridDim.x) {
+        NormRow<T> row[VECS];
+        f32x2 v[VECS][4];
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < VECS; ++c) {
+            row[c] = next[c];
+            widen<T, 8>(row[c].y, v[c]);
+            ss = dot(v[c], v[c], ss);
+        }
+        if (VECS == 1 && m + (int)gridDim.x < a.rows) fetch_row(m + gridDim.x);
+        const float r1 = rms_inverse(block_sum(ss, red[0]), K, a.eps);
         ss = 0.0f;
 #pragma unroll
         for (int c = 0; c < VECS; ++c) {
-            const int k = (c * blockDim.x + threadIdx.x) * 8;
-            if (k < K) {
-                float hv[8], gv[8], w[8], s[8];
-                load<T, 8, ALIGNED>(h + k, K - k, hv);
-                if (g) load<T, 8, ALIGNED>(g + k, K - k, gv);
-                load<float, 8, ALIGNED>(a.post_weight + k, K - k, w);
-                if (a.scale) load<float, 8, ALIGNED>(a.scale + k, K - k, s);
+            const int k = norm_column<ALIGNED>(c);
+            if (k >= K) continue;
+            f32x2 h[4], w[4], f[4];
+            widen<T, 8>(row[c].h, h);
+            widen<float, 8>(fetch<float, 8, ALIGNED>(a.post_weight + k, K - k, stride), w);
+            if (a.gate) {
+                widen<T, 8>(row[c].g, f);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float f = g ? sigmoid(gv[j]) : 1.0f;
-                    if (a.scale) f *= s[j];
-                    v[c][j] = __fmaf_rn(f, v[c][j] * r1 * w[j], hv[j]);
-                    ss = __fmaf_rn(v[c][j], v[c][j], ss);          // columns behind the row's end hold zeros
-                }
-                store<T, 8, ALIGNED>(static_cast<T*>(a.h_out) + (long long)m * K + k, K - k, v[c]);
+                for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], sigmoid2(f[i]));
             }
+            if (a.scale) {
+                widen<float, 8>(fetch<float, 8, ALIGNED>(a.scale + k, K - k, stride), f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], f[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[c][i] = fma2(w[i], mul2(v[c][i], both(r1)), h[i]);      // columns behind the row's end hold zeros
+            ss = dot(v[c], v[c], ss);
+            put<T, 8, ALIGNED>(static_cast<T*>(a.h_out) + (long long)m * K + k, K - k, stride, v[c]);
         }
-        const float r2 = __frsqrt_rn(__fadd_rn(__fdiv_rn(block_sum(ss, red[1]), (float)K), a.eps));
+        const float r2 = rms_inverse(block_sum(ss, red[1]), K, a.eps);
 #pragma unroll
         for (int c = 0; c < VECS; ++c) {
-            const int k = (c * blockDim.x + threadIdx.x) * 8;
-            if (k < K) {
-                float w[8];
-                load<float, 8, ALIGNED>(a.pre_weight + k, K - k, w);
+            const int k = norm_column<ALIGNED>(c);
+            if (k >= K) continue;
+            f32x2 w[4];
+            widen<float, 8>(fetch<float, 8, ALIGNED>(a.pre_weight + k, K - k, stride), w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[c][j] = v[c][j] * r2 * w[j];
-                store<T, 8, ALIGNED>(static_cast<T*>(a.normed) + (long long)m * K + k, K - k, v[c]);
-            }
+            for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], mul2(v[c][i], both(r2)));
+            put<T, 8, ALIGNED>(static_cast<T*>(a.normed) + (long long)m * K + k, K - k, stride, w);
         }
         if (a.rstd && threadIdx.x == 0) {
             a.rstd[2 * (long long)m] = r1;
             a.rstd[2 * (long long)m + 1] = r2;
         }
+        if (VECS > 1 && m + (int)gridDim.x < a.rows) fetch_row(m + gridDim.x);
     }
 }
 
-// Column sums of a block's rows stay in registers and go to `partial` [blocks][3][width]: dw1, dw2, ds.
-template <typename T, int VECS, bool ALIGNED>
-__global__ void __launch_bounds__(1024)
+// Backward, rows of up to 4096 columns: a row's values stay in registers, one vector a thread, and so do the column sums of a block's
+// rows, which go to `partial` [blocks][3][width]: dw1, dw2, ds.  float32 rows are not fetched ahead: no registers are left for them.
+template <typename T> struct NormGrads { Vec<T, 8> h, y, g, dh, dn; };
+
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(512, 1)
 block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial) {
+    constexpr bool AHEAD = sizeof(T) == 2;
     __shared__ float red[2][NORM_MAX_WARPS];
-    const int K = a.width;
-    float sums[VECS][3][8] = {};
+    const int K = a.width, stride = blockDim.x, k = norm_column<ALIGNED>(0);
+    const bool mine = k < K;
+    f32x2 sums[3][4];
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[q][i] = both(0.0f);
+    NormGrads<T> next;
+    auto get = [&](const void* p, long long ld, int m) {
+        return p && mine ? fetch<T, 8, ALIGNED>(static_cast<const T*>(p) + m * ld + k, K - k, stride) : zeros<T, 8>();
+    };
+    auto fetch_row = [&](int m) {
+        next.dn = get(a.dnormed, a.ld_dnormed, m);
+        next.y = get(a.y, a.ld_y, m);
+        next.h = get(a.h, a.ld_h, m);
+        next.g = get(a.gate, a.ld_gate, m);
+        next.dh = get(a.dh_out, a.ld_dh_out, m);
+    };
+    auto weight = [&](const float* p, f32x2 w[4]) {
+        if (p && mine) widen<float, 8>(fetch<float, 8, ALIGNED>(p + k, K - k, stride), w);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = both(p ? 0.0f : 1.0f);
+    };
+    auto out = [&](void* p, int m, const f32x2 v[4]) {
+        if (p && mine) put<T, 8, ALIGNED>(static_cast<T*>(p) + (long long)m * K + k, K - k, stride, v);
+    };
+    if (AHEAD && blockIdx.x < a.rows) fetch_row(blockIdx.x);
+    for (int m = blockIdx.x; m < a.rows; m += gridDim.x) {
+        if (!AHEAD) fetch_row(m);
+        const NormGrads<T> row = next;
+        if (AHEAD && m + (int)gridDim.x < a.rows) fetch_row(m + gridDim.x);
+        const float r1 = a.rstd[2 * (long long)m], r2 = a.rstd[2 * (long long)m + 1];
+        f32x2 yn[4], hn[4], sg[4], dt[4], w1[4], s[4], t[4];
+        widen<T, 8>(row.y, yn);
+        widen<T, 8>(row.h, hn);
+        widen<T, 8>(row.g, sg);
+        widen<T, 8>(row.dn, dt);
+        weight(a.post_weight, w1);
+        weight(a.scale, s);
+        weight(a.pre_weight, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            yn[i] = mul2(yn[i], both(r1));
+            sg[i] = a.gate ? sigmoid2(sg[i]) : both(1.0f);
+            hn[i] = mul2(fma2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]), hn[i]), both(r2));
+            sums[1][i] = fma2(dt[i], hn[i], sums[1][i]);
+            dt[i] = mul2(dt[i], t[i]);
+        }
+        const float c2 = __fdiv_rn(block_sum(dot(dt, hn, 0.0f), red[0]), (float)K);
+        f32x2 d[4];
+        widen<T, 8>(row.dh, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            d[i] = fma2(both(r2), fma2(hn[i], both(-c2), dt[i]), d[i]);
+            const f32x2 p = mul2(yn[i], w1[i]), ds = mul2(d[i], sg[i]), dp = mul2(ds, s[i]);
+            sums[2][i] = fma2(ds, p, sums[2][i]);
+            hn[i] = mul2(mul2(dp, p), fma2(sg[i], both(-1.0f), both(1.0f)));      // of the gate
+            sums[0][i] = fma2(dp, yn[i], sums[0][i]);
+            dt[i] = mul2(dp, w1[i]);
+        }
+        out(a.dh, m, d);
+        if (a.gate) out(a.dgate, m, hn);
+        const float c1 = __fdiv_rn(block_sum(dot(dt, yn, 0.0f), red[1]), (float)K);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dt[i] = mul2(both(r1), fma2(yn[i], both(-c1), dt[i]));
+        out(a.dy_in, m, dt);
+    }
+    if (mine) {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) put<float, 8, ALIGNED>(partial + ((long long)blockIdx.x * 3 + q) * K + k, K - k, stride, sums[q]);
+    }
+}
+
+// Wider rows: nothing is kept between the three passes over a row, whose second and third come from L2, and the column sums are in shared memory.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(512, 1)
+block_norm_backward_wide_kernel(const el_block_norm_t a, float* __restrict__ partial) {
+    __shared__ float red[2][NORM_MAX_WARPS];
+    extern __shared__ float4 sums_[];                         // [3][padded width / 4]: a thread's own columns, as vectors
+    float* sums = reinterpret_cast<float*>(sums_);
+    const int K = a.width, stride = blockDim.x, vecs = (K + 8 * stride - 1) / (8 * stride), padded = vecs * 8 * stride;
+    auto slot = [&](int q, int c, int half) -> float4& { return sums_[((q * vecs + c) * 2 + half) * stride + threadIdx.x]; };
+    for (int i = threadIdx.x; i < 3 * padded; i += stride) sums[i] = 0.0f;
+    __syncthreads();
+    auto get = [&](const void* p, long long ld, int m, int k, f32x2 v[4]) {
+        widen<T, 8>(p ? fetch<T, 8, ALIGNED>(static_cast<const T*>(p) + m * ld + k, K - k, stride) : zeros<T, 8>(), v);
+    };
+    auto weight = [&](const float* p, int k, f32x2 w[4]) {
+        if (p) widen<float, 8>(fetch<float, 8, ALIGNED>(p + k, K - k, stride), w);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = both(1.0f);
+    };
+    auto add_to = [&](int q, int c, const f32x2 v[4]) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float4 s = slot(q, c, half);
+            s.x += lo_of(v[2 * half]); s.y += hi_of(v[2 * half]); s.z += lo_of(v[2 * half + 1]); s.w += hi_of(v[2 * half + 1]);
+            slot(q, c, half) = s;
+        }
+    };
     for (int m = blockIdx.x; m < a.rows; m += gridDim.x) {
         const float r1 = a.rstd[2 * (long long)m], r2 = a.rstd[2 * (long long)m + 1];
-        const T* h = static_cast<const T*>(a.h) + m * a.ld_h;
-        const T* y = static_cast<const T*>(a.y) + m * a.ld_y;
-        const T* g = a.gate ? static_cast<const T*>(a.gate) + m * a.ld_gate : nullptr;
-        const T* dh = a.dh_out ? static_cast<const T*>(a.dh_out) + m * a.ld_dh_out : nullptr;
-        const T* dn = a.dnormed ? static_cast<const T*>(a.dnormed) + m * a.ld_dnormed : nullptr;
-        float yn[VECS][8], hn[VECS][8], sg[VECS][8], dt[VECS][8], dot = 0.0f;
+        // yn, sigmoid of the gate, p = yn w1, hn of a vector
+        auto form = [&](int k, f32x2 yn[4], f32x2 sg[4], f32x2 w1[4], f32x2 s[4], f32x2 hn[4]) {
+            get(a.y, a.ld_y, m, k, yn);
+            get(a.h, a.ld_h, m, k, hn);
+            get(a.gate, a.ld_gate, m, k, sg);
+            weight(a.post_weight, k, w1);
+            weight(a.scale, k, s);
 #pragma unroll
-        for (int c = 0; c < VECS; ++c) {
-            const int k = (c * blockDim.x + threadIdx.x) * 8;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) yn[c][j] = hn[c][j] = sg[c][j] = dt[c][j] = 0.0f;
-            if (k < K) {
-                float w1[8], w2[8], s[8];
-                load<T, 8, ALIGNED>(y + k, K - k, yn[c]);
-                load<T, 8, ALIGNED>(h + k, K - k, hn[c]);
-                if (g) load<T, 8, ALIGNED>(g + k, K - k, sg[c]);
-                if (dn) load<T, 8, ALIGNED>(dn + k, K - k, dt[c]);
-                load<float, 8, ALIGNED>(a.post_weight + k, K - k, w1);
-                load<float, 8, ALIGNED>(a.pre_weight + k, K - k, w2);
-                if (a.scale) load<float, 8, ALIGNED>(a.scale + k, K - k, s);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    yn[c][j] *= r1;
-                    sg[c][j] = g ? sigmoid(sg[c][j]) : 1.0f;
-                    const float f = a.scale ? sg[c][j] * s[j] : sg[c][j];
-                    hn[c][j] = __fmaf_rn(f, yn[c][j] * w1[j], hn[c][j]) * r2;
-                    sums[c][1][j] = __fmaf_rn(dt[c][j], hn[c][j], sums[c][1][j]);
-                    dt[c][j] *= w2[j];
-                    dot = __fmaf_rn(dt[c][j], hn[c][j], dot);
-                }
+            for (int i = 0; i < 4; ++i) {
+                yn[i] = mul2(yn[i], both(r1));
+                sg[i] = a.gate ? sigmoid2(sg[i]) : both(1.0f);
+                hn[i] = mul2(fma2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]), hn[i]), both(r2));
             }
+        };
+        float sum = 0.0f;
+        for (int c = 0; c < vecs; ++c) {
+            const int k = norm_column<ALIGNED>(c);
+            if (k >= K) continue;
+            f32x2 yn[4], sg[4], w1[4], s[4], hn[4], dn[4], w2[4];
+            form(k, yn, sg, w1, s, hn);
+            get(a.dnormed, a.ld_dnormed, m, k, dn);
+            weight(a.pre_weight, k, w2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w2[i] = mul2(w2[i], dn[i]);
+                dn[i] = mul2(dn[i], hn[i]);
+            }
+            sum = dot(w2, hn, sum);
+            add_to(1, c, dn);
         }
-        const float c2 = __fdiv_rn(block_sum(dot, red[0]), (float)K);
-        dot = 0.0f;
+        const float c2 = __fdiv_rn(block_sum(sum, red[0]), (float)K);
+        sum = 0.0f;
+        float c1 = 0.0f;
+        for (int pass = 0; pass < 2; ++pass) {
+            for (int c = 0; c < vecs; ++c) {
+                const int k = norm_column<ALIGNED>(c);
+                if (k >= K) continue;
+                f32x2 yn[4], sg[4], w1[4], s[4], hn[4], d[4], dn[4], w2[4];
+                form(k, yn, sg, w1, s, hn);
+                get(a.dh_out, a.ld_dh_out, m, k, d);
+                get(a.dnormed, a.ld_dnormed, m, k, dn);
+                weight(a.pre_weight, k, w2);
 #pragma unroll
-        for (int c = 0; c < VECS; ++c) {
-            const int k = (c * blockDim.x + threadIdx.x) * 8;
-            if (k < K) {
-                float w1[8], s[8], d[8] = {}, dg[8];
-                if (dh) load<T, 8, ALIGNED>(dh + k, K - k, d);
-                load<float, 8, ALIGNED>(a.post_weight + k, K - k, w1);
-                if (a.scale) load<float, 8, ALIGNED>(a.scale + k, K - k, s);
+                for (int i = 0; i < 4; ++i) d[i] = fma2(both(r2), fma2(hn[i], both(-c2), mul2(dn[i], w2[i])), d[i]);
+                if (pass == 0) {
+                    put<T, 8, ALIGNED>(static_cast<T*>(a.dh) + (long long)m * K + k, K - k, stride, d);
+                    f32x2 ds[4], dg[4], dw[4], dp[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    d[j] = __fmaf_rn(r2, __fmaf_rn(-hn[c][j], c2, dt[c][j]), d[j]);
-                    const float p = yn[c][j] * w1[j], sc = a.scale ? s[j] : 1.0f, ds = d[j] * sg[c][j];
-                    sums[c][2][j] = __fmaf_rn(ds, p, sums[c][2][j]);
-                    dg[j] = ds * sc * p * (1.0f - sg[c][j]);
-                    const float dp = ds * sc;
-                    sums[c][0][j] = __fmaf_rn(dp, yn[c][j], sums[c][0][j]);
-                    dt[c][j] = dp * w1[j];
-                    dot = __fmaf_rn(dt[c][j], yn[c][j], dot);
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x2 p = mul2(yn[i], w1[i]);
+                        dn[i] = mul2(d[i], sg[i]);
+                        ds[i] = mul2(dn[i], p);
+                        dp[i] = mul2(dn[i], s[i]);
+                        dg[i] = mul2(mul2(dp[i], p), fma2(sg[i], both(-1.0f), both(1.0f)));
+                        dw[i] = mul2(dp[i], yn[i]);
+                        dp[i] = mul2(dp[i], w1[i]);
+                    }
+                    add_to(2, c, ds);
+                    add_to(0, c, dw);
+                    if (a.gate && a.dgate) put<T, 8, ALIGNED>(static_cast<T*>(a.dgate) + (long long)m * K + k, K - k, stride, dg);
+                    sum = dot(dp, yn, sum);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[i] = mul2(both(r1), fma2(yn[i], both(-c1), mul2(mul2(mul2(d[i], sg[i]), s[i]), w1[i])));
+                    put<T, 8, ALIGNED>(static_cast<T*>(a.dy_in) + (long long)m * K + k, K - k, stride, d);
                 }
-                if (a.dh) store<T, 8, ALIGNED>(static_cast<T*>(a.dh) + (long long)m * K + k, K - k, d);
-                if (a.dgate && g) store<T, 8, ALIGNED>(static_cast<T*>(a.dgate) + (long long)m * K + k, K - k, dg);
             }
-        }
-        const float c1 = __fdiv_rn(block_sum(dot, red[1]), (float)K);
-        if (a.dy_in) {
-#pragma unroll
-            for (int c = 0; c < VECS; ++c) {
-                const int k = (c * blockDim.x + threadIdx.x) * 8;
-                if (k < K) {
-                    float d[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) d[j] = r1 * __fmaf_rn(-yn[c][j], c1, dt[c][j]);
-                    store<T, 8, ALIGNED>(static_cast<T*>(a.dy_in) + (long long)m * K + k, K - k, d);
-                }
-            }
+            if (pass == 0) c1 = __fdiv_rn(block_sum(sum, red[1]), (float)K);
         }
     }
+    for (int c = 0; c < vecs; ++c) {
+        const int k = norm_column<ALIGNED>(c);
+        if (k >= K) continue;
 #pragma unroll
-    for (int c = 0; c < VECS; ++c) {
-        const int k = (c * blockDim.x + threadIdx.x) * 8;
-        if (k < K) {
-#pragma unroll
-            for (int q = 0; q < 3; ++q)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k + j < K) partial[((long long)blockIdx.x * 3 + q) * K + k + j] = sums[c][q][j];
+        for (int q = 0; q < 3; ++q) {
+            const float4 x = slot(q, c, 0), y = slot(q, c, 1);
+            const f32x2 v[4] = {pair(x.x, x.y), pair(x.z, x.w), pair(y.x, y.y), pair(y.z, y.w)};
+            put<float, 8, ALIGNED>(partial + ((long long)blockIdx.x * 3 + q) * K + k, K - k, stride, v);
         }
     }
 }
 
-static __global__ void __launch_bounds__(256)
-block_norm_sums_kernel(const float* __restrict__ partial, int n_parts, int K, float* __restrict__ dw1, float* __restrict__ dw2, float* __restrict__ ds) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= 3 * K) return;
-    float s = 0.0f;
-#pragma unroll 8
-    for (int p = 0; p < n_parts; ++p) s += partial[(long long)p * 3 * K + i];
-    float* out = i < K ? dw1 : i < 2 * K ? dw2 : ds;
-    if (out) out[i % K] = s;
-}
+struct NormSums {
+    float *dw1, *dw2, *ds;
+    int K;
+    __device__ __forceinline__ void operator()(int i, float v) const {
+        float* out = i < K ? dw1 : i < 2 * K ? dw2 : ds;
+        if (out) out[i % K] = v;
+    }
+};
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
 
-static int norm_threads(int K) {
-    const int vecs = K > 8192 ? 2 : 1;
-    const int t = (K + 8 * vecs - 1) / (8 * vecs);
-    return (t + 31) / 32 * 32;
-}
-static int norm_backward_blocks(const el_block_norm_t& a) {
+constexpr int NORM_HELD = 4096;       // columns of a row that one vector per thread of a block holds
+
+static int norm_threads(int K, int vecs) { return ((K + 8 * vecs - 1) / (8 * vecs) + 31) / 32 * 32; }
+static int norm_vectors(int K) { return K <= NORM_HELD ? 1 : K <= 2 * NORM_HELD ? 2 : 4; }
+static int norm_blocks(int rows, int per_sm) {
     int sms = 148;
     device_sm_count(&sms);
-    return a.rows < sms ? a.rows : sms;
+    return rows < (long long)sms * per_sm ? rows : sms * per_sm;
+}
+// An SM's registers take 512 threads of the backward kernel, of the wide one too.
+static int norm_backward_blocks(const el_block_norm_t& a) {
+    return norm_blocks(a.rows, a.width <= NORM_HELD ? 512 / norm_threads(a.width > 0 ? a.width : 1, 1) : 1);
 }
 size_t block_norm_backward_workspace_bytes(const el_block_norm_t& a) { return (size_t)norm_backward_blocks(a) * 3 * a.width * sizeof(float); }
 
@@ -216,11 +356,7 @@ static bool norm_aligned(const el_block_norm_t& a) {
 }
 
 template <typename F> static int norm_variant(const el_block_norm_t& a, F f) {
-    auto typed = [&](auto t) {
-        const bool al = norm_aligned(a);
-        if (a.width > 8192) return al ? f(t, std::integral_constant<int, 2>(), std::true_type()) : f(t, std::integral_constant<int, 2>(), std::false_type());
-        return al ? f(t, std::integral_constant<int, 1>(), std::true_type()) : f(t, std::integral_constant<int, 1>(), std::false_type());
-    };
+    auto typed = [&](auto t) { return norm_aligned(a) ? f(t, std::true_type()) : f(t, std::false_type()); };
     switch (a.dtype) {
         case EL_F16: return typed(__half());
         case EL_BF16: return typed(__nv_bfloat16());
@@ -229,8 +365,13 @@ template <typename F> static int norm_variant(const el_block_norm_t& a, F f) {
 }
 
 int launch_block_norm(const el_block_norm_t& a, cudaStream_t st) {
-    return norm_variant(a, [&](auto t, auto vecs, auto al) {
-        block_norm_kernel<decltype(t), decltype(vecs)::value, decltype(al)::value><<<a.rows, norm_threads(a.width), 0, st>>>(a);
+    const int vecs = norm_vectors(a.width), threads = norm_threads(a.width, vecs), blocks = norm_blocks(a.rows, vecs == 1 ? 1024 / threads : 1);
+    return norm_variant(a, [&](auto t, auto al) {
+        using T = decltype(t);
+        constexpr bool AL = decltype(al)::value;
+        if (vecs == 1) block_norm_kernel<T, 1, AL><<<blocks, threads, 0, st>>>(a);
+        else if (vecs == 2) block_norm_kernel<T, 2, AL><<<blocks, threads, 0, st>>>(a);
+        else block_norm_kernel<T, 4, AL><<<blocks, threads, 0, st>>>(a);
         return check_launch();
     });
 }
@@ -239,15 +380,28 @@ int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st) {
     const int blocks = norm_backward_blocks(a);
     float* partial = static_cast<float*>(a.workspace);
     if (blocks > 0) {
-        const int rc = norm_variant(a, [&](auto t, auto vecs, auto al) {
-            block_norm_backward_kernel<decltype(t), decltype(vecs)::value, decltype(al)::value><<<blocks, norm_threads(a.width), 0, st>>>(a, partial);
+        const int rc = norm_variant(a, [&](auto t, auto al) {
+            using T = decltype(t);
+            constexpr bool AL = decltype(al)::value;
+            if (a.width <= NORM_HELD) {
+                block_norm_backward_kernel<T, AL><<<blocks, norm_threads(a.width, 1), 0, st>>>(a, partial);
+                return check_launch();
+            }
+            static DeviceOnce once;
+            int dev = 0;
+            EL_CUDA_TRY(cudaGetDevice(&dev));
+            if (!once.is_done(dev)) {
+                EL_CUDA_TRY(cudaFuncSetAttribute(block_norm_backward_wide_kernel<T, AL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 16384 * 4));
+                once.mark(dev);
+            }
+            const int vecs = (a.width + 8 * 512 - 1) / (8 * 512);
+            block_norm_backward_wide_kernel<T, AL><<<blocks, 512, 3 * vecs * 8 * 512 * sizeof(float), st>>>(a, partial);
             return check_launch();
         });
         if (rc != EL_OK) return rc;
     }
-    if (a.dpost_weight || a.dpre_weight || a.dscale)
-        block_norm_sums_kernel<<<(3 * a.width + 255) / 256, 256, 0, st>>>(partial, blocks, a.width, a.dpost_weight, a.dpre_weight, a.dscale);
-    return check_launch();
+    if (!a.dpost_weight && !a.dpre_weight && !a.dscale) return EL_OK;
+    return launch_column_sums(partial, blocks, 3 * a.width, NormSums{a.dpost_weight, a.dpre_weight, a.dscale, a.width}, st);
 }
 
 }  // namespace el

@@ -9,171 +9,242 @@
 
 namespace el {
 using namespace mamba;
+using rowio::add2;
+using rowio::f32x2;
+using rowio::fma2;
+using rowio::hi_of;
+using rowio::lo_of;
+using rowio::mul2;
+using rowio::pair;
 
 constexpr int CONV_LANES = 32;        // threads of a block along the channels; the others are strips of tokens
+
+constexpr int CONV_AHEAD = 4;         // tokens that are fetched together, one such group ahead of the arithmetic
+#ifndef BA
+#define BA 2
+#define BB 2
+#endif
+
+// Where a thread's channels lie: V adjacent ones, or, where vectors are not possible, every 32nd.
+template <int V, bool ALIGNED> struct ConvPlace {
+    int d, valid;
+    __device__ __forceinline__ explicit ConvPlace(int channels) {
+        d = ALIGNED ? (blockIdx.x * CONV_LANES + threadIdx.x) * V : blockIdx.x * CONV_LANES * V + threadIdx.x;
+        valid = channels - d;
+    }
+    __device__ __forceinline__ int channel(int j) const { return ALIGNED ? d + j : d + CONV_LANES * j; }
+};
 
 template <typename T, int W, bool ALIGNED>
 __global__ void __launch_bounds__(128)
 causal_conv_kernel(const el_conv_t a, int strip) {
-    constexpr int V = 8, H = W - 1;
-    const int d = (blockIdx.x * CONV_LANES + threadIdx.x) * V, b = blockIdx.z;
-    if (d >= a.channels) return;
-    const int valid = a.channels - d;
+    constexpr int V = 16 / sizeof(T), P = V / 2, H = W - 1, U = CONV_AHEAD;
+    const ConvPlace<V, ALIGNED> at(a.channels);
+    const int b = blockIdx.z;
+    if (at.valid <= 0) return;
     const int n = a.lengths ? min(max(a.lengths[b], 0), a.length) : a.length;
-    const T* x = static_cast<const T*>(a.x) + b * a.x_stride_b + d;
-    T* y = static_cast<T*>(a.y) + (long long)b * a.length * a.channels + d;
-    const T* first = a.initial_state ? static_cast<const T*>(a.initial_state) + (long long)b * H * a.channels + d : nullptr;
-    auto input = [&](int t, float v[V]) {                     // x[t], the state before token 0; t < n
-        if (t >= 0) load<T, V, ALIGNED>(x + t * a.x_stride_t, valid, v);
-        else if (first) load<T, V, ALIGNED>(first + (long long)(t + H) * a.channels, valid, v);
-        else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = 0.0f;
-        }
+    const T* x = static_cast<const T*>(a.x) + b * a.x_stride_b + at.d;
+    T* y = static_cast<T*>(a.y) + (long long)b * a.length * a.channels + at.d;
+    const T* first = a.initial_state ? static_cast<const T*>(a.initial_state) + (long long)b * H * a.channels + at.d : nullptr;
+    auto input = [&](int t) {                                 // x[t], the state before token 0, zeros from token n on
+        if (t >= n) return zeros<T, V>();
+        if (t >= 0) return fetch<T, V, ALIGNED>(x + t * a.x_stride_t, at.valid, CONV_LANES);
+        return first ? fetch<T, V, ALIGNED>(first + (long long)(t + H) * a.channels, at.valid, CONV_LANES) : zeros<T, V>();
     };
     const int s = blockIdx.y * blockDim.y + threadIdx.y;
     const int t0 = s * strip, t1 = min(t0 + strip, a.length);
     if (t0 < t1) {
-        float w[W][V], bias[V], hist[H][V];
+        Vec<T, V> ahead[U];
+        f32x2 w[W][P], bias[P], win[H + U][P];                // win: x[t-H] .. x[t+U-1]
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = min(d + j, a.channels - 1);
+        for (int u = 0; u < U; ++u) ahead[u] = input(t0 + u);
 #pragma unroll
-            for (int k = 0; k < W; ++k) w[k][j] = a.weight[(long long)c * W + k];
-            bias[j] = a.bias ? a.bias[c] : 0.0f;
+        for (int k = 0; k < H; ++k) widen<T, V>(input(t0 - H + k), win[U + k]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int c0 = min(at.channel(2 * i), a.channels - 1), c1 = min(at.channel(2 * i + 1), a.channels - 1);
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][i] = pair(a.weight[(long long)c0 * W + k], a.weight[(long long)c1 * W + k]);
+            bias[i] = a.bias ? pair(a.bias[c0], a.bias[c1]) : both(0.0f);
         }
+        for (int t = t0; t < t1; t += U) {
 #pragma unroll
-        for (int k = 0; k < H; ++k) {
-            if (t0 - H + k < n) input(t0 - H + k, hist[k]);
-        }
-        const int tn = min(t1, n);
-        int t = t0;
-#pragma unroll 4
-        for (; t < tn; ++t) {
-            float v[V], o[V];
-            load<T, V, ALIGNED>(x + t * a.x_stride_t, valid, v);
+            for (int k = 0; k < H; ++k)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float p = bias[j];
+                for (int i = 0; i < P; ++i) win[k][i] = win[U + k][i];
 #pragma unroll
-                for (int k = 0; k < H; ++k) p = __fmaf_rn(w[k][j], hist[k][j], p);
-                p = __fmaf_rn(w[H][j], v[j], p);
-                o[j] = a.silu ? __fmul_rn(p, sigmoid(p)) : p;
+            for (int u = 0; u < U; ++u) widen<T, V>(ahead[u], win[H + u]);
+            if (t + U < t1) {
 #pragma unroll
-                for (int k = 0; k + 1 < H; ++k) hist[k][j] = hist[k + 1][j];
-                hist[H - 1][j] = v[j];
+                for (int u = 0; u < U; ++u) ahead[u] = input(t + U + u);
             }
-            store<T, V, ALIGNED>(y + (long long)t * a.channels, valid, o);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                f32x2 o[P];
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    o[i] = bias[i];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) o[i] = fma2(w[k][i], win[u + k][i], o[i]);
+                }
+                if (a.silu) {
+#pragma unroll
+                    for (int i = 0; i < P; ++i) o[i] = mul2(o[i], sigmoid2(o[i]));
+                }
+                if (t + u >= n) {
+#pragma unroll
+                    for (int i = 0; i < P; ++i) o[i] = both(0.0f);
+                }
+                if (t + u < t1) put<T, V, ALIGNED>(y + (long long)(t + u) * a.channels, at.valid, CONV_LANES, o);
+            }
         }
-        const float zero[V] = {};
-        for (; t < t1; ++t) store<T, V, ALIGNED>(y + (long long)t * a.channels, valid, zero);
     }
     if (a.final_state && s == 0) {
-        T* last = static_cast<T*>(a.final_state) + (long long)b * H * a.channels + d;
+        T* last = static_cast<T*>(a.final_state) + (long long)b * H * a.channels + at.d;
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-            float v[V];
-            input(n - H + k, v);
-            store<T, V, ALIGNED>(last + (long long)k * a.channels, valid, v);
+            f32x2 v[P];
+            widen<T, V>(input(n - H + k), v);
+            put<T, V, ALIGNED>(last + (long long)k * a.channels, at.valid, CONV_LANES, v);
         }
     }
 }
 
 // dx and the partial sums of dweight and dbias: a block's strips are added in order and stored as one row [W+1][channels] of `partial`.
 template <typename T, int W, bool ALIGNED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, BB)
 causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ partial) {
-    constexpr int V = 4, H = W - 1;
+    constexpr int V = 4, P = V / 2, H = W - 1, U = BA;
     extern __shared__ float red[];                            // [strips of the block][W+1][channels of the block]
-    const int d = (blockIdx.x * CONV_LANES + threadIdx.x) * V, b = blockIdx.z;
-    const int valid = a.channels - d;
-    float dw[W][V] = {}, db[V] = {};
+    const ConvPlace<V, ALIGNED> at(a.channels);
+    const int b = blockIdx.z;
+    f32x2 dw[W][P], db[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        db[i] = both(0.0f);
+#pragma unroll
+        for (int k = 0; k < W; ++k) dw[k][i] = both(0.0f);
+    }
     const int s = blockIdx.y * blockDim.y + threadIdx.y;
     const int t0 = s * strip, t1 = min(t0 + strip, a.length);
-    if (valid > 0 && (t0 < t1 || (s == 0 && a.d_initial_state))) {
+    if (at.valid > 0 && (t0 < t1 || (s == 0 && a.d_initial_state))) {
         const int n = a.lengths ? min(max(a.lengths[b], 0), a.length) : a.length;
-        const T* x = static_cast<const T*>(a.x) + b * a.x_stride_b + d;
-        const T* dy = static_cast<const T*>(a.dy) + b * a.dy_stride_b + d;
-        T* dx = a.dx ? static_cast<T*>(a.dx) + (long long)b * a.length * a.channels + d : nullptr;
-        const long long state_at = (long long)b * H * a.channels + d;
+        const T* x = static_cast<const T*>(a.x) + b * a.x_stride_b + at.d;
+        const T* dy = a.dy ? static_cast<const T*>(a.dy) + b * a.dy_stride_b + at.d : nullptr;
+        T* dx = a.dx ? static_cast<T*>(a.dx) + (long long)b * a.length * a.channels + at.d : nullptr;
+        const long long state_at = (long long)b * H * a.channels + at.d;
         const T* first = a.initial_state ? static_cast<const T*>(a.initial_state) + state_at : nullptr;
         const T* d_last = a.d_final_state ? static_cast<const T*>(a.d_final_state) + state_at : nullptr;
         T* d_first = a.d_initial_state ? static_cast<T*>(a.d_initial_state) + state_at : nullptr;
-        float w[W][V], bias[V], hist[W][V], dp[W][V];         // hist: x[t-(W-1) .. t]; dp: dpre of the same tokens
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = min(d + j, a.channels - 1);
-#pragma unroll
-            for (int k = 0; k < W; ++k) w[k][j] = a.weight[(long long)c * W + k];
-            bias[j] = a.bias ? a.bias[c] : 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-            const int t = t0 - W + k;
-            float v[V] = {};
-            if (t >= 0 && t < n) load<T, V, ALIGNED>(x + t * a.x_stride_t, valid, v);
-            else if (t < 0 && t >= -H && first) load<T, V, ALIGNED>(first + (long long)(t + H) * a.channels, valid, v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) { hist[k][j] = v[j]; dp[k][j] = 0.0f; }
-        }
-        // at token t the gradient of x[t-(W-1)] is complete; the strip's own x are t0 .. t1-1, for the first strip the state's before them too
+        auto input = [&](int t) {
+            if (t >= n) return zeros<T, V>();
+            if (t >= 0) return fetch<T, V, ALIGNED>(x + t * a.x_stride_t, at.valid, CONV_LANES);
+            return first ? fetch<T, V, ALIGNED>(first + (long long)(t + H) * a.channels, at.valid, CONV_LANES) : zeros<T, V>();
+        };
+        auto gradient = [&](int t) { return t < n && dy ? fetch<T, V, ALIGNED>(dy + t * a.dy_stride_t, at.valid, CONV_LANES) : zeros<T, V>(); };
+        // at token t the gradient of x[t-H] is complete; the strip's own x are t0 .. t1-1, for the first strip the state's before them too
         const int end = max(t1, t0) + H;
-#pragma unroll 2
-        for (int t = t0; t < end; ++t) {
-            float v[V] = {}, g[V] = {};
-            const bool live = t < n && a.dy;
-            if (t < n) load<T, V, ALIGNED>(x + t * a.x_stride_t, valid, v);
-            if (live) load<T, V, ALIGNED>(dy + t * a.dy_stride_t, valid, g);
+        Vec<T, V> x_ahead[U], g_ahead[U];
+        f32x2 w[W][P], bias[P], win[H + U][P], dp[H + U][P];  // x and dpre of tokens t-H .. t+U-1
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
+        for (int u = 0; u < U; ++u) {
+            x_ahead[u] = t0 + u < end ? input(t0 + u) : zeros<T, V>();
+            g_ahead[u] = t0 + u < end ? gradient(t0 + u) : zeros<T, V>();
+        }
 #pragma unroll
-                for (int k = 0; k < H; ++k) { hist[k][j] = hist[k + 1][j]; dp[k][j] = dp[k + 1][j]; }
-                hist[H][j] = v[j];
-                float p = bias[j];
+        for (int k = 0; k < H; ++k) {
+            widen<T, V>(input(t0 - H + k), win[U + k]);
 #pragma unroll
-                for (int k = 0; k < W; ++k) p = __fmaf_rn(w[k][j], hist[k][j], p);
-                if (a.silu) g[j] = live ? __fmul_rn(g[j], silu_slope(p, sigmoid(p))) : 0.0f;
-                dp[H][j] = g[j];
+            for (int i = 0; i < P; ++i) dp[U + k][i] = both(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int c0 = min(at.channel(2 * i), a.channels - 1), c1 = min(at.channel(2 * i + 1), a.channels - 1);
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][i] = pair(a.weight[(long long)c0 * W + k], a.weight[(long long)c1 * W + k]);
+            bias[i] = a.bias ? pair(a.bias[c0], a.bias[c1]) : both(0.0f);
+        }
+        for (int t = t0; t < end; t += U) {
+#pragma unroll
+            for (int k = 0; k < H; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    win[k][i] = win[U + k][i];
+                    dp[k][i] = dp[U + k][i];
+                }
+            f32x2 g[U][P];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                widen<T, V>(x_ahead[u], win[H + u]);
+                widen<T, V>(g_ahead[u], g[u]);
             }
-            if (t < t1) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    db[j] += g[j];
-#pragma unroll
-                    for (int k = 0; k < W; ++k) dw[k][j] = __fmaf_rn(g[j], hist[k][j], dw[k][j]);
+            for (int u = 0; u < U; ++u) {
+                if (t + U + u < end) {
+                    x_ahead[u] = input(t + U + u);
+                    g_ahead[u] = gradient(t + U + u);
                 }
             }
-            const int at = t - H;
-            if (at >= t0 || s == 0) {
-                float o[V] = {};
-                if (at < n) {
+            if (a.silu) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int k = 0; k < W; ++k) o[j] = __fmaf_rn(w[k][j], dp[H - k][j], o[j]);
-                    if (d_last && at >= n - H) {              // x[at] is also part of the final state
-                        float f[V];
-                        load<T, V, ALIGNED>(d_last + (long long)(at - (n - H)) * a.channels, valid, f);
+                    for (int i = 0; i < P; ++i) {
+                        f32x2 p = bias[i];
 #pragma unroll
-                        for (int j = 0; j < V; ++j) o[j] += f[j];
+                        for (int k = 0; k < W; ++k) p = fma2(w[k][i], win[u + k][i], p);
+                        g[u][i] = mul2(g[u][i], silu_slope2(p, sigmoid2(p)));
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool real = t + u < n && t + u < end;   // not padding, whose slope may be anything if the bias is not finite
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    dp[H + u][i] = real ? g[u][i] : both(0.0f);
+                    if (t + u < t1) {
+                        db[i] = add2(db[i], dp[H + u][i]);
+#pragma unroll
+                        for (int k = 0; k < W; ++k) dw[k][i] = fma2(dp[H + u][i], win[u + k][i], dw[k][i]);
                     }
                 }
-                if (at >= 0) {
-                    if (dx) store<T, V, ALIGNED>(dx + (long long)at * a.channels, valid, o);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int to = t + u - H;                     // whose gradient is complete
+                if (t + u >= end || (to < t0 && s > 0)) continue;
+                f32x2 o[P];
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    o[i] = both(0.0f);
+                    if (to < n) {
+#pragma unroll
+                        for (int k = 0; k < W; ++k) o[i] = fma2(w[k][i], dp[u + H - k][i], o[i]);
+                    }
+                }
+                if (d_last && to < n && to >= n - H) {        // x[to] is also part of the final state
+                    f32x2 f[P];
+                    widen<T, V>(fetch<T, V, ALIGNED>(d_last + (long long)(to - (n - H)) * a.channels, at.valid, CONV_LANES), f);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) o[i] = add2(o[i], f[i]);
+                }
+                if (to >= 0) {
+                    if (dx) put<T, V, ALIGNED>(dx + (long long)to * a.channels, at.valid, CONV_LANES, o);
                 } else if (d_first) {
-                    store<T, V, ALIGNED>(d_first + (long long)(at + H) * a.channels, valid, o);
+                    put<T, V, ALIGNED>(d_first + (long long)(to + H) * a.channels, at.valid, CONV_LANES, o);
                 }
             }
         }
     }
     if (partial == nullptr) return;
     constexpr int COLS = CONV_LANES * V;
-    float* mine = red + threadIdx.y * (W + 1) * COLS + threadIdx.x * V;
+    float* mine = red + threadIdx.y * (W + 1) * COLS;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+        const int c = ALIGNED ? threadIdx.x * V + j : threadIdx.x + CONV_LANES * j;
 #pragma unroll
-        for (int k = 0; k < W; ++k) mine[k * COLS + j] = dw[k][j];
-        mine[W * COLS + j] = db[j];
+        for (int k = 0; k < W; ++k) mine[k * COLS + c] = j & 1 ? hi_of(dw[k][j / 2]) : lo_of(dw[k][j / 2]);
+        mine[W * COLS + c] = j & 1 ? hi_of(db[j / 2]) : lo_of(db[j / 2]);
     }
     __syncthreads();
     float* row = partial + (long long)(blockIdx.z * gridDim.y + blockIdx.y) * (W + 1) * a.channels;
@@ -185,21 +256,19 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
     }
 }
 
-// dweight [channels, W] and dbias from the rows of `partial`, added in order.
-static __global__ void __launch_bounds__(256)
-causal_conv_sums_kernel(const float* __restrict__ partial, int n_parts, int channels, int W, float* __restrict__ dweight, float* __restrict__ dbias) {
-    const int i = blockIdx.x * 256 + threadIdx.x, all = (W + 1) * channels;
-    if (i >= all) return;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int p = 0; p < n_parts; ++p) sum += partial[(long long)p * all + i];
-    const int k = i / channels, c = i - k * channels;
-    if (k < W) {
-        if (dweight) dweight[(long long)c * W + k] = sum;
-    } else if (dbias) {
-        dbias[c] = sum;
+// Where column i of the sums belongs: dweight [channels, W], then dbias.
+struct ConvSums {
+    float *dweight, *dbias;
+    int channels, W;
+    __device__ __forceinline__ void operator()(int i, float v) const {
+        const int k = i / channels, c = i - k * channels;
+        if (k < W) {
+            if (dweight) dweight[(long long)c * W + k] = v;
+        } else if (dbias) {
+            dbias[c] = v;
+        }
     }
-}
+};
 
 template <typename T, int W>
 __global__ void __launch_bounds__(128)
@@ -270,12 +339,13 @@ template <typename F> static int by_width(int W, F f) {
 }
 
 int launch_causal_conv(const el_conv_t& a, cudaStream_t st) {
-    const int strip = conv_strip(a, (a.channels + 7) / 8, 512);
-    const dim3 grid(ceil_div(a.channels, CONV_LANES * 8), ceil_div(a.length > 0 ? a.length : 1, (long long)strip * FW_STRIPS), a.batch);
+    const int V = a.dtype == EL_F32 ? 4 : 8;
+    const int strip = conv_strip(a, (a.channels + V - 1) / V, 512);
+    const dim3 grid(ceil_div(a.channels, CONV_LANES * V), ceil_div(a.length > 0 ? a.length : 1, (long long)strip * FW_STRIPS), a.batch);
     if (grid.y > 65535 || grid.z > 65535) return EL_ERR_TOO_LARGE;
     const dim3 block(CONV_LANES, FW_STRIPS);
-    const bool al = a.channels % 8 == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, 8) && vectors(a.y, 0, 0, a.dtype, 8) &&
-                    vectors(a.initial_state, 0, 0, a.dtype, 8) && vectors(a.final_state, 0, 0, a.dtype, 8);
+    const bool al = a.channels % V == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, V) && vectors(a.y, 0, 0, a.dtype, V) &&
+                    vectors(a.initial_state, 0, 0, a.dtype, V) && vectors(a.final_state, 0, 0, a.dtype, V);
     return by_type(a.dtype, [&](auto t) {
         return by_width(a.width, [&](auto w) {
             using T = decltype(t);
@@ -307,9 +377,7 @@ int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st) {
         });
     });
     if (rc != EL_OK || !sums) return rc;
-    causal_conv_sums_kernel<<<ceil_div((long long)(a.width + 1) * a.channels, 256), 256, 0, st>>>(partial, a.batch * plan.blocks_t, a.channels, a.width,
-                                                                                                 a.dweight, a.dbias);
-    return check_launch();
+    return launch_column_sums(partial, a.batch * plan.blocks_t, (a.width + 1) * a.channels, ConvSums{a.dweight, a.dbias, a.channels, a.width}, st);
 }
 
 int launch_causal_conv_step(const el_conv_t& a, cudaStream_t st) {

@@ -6,27 +6,98 @@
 namespace el {
 namespace mamba {
 
-// V consecutive channels of a token as float32.  ALIGNED: one or two vector accesses (the host has checked base, strides and that V
-// divides the channels); otherwise element by element, the first `valid` of them, zeros behind.
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void load(const T* p, int valid, float v[V]) {
-    static_assert(V == 4 || V == 8, "vectors of 4 or 8 channels");
-    if constexpr (!ALIGNED) {
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// V values of a row as they lie in memory, and as pairs of float32.  ALIGNED: adjacent ones in one or two vector accesses (the host has
+// checked base, strides and that V divides the row).  Otherwise every STRIDE-th one by itself, STRIDE the number of threads side by side,
+// so that neighbouring threads still read neighbouring values; `valid` is the distance from the first to the row's end, zeros behind it.
+// Held as 32-bit words: registers, whatever T is.
+template <typename T, int V> struct Vec { uint32_t w[V * sizeof(T) / 4]; };
+template <typename T> __device__ __forceinline__ uint32_t bits_of(T v) {
+    if constexpr (sizeof(T) == 4) return __float_as_uint(v);
+    else return *reinterpret_cast<const unsigned short*>(&v);
+}
+template <typename T, int V> __device__ __forceinline__ Vec<T, V> zeros() {
+    Vec<T, V> r;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < valid ? to_float<T>(p[j]) : 0.0f;
-    } else if constexpr (V == 8) {
-        rowio::Io<T>::load8(p, v);
-    } else if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(p);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    for (int i = 0; i < (int)(V * sizeof(T) / 4); ++i) r.w[i] = 0u;
+    return r;
+}
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ Vec<T, V> fetch(const T* p, int valid, int stride) {
+    constexpr int WORDS = V * sizeof(T) / 4;
+    Vec<T, V> r = zeros<T, V>();
+    if constexpr (ALIGNED && WORDS == 2) {
+        const uint2 a = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = a.x; r.w[1] = a.y;
+    } else if constexpr (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4) {
+            const uint4 a = reinterpret_cast<const uint4*>(p)[i / 4];
+            r.w[i] = a.x; r.w[i + 1] = a.y; r.w[i + 2] = a.z; r.w[i + 3] = a.w;
+        }
     } else {
-        rowio::Quad<T> q;
-        q.a = *reinterpret_cast<const uint2*>(p);
-        rowio::f32x2 w[2];
-        rowio::unpack2<T>(q, w);
-        v[0] = rowio::lo_of(w[0]); v[1] = rowio::hi_of(w[0]); v[2] = rowio::lo_of(w[1]); v[3] = rowio::hi_of(w[1]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t b = j * stride < valid ? bits_of<T>(p[j * stride]) : 0u;
+            if constexpr (sizeof(T) == 4) r.w[j] = b;
+            else r.w[j / 2] |= b << (16 * (j & 1));
+        }
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ rowio::f32x2 widen_word(uint32_t w) {            // of a 16-bit type
+    if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        return rowio::pair(f.x, f.y);
+    } else {
+        return rowio::pair(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     }
 }
+template <typename T, int V> __device__ __forceinline__ void widen(const Vec<T, V>& r, rowio::f32x2 v[V / 2]) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = rowio::pair(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+        else v[i] = widen_word<T>(r.w[i]);
+    }
+}
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void put(T* p, int valid, int stride, const rowio::f32x2 v[V / 2]) {       // rounds to T
+    constexpr int WORDS = V * sizeof(T) / 4;
+    uint32_t w[WORDS];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        const float a = rowio::lo_of(v[i]), b = rowio::hi_of(v[i]);
+        if constexpr (sizeof(T) == 4) {
+            w[2 * i] = __float_as_uint(a);
+            w[2 * i + 1] = __float_as_uint(b);
+        } else {
+            w[i] = std::is_same<T, __half>::value ? pack_f16x2(a, b) : pack_bf16x2(a, b);
+        }
+    }
+    if constexpr (ALIGNED && WORDS == 2) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else if constexpr (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (j * stride >= valid) continue;
+            if constexpr (sizeof(T) == 4) {
+                p[j * stride] = __uint_as_float(w[j]);
+            } else {
+                const unsigned short h = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+                p[j * stride] = *reinterpret_cast<const T*>(&h);
+            }
+        }
+    }
+}
+__device__ __forceinline__ rowio::f32x2 both(float v) { return rowio::pair(v, v); }
+
 // Four channels (or states) as they lie in memory, for values that are fetched long before they are used; elements from `valid` on are zeros.
 template <typename T> __device__ __forceinline__ rowio::Quad<T> quad_zero() {
     rowio::Quad<T> q;
@@ -52,32 +123,10 @@ template <typename T> __device__ __forceinline__ float4 widen(const rowio::Quad<
     rowio::unpack2<T>(q, v);
     return make_float4(rowio::lo_of(v[0]), rowio::hi_of(v[0]), rowio::lo_of(v[1]), rowio::hi_of(v[1]));
 }
-template <typename T> __device__ __forceinline__ void store_quad(T* p, int valid, bool aligned, float4 v);
-
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void store(T* p, int valid, const float v[V]) {
-    if constexpr (!ALIGNED) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < valid) p[j] = from_float<T>(v[j]);
-    } else if constexpr (V == 8) {
-        rowio::Io<T>::store8(p, v);
-    } else if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-        *reinterpret_cast<uint2*>(p) = rowio::pack2<T>(rowio::pair(v[0], v[1]), rowio::pair(v[2], v[3])).a;
-    }
-}
-
 template <typename T> __device__ __forceinline__ void store_quad(T* p, int valid, bool aligned, float4 v) {
-    const float f[4] = {v.x, v.y, v.z, v.w};
-    if (aligned && valid > 0) store<T, 4, true>(p, 4, f);
-    else store<T, 4, false>(p, valid, f);
+    const rowio::f32x2 f[2] = {rowio::pair(v.x, v.y), rowio::pair(v.z, v.w)};
+    if (!aligned) put<T, 4, false>(p, valid, 1, f);
+    else if (valid > 0) put<T, 4, true>(p, valid, 1, f);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -108,6 +157,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 __device__ __forceinline__ float exp_minus_abs(float x) { return ex2_denormals(__fmul_rn(-fabsf(x), LOG2E)); }
 // 1 / (1 + e^-x); an exponential that overflows gives 0
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.0f + ex2(__fmul_rn(x, -LOG2E))); }
+__device__ __forceinline__ rowio::f32x2 sigmoid2(rowio::f32x2 x) {
+    using namespace rowio;
+    const f32x2 t = mul2(x, both(-LOG2E)), d = add2(pair(ex2(lo_of(t)), ex2(hi_of(t))), both(1.0f));
+    return pair(rcp(lo_of(d)), rcp(hi_of(d)));
+}
 // 1 / (1 + e^-x) from e = e^-|x|, with all the digits of a small result
 __device__ __forceinline__ float sigmoid_of(float x, float e) {
     const float r = rcp(1.0f + e);
@@ -115,6 +169,10 @@ __device__ __forceinline__ float sigmoid_of(float x, float e) {
 }
 // d/dx of x sigmoid(x), from s = sigmoid(x)
 __device__ __forceinline__ float silu_slope(float x, float s) { return __fmul_rn(s, __fmaf_rn(x, 1.0f - s, 1.0f)); }
+__device__ __forceinline__ rowio::f32x2 silu_slope2(rowio::f32x2 x, rowio::f32x2 s) {
+    using namespace rowio;
+    return mul2(s, fma2(x, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
+}
 
 // log(1 + e^x) from e = e^-|x|: max(x, 0) + log1p(e), log1p(e) = 2 artanh(s) = 2 (s + s^3/3 + s^5/5 + ..), s = e / (2 + e) <= 1/3; the
 // first term left out is s^15/15, 1.4e-8 of the whole at most.  The logarithm of 1 + e in float32 would have an absolute error of 6e-8,
@@ -123,7 +181,6 @@ __device__ __forceinline__ rowio::f32x2 softplus2(float x0, float x1, float e0, 
     using namespace rowio;
     const f32x2 e = pair(e0, e1), d = add2(e, pair(2.0f, 2.0f));
     const f32x2 s = mul2(e, pair(rcp(lo_of(d)), rcp(hi_of(d)))), q = mul2(s, s);
-    auto both = [](float v) { return pair(v, v); };
     f32x2 p = fma2(q, both(1.0f / 13.0f), both(1.0f / 11.0f));
     p = fma2(p, q, both(1.0f / 9.0f));
     p = fma2(p, q, both(1.0f / 7.0f));
@@ -133,6 +190,35 @@ __device__ __forceinline__ rowio::f32x2 softplus2(float x0, float x1, float e0, 
     return add2(pair(max_nan(x0, 0.0f), max_nan(x1, 0.0f)), fma2(s2, mul2(p, q), s2));
 }
 __device__ __forceinline__ float softplus_of(float x, float e) { return rowio::lo_of(softplus2(x, x, e, e)); }
+
+// out[map(i)] = sum of the parts' i-th values, for `cols` of them.  A block covers 32 columns; its W warps each add every W-th part in order, and
+// the first warp adds their results in order: the same bits for a given width.  Few columns take 32 warps: there the chain of loads counts.
+template <typename F>
+__global__ void __launch_bounds__(1024)
+column_sums_kernel(const float* __restrict__ partial, int n_parts, int cols, F store_at) {
+    __shared__ float part[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int k = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (k < cols) {
+#pragma unroll 8
+        for (int p = warp; p < n_parts; p += warps) s += partial[(long long)p * cols + k];
+    }
+    part[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && k < cols) {
+        s = 0.0f;
+        for (int w = 0; w < warps; ++w) s += part[w][lane];
+        store_at(k, s);
+    }
+}
+template <typename F> static int launch_column_sums(const float* partial, int n_parts, int cols, F store_at, cudaStream_t st) {
+    int sms = 148;
+    device_sm_count(&sms);
+    const int blocks = (cols + 31) / 32;
+    column_sums_kernel<<<blocks, blocks <= 2 * sms && n_parts > 64 ? 1024 : 256, 0, st>>>(partial, n_parts, cols, store_at);
+    return check_launch();
+}
 
 }  // namespace mamba
 }  // namespace el

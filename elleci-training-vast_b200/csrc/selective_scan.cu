@@ -92,7 +92,6 @@ template <int TOKENS, int QN> __device__ __forceinline__ void load_twice(const f
     const float4 x = m[0][t][sg], y = m[1][t][sg];
     v[0] = pair(x.x, x.y); v[1] = pair(x.z, x.w); v[2] = pair(y.x, y.y); v[3] = pair(y.z, y.w);
 }
-__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
 __device__ __forceinline__ f32x2 decay_of(f32x2 A, f32x2 delta) {         // A is already times log2(e)
     const f32x2 x = fma2(A, delta, both(DECAY_SHIFT));
     return pair(ex2(lo_of(x)), ex2(hi_of(x)));
@@ -787,36 +786,49 @@ scan_a_sums_kernel(const float* __restrict__ partial, int parts, int channels, i
 
 // ---- one token ----------------------------------------------------------------------------------------------------------
 
-struct Token { float delta, raw, u, z; };
-
-template <typename T>
-__device__ __forceinline__ Token scan_token(const el_scan_t& a, int b, int t, int d, float bias) {
-    Token k;
-    k.u = to_float<T>(static_cast<const T*>(a.u)[b * a.u_stride_b + t * a.u_stride_t + d]);
-    k.raw = to_float<T>(static_cast<const T*>(a.dt)[b * a.dt_stride_b + t * a.dt_stride_t + d]) + bias;
-    k.delta = a.softplus ? softplus_of(k.raw, exp_minus_abs(k.raw)) : k.raw;
-    k.z = a.z ? to_float<T>(static_cast<const T*>(a.z)[b * a.z_stride_b + t * a.z_stride_t + d]) : 0.0f;
-    return k;
-}
-// A thread owns a channel's state.
-template <typename T>
+// LANES lanes share a channel, four states each, and go through the sequences of their block's share: A is read once for them.
+// Bound: memory, the state read and written (128 bytes per channel of 16 states); for few sequences one memory latency.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(128)
-selective_scan_step_kernel(const el_scan_t a) {
-    const int d = blockIdx.x * 128 + threadIdx.x, b = blockIdx.y, N = a.states;
-    if (d >= a.channels) return;
-    const int g = d / (a.channels / a.groups);
-    const long long state_at = ((long long)b * a.channels + d) * N;
-    const Token k = scan_token<T>(a, b, 0, d, a.dt_bias ? a.dt_bias[d] : 0.0f);
-    const T* Bp = static_cast<const T*>(a.B) + b * a.B_stride_b + g * a.B_stride_g;
-    const T* Cp = static_cast<const T*>(a.C) + b * a.C_stride_b + g * a.C_stride_g;
-    float out = a.D ? a.D[d] * k.u : 0.0f;
-    for (int n = 0; n < N; ++n) {
-        const float h = __fmaf_rn(ex2(k.delta * (a.A[(long long)d * N + n] * LOG2E)), a.initial_state[state_at + n], k.delta * k.u * to_float<T>(Bp[n]));
-        out = __fmaf_rn(to_float<T>(Cp[n]), h, out);
-        a.final_state[state_at + n] = h;
+selective_scan_step_kernel(const el_scan_t a, int share) {
+    const int lane = threadIdx.x % LANES, d = (blockIdx.x * 128 + threadIdx.x) / LANES, n0 = lane * 4, N = a.states;
+    const bool real = d < a.channels;
+    const int dc = min(d, a.channels - 1), g = dc / (a.channels / a.groups);
+    const int b0 = blockIdx.y * share, b1 = min(b0 + share, a.batch);
+    const bool aligned_bc = N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C)) % (4 * sizeof(T)) == 0 &&
+                            (a.B_stride_b | a.B_stride_g | a.C_stride_b | a.C_stride_g) % 4 == 0;
+    float A[4];
+    load_states(a.A + (long long)dc * N, n0, N, A);
+    const float bias = a.dt_bias ? a.dt_bias[dc] : 0.0f, D = a.D ? a.D[dc] : 0.0f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) A[n] *= LOG2E;
+#pragma unroll 2
+    for (int b = b0; b < b1; ++b) {
+        const long long at = ((long long)b * a.channels + dc) * N;
+        float h[4];
+        load_states(a.initial_state + at, n0, N, h);
+        const float u = to_float<T>(static_cast<const T*>(a.u)[b * a.u_stride_b + dc]);
+        const float raw = to_float<T>(static_cast<const T*>(a.dt)[b * a.dt_stride_b + dc]) + bias;
+        const float z = a.z ? to_float<T>(static_cast<const T*>(a.z)[b * a.z_stride_b + dc]) : 0.0f;
+        const float4 B = widen<T>(fetch_quad<T>(static_cast<const T*>(a.B) + b * a.B_stride_b + g * a.B_stride_g + n0, N - n0, aligned_bc));
+        const float4 C = widen<T>(fetch_quad<T>(static_cast<const T*>(a.C) + b * a.C_stride_b + g * a.C_stride_g + n0, N - n0, aligned_bc));
+        const float delta = a.softplus ? softplus_of(raw, exp_minus_abs(raw)) : raw, du = delta * u;
+        const float Bv[4] = {B.x, B.y, B.z, B.w}, Cv[4] = {C.x, C.y, C.z, C.w};
+        float y = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            h[n] = __fmaf_rn(ex2(__fmaf_rn(A[n], delta, DECAY_SHIFT)), h[n], du * Bv[n]);
+            y = __fmaf_rn(Cv[n], h[n], y);
+        }
+        if (real) store_states(a.final_state + at, n0, N, h);
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+        if (real && lane == 0) {
+            y = __fmaf_rn(D, u, y);
+            if (a.z) y *= z * sigmoid(z);
+            static_cast<T*>(a.y)[(long long)b * a.channels + d] = from_float<T>(y);
+        }
     }
-    if (a.z) out *= k.z * sigmoid(k.z);
-    static_cast<T*>(a.y)[(long long)b * a.channels + d] = from_float<T>(out);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
@@ -991,10 +1003,25 @@ int launch_selective_scan_backward(const el_scan_t& a, cudaStream_t st) {
 }
 
 int launch_selective_scan_step(const el_scan_t& a, cudaStream_t st) {
-    if (a.batch > 65535) return EL_ERR_TOO_LARGE;
     return scan_by_type(a.dtype, [&](auto t) {
-        selective_scan_step_kernel<decltype(t)><<<dim3((a.channels + 127) / 128, a.batch), 128, 0, st>>>(a);
-        return check_launch();
+        auto launch = [&](auto lanes) {
+            constexpr int LANES = decltype(lanes)::value;
+            const long long blocks = ((long long)a.channels * LANES + 127) / 128;
+            if (blocks > (1ll << 31) - 1) return (int)EL_ERR_TOO_LARGE;
+            int sms = 148;
+            device_sm_count(&sms);
+            // sequences of a block: as many as leave every SM its 16 blocks
+            long long share = blocks * a.batch / (16 * sms);
+            share = share < 1 ? 1 : share > a.batch ? a.batch : share;
+            while ((a.batch + share - 1) / share > 65535) ++share;
+            selective_scan_step_kernel<decltype(t), LANES><<<dim3((unsigned)blocks, (unsigned)((a.batch + share - 1) / share)), 128, 0, st>>>(a, (int)share);
+            return check_launch();
+        };
+        if (a.states <= 4) return launch(std::integral_constant<int, 1>());
+        if (a.states <= 8) return launch(std::integral_constant<int, 2>());
+        if (a.states <= 16) return launch(std::integral_constant<int, 4>());
+        if (a.states <= 32) return launch(std::integral_constant<int, 8>());
+        return launch(std::integral_constant<int, 16>());
     });
 }
 
