@@ -19,11 +19,37 @@ using rowio::pair;
 
 constexpr int CONV_LANES = 32;        // threads of a block along the channels; the others are strips of tokens
 
-constexpr int CONV_AHEAD = 4;         // tokens that are fetched together, one such group ahead of the arithmetic
-#ifndef BA
-#define BA 2
-#define BB 2
-#endif
+constexpr int CONV_SLOTS = 8;         // tokens that are on their way to a thread's slots in shared memory
+constexpr int CONV_V = 4;             // channels of a thread
+
+// What a thread will read of later tokens it copies into its own slots with asynchronous copies, so that tokens ahead cost neither registers
+// nor barriers.  Channels that no vector copy takes go through registers.
+template <typename T, int TENSORS, bool ALIGNED> struct ConvRing {
+    using Slot = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+    Slot* mine;
+    int threads;
+    __device__ __forceinline__ explicit ConvRing(void* shared) {
+        threads = blockDim.x * blockDim.y;
+        mine = static_cast<Slot*>(shared) + threadIdx.y * blockDim.x + threadIdx.x;
+    }
+    __device__ __forceinline__ Slot* at(int t, int tensor) const { return mine + ((t & (CONV_SLOTS - 1)) * TENSORS + tensor) * threads; }
+    __device__ __forceinline__ void request(int t, int tensor, const T* src, int valid) const {
+        Slot* to = at(t, tensor);
+        if constexpr (ALIGNED) {
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+            if constexpr (sizeof(T) == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+            else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        } else {
+            const Vec<T, CONV_V> v = fetch<T, CONV_V, false>(src, valid, CONV_LANES);
+            *to = *reinterpret_cast<const Slot*>(&v);
+        }
+    }
+    __device__ __forceinline__ void read(int t, int tensor, f32x2 v[CONV_V / 2]) const {
+        Vec<T, CONV_V> r;
+        *reinterpret_cast<Slot*>(&r) = *at(t, tensor);
+        widen<T, CONV_V>(r, v);
+    }
+};
 
 // Where a thread's channels lie: V adjacent ones, or, where vectors are not possible, every 32nd.
 template <int V, bool ALIGNED> struct ConvPlace {
@@ -38,7 +64,9 @@ template <int V, bool ALIGNED> struct ConvPlace {
 template <typename T, int W, bool ALIGNED>
 __global__ void __launch_bounds__(128)
 causal_conv_kernel(const el_conv_t a, int strip) {
-    constexpr int V = 16 / sizeof(T), P = V / 2, H = W - 1, U = CONV_AHEAD;
+    constexpr int V = CONV_V, P = V / 2, H = W - 1, U = 4;
+    extern __shared__ uint4 slots[];
+    const ConvRing<T, 1, ALIGNED> ring(slots);
     const ConvPlace<V, ALIGNED> at(a.channels);
     const int b = blockIdx.z;
     if (at.valid <= 0) return;
@@ -54,10 +82,17 @@ causal_conv_kernel(const el_conv_t a, int strip) {
     const int s = blockIdx.y * blockDim.y + threadIdx.y;
     const int t0 = s * strip, t1 = min(t0 + strip, a.length);
     if (t0 < t1) {
-        Vec<T, V> ahead[U];
         f32x2 w[W][P], bias[P], win[H + U][P];                // win: x[t-H] .. x[t+U-1]
+        const int tn = min(t1, n);
+        auto request = [&](int t) {                           // a group of tokens
 #pragma unroll
-        for (int u = 0; u < U; ++u) ahead[u] = input(t0 + u);
+            for (int u = 0; u < U; ++u)
+                if (t + u < tn) ring.request(t + u, 0, x + (t + u) * a.x_stride_t, at.valid);
+            rowio::cp_async_commit();
+        };
+        request(t0);
+        request(t0 + U);
+        static_assert(CONV_SLOTS == 2 * U, "");
 #pragma unroll
         for (int k = 0; k < H; ++k) widen<T, V>(input(t0 - H + k), win[U + k]);
 #pragma unroll
@@ -72,12 +107,15 @@ causal_conv_kernel(const el_conv_t a, int strip) {
             for (int k = 0; k < H; ++k)
 #pragma unroll
                 for (int i = 0; i < P; ++i) win[k][i] = win[U + k][i];
+            rowio::cp_async_wait<1>();
 #pragma unroll
-            for (int u = 0; u < U; ++u) widen<T, V>(ahead[u], win[H + u]);
-            if (t + U < t1) {
+            for (int u = 0; u < U; ++u) {
+                if (t + u < n) ring.read(t + u, 0, win[H + u]);        // a slot that nothing was copied to is not looked at
+                else
 #pragma unroll
-                for (int u = 0; u < U; ++u) ahead[u] = input(t + U + u);
+                    for (int i = 0; i < P; ++i) win[H + u][i] = both(0.0f);
             }
+            request(t + 2 * U);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 f32x2 o[P];
@@ -112,10 +150,11 @@ causal_conv_kernel(const el_conv_t a, int strip) {
 
 // dx and the partial sums of dweight and dbias: a block's strips are added in order and stored as one row [W+1][channels] of `partial`.
 template <typename T, int W, bool ALIGNED>
-__global__ void __launch_bounds__(256, BB)
+__global__ void __launch_bounds__(256, 2)
 causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ partial) {
-    constexpr int V = 4, P = V / 2, H = W - 1, U = BA;
-    extern __shared__ float red[];                            // [strips of the block][W+1][channels of the block]
+    constexpr int V = CONV_V, P = V / 2, H = W - 1, U = 2, GROUPS = CONV_SLOTS / U;
+    extern __shared__ uint4 slots[];                          // then the sums [strips of the block][W+1][channels of the block]
+    const ConvRing<T, 2, ALIGNED> ring(slots);
     const ConvPlace<V, ALIGNED> at(a.channels);
     const int b = blockIdx.z;
     f32x2 dw[W][P], db[P];
@@ -141,16 +180,22 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
             if (t >= 0) return fetch<T, V, ALIGNED>(x + t * a.x_stride_t, at.valid, CONV_LANES);
             return first ? fetch<T, V, ALIGNED>(first + (long long)(t + H) * a.channels, at.valid, CONV_LANES) : zeros<T, V>();
         };
-        auto gradient = [&](int t) { return t < n && dy ? fetch<T, V, ALIGNED>(dy + t * a.dy_stride_t, at.valid, CONV_LANES) : zeros<T, V>(); };
         // at token t the gradient of x[t-H] is complete; the strip's own x are t0 .. t1-1, for the first strip the state's before them too
         const int end = max(t1, t0) + H;
-        Vec<T, V> x_ahead[U], g_ahead[U];
         f32x2 w[W][P], bias[P], win[H + U][P], dp[H + U][P];  // x and dpre of tokens t-H .. t+U-1
+        const int tn = min(end, n);
+        auto request = [&](int t) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            x_ahead[u] = t0 + u < end ? input(t0 + u) : zeros<T, V>();
-            g_ahead[u] = t0 + u < end ? gradient(t0 + u) : zeros<T, V>();
-        }
+            for (int u = 0; u < U; ++u) {
+                if (t + u < tn) {
+                    ring.request(t + u, 0, x + (t + u) * a.x_stride_t, at.valid);
+                    if (dy) ring.request(t + u, 1, dy + (t + u) * a.dy_stride_t, at.valid);
+                }
+            }
+            rowio::cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) request(t0 + i * U);
 #pragma unroll
         for (int k = 0; k < H; ++k) {
             widen<T, V>(input(t0 - H + k), win[U + k]);
@@ -173,18 +218,17 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
                     dp[k][i] = dp[U + k][i];
                 }
             f32x2 g[U][P];
+            rowio::cp_async_wait<GROUPS - 1>();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                widen<T, V>(x_ahead[u], win[H + u]);
-                widen<T, V>(g_ahead[u], g[u]);
-            }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (t + U + u < end) {
-                    x_ahead[u] = input(t + U + u);
-                    g_ahead[u] = gradient(t + U + u);
+                for (int i = 0; i < P; ++i) win[H + u][i] = g[u][i] = both(0.0f);
+                if (t + u < tn) {                             // a slot that nothing was copied to is not looked at
+                    ring.read(t + u, 0, win[H + u]);
+                    if (dy) ring.read(t + u, 1, g[u]);
                 }
             }
+            request(t + CONV_SLOTS);
             if (a.silu) {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -236,7 +280,9 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
             }
         }
     }
+    rowio::cp_async_wait<0>();
     if (partial == nullptr) return;
+    float* red = reinterpret_cast<float*>(slots) + 2 * CONV_SLOTS * V * blockDim.x * blockDim.y * sizeof(T) / sizeof(float);
     constexpr int COLS = CONV_LANES * V;
     float* mine = red + threadIdx.y * (W + 1) * COLS;
 #pragma unroll
@@ -339,19 +385,20 @@ template <typename F> static int by_width(int W, F f) {
 }
 
 int launch_causal_conv(const el_conv_t& a, cudaStream_t st) {
-    const int V = a.dtype == EL_F32 ? 4 : 8;
-    const int strip = conv_strip(a, (a.channels + V - 1) / V, 512);
+    constexpr int V = CONV_V;
+    const int strip = conv_strip(a, (a.channels + V - 1) / V, 1024);
     const dim3 grid(ceil_div(a.channels, CONV_LANES * V), ceil_div(a.length > 0 ? a.length : 1, (long long)strip * FW_STRIPS), a.batch);
     if (grid.y > 65535 || grid.z > 65535) return EL_ERR_TOO_LARGE;
     const dim3 block(CONV_LANES, FW_STRIPS);
+    const size_t shared = (size_t)CONV_SLOTS * CONV_LANES * FW_STRIPS * V * (a.dtype == EL_F32 ? 4 : 2);        // 16 KB at most
     const bool al = a.channels % V == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, V) && vectors(a.y, 0, 0, a.dtype, V) &&
                     vectors(a.initial_state, 0, 0, a.dtype, V) && vectors(a.final_state, 0, 0, a.dtype, V);
     return by_type(a.dtype, [&](auto t) {
         return by_width(a.width, [&](auto w) {
             using T = decltype(t);
             constexpr int W = decltype(w)::value;
-            if (al) causal_conv_kernel<T, W, true><<<grid, block, 0, st>>>(a, strip);
-            else causal_conv_kernel<T, W, false><<<grid, block, 0, st>>>(a, strip);
+            if (al) causal_conv_kernel<T, W, true><<<grid, block, shared, st>>>(a, strip);
+            else causal_conv_kernel<T, W, false><<<grid, block, shared, st>>>(a, strip);
             return check_launch();
         });
     });
@@ -366,14 +413,25 @@ int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st) {
     const bool al = a.channels % 4 == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, 4) && vectors(a.dy, a.dy_stride_b, a.dy_stride_t, a.dtype, 4) &&
                     vectors(a.dx, 0, 0, a.dtype, 4) && vectors(a.initial_state, 0, 0, a.dtype, 4) && vectors(a.d_initial_state, 0, 0, a.dtype, 4) &&
                     vectors(a.d_final_state, 0, 0, a.dtype, 4);
-    const size_t shared = (size_t)BW_STRIPS * (a.width + 1) * CONV_LANES * 4 * sizeof(float);       // 20 KB at most
+    // slots and sums: 84 KB at most (float32)
+    const size_t shared = (size_t)2 * CONV_SLOTS * CONV_LANES * BW_STRIPS * CONV_V * (a.dtype == EL_F32 ? 4 : 2) +
+                          (size_t)BW_STRIPS * (a.width + 1) * CONV_LANES * CONV_V * sizeof(float);
     const int rc = a.batch == 0 ? EL_OK : by_type(a.dtype, [&](auto t) {
         return by_width(a.width, [&](auto w) {
             using T = decltype(t);
             constexpr int W = decltype(w)::value;
-            if (al) causal_conv_backward_kernel<T, W, true><<<grid, block, shared, st>>>(a, plan.strip, partial);
-            else causal_conv_backward_kernel<T, W, false><<<grid, block, shared, st>>>(a, plan.strip, partial);
-            return check_launch();
+            auto launch = [&](auto kernel, DeviceOnce& once) {
+                int dev = 0;
+                EL_CUDA_TRY(cudaGetDevice(&dev));
+                if (!once.is_done(dev)) {
+                    EL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
+                    once.mark(dev);
+                }
+                kernel<<<grid, block, shared, st>>>(a, plan.strip, partial);
+                return check_launch();
+            };
+            static DeviceOnce once[2];
+            return al ? launch(causal_conv_backward_kernel<T, W, true>, once[0]) : launch(causal_conv_backward_kernel<T, W, false>, once[1]);
         });
     });
     if (rc != EL_OK || !sums) return rc;
