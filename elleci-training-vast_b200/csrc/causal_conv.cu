@@ -84,10 +84,14 @@ causal_conv_kernel(const el_conv_t a, int strip) {
     if (t0 < t1) {
         f32x2 w[W][P], bias[P], win[H + U][P];                // win: x[t-H] .. x[t+U-1]
         const int tn = min(t1, n);
+        const T* ask = x + t0 * a.x_stride_t;                 // of the token that is requested next
+        T* to = y + (long long)t0 * a.channels;
         auto request = [&](int t) {                           // a group of tokens
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (t + u < tn) ring.request(t + u, 0, x + (t + u) * a.x_stride_t, at.valid);
+            for (int u = 0; u < U; ++u) {
+                if (t + u < tn) ring.request(t + u, 0, ask, at.valid);
+                ask += a.x_stride_t;
+            }
             rowio::cp_async_commit();
         };
         request(t0);
@@ -102,7 +106,8 @@ causal_conv_kernel(const el_conv_t a, int strip) {
             for (int k = 0; k < W; ++k) w[k][i] = pair(a.weight[(long long)c0 * W + k], a.weight[(long long)c1 * W + k]);
             bias[i] = a.bias ? pair(a.bias[c0], a.bias[c1]) : both(0.0f);
         }
-        for (int t = t0; t < t1; t += U) {
+        auto group = [&](int t, auto edge) {                  // edge: some of the tokens are behind the strip or are padding
+            constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
             for (int k = 0; k < H; ++k)
 #pragma unroll
@@ -110,32 +115,40 @@ causal_conv_kernel(const el_conv_t a, int strip) {
             rowio::cp_async_wait<1>();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (t + u < n) ring.read(t + u, 0, win[H + u]);        // a slot that nothing was copied to is not looked at
+                if (!EDGE || t + u < tn) ring.read(t + u, 0, win[H + u]);      // a slot that nothing was copied to is not looked at
                 else
 #pragma unroll
                     for (int i = 0; i < P; ++i) win[H + u][i] = both(0.0f);
             }
             request(t + 2 * U);
+            f32x2 o[U][P];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                f32x2 o[P];
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    o[i] = bias[i];
+                    o[u][i] = bias[i];
 #pragma unroll
-                    for (int k = 0; k < W; ++k) o[i] = fma2(w[k][i], win[u + k][i], o[i]);
+                    for (int k = 0; k < W; ++k) o[u][i] = fma2(w[k][i], win[u + k][i], o[u][i]);
                 }
-                if (a.silu) {
+            if (a.silu) {
 #pragma unroll
-                    for (int i = 0; i < P; ++i) o[i] = mul2(o[i], sigmoid2(o[i]));
-                }
-                if (t + u >= n) {
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int i = 0; i < P; ++i) o[i] = both(0.0f);
-                }
-                if (t + u < t1) put<T, V, ALIGNED>(y + (long long)(t + u) * a.channels, at.valid, CONV_LANES, o);
+                    for (int i = 0; i < P; ++i) o[u][i] = mul2(o[u][i], sigmoid2(o[u][i]));
             }
-        }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (EDGE && t + u >= n) {
+#pragma unroll
+                    for (int i = 0; i < P; ++i) o[u][i] = both(0.0f);
+                }
+                if (!EDGE || t + u < t1) put<T, V, ALIGNED>(to, at.valid, CONV_LANES, o[u]);
+                to += a.channels;
+            }
+        };
+        int t = t0;
+        for (; t + U <= tn; t += U) group(t, std::false_type());
+        for (; t < t1; t += U) group(t, std::true_type());
     }
     if (a.final_state && s == 0) {
         T* last = static_cast<T*>(a.final_state) + (long long)b * H * a.channels + at.d;
@@ -184,13 +197,16 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
         const int end = max(t1, t0) + H;
         f32x2 w[W][P], bias[P], win[H + U][P], dp[H + U][P];  // x and dpre of tokens t-H .. t+U-1
         const int tn = min(end, n);
+        const T *ask_x = x + t0 * a.x_stride_t, *ask_g = dy + t0 * a.dy_stride_t;         // of the token that is requested next
         auto request = [&](int t) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (t + u < tn) {
-                    ring.request(t + u, 0, x + (t + u) * a.x_stride_t, at.valid);
-                    if (dy) ring.request(t + u, 1, dy + (t + u) * a.dy_stride_t, at.valid);
+                    ring.request(t + u, 0, ask_x, at.valid);
+                    if (dy) ring.request(t + u, 1, ask_g, at.valid);
                 }
+                ask_x += a.x_stride_t;
+                ask_g += a.dy_stride_t;
             }
             rowio::cp_async_commit();
         };
@@ -209,7 +225,10 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
             for (int k = 0; k < W; ++k) w[k][i] = pair(a.weight[(long long)c0 * W + k], a.weight[(long long)c1 * W + k]);
             bias[i] = a.bias ? pair(a.bias[c0], a.bias[c1]) : both(0.0f);
         }
-        for (int t = t0; t < end; t += U) {
+        T* out = dx ? dx + (long long)(t0 - H) * a.channels : nullptr;        // of x[t-H]
+        // edge: some of the tokens are padding or another strip's, or the x whose gradients they complete are, or these are the state's
+        auto group = [&](int t, auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;
 #pragma unroll
             for (int k = 0; k < H; ++k)
 #pragma unroll
@@ -221,9 +240,11 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
             rowio::cp_async_wait<GROUPS - 1>();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                if (EDGE || !dy) {
 #pragma unroll
-                for (int i = 0; i < P; ++i) win[H + u][i] = g[u][i] = both(0.0f);
-                if (t + u < tn) {                             // a slot that nothing was copied to is not looked at
+                    for (int i = 0; i < P; ++i) win[H + u][i] = g[u][i] = both(0.0f);
+                }
+                if (!EDGE || t + u < tn) {                    // a slot that nothing was copied to is not looked at
                     ring.read(t + u, 0, win[H + u]);
                     if (dy) ring.read(t + u, 1, g[u]);
                 }
@@ -242,11 +263,11 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const bool real = t + u < n && t + u < end;   // not padding, whose slope may be anything if the bias is not finite
+                const bool real = !EDGE || t + u < tn;        // not padding, whose slope may be anything if the bias is not finite
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     dp[H + u][i] = real ? g[u][i] : both(0.0f);
-                    if (t + u < t1) {
+                    if (!EDGE || t + u < t1) {
                         db[i] = add2(db[i], dp[H + u][i]);
 #pragma unroll
                         for (int k = 0; k < W; ++k) dw[k][i] = fma2(dp[H + u][i], win[u + k][i], dw[k][i]);
@@ -256,29 +277,36 @@ causal_conv_backward_kernel(const el_conv_t a, int strip, float* __restrict__ pa
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int to = t + u - H;                     // whose gradient is complete
-                if (t + u >= end || (to < t0 && s > 0)) continue;
+                T* here = out;
+                if (dx) out += a.channels;
+                if (EDGE && (t + u >= end || (to < t0 && s > 0))) continue;
                 f32x2 o[P];
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     o[i] = both(0.0f);
-                    if (to < n) {
+                    if (!EDGE || to < n) {
+                        o[i] = mul2(w[0][i], dp[u + H][i]);
 #pragma unroll
-                        for (int k = 0; k < W; ++k) o[i] = fma2(w[k][i], dp[u + H - k][i], o[i]);
+                        for (int k = 1; k < W; ++k) o[i] = fma2(w[k][i], dp[u + H - k][i], o[i]);
                     }
                 }
-                if (d_last && to < n && to >= n - H) {        // x[to] is also part of the final state
+                if (EDGE && d_last && to < n && to >= n - H) {        // x[to] is also part of the final state
                     f32x2 f[P];
                     widen<T, V>(fetch<T, V, ALIGNED>(d_last + (long long)(to - (n - H)) * a.channels, at.valid, CONV_LANES), f);
 #pragma unroll
                     for (int i = 0; i < P; ++i) o[i] = add2(o[i], f[i]);
                 }
-                if (to >= 0) {
-                    if (dx) put<T, V, ALIGNED>(dx + (long long)to * a.channels, at.valid, CONV_LANES, o);
+                if (!EDGE || to >= 0) {
+                    if (dx) put<T, V, ALIGNED>(here, at.valid, CONV_LANES, o);
                 } else if (d_first) {
                     put<T, V, ALIGNED>(d_first + (long long)(to + H) * a.channels, at.valid, CONV_LANES, o);
                 }
             }
-        }
+        };
+        int t = t0;
+        for (; t < t0 + H && t < end; t += U) group(t, std::true_type());
+        for (; t + U <= t1 && t + U <= tn; t += U) group(t, std::false_type());
+        for (; t < end; t += U) group(t, std::true_type());
     }
     rowio::cp_async_wait<0>();
     if (partial == nullptr) return;
@@ -347,13 +375,13 @@ static bool vectors(const void* p, long long s0, long long s1, int dtype, int V)
 
 static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Tokens of a strip: long strips read fewer tokens twice, short ones give every SM work.
-static int conv_strip(const el_conv_t& a, int vectors_per_token, int blocks_of) {
+// Tokens of a strip: long strips read fewer tokens twice, short ones give every SM its `threads_of` threads.
+static int conv_strip(const el_conv_t& a, int vectors_per_token, int threads_of) {
     int sms = 148;
     device_sm_count(&sms);
     const long long threads = (long long)a.batch * vectors_per_token * a.length;       // at one token a strip
     int strip = 32;
-    while (strip > 4 && threads / strip < (long long)sms * blocks_of) strip >>= 1;
+    while (strip > 8 && threads / strip < (long long)sms * threads_of) strip >>= 1;
     return strip;
 }
 
@@ -361,7 +389,7 @@ constexpr int FW_STRIPS = 4, BW_STRIPS = 8;
 
 struct ConvBackwardPlan { int strip, blocks_t; };
 static ConvBackwardPlan conv_backward_plan(const el_conv_t& a) {
-    const int strip = conv_strip(a, (a.channels + 3) / 4, 1024);
+    const int strip = conv_strip(a, (a.channels + 3) / 4, 768);
     return {strip, ceil_div(a.length > 0 ? a.length : 1, (long long)strip * BW_STRIPS)};
 }
 
