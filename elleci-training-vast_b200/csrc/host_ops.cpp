@@ -9,6 +9,7 @@
 // No state of its own but the handles that set_hooks hands over: the status word of each device, the function that turns a status
 // into an exception and the one that checks the device's status word.  Scratch that a call needs and leaves is allocated per call.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -660,6 +661,13 @@ const Tensor& state_out_arg(PyObject* o, const Tensor& state) {
 void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// a step has no gradient: called where one would be recorded, it refuses
+void no_gradient(const char* name, PyObject* const* a, std::initializer_list<int> tensors) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (int i : tensors)
+        if (!is_none(a[i]) && THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).requires_grad())
+            raise(std::string(name) + " has no gradient: call it without gradient recording");
+}
 long long stride_of(const Tensor& t, int64_t dim) { return t.defined() && t.size(dim) > 1 ? t.stride(dim) : 0; }
 int int_size(int64_t n) {
     EL_REQUIRE(n <= INT32_MAX, "a size does not fit 32 bits");
@@ -752,6 +760,7 @@ PyObject* causal_conv_backward(PyObject* const* a) {
 
 // causal_conv_step(x, state, weight, bias, silu, state_out) -> y
 PyObject* causal_conv_step(PyObject* const* a) {
+    no_gradient("causal_conv_step", a, {0, 1, 2, 3});
     ConvCall k;
     conv_call(k, a[0], a[2], a[3], int_arg(a[4]) != 0, true);
     const Tensor& x = k.x;
@@ -773,6 +782,7 @@ struct ScanCall {
     std::vector<Tensor> keep;
     Tensor u;
     int64_t B = 0, L = 0, D = 0, G = 0, N = 0;
+    std::vector<int64_t> shared;            // B's and C's sizes
 };
 // u, dt [batch, length, channels], A [channels, states], B, C [batch, length, groups, states], D, z, dt_bias; a step has no length
 void scan_call(ScanCall& k, PyObject* const* a, bool softplus, bool step) {
@@ -781,16 +791,17 @@ void scan_call(ScanCall& k, PyObject* const* a, bool softplus, bool step) {
     EL_REQUIRE(u.dim() == (step ? 2 : 3), step ? "u must be [batch, channels]" : "u must be [batch, length, channels]");
     const Tensor &A = cuda_arg(a[2], "A"), &Bm = cuda_arg(a[3], "B");
     EL_REQUIRE(A.dim() == 2 && A.size(1) >= 1 && A.size(1) <= 64, "A must be [channels, states] with 1 to 64 states");
-    EL_REQUIRE(Bm.dim() == u.dim() + 1, step ? "B must be [batch, groups, states]" : "B must be [batch, length, groups, states]");
+    const bool grouped = Bm.dim() == u.dim() + 1;             // or one group, without a dimension of its own
+    EL_REQUIRE(grouped || Bm.dim() == u.dim(), step ? "B must be [batch, (groups,) states]" : "B must be [batch, length, (groups,) states]");
     k.B = u.size(0);
     k.L = step ? 1 : u.size(1);
     k.D = u.size(-1);
     k.N = A.size(1);
-    k.G = Bm.size(-2);
+    k.G = grouped ? Bm.size(-2) : 1;
     EL_REQUIRE(k.G >= 1 && k.D % k.G == 0, "the channels must be a multiple of B's groups");
     k.u = tokens_arg(a[0], "u", u, u.sizes());
     std::vector<int64_t> shared(u.sizes().begin(), u.sizes().end() - 1);
-    shared.push_back(k.G);
+    if (grouped) shared.push_back(k.G);
     shared.push_back(k.N);
     Tensor dt = tokens_arg(a[1], "dt", u, u.sizes()), B2 = tokens_arg(a[3], "B", u, shared), C2 = tokens_arg(a[4], "C", u, shared);
     Tensor A2 = dense_arg(a[2], "A", u, at::kFloat, {k.D, k.N}), Dv = maybe_dense(a[5], "D", u, at::kFloat, {k.D});
@@ -813,8 +824,8 @@ void scan_call(ScanCall& k, PyObject* const* a, bool softplus, bool step) {
     c.z_stride_b = z.defined() ? stride_of(z, 0) : 0;
     c.B_stride_b = stride_of(B2, 0);
     c.C_stride_b = stride_of(C2, 0);
-    c.B_stride_g = stride_of(B2, -2);
-    c.C_stride_g = stride_of(C2, -2);
+    c.B_stride_g = grouped ? stride_of(B2, -2) : 0;
+    c.C_stride_g = grouped ? stride_of(C2, -2) : 0;
     if (!step) {
         c.u_stride_t = stride_of(k.u, 1);
         c.dt_stride_t = stride_of(dt, 1);
@@ -825,6 +836,7 @@ void scan_call(ScanCall& k, PyObject* const* a, bool softplus, bool step) {
     c.A = ptr<float>(A2);
     c.D = ptr<float>(Dv);
     c.dt_bias = ptr<float>(bias);
+    k.shared = std::move(shared);
     k.keep = {dt, B2, C2, A2, Dv, z, bias};
 }
 
@@ -871,8 +883,8 @@ PyObject* selective_scan_backward(PyObject* const* a) {
     if (want & 1) du = new_empty(u, u.sizes(), io);
     if (want & 2) ddt = new_empty(u, u.sizes(), io);
     if (want & 4) dA = new_empty(u, {k.D, k.N}, at::kFloat);
-    if (want & 8) dB = new_empty(u, {k.B, k.L, k.G, k.N}, io);
-    if (want & 16) dC = new_empty(u, {k.B, k.L, k.G, k.N}, io);
+    if (want & 8) dB = new_empty(u, k.shared, io);
+    if (want & 16) dC = new_empty(u, k.shared, io);
     if (want & 32) dD = new_empty(u, {k.D}, at::kFloat);
     if ((want & 64) && c.z) dz = new_empty(u, u.sizes(), io);
     if (want & 128) dbias = new_empty(u, {k.D}, at::kFloat);
@@ -901,6 +913,7 @@ PyObject* selective_scan_backward(PyObject* const* a) {
 
 // selective_scan_step(u, dt, A, B, C, D, z, dt_bias, softplus, state, state_out) -> y
 PyObject* selective_scan_step(PyObject* const* a) {
+    no_gradient("selective_scan_step", a, {0, 1, 2, 3, 4, 5, 6, 7, 9});
     ScanCall k;
     scan_call(k, a, int_arg(a[8]) != 0, true);
     const Tensor& u = k.u;

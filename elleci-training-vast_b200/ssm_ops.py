@@ -28,7 +28,11 @@ _ACTIVATIONS = {"silu": 1, "swish": 1, None: 0}
 
 
 def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _bits(wanted) -> int:
@@ -82,7 +86,6 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     """One token x [batch, channels] of `causal_conv`.  `state` [batch, width-1, channels] becomes the state after the token in place, or,
     with `state_out` (a tensor like it; for callers that may take the token back), is kept and the new state goes there.  Not
     differentiable."""
-    _require(not _wants_grad(x, weight, bias, state), "causal_conv_step has no gradient: call it without gradient recording")
     return host_ops().causal_conv_step(x, state, weight, bias, _silu(activation), state_out)
 
 
@@ -107,11 +110,6 @@ class _SelectiveScan(Function):
         return du, ddt, dA, dB, dC, dD, dz, ddt_bias, None, d_first, None, None
 
 
-def _with_groups(t: torch.Tensor, dims: int) -> torch.Tensor:
-    """[.., states] of one group as [.., 1, states]."""
-    return t.unsqueeze(-2) if isinstance(t, torch.Tensor) and t.dim() == dims else t
-
-
 def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor] = None,
                    z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = True,
                    initial_state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
@@ -124,7 +122,6 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     [batch, length, states], or [batch, length, groups, states] where channels / groups consecutive channels share a group.  `initial_state`
     [batch, channels, states] float32 (zeros if None); with `return_final_state` the state after each sequence's last token is returned too.
     Differentiable in every tensor; the forward pass then keeps the state of every sixteenth token."""
-    B, C = _with_groups(B, 3), _with_groups(C, 3)
     if _wants_grad(u, dt, A, B, C, D, z, dt_bias, initial_state):
         y, state = _SelectiveScan.apply(u, dt, A, B, C, D, z, dt_bias, int(dt_softplus), initial_state, lengths, int(return_final_state))
     else:
@@ -139,8 +136,7 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     """One token of `selective_scan`: u, dt, z [batch, channels], B and C [batch, states] or [batch, groups, states].  `state`
     [batch, channels, states] float32 becomes the state after the token in place, or goes to `state_out` as in `causal_conv_step`.
     Not differentiable."""
-    _require(not _wants_grad(u, dt, A, B, C, state, D, z, dt_bias), "selective_scan_step has no gradient: call it without gradient recording")
-    return host_ops().selective_scan_step(u, dt, A, _with_groups(B, 2), _with_groups(C, 2), D, z, dt_bias, int(dt_softplus), state, state_out)
+    return host_ops().selective_scan_step(u, dt, A, B, C, D, z, dt_bias, int(dt_softplus), state, state_out)
 
 
 class _BlockNorm(Function):
