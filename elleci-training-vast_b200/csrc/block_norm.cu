@@ -4,6 +4,8 @@
 // backward (yn = y r1, hn = h' r2, both formed again from the inputs):
 //   dh = dh' + r2 (dn w2 - hn mean(dn w2 hn));  dw2 = sum dn hn;  ds = sum dh sigmoid(g) p;  dg = dh s p sigmoid'(g)
 //   dp = dh s sigmoid(g);  dw1 = sum dp yn;  dy = r1 (dp w1 - yn mean(dp w1 yn))
+// The second mean is linear in the first one, c2: with q = s sigmoid(g) w1 yn it is mean((dh' + r2 dn w2) q) - c2 r2 mean(hn q), so that a row's
+// three sums are taken together, behind one barrier.
 // Row sums in float32: a thread adds 8 to 32 squares, the block adds the threads' in a fixed order.
 //
 // Blocks walk over the rows; a thread owns the same vectors of 8 columns in each.  Bound: memory, 5 values read or written per column forward, 8
@@ -33,6 +35,25 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// The same of three sums at once.
+__device__ __forceinline__ void block_sums(float v[3], float (*red)[NORM_MAX_WARPS]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int q = 0; q < 3; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+        for (int q = 0; q < 3; ++q) red[q][threadIdx.x >> 5] = v[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 3; ++q) v[q] = lane < (int)(blockDim.x >> 5) ? red[q][lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int q = 0; q < 3; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
 }
 
 // 1 / sqrt(sum / K + eps)
@@ -131,7 +152,7 @@ template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(512, 1)
 block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial) {
     constexpr bool AHEAD = sizeof(T) == 2;
-    __shared__ float red[2][NORM_MAX_WARPS];
+    __shared__ float red[2][3][NORM_MAX_WARPS];
     const int K = a.width, stride = blockDim.x, k = norm_column<ALIGNED>(0);
     const bool mine = k < K;
     f32x2 sums[3][4];
@@ -160,12 +181,13 @@ block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial)
         if (p && mine) put<T, 8, ALIGNED>(static_cast<T*>(p) + (long long)m * K + k, K - k, stride, v);
     };
     if (AHEAD && blockIdx.x < a.rows) fetch_row(blockIdx.x);
-    for (int m = blockIdx.x; m < a.rows; m += gridDim.x) {
+    int turn = 0;
+    for (int m = blockIdx.x; m < a.rows; m += gridDim.x, turn ^= 1) {
         if (!AHEAD) fetch_row(m);
         const NormGrads<T> row = next;
         if (AHEAD && m + (int)gridDim.x < a.rows) fetch_row(m + gridDim.x);
         const float r1 = a.rstd[2 * (long long)m], r2 = a.rstd[2 * (long long)m + 1];
-        f32x2 yn[4], hn[4], sg[4], dt[4], w1[4], s[4], t[4];
+        f32x2 yn[4], hn[4], sg[4], dt[4], w1[4], s[4], t[4], q[4];
         widen<T, 8>(row.y, yn);
         widen<T, 8>(row.h, hn);
         widen<T, 8>(row.g, sg);
@@ -177,27 +199,28 @@ block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial)
         for (int i = 0; i < 4; ++i) {
             yn[i] = mul2(yn[i], both(r1));
             sg[i] = a.gate ? sigmoid2(sg[i]) : both(1.0f);
-            hn[i] = mul2(fma2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]), hn[i]), both(r2));
+            q[i] = mul2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]));
+            hn[i] = mul2(add2(q[i], hn[i]), both(r2));
             sums[1][i] = fma2(dt[i], hn[i], sums[1][i]);
             dt[i] = mul2(dt[i], t[i]);
         }
-        const float c2 = __fdiv_rn(block_sum(dot(dt, hn, 0.0f), red[0]), (float)K);
-        f32x2 d[4];
-        widen<T, 8>(row.dh, d);
+        widen<T, 8>(row.dh, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = fma2(both(r2), dt[i], t[i]);
+        float v[3] = {dot(dt, hn, 0.0f), dot(t, q, 0.0f), dot(hn, q, 0.0f)};
+        block_sums(v, red[turn]);
+        const float c2 = __fdiv_rn(v[0], (float)K), c1 = __fdiv_rn(__fmaf_rn(-__fmul_rn(c2, r2), v[2], v[1]), (float)K);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            d[i] = fma2(both(r2), fma2(hn[i], both(-c2), dt[i]), d[i]);
-            const f32x2 p = mul2(yn[i], w1[i]), ds = mul2(d[i], sg[i]), dp = mul2(ds, s[i]);
+            t[i] = fma2(hn[i], both(-__fmul_rn(c2, r2)), t[i]);            // dh
+            const f32x2 p = mul2(yn[i], w1[i]), ds = mul2(t[i], sg[i]), dp = mul2(ds, s[i]);
             sums[2][i] = fma2(ds, p, sums[2][i]);
             hn[i] = mul2(mul2(dp, p), fma2(sg[i], both(-1.0f), both(1.0f)));      // of the gate
             sums[0][i] = fma2(dp, yn[i], sums[0][i]);
-            dt[i] = mul2(dp, w1[i]);
+            dt[i] = mul2(both(r1), fma2(yn[i], both(-c1), mul2(dp, w1[i])));
         }
-        out(a.dh, m, d);
+        out(a.dh, m, t);
         if (a.gate) out(a.dgate, m, hn);
-        const float c1 = __fdiv_rn(block_sum(dot(dt, yn, 0.0f), red[1]), (float)K);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dt[i] = mul2(both(r1), fma2(yn[i], both(-c1), dt[i]));
         out(a.dy_in, m, dt);
     }
     if (mine) {
@@ -206,11 +229,11 @@ block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial)
     }
 }
 
-// Wider rows: nothing is kept between the three passes over a row, whose second and third come from L2, and the column sums are in shared memory.
+// Wider rows: nothing is kept between the two passes over a row, the second one's values come from L2, and the column sums are in shared memory.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(512, 1)
 block_norm_backward_wide_kernel(const el_block_norm_t a, float* __restrict__ partial) {
-    __shared__ float red[2][NORM_MAX_WARPS];
+    __shared__ float red[2][3][NORM_MAX_WARPS];
     extern __shared__ float4 sums_[];                         // [3][padded width / 4]: a thread's own columns, as vectors
     float* sums = reinterpret_cast<float*>(sums_);
     const int K = a.width, stride = blockDim.x, vecs = (K + 8 * stride - 1) / (8 * stride), padded = vecs * 8 * stride;
@@ -234,76 +257,64 @@ block_norm_backward_wide_kernel(const el_block_norm_t a, float* __restrict__ par
             slot(q, c, half) = s;
         }
     };
-    for (int m = blockIdx.x; m < a.rows; m += gridDim.x) {
+    int turn = 0;
+    for (int m = blockIdx.x; m < a.rows; m += gridDim.x, turn ^= 1) {
         const float r1 = a.rstd[2 * (long long)m], r2 = a.rstd[2 * (long long)m + 1];
-        // yn, sigmoid of the gate, p = yn w1, hn of a vector
-        auto form = [&](int k, f32x2 yn[4], f32x2 sg[4], f32x2 w1[4], f32x2 s[4], f32x2 hn[4]) {
+        // of a vector: yn, sigmoid of the gate, w1, scale, q, hn, dn and dh' + r2 dn w2
+        auto form = [&](int k, f32x2 yn[4], f32x2 sg[4], f32x2 w1[4], f32x2 s[4], f32x2 q[4], f32x2 hn[4], f32x2 dn[4], f32x2 d[4]) {
+            f32x2 w2[4];
             get(a.y, a.ld_y, m, k, yn);
             get(a.h, a.ld_h, m, k, hn);
             get(a.gate, a.ld_gate, m, k, sg);
+            get(a.dnormed, a.ld_dnormed, m, k, dn);
+            get(a.dh_out, a.ld_dh_out, m, k, d);
             weight(a.post_weight, k, w1);
             weight(a.scale, k, s);
+            weight(a.pre_weight, k, w2);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 yn[i] = mul2(yn[i], both(r1));
                 sg[i] = a.gate ? sigmoid2(sg[i]) : both(1.0f);
-                hn[i] = mul2(fma2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]), hn[i]), both(r2));
+                q[i] = mul2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]));
+                hn[i] = mul2(add2(q[i], hn[i]), both(r2));
+                w2[i] = mul2(w2[i], dn[i]);
+                d[i] = fma2(both(r2), w2[i], d[i]);
+                dn[i] = mul2(dn[i], hn[i]);                    // what the sum for w2 takes
+                w2[i] = mul2(w2[i], hn[i]);
             }
+            return lo_of(add2(add2(w2[0], w2[1]), add2(w2[2], w2[3]))) + hi_of(add2(add2(w2[0], w2[1]), add2(w2[2], w2[3])));
         };
-        float sum = 0.0f;
+        float v[3] = {};
         for (int c = 0; c < vecs; ++c) {
             const int k = norm_column<ALIGNED>(c);
             if (k >= K) continue;
-            f32x2 yn[4], sg[4], w1[4], s[4], hn[4], dn[4], w2[4];
-            form(k, yn, sg, w1, s, hn);
-            get(a.dnormed, a.ld_dnormed, m, k, dn);
-            weight(a.pre_weight, k, w2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w2[i] = mul2(w2[i], dn[i]);
-                dn[i] = mul2(dn[i], hn[i]);
-            }
-            sum = dot(w2, hn, sum);
+            f32x2 yn[4], sg[4], w1[4], s[4], q[4], hn[4], dn[4], d[4];
+            v[0] += form(k, yn, sg, w1, s, q, hn, dn, d);
+            v[1] = dot(d, q, v[1]);
+            v[2] = dot(hn, q, v[2]);
             add_to(1, c, dn);
         }
-        const float c2 = __fdiv_rn(block_sum(sum, red[0]), (float)K);
-        sum = 0.0f;
-        float c1 = 0.0f;
-        for (int pass = 0; pass < 2; ++pass) {
-            for (int c = 0; c < vecs; ++c) {
-                const int k = norm_column<ALIGNED>(c);
-                if (k >= K) continue;
-                f32x2 yn[4], sg[4], w1[4], s[4], hn[4], d[4], dn[4], w2[4];
-                form(k, yn, sg, w1, s, hn);
-                get(a.dh_out, a.ld_dh_out, m, k, d);
-                get(a.dnormed, a.ld_dnormed, m, k, dn);
-                weight(a.pre_weight, k, w2);
+        block_sums(v, red[turn]);
+        const float c2 = __fdiv_rn(v[0], (float)K), c1 = __fdiv_rn(__fmaf_rn(-__fmul_rn(c2, r2), v[2], v[1]), (float)K);
+        for (int c = 0; c < vecs; ++c) {
+            const int k = norm_column<ALIGNED>(c);
+            if (k >= K) continue;
+            f32x2 yn[4], sg[4], w1[4], s[4], q[4], hn[4], dn[4], d[4], ds[4], dw[4];
+            form(k, yn, sg, w1, s, q, hn, dn, d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[i] = fma2(both(r2), fma2(hn[i], both(-c2), mul2(dn[i], w2[i])), d[i]);
-                if (pass == 0) {
-                    put<T, 8, ALIGNED>(static_cast<T*>(a.dh) + (long long)m * K + k, K - k, stride, d);
-                    f32x2 ds[4], dg[4], dw[4], dp[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x2 p = mul2(yn[i], w1[i]);
-                        dn[i] = mul2(d[i], sg[i]);
-                        ds[i] = mul2(dn[i], p);
-                        dp[i] = mul2(dn[i], s[i]);
-                        dg[i] = mul2(mul2(dp[i], p), fma2(sg[i], both(-1.0f), both(1.0f)));
-                        dw[i] = mul2(dp[i], yn[i]);
-                        dp[i] = mul2(dp[i], w1[i]);
-                    }
-                    add_to(2, c, ds);
-                    add_to(0, c, dw);
-                    if (a.gate && a.dgate) put<T, 8, ALIGNED>(static_cast<T*>(a.dgate) + (long long)m * K + k, K - k, stride, dg);
-                    sum = dot(dp, yn, sum);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = mul2(both(r1), fma2(yn[i], both(-c1), mul2(mul2(mul2(d[i], sg[i]), s[i]), w1[i])));
-                    put<T, 8, ALIGNED>(static_cast<T*>(a.dy_in) + (long long)m * K + k, K - k, stride, d);
-                }
+            for (int i = 0; i < 4; ++i) {
+                d[i] = fma2(hn[i], both(-__fmul_rn(c2, r2)), d[i]);        // dh
+                const f32x2 p = mul2(yn[i], w1[i]), g = mul2(d[i], sg[i]), dp = mul2(g, s[i]);
+                ds[i] = mul2(g, p);
+                dw[i] = mul2(dp, yn[i]);
+                hn[i] = mul2(mul2(dp, p), fma2(sg[i], both(-1.0f), both(1.0f)));      // of the gate
+                dn[i] = mul2(both(r1), fma2(yn[i], both(-c1), mul2(dp, w1[i])));      // of y
             }
-            if (pass == 0) c1 = __fdiv_rn(block_sum(sum, red[1]), (float)K);
+            add_to(2, c, ds);
+            add_to(0, c, dw);
+            put<T, 8, ALIGNED>(static_cast<T*>(a.dh) + (long long)m * K + k, K - k, stride, d);
+            if (a.gate && a.dgate) put<T, 8, ALIGNED>(static_cast<T*>(a.dgate) + (long long)m * K + k, K - k, stride, hn);
+            put<T, 8, ALIGNED>(static_cast<T*>(a.dy_in) + (long long)m * K + k, K - k, stride, dn);
         }
     }
     for (int c = 0; c < vecs; ++c) {
