@@ -195,11 +195,13 @@ int launch_decode_preq(const int8_t* xq, const float* absmax, const uint8_t* Wp,
 }
 
 // ---- between the projections of a Mamba block: what every entry point of an operator checks ----------------------------------
+constexpr int MAX_LENGTH = 0x7fff0000;           // tokens of a sequence: the kernels count a tile beyond its end
 static int check_conv(const el_conv_t* a) {
     if (!a) return EL_ERR_NULL_PTR;
     if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->channels < 0 || a->x_stride_b < 0 || a->x_stride_t < 0 || a->dy_stride_b < 0 ||
         a->dy_stride_t < 0)
         return EL_ERR_INVALID_ARG;
+    if (a->length > MAX_LENGTH) return EL_ERR_TOO_LARGE;
     return a->width >= 2 && a->width <= 4 ? EL_OK : EL_ERR_UNSUPPORTED_SHAPE;
 }
 static int check_scan(const el_scan_t* a) {
@@ -210,6 +212,7 @@ static int check_scan(const el_scan_t* a) {
                                  a->B_stride_t, a->B_stride_g, a->C_stride_b, a->C_stride_t, a->C_stride_g, a->dy_stride_b, a->dy_stride_t};
     for (long long s : strides)
         if (s < 0) return EL_ERR_INVALID_ARG;
+    if (a->length > MAX_LENGTH) return EL_ERR_TOO_LARGE;
     return a->states <= 64 ? EL_OK : EL_ERR_UNSUPPORTED_SHAPE;
 }
 static int check_norm(const el_block_norm_t* a) {
