@@ -121,7 +121,7 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     dt and z are like u; A is [channels, states] (1 to 64 states; negative for a state that decays), D and dt_bias [channels]; B and C are
     [batch, length, states], or [batch, length, groups, states] where channels / groups consecutive channels share a group.  `initial_state`
     [batch, channels, states] float32 (zeros if None); with `return_final_state` the state after each sequence's last token is returned too.
-    Differentiable in every tensor; the forward pass then keeps the state of every sixteenth token."""
+    Differentiable in every tensor; the forward pass then keeps the state of every eighth token."""
     if _wants_grad(u, dt, A, B, C, D, z, dt_bias, initial_state):
         y, state = _SelectiveScan.apply(u, dt, A, B, C, D, z, dt_bias, int(dt_softplus), initial_state, lengths, int(return_final_state))
     else:
