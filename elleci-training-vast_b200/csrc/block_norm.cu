@@ -58,15 +58,38 @@ __device__ __forceinline__ void block_sums(float v[3], float (*red)[NORM_MAX_WAR
 
 // 1 / sqrt(sum / K + eps)
 __device__ __forceinline__ float rms_inverse(float sum, int K, float eps) { return __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)K), eps)); }
-__device__ __forceinline__ float dot(const f32x2 a[4], const f32x2 b[4], float sum) {
+template <int P = 4> __device__ __forceinline__ float dot(const f32x2 a[P], const f32x2 b[P], float sum) {
     f32x2 s = mul2(a[0], b[0]);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) s = fma2(a[i], b[i], s);
+    for (int i = 1; i < P; ++i) s = fma2(a[i], b[i], s);
     return sum + (lo_of(s) + hi_of(s));
 }
 
 // First column of a thread's vector c, and the distance of its elements: adjacent, or as many apart as the block has threads.
 template <bool ALIGNED> __device__ __forceinline__ int norm_column(int c) { return ALIGNED ? (c * blockDim.x + threadIdx.x) * 8 : c * 8 * blockDim.x + threadIdx.x; }
+
+// A thread's columns of the weights, ones for a scale that is not there, in its own slots of shared memory: 48 KB at 4096 columns, which the rows would
+// drive out of the L1 cache (backward 4096 x 4096 bfloat16: 78 us with the weights read from there, 67 so).
+template <int V, bool ALIGNED> struct HeldWeights {
+    float4* mine;
+    __device__ __forceinline__ void hold(int q, const float* p, int k, int K) {
+        f32x2 w[V / 2];
+        if (p && k < K) widen<float, V>(fetch<float, V, ALIGNED>(p + k, K - k, blockDim.x), w);
+        else
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) w[i] = both(1.0f);
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) mine[(q * (V / 4) + i) * blockDim.x] = make_float4(lo_of(w[2 * i]), hi_of(w[2 * i]), lo_of(w[2 * i + 1]), hi_of(w[2 * i + 1]));
+    }
+    __device__ __forceinline__ void read(int q, f32x2 w[V / 2]) const {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float4 x = mine[(q * (V / 4) + i) * blockDim.x];
+            w[2 * i] = pair(x.x, x.y);
+            w[2 * i + 1] = pair(x.z, x.w);
+        }
+    }
+};
 
 template <typename T> struct NormRow { Vec<T, 8> h, y, g; };
 
@@ -74,7 +97,13 @@ template <typename T, int VECS, bool ALIGNED>
 __global__ void __launch_bounds__(512, VECS == 1 ? 2 : 1)
 block_norm_kernel(const el_block_norm_t a) {
     __shared__ float red[2][NORM_MAX_WARPS];
+    extern __shared__ uint4 slots[];                          // one vector a thread: its weights
     const int K = a.width, stride = blockDim.x;
+    HeldWeights<8, ALIGNED> held{reinterpret_cast<float4*>(slots) + threadIdx.x};
+    auto weight = [&](int q, const float* p, int k, f32x2 w[4]) {
+        if (VECS == 1) held.read(q, w);
+        else widen<float, 8>(fetch<float, 8, ALIGNED>(p + k, K - k, stride), w);
+    };
     NormRow<T> next[VECS];
     auto fetch_row = [&](int m) {
 #pragma unroll
@@ -90,6 +119,11 @@ block_norm_kernel(const el_block_norm_t a) {
     };
     int m = blockIdx.x;
     if (m < a.rows) fetch_row(m);
+    if (VECS == 1) {
+        held.hold(0, a.post_weight, norm_column<ALIGNED>(0), K);
+        held.hold(1, a.pre_weight, norm_column<ALIGNED>(0), K);
+        if (a.scale) held.hold(2, a.scale, norm_column<ALIGNED>(0), K);
+    }
     for (; m < a.rows; m += gridDim.x) {
         NormRow<T> row[VECS];
         f32x2 v[VECS][4];
@@ -109,14 +143,14 @@ block_norm_kernel(const el_block_norm_t a) {
             if (k >= K) continue;
             f32x2 h[4], w[4], f[4];
             widen<T, 8>(row[c].h, h);
-            widen<float, 8>(fetch<float, 8, ALIGNED>(a.post_weight + k, K - k, stride), w);
+            weight(0, a.post_weight, k, w);
             if (a.gate) {
                 widen<T, 8>(row[c].g, f);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], sigmoid2(f[i]));
             }
             if (a.scale) {
-                widen<float, 8>(fetch<float, 8, ALIGNED>(a.scale + k, K - k, stride), f);
+                weight(2, a.scale, k, f);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], f[i]);
             }
@@ -131,7 +165,7 @@ block_norm_kernel(const el_block_norm_t a) {
             const int k = norm_column<ALIGNED>(c);
             if (k >= K) continue;
             f32x2 w[4];
-            widen<float, 8>(fetch<float, 8, ALIGNED>(a.pre_weight + k, K - k, stride), w);
+            weight(1, a.pre_weight, k, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], mul2(v[c][i], both(r2)));
             put<T, 8, ALIGNED>(static_cast<T*>(a.normed) + (long long)m * K + k, K - k, stride, w);
@@ -144,59 +178,91 @@ block_norm_kernel(const el_block_norm_t a) {
     }
 }
 
-// Backward, rows of up to 4096 columns: a row's values stay in registers, one vector a thread, and so do the column sums of a block's
-// rows, which go to `partial` [blocks][3][width]: dw1, dw2, ds.  float32 rows are not fetched ahead: no registers are left for them.
-template <typename T> struct NormGrads { Vec<T, 8> h, y, g, dh, dn; };
+// Backward, rows of up to 4096 columns: a row's values stay in registers, one vector of 16 bytes a thread, and so do the column sums of a block's
+// rows, which go to `partial` [blocks][3][width]: dw1, dw2, ds.  The next row is on asynchronous copies into the threads' own slots in shared
+// memory (one row ahead; two or three gain nothing); rows that no vector copy takes are fetched into registers.  4096 x 4096, bfloat16 67 us, float32 98.
+template <typename T> constexpr int NORM_V = 16 / sizeof(T);
+template <typename T> constexpr int NORM_THREADS = sizeof(T) == 2 ? 512 : 1024;        // of an SM: what its registers take
+template <typename T> struct NormGrads { Vec<T, NORM_V<T>> v[5]; };              // dnormed, y, h, gate, dh_out
 
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(NORM_THREADS<T>, 1)
 block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial) {
-    constexpr bool AHEAD = sizeof(T) == 2;
     __shared__ float red[2][3][NORM_MAX_WARPS];
-    const int K = a.width, stride = blockDim.x, k = norm_column<ALIGNED>(0);
+    constexpr int V = NORM_V<T>, P = V / 2;
+    const int K = a.width, stride = blockDim.x, k = ALIGNED ? threadIdx.x * V : threadIdx.x;
     const bool mine = k < K;
-    f32x2 sums[3][4];
+    f32x2 sums[3][P];
 #pragma unroll
     for (int q = 0; q < 3; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[q][i] = both(0.0f);
+        for (int i = 0; i < P; ++i) sums[q][i] = both(0.0f);
+    extern __shared__ uint4 slots[];                          // [tensor][thread], then the weights
+    const void* const from[5] = {a.dnormed, a.y, a.h, a.gate, a.dh_out};
+    const long long pitch[5] = {a.ld_dnormed, a.ld_y, a.ld_h, a.ld_gate, a.ld_dh_out};
+    uint4* const mine_ahead = slots + threadIdx.x;
+    HeldWeights<V, ALIGNED> held{reinterpret_cast<float4*>(slots + (ALIGNED ? 5 * stride : 0)) + threadIdx.x};
     NormGrads<T> next;
-    auto get = [&](const void* p, long long ld, int m) {
-        return p && mine ? fetch<T, 8, ALIGNED>(static_cast<const T*>(p) + m * ld + k, K - k, stride) : zeros<T, 8>();
-    };
-    auto fetch_row = [&](int m) {
-        next.dn = get(a.dnormed, a.ld_dnormed, m);
-        next.y = get(a.y, a.ld_y, m);
-        next.h = get(a.h, a.ld_h, m);
-        next.g = get(a.gate, a.ld_gate, m);
-        next.dh = get(a.dh_out, a.ld_dh_out, m);
-    };
-    auto weight = [&](const float* p, f32x2 w[4]) {
-        if (p && mine) widen<float, 8>(fetch<float, 8, ALIGNED>(p + k, K - k, stride), w);
-        else
+    auto request = [&](int m) {
+        if (m < a.rows && mine) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = both(p ? 0.0f : 1.0f);
+            for (int q = 0; q < 5; ++q) {
+                if (!from[q]) continue;
+                const T* src = static_cast<const T*>(from[q]) + m * pitch[q] + k;
+                if constexpr (ALIGNED) rowio::cp_async16(mine_ahead + q * stride, src);
+                else next.v[q] = fetch<T, V, false>(src, K - k, stride);
+            }
+        }
+        if (ALIGNED) rowio::cp_async_commit();
     };
-    auto out = [&](void* p, int m, const f32x2 v[4]) {
-        if (p && mine) put<T, 8, ALIGNED>(static_cast<T*>(p) + (long long)m * K + k, K - k, stride, v);
+    auto take = [&]() {                                       // zeros for a tensor that is not there
+        NormGrads<T> row;
+#pragma unroll
+        for (int q = 0; q < 5; ++q) {
+            row.v[q] = zeros<T, V>();
+            if (!from[q] || !mine) continue;
+            if constexpr (ALIGNED) {
+                const uint4 x = mine_ahead[q * stride];
+                row.v[q].w[0] = x.x; row.v[q].w[1] = x.y; row.v[q].w[2] = x.z; row.v[q].w[3] = x.w;
+            } else {
+                row.v[q] = next.v[q];
+            }
+        }
+        return row;
     };
-    if (AHEAD && blockIdx.x < a.rows) fetch_row(blockIdx.x);
+    auto out = [&](void* p, int m, const f32x2 v[P]) {
+        if (p && mine) put<T, V, ALIGNED>(static_cast<T*>(p) + (long long)m * K + k, K - k, stride, v);
+    };
+    const int G = gridDim.x;
+    request(blockIdx.x);
+    held.hold(0, a.post_weight, k, K);
+    held.hold(1, a.scale, k, K);
+    held.hold(2, a.pre_weight, k, K);
+    float r1_next = 0.0f, r2_next = 0.0f;
+    auto rms = [&](int m) {                                   // one row ahead too: nothing of a row can start without them
+        if (m < a.rows) {
+            r1_next = a.rstd[2 * (long long)m];
+            r2_next = a.rstd[2 * (long long)m + 1];
+        }
+    };
+    rms(blockIdx.x);
     int turn = 0;
-    for (int m = blockIdx.x; m < a.rows; m += gridDim.x, turn ^= 1) {
-        if (!AHEAD) fetch_row(m);
-        const NormGrads<T> row = next;
-        if (AHEAD && m + (int)gridDim.x < a.rows) fetch_row(m + gridDim.x);
-        const float r1 = a.rstd[2 * (long long)m], r2 = a.rstd[2 * (long long)m + 1];
-        f32x2 yn[4], hn[4], sg[4], dt[4], w1[4], s[4], t[4], q[4];
-        widen<T, 8>(row.y, yn);
-        widen<T, 8>(row.h, hn);
-        widen<T, 8>(row.g, sg);
-        widen<T, 8>(row.dn, dt);
-        weight(a.post_weight, w1);
-        weight(a.scale, s);
-        weight(a.pre_weight, t);
+    for (int m = blockIdx.x; m < a.rows; m += G, turn ^= 1) {
+        if (ALIGNED) rowio::cp_async_wait<0>();
+        const NormGrads<T> row = take();
+        const float r1 = r1_next, r2 = r2_next;
+        rms(m + G);
+        request(m + G);
+        f32x2 yn[P], hn[P], sg[P], dt[P], w1[P], s[P], t[P], q[P];
+        widen<T, V>(row.v[1], yn);
+        widen<T, V>(row.v[2], hn);
+        widen<T, V>(row.v[3], sg);
+        widen<T, V>(row.v[0], dt);
+        held.read(0, w1);
+        held.read(1, s);
+        held.read(2, t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < P; ++i) {
             yn[i] = mul2(yn[i], both(r1));
             sg[i] = a.gate ? sigmoid2(sg[i]) : both(1.0f);
             q[i] = mul2(mul2(sg[i], s[i]), mul2(yn[i], w1[i]));
@@ -204,14 +270,14 @@ block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial)
             sums[1][i] = fma2(dt[i], hn[i], sums[1][i]);
             dt[i] = mul2(dt[i], t[i]);
         }
-        widen<T, 8>(row.dh, t);
+        widen<T, V>(row.v[4], t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = fma2(both(r2), dt[i], t[i]);
-        float v[3] = {dot(dt, hn, 0.0f), dot(t, q, 0.0f), dot(hn, q, 0.0f)};
+        for (int i = 0; i < P; ++i) t[i] = fma2(both(r2), dt[i], t[i]);
+        float v[3] = {dot<P>(dt, hn, 0.0f), dot<P>(t, q, 0.0f), dot<P>(hn, q, 0.0f)};
         block_sums(v, red[turn]);
         const float c2 = __fdiv_rn(v[0], (float)K), c1 = __fdiv_rn(__fmaf_rn(-__fmul_rn(c2, r2), v[2], v[1]), (float)K);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < P; ++i) {
             t[i] = fma2(hn[i], both(-__fmul_rn(c2, r2)), t[i]);            // dh
             const f32x2 p = mul2(yn[i], w1[i]), ds = mul2(t[i], sg[i]), dp = mul2(ds, s[i]);
             sums[2][i] = fma2(ds, p, sums[2][i]);
@@ -225,7 +291,7 @@ block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial)
     }
     if (mine) {
 #pragma unroll
-        for (int q = 0; q < 3; ++q) put<float, 8, ALIGNED>(partial + ((long long)blockIdx.x * 3 + q) * K + k, K - k, stride, sums[q]);
+        for (int q = 0; q < 3; ++q) put<float, V, ALIGNED>(partial + ((long long)blockIdx.x * 3 + q) * K + k, K - k, stride, sums[q]);
     }
 }
 
@@ -340,7 +406,7 @@ struct NormSums {
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
 
-constexpr int NORM_HELD = 4096;       // columns of a row that one vector per thread of a block holds
+constexpr int NORM_HELD = 4096;       // columns of a row that the kernels hold, one vector a thread
 
 static int norm_threads(int K, int vecs) { return ((K + 8 * vecs - 1) / (8 * vecs) + 31) / 32 * 32; }
 static int norm_vectors(int K) { return K <= NORM_HELD ? 1 : K <= 2 * NORM_HELD ? 2 : 4; }
@@ -349,9 +415,13 @@ static int norm_blocks(int rows, int per_sm) {
     device_sm_count(&sms);
     return rows < (long long)sms * per_sm ? rows : sms * per_sm;
 }
-// An SM's registers take 512 threads of the backward kernel, of the wide one too.
+static int norm_held_threads(const el_block_norm_t& a) {       // of a block of the backward kernel that holds its rows
+    const int V = a.dtype == EL_F32 ? NORM_V<float> : NORM_V<__half>;
+    return ((a.width + V - 1) / V + 31) / 32 * 32;
+}
 static int norm_backward_blocks(const el_block_norm_t& a) {
-    return norm_blocks(a.rows, a.width <= NORM_HELD ? 512 / norm_threads(a.width > 0 ? a.width : 1, 1) : 1);
+    if (a.width > NORM_HELD || a.width == 0) return norm_blocks(a.rows, 1);
+    return norm_blocks(a.rows, (a.dtype == EL_F32 ? NORM_THREADS<float> : NORM_THREADS<__half>) / norm_held_threads(a));
 }
 size_t block_norm_backward_workspace_bytes(const el_block_norm_t& a) { return (size_t)norm_backward_blocks(a) * 3 * a.width * sizeof(float); }
 
@@ -364,6 +434,17 @@ static bool norm_aligned(const el_block_norm_t& a) {
     for (long long l : ld)
         if (l % 8 != 0) return false;
     return true;
+}
+
+// Allows a kernel the shared memory that its widest rows take, once per device.
+template <typename K> static int norm_shared(K kernel, int bytes, DeviceOnce& once) {
+    int dev = 0;
+    EL_CUDA_TRY(cudaGetDevice(&dev));
+    if (!once.is_done(dev)) {
+        EL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        once.mark(dev);
+    }
+    return EL_OK;
 }
 
 template <typename F> static int norm_variant(const el_block_norm_t& a, F f) {
@@ -380,9 +461,16 @@ int launch_block_norm(const el_block_norm_t& a, cudaStream_t st) {
     return norm_variant(a, [&](auto t, auto al) {
         using T = decltype(t);
         constexpr bool AL = decltype(al)::value;
-        if (vecs == 1) block_norm_kernel<T, 1, AL><<<blocks, threads, 0, st>>>(a);
-        else if (vecs == 2) block_norm_kernel<T, 2, AL><<<blocks, threads, 0, st>>>(a);
-        else block_norm_kernel<T, 4, AL><<<blocks, threads, 0, st>>>(a);
+        if (vecs == 1) {
+            static DeviceOnce once;
+            const int rc = norm_shared(block_norm_kernel<T, 1, AL>, 3 * 8 * 512 * (int)sizeof(float), once);
+            if (rc != EL_OK) return rc;
+            block_norm_kernel<T, 1, AL><<<blocks, threads, 3 * 8 * threads * sizeof(float), st>>>(a);
+        } else if (vecs == 2) {
+            block_norm_kernel<T, 2, AL><<<blocks, threads, 0, st>>>(a);
+        } else {
+            block_norm_kernel<T, 4, AL><<<blocks, threads, 0, st>>>(a);
+        }
         return check_launch();
     });
 }
@@ -394,17 +482,15 @@ int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st) {
         const int rc = norm_variant(a, [&](auto t, auto al) {
             using T = decltype(t);
             constexpr bool AL = decltype(al)::value;
+            static DeviceOnce once[2];
             if (a.width <= NORM_HELD) {
-                block_norm_backward_kernel<T, AL><<<blocks, norm_threads(a.width, 1), 0, st>>>(a, partial);
+                const int threads = norm_held_threads(a), rc = norm_shared(block_norm_backward_kernel<T, AL>, NORM_THREADS<T> * (5 * 16 + 3 * NORM_V<T> * 4), once[0]);
+                if (rc != EL_OK) return rc;
+                block_norm_backward_kernel<T, AL><<<blocks, threads, threads * ((AL ? 5 * 16 : 0) + 3 * NORM_V<T> * sizeof(float)), st>>>(a, partial);
                 return check_launch();
             }
-            static DeviceOnce once;
-            int dev = 0;
-            EL_CUDA_TRY(cudaGetDevice(&dev));
-            if (!once.is_done(dev)) {
-                EL_CUDA_TRY(cudaFuncSetAttribute(block_norm_backward_wide_kernel<T, AL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 16384 * 4));
-                once.mark(dev);
-            }
+            const int rc = norm_shared(block_norm_backward_wide_kernel<T, AL>, 3 * 16384 * 4, once[1]);
+            if (rc != EL_OK) return rc;
             const int vecs = (a.width + 8 * 512 - 1) / (8 * 512);
             block_norm_backward_wide_kernel<T, AL><<<blocks, 512, 3 * vecs * 8 * 512 * sizeof(float), st>>>(a, partial);
             return check_launch();

@@ -345,6 +345,13 @@ def test_norm_forward_and_gradients(ops, M, K, dtype):
     _check_norm(ops, *_norm_case(M, K, dtype, True, True), wide=M == 7)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K", [(3, 4088), (160, 4096), (3, 4095), (2, 4104), (2, 8192), (1, 8193)])
+def test_norm_where_the_kernels_change(ops, M, K, dtype):
+    """Rows of up to 4096, 8192 and 16384 columns run differently."""
+    _check_norm(ops, *_norm_case(M, K, dtype, True, True))
+
+
 @pytest.mark.parametrize("gated,scaled", [(False, True), (True, False), (False, False)])
 def test_norm_without_gate_or_scale(ops, gated, scaled):
     _check_norm(ops, *_norm_case(33, 200, torch.float32, gated, scaled))
