@@ -55,9 +55,10 @@ struct Shape {
 // Where a warp works: its channels d0 .. d0 + n - 1 of group g in sequence b.
 struct WarpPlace { int b, g, d0, n; };
 
-// SPL states of a channel that has N, from number n0 on.
-__device__ __forceinline__ void load_states(const float* p, int n0, int N, float v[4]) {
-    if (N % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+// Four states of a channel that has N, from number n0 on; `whole`: all channels' states lie on 16-byte boundaries and N is a multiple of 4.
+__device__ __forceinline__ bool whole_states(const float* p, int N) { return N % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+__device__ __forceinline__ void load_states(const float* p, int n0, int N, bool whole, float v[4]) {
+    if (whole) {
         const float4 x = n0 < N ? *reinterpret_cast<const float4*>(p + n0) : make_float4(0.f, 0.f, 0.f, 0.f);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
         return;
@@ -65,8 +66,8 @@ __device__ __forceinline__ void load_states(const float* p, int n0, int N, float
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = n0 + j < N ? p[n0 + j] : 0.0f;
 }
-__device__ __forceinline__ void store_states(float* p, int n0, int N, const float v[4]) {
-    if (N % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+__device__ __forceinline__ void store_states(float* p, int n0, int N, bool whole, const float v[4]) {
+    if (whole) {
         if (n0 < N) *reinterpret_cast<float4*>(p + n0) = make_float4(v[0], v[1], v[2], v[3]);
         return;
     }
@@ -75,22 +76,22 @@ __device__ __forceinline__ void store_states(float* p, int n0, int N, const floa
         if (n0 + j < N) p[n0 + j] = v[j];
 }
 // The same of two adjacent channels, as far as they exist, each pair of values one operand.
-__device__ __forceinline__ void load_states2(const float* p, int channels, int n0, int N, f32x2 v[4]) {
+__device__ __forceinline__ void load_states2(const float* p, int channels, int n0, int N, bool whole, f32x2 v[4]) {
     float x[2][4] = {};
-    if (channels > 0) load_states(p, n0, N, x[0]);
-    if (channels > 1) load_states(p + N, n0, N, x[1]);
+    if (channels > 0) load_states(p, n0, N, whole, x[0]);
+    if (channels > 1) load_states(p + N, n0, N, whole, x[1]);
 #pragma unroll
     for (int n = 0; n < 4; ++n) v[n] = pair(x[0][n], x[1][n]);
 }
-__device__ __forceinline__ void store_states2(float* p, int channels, int n0, int N, const f32x2 v[4]) {
+__device__ __forceinline__ void store_states2(float* p, int channels, int n0, int N, bool whole, const f32x2 v[4]) {
     const float lo[4] = {lo_of(v[0]), lo_of(v[1]), lo_of(v[2]), lo_of(v[3])}, hi[4] = {hi_of(v[0]), hi_of(v[1]), hi_of(v[2]), hi_of(v[3])};
-    if (channels > 0) store_states(p, n0, N, lo);
-    if (channels > 1) store_states(p + N, n0, N, hi);
+    if (channels > 0) store_states(p, n0, N, whole, lo);
+    if (channels > 1) store_states(p + N, n0, N, whole, hi);
 }
 // The four values of lane group sg as operands for two channels, from token t of a tile's b or c.
-template <int TOKENS, int QN> __device__ __forceinline__ void load_twice(const float4 (&m)[2][TOKENS][QN], int t, int sg, f32x2 v[4]) {
-    const float4 x = m[0][t][sg], y = m[1][t][sg];
-    v[0] = pair(x.x, x.y); v[1] = pair(x.z, x.w); v[2] = pair(y.x, y.y); v[3] = pair(y.z, y.w);
+template <int TOKENS, int QN> __device__ __forceinline__ void load_twice(const float4 (&m)[TOKENS][QN], int t, int sg, f32x2 v[4]) {
+    const float4 x = m[t][sg];
+    v[0] = both(x.x); v[1] = both(x.y); v[2] = both(x.z); v[3] = both(x.w);
 }
 __device__ __forceinline__ f32x2 decay_of(f32x2 A, f32x2 delta) {         // A is already times log2(e)
     const f32x2 x = fma2(A, delta, both(DECAY_SHIFT));
@@ -126,8 +127,8 @@ struct Tile {
     // Of channels 2 i, 2 i + 1: delta, delta, delta u, delta u.  Even i lie before odd ones, 64 bytes apart modulo the banks: neither a
     // quad's two stores nor the loads meet a bank twice.
     float4 steps[2][TILE * S::CW / 4 + 4];
-    // Of states 2 i, 2 i + 1, each value twice: an operand for two channels.  Even i before odd ones too.
-    float4 b[2][TILE][S::NS / 4], c[2][TILE][S::NS / 4];
+    // Each value once: in shared memory twice, as operands for two channels, they save moves but cost wavefronts (256 us forward, 893 backward; so 245 and 871).
+    float4 b[TILE][S::NS / 4], c[TILE][S::NS / 4];
     // C h of a lane's states; the lane that writes y adds them.  The rows are 16 floats longer than they need: its vector reads then meet no
     // bank twice.
     float y[TILE][S::SG * S::CW + 16];
@@ -208,12 +209,10 @@ struct ScanInputs {
             for (int i = 0; i < BCS; ++i) {
                 const int q = lane + 32 * i, r = q / (S::NS / 4), n = q % (S::NS / 4);
                 const float4 bv = widen<T>(b_next[i]);
-                tile.b[0][r][n] = make_float4(bv.x, bv.x, bv.y, bv.y);
-                tile.b[1][r][n] = make_float4(bv.z, bv.z, bv.w, bv.w);
+                tile.b[r][n] = bv;
                 if (!LOCAL) {
                     const float4 cv = widen<T>(c_next[i]);
-                    tile.c[0][r][n] = make_float4(cv.x, cv.x, cv.y, cv.y);
-                    tile.c[1][r][n] = make_float4(cv.z, cv.z, cv.w, cv.w);
+                    tile.c[r][n] = cv;
                 }
             }
         };
@@ -302,29 +301,30 @@ selective_scan_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bo
     const int d0 = p.d0 + 2 * cg, channels = p.n - 2 * cg;    // the lane's: d0, d0 + 1, as far as they exist
     f32x2 A[4], h[4];                                         // the two channels' values
     float dsum[2] = {};
-    load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, A);
+    load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, whole_states(a.A, N), A);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         A[n] = mul2(A[n], both(LOG2E));
         h[n] = both(0.0f);
     }
     if (!LOCAL) {
-        if (a.initial_state) load_states2(a.initial_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, h);
+        if (a.initial_state) load_states2(a.initial_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, whole_states(a.initial_state, N), h);
         for (int j = 0; j < chunk; ++j) {                     // the chunks before this one, each a state of its own and a decay
             const long long at = ((long long)p.b * split.chunks + j) * a.channels + d0;
             f32x2 own[4];
-            load_states2(split.states + at * N, channels, sg * 4, N, own);
+            load_states2(split.states + at * N, channels, sg * 4, N, whole_states(split.states, N), own);
             const f32x2 delta = pair(channels > 0 ? split.deltas[at] : 0.0f, channels > 1 ? split.deltas[at + 1] : 0.0f);
 #pragma unroll
             for (int n = 0; n < 4; ++n) h[n] = fma2(decay_of(A[n], delta), h[n], own[n]);
         }
     }
     const int kept = (a.length + KEEP - 1) / KEEP;
+    const bool whole_kept = whole_states(a.checkpoints, N);
     int k = 0;
     for (int t0 = begin; t0 < stop; t0 += TILE, ++k) {
         Tile<S>& tile = tiles[k & 1];
         float* keep = !LOCAL && a.checkpoints ? a.checkpoints + (((long long)p.b * kept + t0 / KEEP) * a.channels + d0) * N : nullptr;
-        if (keep) store_states2(keep, channels, sg * 4, N, h);
+        if (keep) store_states2(keep, channels, sg * 4, N, whole_kept, h);
         couple_wait(barrier + 2 * (k & 1));
         // The tile's tokens in groups: while one group's states are formed, the exponentials of the next are on their way.  Tokens behind
         // the sequence's end have delta = B = C = 0 and leave the states as they are.
@@ -351,7 +351,7 @@ selective_scan_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bo
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
             if (g + 1 < GROUPS) prepare(g + 1, (g + 1) & 1);
-            if (g * GROUP == KEEP && keep && t0 + KEEP < stop) store_states2(keep + (long long)a.channels * N, channels, sg * 4, N, h);
+            if (g * GROUP == KEEP && keep && t0 + KEEP < stop) store_states2(keep + (long long)a.channels * N, channels, sg * 4, N, whole_kept, h);
 #pragma unroll
             for (int k = 0; k < GROUP; ++k) {
                 const int t = g * GROUP + k;
@@ -371,11 +371,11 @@ selective_scan_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bo
     }
     if (LOCAL) {
         const long long at = ((long long)p.b * split.chunks + chunk) * a.channels + d0;
-        store_states2(split.states + at * N, channels, sg * 4, N, h);
+        store_states2(split.states + at * N, channels, sg * 4, N, whole_states(split.states, N), h);
         if (sg == 0 && channels > 0) split.deltas[at] = dsum[0];
         if (sg == 0 && channels > 1) split.deltas[at + 1] = dsum[1];
     } else if (a.final_state && chunk == split.chunks - 1) {
-        store_states2(a.final_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, h);
+        store_states2(a.final_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, whole_states(a.final_state, N), h);
     }
 }
 
@@ -391,7 +391,7 @@ selective_scan_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bo
 template <typename S>
 struct BackTile {
     float4 steps[2][KEEP * S::CW / 4 + 4];            // as in Tile
-    float4 b[2][KEEP][S::NS / 4], c[2][KEEP][S::NS / 4];
+    float4 b[KEEP][S::NS / 4], c[KEEP][S::NS / 4];
     float dyg[KEEP][S::CW];
     float4 h[KEEP][2][32];                            // state before the token: a lane's [state 0, 1 or 2, 3][channel]; then the sums [3][SG][CW]
     float bc[2][KEEP][2][S::NS];                      // dB and dC of the warp's channels, of two tiles
@@ -471,25 +471,25 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     const int d0 = p.d0 + 2 * cg, channels = p.n - 2 * cg;
     f32x2 A[4], adj[4], h[4], dA[4];                          // adj: gradient of the state before the token in hand
     float dsum[2] = {};
-    load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, A);
+    load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, whole_states(a.A, N), A);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         A[n] = mul2(A[n], both(LOG2E));
         adj[n] = dA[n] = both(0.0f);
     }
     if (!LOCAL) {
-        if (a.d_final_state) load_states2(a.d_final_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, adj);
+        if (a.d_final_state) load_states2(a.d_final_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, whole_states(a.d_final_state, N), adj);
         for (int j = split.chunks - 1; j > chunk; --j) {
             const long long at = ((long long)p.b * split.chunks + j) * a.channels + d0;
             f32x2 own[4];
-            load_states2(split.states + at * N, channels, sg * 4, N, own);
+            load_states2(split.states + at * N, channels, sg * 4, N, whole_states(split.states, N), own);
             const f32x2 delta = pair(channels > 0 ? split.deltas[at] : 0.0f, channels > 1 ? split.deltas[at + 1] : 0.0f);
 #pragma unroll
             for (int n = 0; n < 4; ++n) adj[n] = fma2(decay_of(A[n], delta), adj[n], own[n]);
         }
     }
     const int quad = lane % S::QUADS * 4, row = lane / S::QUADS, valid = p.n - quad;
-    float dD[4] = {}, dbias[4] = {};
+    f32x2 dD[2] = {both(0.0f), both(0.0f)}, dbias[2] = {both(0.0f), both(0.0f)};
     if (row == 0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -515,8 +515,9 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
         if (n < N && t < end) bc[m * bc_all + (long long)t * a.groups * N + n] = v;
     };
 
-    Quad<T> u[PAIRS], z[PAIRS], dy[PAIRS], u_next[PAIRS], dt_next[PAIRS], z_next[PAIRS], dy_next[PAIRS], b_next[BCS], c_next[BCS];
+    Quad<T> u[PAIRS], u_next[PAIRS], dt_next[PAIRS], z_next[PAIRS], dy_next[PAIRS], b_next[BCS], c_next[BCS];
     const int kept = (a.length + KEEP - 1) / KEEP;
+    const bool whole_kept = whole_states(a.checkpoints, N);
     auto fetch = [&](int t0) {                                // a tile's inputs; zeros behind the sequence's end
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
@@ -549,17 +550,18 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            float skip = j & 1 ? hi_of(dD[j / 2]) : lo_of(dD[j / 2]), step = j & 1 ? hi_of(dbias[j / 2]) : lo_of(dbias[j / 2]);
 #pragma unroll
             for (int o = S::QUADS; o < 32; o <<= 1) {         // over the rows
-                dD[j] += __shfl_xor_sync(0xffffffffu, dD[j], o);
-                dbias[j] += __shfl_xor_sync(0xffffffffu, dbias[j], o);
+                skip += __shfl_xor_sync(0xffffffffu, skip, o);
+                step += __shfl_xor_sync(0xffffffffu, step, o);
             }
             if (row == 0 && j < valid) {
-                put(p.d0 + quad + j, N, dD[j]);
-                put(p.d0 + quad + j, N + 1, dbias[j]);
+                put(p.d0 + quad + j, N, skip);
+                put(p.d0 + quad + j, N + 1, step);
             }
-            dD[j] = dbias[j] = 0.0f;
         }
+        dD[0] = dD[1] = dbias[0] = dbias[1] = both(0.0f);
     };
     const int n_tiles = stop > begin ? (stop - begin + KEEP - 1) / KEEP : 0;
     if (!LOCAL) {                                             // padding
@@ -576,44 +578,46 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     for (int k = n_tiles - 1; k >= 0; --k) {
         const int t0 = begin + k * KEEP;
         // on its way while the steps are formed: one tile ahead it would take registers from the walk over the tokens
-        if (!LOCAL) load_states2(a.checkpoints + (((long long)p.b * kept + t0 / KEEP) * a.channels + d0) * N, channels, sg * 4, N, h);
+        if (!LOCAL) load_states2(a.checkpoints + (((long long)p.b * kept + t0 / KEEP) * a.channels + d0) * N, channels, sg * 4, N, whole_kept, h);
         __syncwarp();                                         // the last tile has been read
-        float raw_sig[PAIRS][4];
+        f32x2 raw_sig[PAIRS][2], dz_of[PAIRS][2];             // what ddelta and the ungated y are multiplied by for ddt and dz
         const float4 bias = *reinterpret_cast<const float4*>(&tile.bias[quad]);
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
             const int r = row + i * ROWS;
             if (!LOCAL) u[i] = u_next[i];
-            if (zp) z[i] = z_next[i];
-            dy[i] = dy_next[i];
-            const float4 uv = LOCAL ? make_float4(0.f, 0.f, 0.f, 0.f) : widen<T>(u[i]), dv = widen<T>(dt_next[i]), yv = widen<T>(dy[i]);
-            const float raw[4] = {dv.x + bias.x, dv.y + bias.y, dv.z + bias.z, dv.w + bias.w};
-            float g[4] = {yv.x, yv.y, yv.z, yv.w}, delta[4];
+            const float4 uv = LOCAL ? make_float4(0.f, 0.f, 0.f, 0.f) : widen<T>(u[i]), dv = widen<T>(dt_next[i]), yv = widen<T>(dy_next[i]);
+            const f32x2 raw[2] = {add2(pair(dv.x, dv.y), pair(bias.x, bias.y)), add2(pair(dv.z, dv.w), pair(bias.z, bias.w))};
+            f32x2 g[2] = {pair(yv.x, yv.y), pair(yv.z, yv.w)}, delta[2] = {raw[0], raw[1]};
+            raw_sig[i][0] = raw_sig[i][1] = both(1.0f);
             if (a.softplus) {
-                float e[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    e[j] = exp_minus_abs(raw[j]);
-                    raw_sig[i][j] = sigmoid_of(raw[j], e[j]);
+                for (int j = 0; j < 2; ++j) {
+                    const float e0 = exp_minus_abs(lo_of(raw[j])), e1 = exp_minus_abs(hi_of(raw[j]));
+                    raw_sig[i][j] = pair(sigmoid_of(lo_of(raw[j]), e0), sigmoid_of(hi_of(raw[j]), e1));
+                    delta[j] = softplus2(lo_of(raw[j]), hi_of(raw[j]), e0, e1);
                 }
-                const f32x2 s0 = softplus2(raw[0], raw[1], e[0], e[1]), s1 = softplus2(raw[2], raw[3], e[2], e[3]);
-                delta[0] = lo_of(s0); delta[1] = hi_of(s0); delta[2] = lo_of(s1); delta[3] = hi_of(s1);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { delta[j] = raw[j]; raw_sig[i][j] = 1.0f; }
             }
             if (zp) {
-                const float4 zv = widen<T>(z[i]);
-                g[0] *= zv.x * sigmoid(zv.x); g[1] *= zv.y * sigmoid(zv.y); g[2] *= zv.z * sigmoid(zv.z); g[3] *= zv.w * sigmoid(zv.w);
+                const float4 zv = widen<T>(z_next[i]);
+                const f32x2 zz[2] = {pair(zv.x, zv.y), pair(zv.z, zv.w)};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const f32x2 s = sigmoid2(zz[j]);
+                    dz_of[i][j] = mul2(g[j], silu_slope2(zz[j], s));
+                    g[j] = mul2(g[j], mul2(zz[j], s));
+                }
             }
             const uint32_t live = t0 + r < stop ? 0xffffffffu : 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) delta[j] = __uint_as_float(__float_as_uint(delta[j]) & live);
             if (FULL || r < KEEP) {
                 const int at = r * S::QUADS + quad / 4;
-                tile.steps[0][at] = make_float4(delta[0], delta[1], __fmul_rn(delta[0], uv.x), __fmul_rn(delta[1], uv.y));
-                tile.steps[1][at] = make_float4(delta[2], delta[3], __fmul_rn(delta[2], uv.z), __fmul_rn(delta[3], uv.w));
-                *reinterpret_cast<float4*>(&tile.dyg[r][quad]) = make_float4(g[0], g[1], g[2], g[3]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    delta[j] = pair(__uint_as_float(__float_as_uint(lo_of(delta[j])) & live), __uint_as_float(__float_as_uint(hi_of(delta[j])) & live));
+                    const f32x2 d_u = mul2(delta[j], j ? pair(uv.z, uv.w) : pair(uv.x, uv.y));
+                    tile.steps[j][at] = make_float4(lo_of(delta[j]), hi_of(delta[j]), lo_of(d_u), hi_of(d_u));
+                }
+                *reinterpret_cast<float4*>(&tile.dyg[r][quad]) = make_float4(lo_of(g[0]), hi_of(g[0]), lo_of(g[1]), hi_of(g[1]));
             }
         }
 #pragma unroll
@@ -622,17 +626,15 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             if (BCQ % 32 != 0 && q >= BCQ) continue;
             if (!LOCAL) {
                 const float4 bv = widen<T>(b_next[i]);
-                tile.b[0][r][n] = make_float4(bv.x, bv.x, bv.y, bv.y);
-                tile.b[1][r][n] = make_float4(bv.z, bv.z, bv.w, bv.w);
+                tile.b[r][n] = bv;
             }
             const float4 cv = widen<T>(c_next[i]);
-            tile.c[0][r][n] = make_float4(cv.x, cv.x, cv.y, cv.y);
-            tile.c[1][r][n] = make_float4(cv.z, cv.z, cv.w, cv.w);
+            tile.c[r][n] = cv;
         }
         __syncwarp();
         if (k > 0) fetch(t0 - KEEP);
         if (!LOCAL) {                                         // the tile's states
-#pragma unroll 2                                              // all eight: 962 us instead of 912, for registers
+#pragma unroll 4                                              // 4 x 1024 x 8192: two 924 us, four 893, eight 933 (registers)
             for (int t = 0; t < KEEP; ++t) {
                 tile.h[t][0][lane] = make_float4(lo_of(h[0]), hi_of(h[0]), lo_of(h[1]), hi_of(h[1]));
                 tile.h[t][1][lane] = make_float4(lo_of(h[2]), hi_of(h[2]), lo_of(h[3]), hi_of(h[3]));
@@ -643,7 +645,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
                 for (int n = 0; n < 4; ++n) h[n] = fma2(decay_of(A[n], pair(s.x, s.y)), h[n], mul2(pair(s.z, s.w), B[n]));
             }
         }
-#pragma unroll 2
+#pragma unroll 4
         for (int t = KEEP - 1; t >= 0; --t) {
             f32x2 C[4], g[4];
             load_twice(tile.c, t, sg, C);
@@ -696,60 +698,53 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
         for (int i = 0; i < PAIRS; ++i) {
             const int r = row + i * ROWS, t = t0 + r;
             const float* in = reinterpret_cast<const float*>(tile.h[r % KEEP]) + quad;
-            float sum[3][4] = {};
+            f32x2 sum[3][2];
 #pragma unroll
-            for (int q = 0; q < 3; ++q)
+            for (int q = 0; q < 3; ++q) {
+                sum[q][0] = sum[q][1] = both(0.0f);
 #pragma unroll
                 for (int s = 0; s < S::SG; ++s) {             // odd rows start with the other half of the banks
                     const float4 v = *reinterpret_cast<const float4*>(in + q * S::SG * S::CW + (s ^ (r & 1)) * S::CW);
-                    sum[q][0] += v.x; sum[q][1] += v.y; sum[q][2] += v.z; sum[q][3] += v.w;
+                    sum[q][0] = add2(sum[q][0], pair(v.x, v.y));
+                    sum[q][1] = add2(sum[q][1], pair(v.z, v.w));
                 }
-            const float4 uv = widen<T>(u[i]), yv = widen<T>(dy[i]);
-            const float uu[4] = {uv.x, uv.y, uv.z, uv.w}, dd[4] = {yv.x, yv.y, yv.z, yv.w};
-            float zz[4] = {};
-            if (zp) {
-                const float4 zv = widen<T>(z[i]);
-                zz[0] = zv.x; zz[1] = zv.y; zz[2] = zv.z; zz[3] = zv.w;
             }
-            const float2 d01 = *reinterpret_cast<const float2*>(&tile.steps[0][r % KEEP * S::QUADS + quad / 4]);
-            const float2 d23 = *reinterpret_cast<const float2*>(&tile.steps[1][r % KEEP * S::QUADS + quad / 4]);
-            const float delta[4] = {d01.x, d01.y, d23.x, d23.y};
+            const float4 uv = widen<T>(u[i]), gv = *reinterpret_cast<const float4*>(&tile.dyg[r % KEEP][quad]);
             const float4 Dv = *reinterpret_cast<const float4*>(&tile.D[quad]);
-            const float D[4] = {Dv.x, Dv.y, Dv.z, Dv.w};
-            float o_u[4], o_t[4], o_z[4];
+            float4 o_u, o_t, o_z;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float dyg = dd[j];
-                if (zp) {
-                    const float s = sigmoid(zz[j]);
-                    dyg *= zz[j] * s;
-                    o_z[j] = dd[j] * __fmaf_rn(D[j], uu[j], sum[0][j]) * silu_slope(zz[j], s);
-                }
-                o_u[j] = __fmaf_rn(D[j], dyg, delta[j] * sum[1][j]);
-                o_t[j] = __fmaf_rn(sum[2][j], LN2, uu[j] * sum[1][j]) * raw_sig[i][j];       // A was times log2(e)
-                if (FULL || r < KEEP) {
-                    dD[j] = __fmaf_rn(dyg, uu[j], dD[j]);
-                    dbias[j] += t < stop ? o_t[j] : 0.0f;
+            for (int j = 0; j < 2; ++j) {
+                const float2 dl = *reinterpret_cast<const float2*>(&tile.steps[j][r % KEEP * S::QUADS + quad / 4]);
+                const f32x2 uu = j ? pair(uv.z, uv.w) : pair(uv.x, uv.y), dyg = j ? pair(gv.z, gv.w) : pair(gv.x, gv.y), D = j ? pair(Dv.z, Dv.w) : pair(Dv.x, Dv.y);
+                const f32x2 ou = fma2(D, dyg, mul2(pair(dl.x, dl.y), sum[1][j]));
+                const f32x2 ot = mul2(fma2(sum[2][j], both(LN2), mul2(uu, sum[1][j])), raw_sig[i][j]);       // A was times log2(e)
+                const f32x2 oz = zp ? mul2(dz_of[i][j], fma2(D, uu, sum[0][j])) : both(0.0f);
+                (j ? o_u.z : o_u.x) = lo_of(ou); (j ? o_u.w : o_u.y) = hi_of(ou);
+                (j ? o_t.z : o_t.x) = lo_of(ot); (j ? o_t.w : o_t.y) = hi_of(ot);
+                (j ? o_z.z : o_z.x) = lo_of(oz); (j ? o_z.w : o_z.y) = hi_of(oz);
+                if ((FULL || r < KEEP) && t < stop) {
+                    dD[j] = fma2(dyg, uu, dD[j]);
+                    dbias[j] = add2(dbias[j], ot);
                 }
             }
             if ((FULL || r < KEEP) && t < end) {
-                const bool on = t < stop;
                 const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (du) store_quad<T>(du + (long long)t * a.channels, valid, aligned, on ? make_float4(o_u[0], o_u[1], o_u[2], o_u[3]) : zero);
-                if (ddt) store_quad<T>(ddt + (long long)t * a.channels, valid, aligned, on ? make_float4(o_t[0], o_t[1], o_t[2], o_t[3]) : zero);
-                if (dz) store_quad<T>(dz + (long long)t * a.channels, valid, aligned, on ? make_float4(o_z[0], o_z[1], o_z[2], o_z[3]) : zero);
+                const bool on = t < stop;
+                if (du) store_quad<T>(du + (long long)t * a.channels, valid, aligned, on ? o_u : zero);
+                if (ddt) store_quad<T>(ddt + (long long)t * a.channels, valid, aligned, on ? o_t : zero);
+                if (dz) store_quad<T>(dz + (long long)t * a.channels, valid, aligned, on ? o_z : zero);
             }
         }
         if (k % FLUSH == 0) flush(k / FLUSH == (n_tiles - 1) / FLUSH);
     }
     if (LOCAL) {
         const long long at = ((long long)p.b * split.chunks + chunk) * a.channels + d0;
-        store_states2(split.states + at * N, channels, sg * 4, N, adj);
+        store_states2(split.states + at * N, channels, sg * 4, N, whole_states(split.states, N), adj);
         if (sg == 0 && channels > 0) split.deltas[at] = dsum[0];
         if (sg == 0 && channels > 1) split.deltas[at + 1] = dsum[1];
         return;
     }
-    if (a.d_initial_state && chunk == 0) store_states2(a.d_initial_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, adj);
+    if (a.d_initial_state && chunk == 0) store_states2(a.d_initial_state + ((long long)p.b * a.channels + d0) * N, channels, sg * 4, N, whole_states(a.d_initial_state, N), adj);
     if (n_tiles == 0) flush(true);
 }
 
@@ -798,15 +793,16 @@ selective_scan_step_kernel(const el_scan_t a, int share) {
     const bool aligned_bc = N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C)) % (4 * sizeof(T)) == 0 &&
                             (a.B_stride_b | a.B_stride_g | a.C_stride_b | a.C_stride_g) % 4 == 0;
     float A[4];
-    load_states(a.A + (long long)dc * N, n0, N, A);
+    load_states(a.A + (long long)dc * N, n0, N, whole_states(a.A, N), A);
     const float bias = a.dt_bias ? a.dt_bias[dc] : 0.0f, D = a.D ? a.D[dc] : 0.0f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) A[n] *= LOG2E;
+    const bool whole = whole_states(a.initial_state, N) && whole_states(a.final_state, N);
     // The next sequence's inputs are fetched ahead: the compiler itself cannot move loads of a state before the stores of another one.  64 sequences of
     // 8192 channels: 25.6 -> 20.5 us; two ahead 20.8.
     struct Inputs { float h[4]; T u, dt, z; Quad<T> B, C; };
     auto fetch = [&](int b, Inputs& in) {
-        load_states(a.initial_state + ((long long)b * a.channels + dc) * N, n0, N, in.h);
+        load_states(a.initial_state + ((long long)b * a.channels + dc) * N, n0, N, whole, in.h);
         in.u = static_cast<const T*>(a.u)[b * a.u_stride_b + dc];
         in.dt = static_cast<const T*>(a.dt)[b * a.dt_stride_b + dc];
         in.z = a.z ? static_cast<const T*>(a.z)[b * a.z_stride_b + dc] : T(0.0f);
@@ -829,7 +825,7 @@ selective_scan_step_kernel(const el_scan_t a, int share) {
             h[n] = __fmaf_rn(ex2(__fmaf_rn(A[n], delta, DECAY_SHIFT)), now.h[n], du * Bv[n]);
             y = __fmaf_rn(Cv[n], h[n], y);
         }
-        if (real) store_states(a.final_state + at, n0, N, h);
+        if (real) store_states(a.final_state + at, n0, N, whole, h);
 #pragma unroll
         for (int o = 1; o < LANES; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
         if (real && lane == 0) {
