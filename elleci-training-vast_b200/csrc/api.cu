@@ -690,7 +690,7 @@ int el_selective_scan(const el_scan_t* a, el_stream_t stream) {
     const size_t need = selective_scan_workspace_bytes(*a);
     if (!a->A || (a->length > 0 && (!a->u || !a->dt || !a->B || !a->C || !a->y)) || (need > 0 && !a->workspace)) return EL_ERR_NULL_PTR;
     if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
-    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(a->checkpoints) % 16 != 0) return EL_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
     return launch_selective_scan(*a, (cudaStream_t)stream);
 }
 
@@ -703,7 +703,7 @@ int el_selective_scan_backward(const el_scan_t* a, el_stream_t stream) {
     if (!a->A || (a->length > 0 && a->batch > 0 && (!a->u || !a->dt || !a->B || !a->C || !a->checkpoints)) || (need > 0 && !a->workspace))
         return EL_ERR_NULL_PTR;
     if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
-    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(a->checkpoints) % 16 != 0) return EL_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
     return launch_selective_scan_backward(*a, (cudaStream_t)stream);
 }
 

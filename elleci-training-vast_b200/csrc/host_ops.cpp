@@ -886,7 +886,7 @@ PyObject* selective_scan_backward(PyObject* const* a) {
     if (want & 8) dB = new_empty(u, k.shared, io);
     if (want & 16) dC = new_empty(u, k.shared, io);
     if (want & 32) dD = new_empty(u, {k.D}, at::kFloat);
-    if ((want & 64) && c.z) dz = new_empty(u, u.sizes(), io);
+    if ((want & 64) && !is_none(a[6])) dz = new_empty(u, u.sizes(), io);
     if (want & 128) dbias = new_empty(u, {k.D}, at::kFloat);
     if (want & 256) d_first = new_empty(u, {k.B, k.D, k.N}, at::kFloat);
     c.checkpoints = ptr<float>(kept);
@@ -1004,8 +1004,8 @@ PyObject* block_norm_backward(PyObject* const* a) {
     if (!is_none(a[9])) dn = norm_rows(a[9], "dnormed", shaped);
     Tensor dh = new_empty(h, shaped.sizes(), h.scalar_type()), dy = new_empty(h, shaped.sizes(), h.scalar_type()), dg, ds;
     Tensor dw1 = new_empty(h, {K}, at::kFloat), dw2 = new_empty(h, {K}, at::kFloat);
-    if (c.gate) dg = new_empty(h, shaped.sizes(), h.scalar_type());
-    if (c.scale) ds = new_empty(h, {K}, at::kFloat);
+    if (k.g.t.defined()) dg = new_empty(h, shaped.sizes(), h.scalar_type());
+    if (k.scale.defined()) ds = new_empty(h, {K}, at::kFloat);
     c.rstd = ptr<float>(rstd);
     if (dh_out.t.defined()) {
         c.dh_out = ptr(dh_out.t);

@@ -15,7 +15,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 // checked base, strides and that V divides the row).  Otherwise every STRIDE-th one by itself, STRIDE the number of threads side by side,
 // so that neighbouring threads still read neighbouring values; `valid` is the distance from the first to the row's end, zeros behind it.
 // Held as 32-bit words: registers, whatever T is.
-template <typename T, int V> struct Vec { uint32_t w[V * sizeof(T) / 4]; };
+template <typename T, int V> struct alignas(V * sizeof(T) < 16 ? 8 : 16) Vec { uint32_t w[V * sizeof(T) / 4]; };
 template <typename T> __device__ __forceinline__ uint32_t bits_of(T v) {
     if constexpr (sizeof(T) == 4) return __float_as_uint(v);
     else return *reinterpret_cast<const unsigned short*>(&v);

@@ -866,7 +866,7 @@ static ScanSplit scan_split(const el_scan_t& a, long long warps, int slots, int 
     int sms = 148;
     device_sm_count(&sms);
     ScanSplit s = {1, a.length > 0 ? a.length : 1, states, nullptr};
-    if (warps < (long long)enough * sms) {
+    if (warps > 0 && warps < (long long)enough * sms) {
         long long chunks = (long long)slots * sms / warps;
         if (chunks > 32) chunks = 32;                         // a chunk's first warps go through those before it one by one
         if (chunks > a.length / 64) chunks = a.length / 64;

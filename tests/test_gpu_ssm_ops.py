@@ -443,6 +443,42 @@ def test_operators_can_be_recorded_in_a_graph(ops, name):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("name", ["conv", "scan", "norm"])
+def test_each_gradient_alone_is_the_one_of_all(ops, name):
+    """Whatever else needs no gradient, and whichever output has one."""
+    call, t, douts = _three(ops)[name]
+    douts = [d.to(DEV) for d in douts]
+    gpu = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    whole = dict(zip(gpu, torch.autograd.grad(call(**gpu), list(gpu.values()), douts)))
+    for k in gpu:
+        alone = {j: v.detach() for j, v in gpu.items()}
+        alone[k].requires_grad_(True)
+        outs = call(**alone)
+        assert torch.equal(torch.autograd.grad(outs, alone[k], douts, retain_graph=True)[0], whole[k]), k
+        parts = [torch.autograd.grad(o, alone[k], d, retain_graph=True, allow_unused=True)[0] for o, d in zip(outs, douts)]
+        total = sum(p.double() for p in parts if p is not None)
+        assert float((total - whole[k].double()).norm()) <= 1e-5 * float(sum(p.double().norm() for p in parts if p is not None)) + 1e-30, k
+
+
+@pytest.mark.parametrize("name", ["conv", "scan", "norm"])
+def test_no_sequences_at_all(ops, name):
+    call, t, douts = _three(ops)[name]
+    lead = {"conv": ("x", "initial_state"), "scan": ("u", "dt", "B", "C", "z", "initial_state"), "norm": ("h", "y", "gate")}[name]
+    gpu = {k: (v[:0] if k in lead else v).to(DEV).requires_grad_(True) for k, v in t.items()}
+    outs = call(**gpu)
+    assert all(o.numel() == 0 for o in outs)
+    for k, g in zip(gpu, torch.autograd.grad(outs, list(gpu.values()), [d[:0].to(DEV) for d in douts])):
+        assert g.shape == gpu[k].shape and not g.any(), k
+
+
+def test_second_derivatives_are_refused(ops):
+    call, t, douts = _three(ops)["norm"]
+    gpu = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    g = torch.autograd.grad(call(**gpu), gpu["h"], [d.to(DEV) for d in douts], create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_offsets_beyond_32_bits(ops):
     """Windows of a tensor whose last rows lie more than 2^31 elements behind the first."""
     L, pitch, D = 140000, 16384, 32
