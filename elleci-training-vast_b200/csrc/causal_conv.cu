@@ -4,7 +4,9 @@
 //   dpre = dy * slope(pre),  dx[t] = sum_i w[W-1-i] dpre[t + i],  dw[j] = sum_t dpre[t] x[t - (W-1) + j],  dbias = sum_t dpre[t]
 //
 // A thread owns a vector of channels and walks over a strip of tokens with the last W-1 inputs (backward: and W dpre) in registers, so
-// every input is read once but for the W-1 tokens at a strip's ends.  Bound: memory, one read and one write per value (backward two and one).
+// every input is read once but for the W-1 tokens at a strip's ends.  Floor: memory, one read and one write per value
+// (backward two and one).  4 x 1024 tokens of 8192 channels: forward 33 us in bfloat16 (floor 20), 48 in float32 (41); backward 68 (31) and 83 (61): the
+// 16-bit types are bound by instructions and latencies, not by bytes.
 #include "mamba_common.cuh"
 
 namespace el {

@@ -111,7 +111,7 @@ template <typename T> __device__ __forceinline__ rowio::Quad<T> fetch_quad(const
     if (aligned) {
         q.a = *reinterpret_cast<const decltype(q.a)*>(p);
     } else {
-        T v[4];
+        alignas(16) T v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = j < valid ? p[j] : T(0.0f);
         q = *reinterpret_cast<const rowio::Quad<T>*>(v);
@@ -168,7 +168,6 @@ __device__ __forceinline__ float sigmoid_of(float x, float e) {
     return x < 0.0f ? __fmul_rn(e, r) : r;
 }
 // d/dx of x sigmoid(x), from s = sigmoid(x)
-__device__ __forceinline__ float silu_slope(float x, float s) { return __fmul_rn(s, __fmaf_rn(x, 1.0f - s, 1.0f)); }
 __device__ __forceinline__ rowio::f32x2 silu_slope2(rowio::f32x2 x, rowio::f32x2 s) {
     using namespace rowio;
     return mul2(s, fma2(x, fma2(s, both(-1.0f), both(1.0f)), both(1.0f)));
