@@ -9,6 +9,7 @@
 // No state of its own but the handles that set_hooks hands over: the status word of each device, the function that turns a status
 // into an exception and the one that checks the device's status word.  Scratch that a call needs and leaves is allocated per call.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -661,6 +662,13 @@ const Tensor& state_out_arg(PyObject* o, const Tensor& state) {
 void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// Forward-mode derivatives are not formed: a tangent would be lost without a word, so an argument that has one is refused.  (Where autograd records the
+// call, the same is refused behind it.)
+void no_tangent(const char* name, PyObject* const* a, std::initializer_list<int> tensors) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (int i : tensors)
+        if (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i])._fw_grad(0).defined()) raise(std::string(name) + " has no forward-mode derivative");
+}
 // a step has no gradient: called where one would be recorded, it refuses
 void no_gradient(const char* name, PyObject* const* a, std::initializer_list<int> tensors) {
     if (!c10::GradMode::is_enabled()) return;
@@ -708,6 +716,7 @@ void conv_call(ConvCall& k, PyObject* x_arg, PyObject* weight, PyObject* bias, b
 
 // causal_conv(x, weight, bias, silu, initial_state, lengths, final_state wanted) -> (y, final state or None)
 PyObject* causal_conv(PyObject* const* a) {
+    no_tangent("causal_conv", a, {0, 1, 2, 4});
     ConvCall k;
     conv_call(k, a[0], a[1], a[2], int_arg(a[3]) != 0, false);
     const Tensor& x = k.x;
@@ -727,6 +736,7 @@ PyObject* causal_conv(PyObject* const* a) {
 // causal_conv_backward(x, weight, bias, silu, initial_state, lengths, dy, d_final_state, wanted) -> (dx, dweight, dbias, d_initial_state),
 // `wanted`: bits 0 .. 3 in this order
 PyObject* causal_conv_backward(PyObject* const* a) {
+    no_tangent("causal_conv_backward", a, {0, 1, 2, 4, 6, 7});
     ConvCall k;
     conv_call(k, a[0], a[1], a[2], int_arg(a[3]) != 0, false);
     const Tensor& x = k.x;
@@ -761,6 +771,7 @@ PyObject* causal_conv_backward(PyObject* const* a) {
 // causal_conv_step(x, state, weight, bias, silu, state_out) -> y
 PyObject* causal_conv_step(PyObject* const* a) {
     no_gradient("causal_conv_step", a, {0, 1, 2, 3});
+    no_tangent("causal_conv_step", a, {0, 1, 2, 3});
     ConvCall k;
     conv_call(k, a[0], a[2], a[3], int_arg(a[4]) != 0, true);
     const Tensor& x = k.x;
@@ -843,6 +854,7 @@ void scan_call(ScanCall& k, PyObject* const* a, bool softplus, bool step) {
 // selective_scan(u, dt, A, B, C, D, z, dt_bias, softplus, initial_state, lengths, final_state wanted, checkpoints wanted)
 // -> (y, final state or None, checkpoints or None)
 PyObject* selective_scan(PyObject* const* a) {
+    no_tangent("selective_scan", a, {0, 1, 2, 3, 4, 5, 6, 7, 9});
     ScanCall k;
     scan_call(k, a, int_arg(a[8]) != 0, false);
     const Tensor& u = k.u;
@@ -867,6 +879,7 @@ PyObject* selective_scan(PyObject* const* a) {
 // selective_scan_backward(u, dt, A, B, C, D, z, dt_bias, softplus, initial_state, lengths, checkpoints, dy, d_final_state, wanted)
 // -> (du, ddt, dA, dB, dC, dD, dz, ddt_bias, d_initial_state), `wanted`: bits 0 .. 8 in this order
 PyObject* selective_scan_backward(PyObject* const* a) {
+    no_tangent("selective_scan_backward", a, {0, 1, 2, 3, 4, 5, 6, 7, 9, 12, 13});
     ScanCall k;
     scan_call(k, a, int_arg(a[8]) != 0, false);
     const Tensor& u = k.u;
@@ -914,6 +927,7 @@ PyObject* selective_scan_backward(PyObject* const* a) {
 // selective_scan_step(u, dt, A, B, C, D, z, dt_bias, softplus, state, state_out) -> y
 PyObject* selective_scan_step(PyObject* const* a) {
     no_gradient("selective_scan_step", a, {0, 1, 2, 3, 4, 5, 6, 7, 9});
+    no_tangent("selective_scan_step", a, {0, 1, 2, 3, 4, 5, 6, 7, 9});
     ScanCall k;
     scan_call(k, a, int_arg(a[8]) != 0, true);
     const Tensor& u = k.u;
@@ -975,6 +989,7 @@ void norm_call(NormCall& k, PyObject* const* a) {
 
 // block_norm(h, y, post_weight, pre_weight, gate, scale, eps, rstd wanted) -> (h_out, normed, rstd or None)
 PyObject* block_norm(PyObject* const* a) {
+    no_tangent("block_norm", a, {0, 1, 2, 3, 4, 5});
     NormCall k;
     norm_call(k, a);
     const Tensor& h = k.h.t;
@@ -991,6 +1006,7 @@ PyObject* block_norm(PyObject* const* a) {
 
 // block_norm_backward(h, y, post_weight, pre_weight, gate, scale, eps, rstd, dh_out, dnormed) -> (dh, dy, dpost_weight, dpre_weight, dgate, dscale)
 PyObject* block_norm_backward(PyObject* const* a) {
+    no_tangent("block_norm_backward", a, {0, 1, 2, 3, 4, 5, 8, 9});
     NormCall k;
     norm_call(k, a);
     const Tensor& h = k.h.t;

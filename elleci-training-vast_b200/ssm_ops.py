@@ -8,7 +8,8 @@ The reference's block runs them as tensor operations (core/mamba/mamba2.py:136,1
 (include/elleci_int2.h) per direction, queued on the current CUDA stream.  Activations are float16, bfloat16 or float32, channel-last,
 all of one dtype; tensors whose channels are contiguous (slices of a wider projection) are read in place.  Parameters are float32, sums
 and states are held in float32, and every output is rounded once.  Gradients do not depend on the order in which blocks run: the same
-call gives the same bits.  `RuntimeError` on bad arguments.
+call gives the same bits.  Derivatives are reverse-mode ones of the first order; a tensor with a forward-mode tangent is refused.
+`RuntimeError` on bad arguments.
 
 `lengths` (int32 or int64 [batch]): sequence b has lengths[b] tokens and padding behind them.  Padding is not read (it may hold
 anything, NaN included), its outputs and gradients are zeros and it leaves the state as it is.
