@@ -68,6 +68,16 @@ class MambaBlockInt2(nn.Module):
         return MambaState(torch.zeros(batch, self.d_conv - 1, self.d_inner, dtype=dtype, device=device),
                           torch.zeros(batch, self.d_inner, self.d_state, device=device))
 
+    @staticmethod
+    def _before(state: Optional[MambaState]) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """The state's tensors for a forward pass that then overwrites them.  Where gradients are recorded the operators keep what they start from for
+        the backward pass, so they get copies."""
+        if state is None:
+            return None, None
+        if not torch.is_grad_enabled():
+            return state.conv, state.ssm
+        return state.conv.detach().clone(), state.ssm.detach().clone()
+
     def _selection(self, u: torch.Tensor):
         """(step sizes, B, C) of the convolved channels; B and C are windows of one projection's output, read in place."""
         p = self.x_proj(u)
@@ -80,18 +90,19 @@ class MambaBlockInt2(nn.Module):
 
     def forward(self, h: torch.Tensor, x: torch.Tensor, state: Optional[MambaState] = None,
                 lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """h, x [batch, length, d_model].  `state` (no gradient goes into it): the text goes on from it, and it becomes the state after each
-        sequence's last token.  `lengths` as in ssm_ops."""
+        """h, x [batch, length, d_model].  `state` (no gradient goes into it): the text goes on from it, and its tensors become the state after
+        each sequence's last token, in place; a backward pass after that is that of the piece that was given.  `lengths` as in ssm_ops."""
+        conv_before, ssm_before = self._before(state)
         xz = self.in_proj(x)
         u, z = xz[..., :self.d_inner], xz[..., self.d_inner:]
-        u = ssm_ops.causal_conv(u, self.conv_weight, self.conv_bias, initial_state=None if state is None else state.conv, lengths=lengths,
+        u = ssm_ops.causal_conv(u, self.conv_weight, self.conv_bias, initial_state=conv_before, lengths=lengths,
                                 return_final_state=state is not None)
         if state is not None:
             u, last = u
             state.conv.copy_(last.detach())
         dt, B, C = self._selection(u)
         y = ssm_ops.selective_scan(u, dt, -torch.exp(self.A_log), B, C, D=self.D, z=z, dt_bias=self.dt_bias,
-                                   initial_state=None if state is None else state.ssm, lengths=lengths, return_final_state=state is not None)
+                                   initial_state=ssm_before, lengths=lengths, return_final_state=state is not None)
         if state is not None:
             y, last = y
             state.ssm.copy_(last.detach())

@@ -69,3 +69,35 @@ def test_block_equals_its_definition(pkg, gated):
         _near(a, b, name, 0.02)
     for name in want:
         _near(got[name], want[name], name, 0.04)
+
+
+def _piecewise(pkg, block, h, x, state):
+    """The block's forward pass from its operators, the state's tensors replaced instead of written."""
+    ops, inner = pkg.ssm_ops, block.d_inner
+    xz = block.in_proj(x)
+    u, conv = ops.causal_conv(xz[..., :inner], block.conv_weight, block.conv_bias, initial_state=state[0], return_final_state=True)
+    dt, B, C = block._selection(u)
+    y, ssm = ops.selective_scan(u, dt, -torch.exp(block.A_log), B, C, D=block.D, z=xz[..., inner:], dt_bias=block.dt_bias, initial_state=state[1],
+                                return_final_state=True)
+    return block._join(h, y, x), (conv.detach(), ssm.detach())
+
+
+def test_training_on_a_text_in_pieces(pkg):
+    """Backward after each piece, the state going on from one to the next: the gradients are those of the operators on each piece, bit for bit."""
+    block = _block(pkg).train()
+    pkg.set_all_int2_lr(block, 0.0)
+    twin = copy.deepcopy(block)
+    h, x = _inputs(2, 75, 256)
+    g = torch.Generator().manual_seed(1)
+    grads = [torch.randn(2, 75, 256, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    state = block.new_state(2)
+    conv, ssm = state.conv, state.ssm
+    own = (conv.clone(), ssm.clone())
+    for a, b in ((0, 33), (33, 34), (34, 75)):
+        torch.autograd.backward(block(h[:, a:b], x[:, a:b], state), [v[:, a:b] for v in grads])
+        out, own = _piecewise(pkg, twin, h[:, a:b], x[:, a:b], own)
+        torch.autograd.backward(out, [v[:, a:b] for v in grads])
+        assert torch.equal(state.conv, own[0]) and torch.equal(state.ssm, own[1])
+        assert state.conv is conv and state.ssm is ssm, "the state's tensors are updated in place"
+    for (name, p), q in zip(block.named_parameters(), twin.parameters()):
+        assert (p.grad is None) == (q.grad is None) and (p.grad is None or torch.equal(p.grad, q.grad)), name
