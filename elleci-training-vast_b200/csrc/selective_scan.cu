@@ -99,6 +99,21 @@ __device__ __forceinline__ f32x2 decay_of(f32x2 A, f32x2 delta) {         // A i
     const f32x2 x = fma2(A, delta, both(DECAY_SHIFT));
     return pair(ex2(lo_of(x)), ex2(hi_of(x)));
 }
+// The state behind a chunk: h before it, decayed over the whole chunk, and what the chunk adds.  A token's decay may be far from 0 and infinity while
+// the product over a chunk is not: 0 times infinity would turn a state (or gradient) of zero into a NaN that token by token never arises.  So large
+// powers are applied in three steps, each of them finite; beyond 2^300 every state other than zero leaves float32 anyway.
+__device__ __forceinline__ f32x2 after_chunk(f32x2 A, f32x2 delta, f32x2 h, f32x2 own) {
+    const f32x2 x = fma2(A, delta, both(DECAY_SHIFT));
+    float f[2] = {lo_of(x), hi_of(x)}, g[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const bool far = fabsf(f[k]) > 120.0f;                // not a NaN, which stays one
+        f[k] = ex2(far ? fminf(fmaxf(f[k], -300.0f), 300.0f) * (1.0f / 3.0f) : f[k]);
+        g[k] = far ? f[k] : 1.0f;
+    }
+    const f32x2 rest = pair(g[0], g[1]);
+    return fma2(pair(f[0], f[1]), mul2(rest, mul2(rest, h)), own);
+}
 
 // A sequence in chunks: `states` [batch][chunks][channels][states] and `deltas` [batch][chunks][channels] take what each adds on its own.
 struct ScanSplit { int chunks, tokens; float* states; float* deltas; };
@@ -317,7 +332,7 @@ selective_scan_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bo
             load_states2(split.states + at * N, channels, sg * 4, N, whole_states(split.states, N), own);
             const f32x2 delta = pair(channels > 0 ? split.deltas[at] : 0.0f, channels > 1 ? split.deltas[at + 1] : 0.0f);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) h[n] = fma2(decay_of(A[n], delta), h[n], own[n]);
+            for (int n = 0; n < 4; ++n) h[n] = after_chunk(A[n], delta, h[n], own[n]);
         }
     }
     const int kept = (a.length + KEEP - 1) / KEEP;
@@ -487,7 +502,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             load_states2(split.states + at * N, channels, sg * 4, N, whole_states(split.states, N), own);
             const f32x2 delta = pair(channels > 0 ? split.deltas[at] : 0.0f, channels > 1 ? split.deltas[at + 1] : 0.0f);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) adj[n] = fma2(decay_of(A[n], delta), adj[n], own[n]);
+            for (int n = 0; n < 4; ++n) adj[n] = after_chunk(A[n], delta, adj[n], own[n]);
         }
     }
     const int quad = lane % S::QUADS * 4, row = lane / S::QUADS, valid = p.n - quad;

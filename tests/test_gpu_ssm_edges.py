@@ -35,3 +35,40 @@ def test_forward_mode_is_refused_where_gradients_are_recorded(ops, name):
         outs = call(**gpu)
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(outs, list(gpu.values()), [fwAD.make_dual(d, d) for d in douts])
+
+
+# ---- states that grow ---------------------------------------------------------------------------------------------------
+
+def _growing(L, u_from, dy_to):
+    """A state that grows by e^2 per token: e^160 over the 80 tokens of a chunk, which float32 does not hold.  Inputs that are zero before token
+    u_from and output gradients that are zero from token dy_to on keep everything that is formed token by token finite."""
+    t, _, dy, ds = _scan_case(1, L, 64, 16, 1, torch.float32, state=False, gated=False, bias=False)
+    t["A"] = 4.0 + 0.01 * t["A"]
+    t["dt"] = torch.full_like(t["dt"], 0.5)
+    t["u"][:, :u_from] = 0.0
+    dy[:, dy_to:] = 0.0
+    return t, dy
+
+
+def test_scan_of_growing_states_in_chunks_keeps_zeros(ops):
+    L = 2500
+    t, _ = _growing(L, L - 10, 0)
+    d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+    y, s = ops.selective_scan(**d, dt_softplus=False, return_final_state=True)
+    yr, sr = R.selective_scan(**{k: None if v is None else v.double() for k, v in t.items()}, softplus=False)
+    _close("y", y, yr, 4 * 10 + 16 + 16)                  # ten tokens have a state other than zero
+    _close("state", s, sr, 4 * 10 + 16)
+
+
+def test_scan_gradients_of_growing_states_in_chunks_keep_zeros(ops):
+    L = 2500
+    t, dy = _growing(L, L - 10, 10)
+    gpu, ref = _leaves(t)
+    y = ops.selective_scan(**gpu, dt_softplus=False)
+    yr, _ = R.selective_scan(**ref, softplus=False)
+    names = [k for k, v in gpu.items() if v is not None]
+    got = torch.autograd.grad(y, [gpu[k] for k in names], dy.to(DEV))
+    want = _reference_grads([yr], [ref[k] for k in names], [dy.double()])
+    for k, a, b in zip(names, got, want):
+        _close("d" + k, a, b, 8 * 10 + 2 * 16 + 32)
+    assert got[0][:, :10].any()
