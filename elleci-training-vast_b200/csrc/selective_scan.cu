@@ -709,7 +709,8 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < BACK_WARPS; ++w) v += reinterpret_cast<const float*>(tiles[w].bc[k & 1])[i];
-            store_bc(t0 + i / (2 * S::NS), i / S::NS & 1, i % S::NS, v);
+            const int t = t0 + i / (2 * S::NS);
+            store_bc(t, i / S::NS & 1, i % S::NS, t < stop ? v : 0.0f);      // of padding: zero times a state that may not be finite
         }
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {

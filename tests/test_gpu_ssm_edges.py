@@ -72,3 +72,29 @@ def test_scan_gradients_of_growing_states_in_chunks_keep_zeros(ops):
     for k, a, b in zip(names, got, want):
         _close("d" + k, a, b, 8 * 10 + 2 * 16 + 32)
     assert got[0][:, :10].any()
+
+
+# ---- padding ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("what", ["initial state", "final state's gradient", "token"])
+@pytest.mark.parametrize("N,G", [(16, 1), (12, 2), (64, 1)])
+def test_padding_has_zero_gradients_whatever_the_states_hold(ops, what, N, G):
+    """Lengths that end inside a tile; a state or a gradient that is not finite in a sequence that has padding."""
+    t, lengths, dy, ds = _scan_case(3, 21, 32, N, G, torch.float32)
+    lengths = torch.tensor([13, 21, 1])
+    for v in (t["u"], t["dt"], t["z"], t["B"], t["C"], dy):
+        _poison(v, lengths)
+    if what == "initial state":
+        t["initial_state"][0, 3], t["initial_state"][2, 5, 1] = INF, NAN
+    elif what == "token":
+        t["u"][0, 12, 3] = INF
+    else:
+        ds[0, 3, 2], ds[2, 5] = NAN, INF
+    gpu, _ = _leaves(t)
+    y, s = ops.selective_scan(**gpu, lengths=lengths.to(DEV), return_final_state=True)
+    names = ("u", "dt", "z", "B", "C")
+    for k, g in zip(names, torch.autograd.grad((y, s), [gpu[k] for k in names], (dy.to(DEV), ds.to(DEV)))):
+        for b, n in enumerate(lengths.tolist()):
+            assert not g[b, n:].any(), (k, b)              # a NaN is not zero either
+    for b, n in enumerate(lengths.tolist()):
+        assert not y[b, n:].any()
