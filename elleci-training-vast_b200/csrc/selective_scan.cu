@@ -98,7 +98,15 @@ template <int TOKENS, int QN> __device__ __forceinline__ void load_twice(const f
 __device__ __forceinline__ f32x2 decay_of(f32x2 A, f32x2 delta) {         // A is already times log2(e)
     const f32x2 x = fma2(A, delta, both(DECAY_SHIFT));
     return pair(ex2(lo_of(x)), ex2(hi_of(x)));
+}// Decay rates times log2(e).  Infinite ones (a state that forgets at once; A log2(e) may overflow too) become the largest finite value, which decays as
+// much for any step size above 1e-36: 0 times infinity would be NaN for the tokens behind a tile's last one, whose delta is 0 and which leave the
+// state as it is.
+__device__ __forceinline__ float rate_of(float A) {
+    const float x = __fmul_rn(A, LOG2E);
+    return isinf(x) ? copysignf(3.402823466e38f, x) : x;
 }
+__device__ __forceinline__ f32x2 rates_of(f32x2 A) { return pair(rate_of(lo_of(A)), rate_of(hi_of(A))); }
+
 // The state behind a chunk: h before it, decayed over the whole chunk, and what the chunk adds.  A token's decay may be far from 0 and infinity while
 // the product over a chunk is not: 0 times infinity would turn a state (or gradient) of zero into a NaN that token by token never arises.  So large
 // powers are applied in three steps, each of them finite; beyond 2^300 every state other than zero leaves float32 anyway.
@@ -321,7 +329,7 @@ selective_scan_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bo
     load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, whole_states(a.A, N), A);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        A[n] = mul2(A[n], both(LOG2E));
+        A[n] = rates_of(A[n]);
         h[n] = both(0.0f);
     }
     if (!LOCAL) {
@@ -491,7 +499,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     load_states2(a.A + (long long)d0 * N, channels, sg * 4, N, whole_states(a.A, N), A);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        A[n] = mul2(A[n], both(LOG2E));
+        A[n] = rates_of(A[n]);
         adj[n] = dA[n] = both(0.0f);
     }
     if (!LOCAL) {
@@ -814,7 +822,7 @@ selective_scan_step_kernel(const el_scan_t a, int share) {
     load_states(a.A + (long long)dc * N, n0, N, whole_states(a.A, N), A);
     const float bias = a.dt_bias ? a.dt_bias[dc] : 0.0f, D = a.D ? a.D[dc] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) A[n] *= LOG2E;
+    for (int n = 0; n < 4; ++n) A[n] = rate_of(A[n]);
     const bool whole = whole_states(a.initial_state, N) && whole_states(a.final_state, N);
     // The next sequence's inputs are fetched ahead: the compiler itself cannot move loads of a state before the stores of another one.  64 sequences of
     // 8192 channels: 25.6 -> 20.5 us; two ahead 20.8.

@@ -98,3 +98,25 @@ def test_padding_has_zero_gradients_whatever_the_states_hold(ops, what, N, G):
             assert not g[b, n:].any(), (k, b)              # a NaN is not zero either
     for b, n in enumerate(lengths.tolist()):
         assert not y[b, n:].any()
+
+
+# ---- decay rates without bound --------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("L,mask", [(21, "full"), (16, "full"), (21, "ragged"), (1500, "full")])
+def test_scan_of_states_that_forget_at_once(ops, L, mask):
+    """A = -inf: exp(delta A) is 0 for every token, and padding of a tile leaves the state as it is.  (The gradient of the step sizes is
+    -inf * 0 in the definition and is not looked at.)"""
+    t, lengths, dy, ds = _scan_case(2, L, 32, 16, 1, torch.float32, mask)
+    t["A"][3, 2], t["A"][:, 7], t["A"][5] = -INF, -INF, -3e38
+    gpu, ref = _leaves(t)
+    dev_lengths = None if lengths is None else lengths.to(DEV)
+    y, s = ops.selective_scan(**gpu, lengths=dev_lengths, return_final_state=True)
+    yr, sr = R.selective_scan(**{k: v if k != "A" else v.detach().masked_fill(t["A"].isinf(), -3.4e38).requires_grad_(True) for k, v in ref.items()}, lengths=lengths)
+    _close("y", y, yr, 4 * L + 32)
+    _close("state", s, sr, 4 * L + 16)
+    names = ("u", "B", "C", "D", "z", "initial_state")
+    got = torch.autograd.grad((y, s), [gpu[k] for k in (*names, "A")], (dy.to(DEV), ds.to(DEV)))
+    want = _reference_grads((yr, sr), [ref[k] for k in names], (dy.double().nan_to_num(0.0), ds.double()))
+    for k, a, b in zip(names, got, want):
+        _close("d" + k, a, b, 8 * L + 64 + (2 * L if k == "D" else 32 if k in "BC" else 0))
+    assert torch.isfinite(got[-1]).all() and not got[-1][:, 7].any()
