@@ -416,11 +416,40 @@ template <typename F> static int by_width(int W, F f) {
     }
 }
 
+// n sequences of a call from number b0 on, as a call of their own.
+static el_conv_t conv_sequences(const el_conv_t& a, int b0, int n) {
+    const int e = a.dtype == EL_F32 ? 4 : 2;
+    const long long tokens = (long long)a.length * a.channels, state = (long long)(a.width - 1) * a.channels;
+    auto from = [&](auto* p, long long pitch) { return p ? reinterpret_cast<decltype(p)>(reinterpret_cast<uintptr_t>(p) + (uintptr_t)(b0 * pitch * e)) : p; };
+    el_conv_t s = a;
+    s.batch = n;
+    s.x = from(a.x, a.x_stride_b);
+    s.dy = from(a.dy, a.dy_stride_b);
+    s.y = from(a.y, tokens);
+    s.dx = from(a.dx, tokens);
+    s.initial_state = from(a.initial_state, state);
+    s.final_state = from(a.final_state, state);
+    s.d_initial_state = from(a.d_initial_state, state);
+    s.d_final_state = from(a.d_final_state, state);
+    if (a.lengths) s.lengths = a.lengths + b0;
+    return s;
+}
+// launch(call, first sequence) of as many sequences at a time as a grid has rows
+template <typename F> static int by_sequences(const el_conv_t& a, F launch) {
+    constexpr int ROWS = 65535;
+    if (a.batch <= ROWS) return launch(a, 0);
+    for (long long b0 = 0; b0 < a.batch; b0 += ROWS) {
+        const int rc = launch(conv_sequences(a, (int)b0, (int)(a.batch - b0 < ROWS ? a.batch - b0 : ROWS)), (int)b0);
+        if (rc != EL_OK) return rc;
+    }
+    return EL_OK;
+}
+
 int launch_causal_conv(const el_conv_t& a, cudaStream_t st) {
     constexpr int V = CONV_V;
     const int strip = conv_strip(a, 64);
-    const dim3 grid(ceil_div(a.channels, CONV_LANES * V), ceil_div(a.length > 0 ? a.length : 1, (long long)strip * FW_STRIPS), a.batch);
-    if (grid.y > 65535 || grid.z > 65535) return EL_ERR_TOO_LARGE;
+    const unsigned blocks_t = ceil_div(a.length > 0 ? a.length : 1, (long long)strip * FW_STRIPS);
+    if (blocks_t > 65535) return EL_ERR_TOO_LARGE;
     const dim3 block(CONV_LANES, FW_STRIPS);
     const size_t shared = (size_t)CONV_SLOTS * CONV_LANES * FW_STRIPS * V * (a.dtype == EL_F32 ? 4 : 2);        // 16 KB at most
     const bool al = a.channels % V == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, V) && vectors(a.y, 0, 0, a.dtype, V) &&
@@ -429,17 +458,20 @@ int launch_causal_conv(const el_conv_t& a, cudaStream_t st) {
         return by_width(a.width, [&](auto w) {
             using T = decltype(t);
             constexpr int W = decltype(w)::value;
-            if (al) causal_conv_kernel<T, W, true><<<grid, block, shared, st>>>(a, strip);
-            else causal_conv_kernel<T, W, false><<<grid, block, shared, st>>>(a, strip);
-            return check_launch();
+            return by_sequences(a, [&](const el_conv_t& part, int) {
+                const dim3 grid(ceil_div(a.channels, CONV_LANES * V), blocks_t, part.batch);
+                if (al) causal_conv_kernel<T, W, true><<<grid, block, shared, st>>>(part, strip);
+                else causal_conv_kernel<T, W, false><<<grid, block, shared, st>>>(part, strip);
+                return check_launch();
+            });
         });
     });
 }
 
 int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st) {
     const ConvBackwardPlan plan = conv_backward_plan(a);
-    const dim3 grid(ceil_div(a.channels, CONV_LANES * 4), plan.blocks_t, a.batch), block(CONV_LANES, BW_STRIPS);
-    if (grid.y > 65535 || grid.z > 65535) return EL_ERR_TOO_LARGE;
+    const dim3 block(CONV_LANES, BW_STRIPS);
+    if (plan.blocks_t > 65535) return EL_ERR_TOO_LARGE;
     const bool sums = a.dweight || a.dbias;
     float* partial = sums ? static_cast<float*>(a.workspace) : nullptr;
     const bool al = a.channels % 4 == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, 4) && vectors(a.dy, a.dy_stride_b, a.dy_stride_t, a.dtype, 4) &&
@@ -459,8 +491,11 @@ int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st) {
                     EL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
                     once.mark(dev);
                 }
-                kernel<<<grid, block, shared, st>>>(a, plan.strip, partial);
-                return check_launch();
+                return by_sequences(a, [&](const el_conv_t& part, int b0) {
+                    const dim3 grid(ceil_div(a.channels, CONV_LANES * 4), plan.blocks_t, part.batch);
+                    kernel<<<grid, block, shared, st>>>(part, plan.strip, partial ? partial + (size_t)b0 * plan.blocks_t * (a.width + 1) * a.channels : nullptr);
+                    return check_launch();
+                });
             };
             static DeviceOnce once[2];
             return al ? launch(causal_conv_backward_kernel<T, W, true>, once[0]) : launch(causal_conv_backward_kernel<T, W, false>, once[1]);
@@ -471,12 +506,12 @@ int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st) {
 }
 
 int launch_causal_conv_step(const el_conv_t& a, cudaStream_t st) {
-    const dim3 grid(ceil_div(a.channels, 128), a.batch);
-    if (grid.y > 65535) return EL_ERR_TOO_LARGE;
     return by_type(a.dtype, [&](auto t) {
         return by_width(a.width, [&](auto w) {
-            causal_conv_step_kernel<decltype(t), decltype(w)::value><<<grid, 128, 0, st>>>(a);
-            return check_launch();
+            return by_sequences(a, [&](const el_conv_t& part, int) {
+                causal_conv_step_kernel<decltype(t), decltype(w)::value><<<dim3(ceil_div(a.channels, 128), part.batch), 128, 0, st>>>(part);
+                return check_launch();
+            });
         });
     });
 }

@@ -120,3 +120,57 @@ def test_scan_of_states_that_forget_at_once(ops, L, mask):
     for k, a, b in zip(names, got, want):
         _close("d" + k, a, b, 8 * L + 64 + (2 * L if k == "D" else 32 if k in "BC" else 0))
     assert torch.isfinite(got[-1]).all() and not got[-1][:, 7].any()
+
+
+# ---- sizes that one launch does not hold ----------------------------------------------------------------------------------
+
+def _conv_reference(x, weight, bias, first=None, lengths=None):
+    """(y, final state) of all tokens at once, with SiLU."""
+    B, L, D = x.shape
+    W = weight.shape[1]
+    live = None if lengths is None else (torch.arange(L, device=x.device) < lengths[:, None])[..., None]
+    x = x if live is None else torch.where(live, x, 0.0)
+    rows = torch.cat([x.new_zeros(B, W - 1, D) if first is None else first, x], 1)
+    y = F.silu(bias + sum(weight[:, j] * rows[:, j:j + L] for j in range(W)))
+    end = torch.full((B,), L, device=x.device) if lengths is None else lengths.long()
+    at = end[:, None] + torch.arange(W - 1, device=x.device)
+    return y if live is None else torch.where(live, y, 0.0), rows[torch.arange(B, device=x.device)[:, None], at]
+
+
+def _check_conv_at_once(ops, B, L, D, W, dtype, ragged):
+    g = torch.Generator(device=DEV).manual_seed(B + L + D + W)
+
+    def randn(*shape, dtype=torch.float32):
+        return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+    lengths = torch.randint(0, L + 1, (B,), generator=g, device=DEV) if ragged else None
+    t = dict(x=randn(B, L, D, dtype=dtype), weight=randn(D, W) * 0.5, bias=randn(D), first=randn(B, W - 1, D, dtype=dtype))
+    dy, ds = randn(B, L, D, dtype=dtype), randn(B, W - 1, D, dtype=dtype)
+    ref = {k: v.double().requires_grad_(True) for k, v in t.items()}
+    yr, sr = _conv_reference(**ref, lengths=lengths)
+    want = torch.autograd.grad((yr, sr), list(ref.values()), (dy.double(), ds.double()))
+    if ragged:
+        behind = torch.arange(L, device=DEV) >= lengths[:, None]
+        t["x"][behind], dy[behind] = NAN, NAN
+    gpu = {k: v.requires_grad_(True) for k, v in t.items()}
+    y, s = ops.causal_conv(gpu["x"], gpu["weight"], gpu["bias"], initial_state=gpu["first"], lengths=lengths, return_final_state=True)
+    _close("y", y, yr, W + 8)
+    assert torch.equal(s.double(), sr)
+    for k, a, b in zip(gpu, torch.autograd.grad((y, s), list(gpu.values()), (dy, ds)), want):
+        _close("d" + k, a, b, (B * L if k in ("weight", "bias") else W) + 16)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 12), (torch.bfloat16, 8), (torch.float16, 5)])
+def test_conv_of_more_sequences_than_a_grid_has_rows(ops, dtype, D):
+    B = 2 * 65535 + 3
+    _check_conv_at_once(ops, B, 2, D, 3, dtype, True)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, state = (torch.randn(*s, generator=g, device=DEV).to(dtype) for s in ((B, D), (B, 3, D)))
+    w = torch.randn(D, 4, generator=g, device=DEV)
+    want = torch.cat([state, x[:, None]], 1)
+    y = ops.causal_conv_step(x, state, w)
+    assert torch.equal(state, want[:, 1:])
+    pre = (want.double() * w.double().t()).sum(1)
+    _close("y", y, F.silu(pre), 4 + 8)
+
+
