@@ -377,23 +377,25 @@ static bool vectors(const void* p, long long s0, long long s1, int dtype, int V)
 
 static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+constexpr int FW_STRIPS = 4, BW_STRIPS = 8;
+
 // Tokens of a strip, at most `longest`.  A strip costs its start (weights, the first tokens' latency, W-1 tokens read again) and its end, so it is long; but
 // every SM is given 400 threads first.  Strips of up to 32 / 64 / 128 tokens, us: forward 4 x 1024 x 8192 35.7 / 33.4 / 36.1; backward 78.6 / 76.7 / 68.4.
 // 1024 threads an SM instead: 3 x 1999 x 1504 forward 13.0 -> 19.0, backward 28.0 -> 35.0.
-static int conv_strip(const el_conv_t& a, int longest) {
+// Millions of tokens take longer strips, `strips` of them a block, so that a grid's 65535 rows hold them.
+static int conv_strip(const el_conv_t& a, int longest, int strips) {
     int sms = 148;
     device_sm_count(&sms);
     const long long threads = (long long)a.batch * ((a.channels + CONV_V - 1) / CONV_V) * a.length;        // at one token a strip
     int strip = longest;
     while (strip > 8 && threads / strip < (long long)sms * 400) strip >>= 1;
+    while (ceil_div(a.length, (long long)strip * strips) > 65535) strip <<= 1;
     return strip;
 }
 
-constexpr int FW_STRIPS = 4, BW_STRIPS = 8;
-
 struct ConvBackwardPlan { int strip, blocks_t; };
 static ConvBackwardPlan conv_backward_plan(const el_conv_t& a) {
-    const int strip = conv_strip(a, 128);
+    const int strip = conv_strip(a, 128, BW_STRIPS);
     return {strip, ceil_div(a.length > 0 ? a.length : 1, (long long)strip * BW_STRIPS)};
 }
 
@@ -447,9 +449,8 @@ template <typename F> static int by_sequences(const el_conv_t& a, F launch) {
 
 int launch_causal_conv(const el_conv_t& a, cudaStream_t st) {
     constexpr int V = CONV_V;
-    const int strip = conv_strip(a, 64);
+    const int strip = conv_strip(a, 64, FW_STRIPS);
     const unsigned blocks_t = ceil_div(a.length > 0 ? a.length : 1, (long long)strip * FW_STRIPS);
-    if (blocks_t > 65535) return EL_ERR_TOO_LARGE;
     const dim3 block(CONV_LANES, FW_STRIPS);
     const size_t shared = (size_t)CONV_SLOTS * CONV_LANES * FW_STRIPS * V * (a.dtype == EL_F32 ? 4 : 2);        // 16 KB at most
     const bool al = a.channels % V == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, V) && vectors(a.y, 0, 0, a.dtype, V) &&
@@ -471,7 +472,6 @@ int launch_causal_conv(const el_conv_t& a, cudaStream_t st) {
 int launch_causal_conv_backward(const el_conv_t& a, cudaStream_t st) {
     const ConvBackwardPlan plan = conv_backward_plan(a);
     const dim3 block(CONV_LANES, BW_STRIPS);
-    if (plan.blocks_t > 65535) return EL_ERR_TOO_LARGE;
     const bool sums = a.dweight || a.dbias;
     float* partial = sums ? static_cast<float*>(a.workspace) : nullptr;
     const bool al = a.channels % 4 == 0 && vectors(a.x, a.x_stride_b, a.x_stride_t, a.dtype, 4) && vectors(a.dy, a.dy_stride_b, a.dy_stride_t, a.dtype, 4) &&

@@ -174,3 +174,22 @@ def test_conv_of_more_sequences_than_a_grid_has_rows(ops, dtype, D):
     _close("y", y, F.silu(pre), 4 + 8)
 
 
+def test_conv_of_one_sequence_of_millions_of_tokens(ops):
+    """More strips than a grid has rows, forward and backward: each output and each gradient of an input is formed from the same few tokens as in
+    pieces."""
+    L, D = 68_000_000, 4
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(1, L, D, generator=g, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    dy = torch.randn(1, L, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    w = torch.randn(D, 4, generator=g, device=DEV)
+    whole = ops.causal_conv(x, w)
+    dx, = torch.autograd.grad(whole, x, dy)
+    whole = whole.detach()
+    cuts = (0, 16_000_000, 32_000_000, 48_000_000, 64_000_000, L)
+    for a, b in zip(cuts, cuts[1:]):
+        lead = min(a, 3)                                   # the tokens before a piece, with it, in place of a state
+        piece = x.detach()[:, a - lead:b].requires_grad_(True)
+        y = ops.causal_conv(piece, w)
+        assert torch.equal(y[:, lead:], whole[:, a:b])
+        gp, = torch.autograd.grad(y, piece, dy[:, a - lead:b])
+        assert torch.equal(gp[:, lead:b - a + lead - 3], dx[:, a:b - 3])
