@@ -639,13 +639,14 @@ Tensor maybe_dense(PyObject* o, const char* name, const Tensor& x, at::ScalarTyp
     return is_none(o) ? Tensor() : dense_arg(o, name, x, dt, sizes);
 }
 Tensor maybe_tokens(PyObject* o, const char* name, const Tensor& x, at::IntArrayRef sizes) { return is_none(o) ? Tensor() : tokens_arg(o, name, x, sizes); }
-Tensor lengths_arg(PyObject* o, const Tensor& x, int64_t batch) {
+// int32 values go to the kernels as they are, which clamp them to 0 .. length; int64 ones are clamped before they are narrowed
+Tensor lengths_arg(PyObject* o, const Tensor& x, int64_t batch, int64_t length) {
     if (is_none(o)) return Tensor();
     const Tensor& t = cuda_arg(o, "lengths");
     if (t.device() != x.device()) raise("lengths is on another device");
     EL_REQUIRE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, "lengths must be int32 or int64");
     EL_REQUIRE(t.dim() == 1 && t.size(0) == batch, "lengths must have one entry per sequence");
-    return t.to(at::kInt).contiguous();
+    return (t.scalar_type() == at::kLong ? t.clamp(0, length).to(at::kInt) : t).contiguous();
 }
 // the state that a step writes: a dense tensor like `state`, either state itself or one apart from it
 const Tensor& state_out_arg(PyObject* o, const Tensor& state) {
@@ -722,7 +723,7 @@ PyObject* causal_conv(PyObject* const* a) {
     const Tensor& x = k.x;
     const c10::cuda::CUDAGuard device(x.device());
     const int64_t B = x.size(0), H = k.c.width - 1, D = x.size(2);
-    Tensor first = maybe_dense(a[4], "initial_state", x, x.scalar_type(), {B, H, D}), lengths = lengths_arg(a[5], x, B);
+    Tensor first = maybe_dense(a[4], "initial_state", x, x.scalar_type(), {B, H, D}), lengths = lengths_arg(a[5], x, B, x.size(1));
     k.c.initial_state = ptr(first);
     k.c.lengths = ptr<int32_t>(lengths);
     Tensor y = new_empty(x, x.sizes(), x.scalar_type()), last;
@@ -743,7 +744,7 @@ PyObject* causal_conv_backward(PyObject* const* a) {
     const c10::cuda::CUDAGuard device(x.device());
     const int64_t B = x.size(0), H = k.c.width - 1, D = x.size(2);
     const int want = (int)int_arg(a[8]);
-    Tensor first = maybe_dense(a[4], "initial_state", x, x.scalar_type(), {B, H, D}), lengths = lengths_arg(a[5], x, B);
+    Tensor first = maybe_dense(a[4], "initial_state", x, x.scalar_type(), {B, H, D}), lengths = lengths_arg(a[5], x, B, x.size(1));
     Tensor dy = maybe_tokens(a[6], "dy", x, x.sizes()), d_last = maybe_dense(a[7], "d_final_state", x, x.scalar_type(), {B, H, D});
     Tensor dx, dw, db, d_first;
     if (want & 1) dx = new_empty(x, x.sizes(), x.scalar_type());
@@ -859,7 +860,7 @@ PyObject* selective_scan(PyObject* const* a) {
     scan_call(k, a, int_arg(a[8]) != 0, false);
     const Tensor& u = k.u;
     const c10::cuda::CUDAGuard device(u.device());
-    Tensor first = maybe_dense(a[9], "initial_state", u, at::kFloat, {k.B, k.D, k.N}), lengths = lengths_arg(a[10], u, k.B);
+    Tensor first = maybe_dense(a[9], "initial_state", u, at::kFloat, {k.B, k.D, k.N}), lengths = lengths_arg(a[10], u, k.B, k.L);
     el_scan_t& c = k.c;
     c.initial_state = ptr<float>(first);
     c.lengths = ptr<int32_t>(lengths);
@@ -884,7 +885,7 @@ PyObject* selective_scan_backward(PyObject* const* a) {
     scan_call(k, a, int_arg(a[8]) != 0, false);
     const Tensor& u = k.u;
     const c10::cuda::CUDAGuard device(u.device());
-    Tensor first = maybe_dense(a[9], "initial_state", u, at::kFloat, {k.B, k.D, k.N}), lengths = lengths_arg(a[10], u, k.B);
+    Tensor first = maybe_dense(a[9], "initial_state", u, at::kFloat, {k.B, k.D, k.N}), lengths = lengths_arg(a[10], u, k.B, k.L);
     el_scan_t& c = k.c;
     c.initial_state = ptr<float>(first);
     c.lengths = ptr<int32_t>(lengths);

@@ -11,7 +11,7 @@ and states are held in float32, and every output is rounded once.  Gradients do 
 call gives the same bits.  Derivatives are reverse-mode ones of the first order; a tensor with a forward-mode tangent is refused.
 `RuntimeError` on bad arguments.
 
-`lengths` (int32 or int64 [batch]): sequence b has lengths[b] tokens and padding behind them.  Padding is not read (it may hold
+`lengths` (int32 or int64 [batch], clamped to 0 .. length): sequence b has lengths[b] tokens and padding behind them.  Padding is not read (it may hold
 anything, NaN included), its outputs and gradients are zeros and it leaves the state as it is.
 """
 from __future__ import annotations

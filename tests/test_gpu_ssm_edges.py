@@ -193,3 +193,20 @@ def test_conv_of_one_sequence_of_millions_of_tokens(ops):
         assert torch.equal(y[:, lead:], whole[:, a:b])
         gp, = torch.autograd.grad(y, piece, dy[:, a - lead:b])
         assert torch.equal(gp[:, lead:b - a + lead - 3], dx[:, a:b - 3])
+
+
+@pytest.mark.parametrize("name", ["conv", "scan"])
+def test_lengths_beyond_32_bits_are_clamped(ops, name):
+    t, *_ = _scan_case(4, 10, 16, 8, 1, torch.float32)
+    d = {k: v.to(DEV) for k, v in t.items()}
+    w = _randn(_gen(1), 16, 4).to(DEV)
+
+    def call(lengths):
+        if name == "conv":
+            return ops.causal_conv(d["u"], w, lengths=lengths, return_final_state=True)
+        return ops.selective_scan(**d, lengths=lengths, return_final_state=True)
+
+    got = call(torch.tensor([2 ** 32 + 3, -2 ** 32 + 5, 2 ** 31, -1], device=DEV))
+    want = call(torch.tensor([10, 0, 10, 0], device=DEV, dtype=torch.int32))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
