@@ -898,7 +898,7 @@ static ScanSplit scan_split(const el_scan_t& a, long long warps, int slots, int 
         if (chunks > a.length / 64) chunks = a.length / 64;
         if (chunks >= 2) {
             s.tokens = (int)((a.length + chunks - 1) / chunks + TILE - 1) / TILE * TILE;
-            s.chunks = (a.length + s.tokens - 1) / s.tokens;
+            s.chunks = (int)(((long long)a.length + s.tokens - 1) / s.tokens);       // length + tokens may pass 31 bits; a chunk's end does not
         }
     }
     s.deltas = states + (size_t)a.batch * s.chunks * a.channels * a.states;

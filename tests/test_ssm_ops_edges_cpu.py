@@ -20,6 +20,20 @@ def _scan_args(pkg, length, channels=1, states=1):
     return buf
 
 
+@pytest.mark.parametrize("length", [1 << 20, (1 << 31) - (1 << 27), (1 << 31) - (1 << 26) - 40, 0x7fff0000])
+def test_workspaces_of_the_longest_sequences(pkg, length):
+    """One channel: 32 chunks, each with a state and a sum of step sizes; backward adds dB and dC of every token and a chunk's dA, dD, dbias."""
+    lib = pkg._lib.lib()
+    assert lib.el_selective_scan_workspace_bytes(_scan_args(pkg, length)) == 32 * 2 * 4
+    assert lib.el_selective_scan_backward_workspace_bytes(_scan_args(pkg, length)) == (2 * length + 32 * 3 + 32 * 2) * 4
+
+
+def test_longer_sequences_are_refused(pkg):
+    lib = pkg._lib
+    assert lib.lib().el_selective_scan(_scan_args(pkg, 0x7fff0001), None) == lib.EL_ERR_TOO_LARGE
+    assert lib.lib().el_selective_scan_workspace_bytes(_scan_args(pkg, 0x7fff0001)) == 0
+
+
 def _calls(o):
     t, w, s = torch.zeros(2, 3, 8), torch.zeros(8, 4), torch.zeros(2, 3, 8)
     return {"causal_conv": (o.causal_conv, dict(x=t, weight=w, bias=t, initial_state=s)),
