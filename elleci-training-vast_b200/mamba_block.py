@@ -91,7 +91,12 @@ class MambaBlockInt2(nn.Module):
     def forward(self, h: torch.Tensor, x: torch.Tensor, state: Optional[MambaState] = None,
                 lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """h, x [batch, length, d_model].  `state` (no gradient goes into it): the text goes on from it, and its tensors become the state after
-        each sequence's last token, in place; a backward pass after that is that of the piece that was given.  `lengths` as in ssm_ops."""
+        each sequence's last token, in place; a backward pass after that is that of the piece that was given.  `lengths` as in ssm_ops: h and x
+        may hold anything behind a sequence's end, both outputs and all gradients are zeros there."""
+        # the projections and norms run over padding too: zeros on the way in and, for the gradients, on the way out
+        live = None if lengths is None else (torch.arange(x.shape[1], device=x.device) < lengths[:, None])[..., None]
+        if live is not None:
+            h, x = torch.where(live, h, 0.0), torch.where(live, x, 0.0)
         conv_before, ssm_before = self._before(state)
         xz = self.in_proj(x)
         u, z = xz[..., :self.d_inner], xz[..., self.d_inner:]
@@ -106,7 +111,8 @@ class MambaBlockInt2(nn.Module):
         if state is not None:
             y, last = y
             state.ssm.copy_(last.detach())
-        return self._join(h, y, x)
+        out, normed = self._join(h, y, x)
+        return (out, normed) if live is None else (torch.where(live, out, 0.0), torch.where(live, normed, 0.0))
 
     @torch.no_grad()
     def step(self, h: torch.Tensor, x: torch.Tensor, state: MambaState) -> Tuple[torch.Tensor, torch.Tensor]:

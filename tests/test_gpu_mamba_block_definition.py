@@ -101,3 +101,28 @@ def test_training_on_a_text_in_pieces(pkg):
         assert state.conv is conv and state.ssm is ssm, "the state's tensors are updated in place"
     for (name, p), q in zip(block.named_parameters(), twin.parameters()):
         assert (p.grad is None) == (q.grad is None) and (p.grad is None or torch.equal(p.grad, q.grad)), name
+
+
+def test_padding_of_the_block_may_hold_anything(pkg):
+    """Outputs and gradients of padding are zeros, and no parameter's gradient has seen it, whatever lies in the padding of the inputs and of the outputs'
+    gradients."""
+    lengths = torch.tensor([40, 0, 7, 1], device=DEV)
+    behind = torch.arange(40, device=DEV) >= lengths[:, None]
+    results = []
+    for fill in (0.0, float("nan"), float("inf")):
+        block = _block(pkg).train()
+        h, x = _inputs(4, 40, 256)
+        g = torch.Generator().manual_seed(1)
+        grads = [torch.randn(4, 40, 256, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)]
+        for t in (h, x, *grads):
+            t[behind] = fill
+        h.requires_grad_(True)
+        x.requires_grad_(True)
+        out = block(h, x, lengths=lengths)
+        torch.autograd.backward(out, grads)
+        for t in (*out, h.grad, x.grad):
+            assert not t[behind].any() and torch.isfinite(t).all()
+        results.append([*out, h.grad, x.grad, *(p.grad for n, p in block.named_parameters() if not n.endswith("gamma"))])
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
