@@ -210,3 +210,102 @@ def test_lengths_beyond_32_bits_are_clamped(ops, name):
     want = call(torch.tensor([10, 0, 10, 0], device=DEV, dtype=torch.int32))
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ---- loops that only larger sizes reach -----------------------------------------------------------------------------------
+
+def _sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def _plan(pkg, name, ints):
+    """A workspace size, which shows how a call is cut up: leading fields of its struct, all pointers null."""
+    buf = (ctypes.c_int32 * 160)()
+    for i, v in enumerate(ints):
+        buf[i] = v
+    return getattr(pkg._lib.lib(), name)(buf)
+
+
+@pytest.mark.parametrize("B,L,D,W,dtype,ragged,strip", [(1, 517, 7400, 4, torch.bfloat16, False, 16), (3, 1999, 1504, 4, torch.float16, True, 32),
+                                                        (2, 1001, 7607, 3, torch.bfloat16, True, 64), (4, 1024, 8192, 4, torch.bfloat16, False, 128),
+                                                        (2, 1024, 8192, 2, torch.float32, True, 64)])
+def test_conv_where_a_strip_is_longer_than_its_slots(pkg, ops, B, L, D, W, dtype, ragged, strip):
+    """A thread's slots hold 8 tokens: strips of 16 to 128 go round them."""
+    if _sms() == 148:
+        blocks = -(-L // (8 * strip))
+        assert _plan(pkg, "el_causal_conv_backward_workspace_bytes", [pkg._lib.EL_BF16, B, L, D, W]) == B * blocks * (W + 1) * D * 4
+    _check_conv_at_once(ops, B, L, D, W, dtype, ragged)
+
+
+def _scan_reference(u, dt, A, B, C, D, z, dt_bias, initial_state, lengths):
+    """(y, final state), token by token for all sequences at once."""
+    nb, L, ch = u.shape
+    G, h, ys = B.shape[2], initial_state, []
+    steps = [v.unbind(1) for v in (u, F.softplus(dt + dt_bias, threshold=1e9), B, C, z)]
+    for i, (ut, delta, Bt, Ct, zt) in enumerate(zip(*steps)):
+        Bt, Ct = (m.repeat_interleave(ch // G, 1) for m in (Bt, Ct))
+        new = torch.exp(delta[..., None] * A) * h + (delta * ut)[..., None] * Bt
+        on = (i < lengths)[:, None]
+        y = (new * Ct).sum(-1) + D * ut
+        ys.append(torch.where(on, y * F.silu(zt), 0.0))
+        h = torch.where(on[..., None], new, h)
+    return torch.stack(ys, 1), h
+
+
+@pytest.mark.parametrize("B,L,D,N,G,dtype,ragged", [(4, 300, 7168, 16, 1, torch.bfloat16, False), (4, 277, 7184, 16, 2, torch.float32, True),
+                                                    (2, 290, 1800, 64, 1, torch.float32, True)])
+def test_scan_backward_of_many_tiles_in_one_piece(pkg, ops, B, L, D, N, G, dtype, ragged):
+    """So many channels that the sequences are not cut: a warp takes more than the 16 tiles after which its sums over tokens go to memory."""
+    lanes = max(N // 4, 1)
+    width = 8 * 64 // lanes                                # channels of a block's eight warps
+    blocks = -(-(D // G) // width)
+    if _sms() == 148:
+        assert _plan(pkg, "el_selective_scan_backward_workspace_bytes", [pkg._lib.EL_BF16, B, L, D, G, N]) == 4 * (2 * blocks * B * L * G * N + B * D * (N + 2))
+    assert L > 2 * 128
+    t, _, dy, ds = _scan_case(B, L, D, N, G, dtype)
+    lengths = torch.tensor([L, 0, L - 3, 130][:B]) if ragged else torch.full((B,), L)
+    dev = {k: v.to(DEV) for k, v in t.items()}
+    dy, ds = dy.to(DEV), ds.to(DEV)
+    ref = {k: v.double().requires_grad_(True) for k, v in dev.items()}
+    yr, sr = _scan_reference(**ref, lengths=lengths.to(DEV))
+    want = torch.autograd.grad((yr, sr), list(ref.values()), (dy.double(), ds.double()))
+    yr, sr = yr.detach(), sr.detach()
+    for v in [dev[k] for k in ("u", "dt", "z", "B", "C")] + [dy]:
+        _poison(v, lengths)
+    gpu = {k: v.requires_grad_(True) for k, v in dev.items()}
+    y, s = ops.selective_scan(**gpu, lengths=lengths.to(DEV) if ragged else None, return_final_state=True)
+    _close("y", y, yr, 4 * L + N + 16)
+    _close("state", s, sr, 4 * L + 16)
+    got = torch.autograd.grad((y, s), list(gpu.values()), (dy, ds))
+    terms = dict(A=B * L, D=B * L, dt_bias=B * L, B=D // G, C=D // G)
+    for k, a, b in zip(gpu, got, want):
+        _close("d" + k, a, b, 8 * L + 2 * N + 32 + terms.get(k, 0))
+
+
+@pytest.mark.parametrize("B,D,N,G,dtype", [(64, 8192, 16, 1, torch.bfloat16), (61, 8190, 16, 2, torch.float32), (100, 4100, 12, 1, torch.float16),
+                                           (33, 2056, 64, 4, torch.bfloat16)])
+def test_scan_step_of_blocks_that_take_several_sequences(ops, B, D, N, G, dtype):
+    """In place and beside the old state; a block goes through its sequences with the next one's state under way."""
+    lanes = max(1, 1 << (N - 1).bit_length() >> 2)
+    assert -(-D * lanes // 128) * B // (16 * _sms()) >= 2
+    t, *_ = _scan_case(B, 1, D, N, G, dtype)
+    d = {k: v.to(DEV) for k, v in t.items()}
+    tok = {k: d[k][:, 0] for k in ("u", "dt", "B", "C", "z")}
+    rest = {k: d[k] for k in ("A", "D", "dt_bias")}
+    yr, sr = _scan_reference(**{k: v.double() for k, v in d.items()}, lengths=torch.ones(B, device=DEV))
+    old, other = d["initial_state"].clone(), torch.full_like(d["initial_state"], NAN)
+    y = ops.selective_scan_step(**tok, **rest, state=old, state_out=other)
+    assert torch.equal(old, d["initial_state"])
+    _close("y", y, yr[:, 0], 4 + N + 16)
+    _close("state", other, sr, 4 + 16)
+    again = ops.selective_scan_step(**tok, **rest, state=old)
+    assert torch.equal(again, y) and torch.equal(old, other)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,K", [(700, 4096), (5000, 256), (400, 4095), (400, 8200), (500, 16384), (600, 8192)])
+def test_norm_of_blocks_that_take_several_rows(ops, M, K, dtype):
+    """Rows in plenty: the next row fetched while this one is worked on, the sums' buffers in turn, column sums over a block's rows."""
+    threads = -(-(-(-K // 8)) // 32) * 32                  # of a row's block, 16-bit types; two blocks an SM where it has 512
+    assert M > _sms() * (max(1024 // threads, 1) if K <= 4096 else 1)
+    _check_norm(ops, *_norm_case(M, K, dtype, True, True))
