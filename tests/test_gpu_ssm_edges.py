@@ -309,3 +309,18 @@ def test_norm_of_blocks_that_take_several_rows(ops, M, K, dtype):
     threads = -(-(-(-K // 8)) // 32) * 32                  # of a row's block, 16-bit types; two blocks an SM where it has 512
     assert M > _sms() * (max(1024 // threads, 1) if K <= 4096 else 1)
     _check_norm(ops, *_norm_case(M, K, dtype, True, True))
+
+
+# ---- step sizes -----------------------------------------------------------------------------------------------------------
+
+def test_relative_error_of_step_sizes(ops):
+    """From a state of zero, with u, B and C of one, the first y is the step size itself.  The exponential: a product with log2(e) rounded to 2^-24 and
+    log2(e) to 1.4e-8, both of the exponent, 7.3e-8 |x|, and two units in the last place, 2^-22.  The logarithm's series: its argument e / (2 + e) with an addition, a reciprocal of
+    one unit in the last place and a product, 2^-24 + 2^-23 + 2^-24; its sum 2^-24 twice and 1.4e-8 for the terms left out; the largest together 4.1e-7.
+    Below 2^-126 two units of 2^-149."""
+    x = torch.cat([torch.linspace(-100, 30, 4001), torch.linspace(-8, 1, 4001)])
+    one = torch.ones(1, 1, 1, device=DEV)
+    y = ops.selective_scan(one.expand(1, 1, len(x)), x[None, None].to(DEV), -torch.ones(len(x), 1, device=DEV), one, one)
+    want = F.softplus(x.double(), threshold=1e9)
+    off = (y[0, 0].double().cpu() - want).abs()
+    assert bool((off <= want * (7.3e-8 * x.double().abs() + 2.0 ** -22 + 4.1e-7) + 2 * 2.0 ** -149).all()), float((off / want).max())
