@@ -122,6 +122,16 @@ def test_scan_of_states_that_forget_at_once(ops, L, mask):
     assert torch.isfinite(got[-1]).all() and not got[-1][:, 7].any()
 
 
+def test_scan_step_of_states_that_forget_at_once(ops):
+    t, *_ = _scan_case(2, 1, 32, 16, 1, torch.float32)
+    t["A"][3, 2], t["A"][:, 7], t["A"][5] = -INF, -INF, -3e38
+    d = {k: v.to(DEV) for k, v in t.items()}
+    whole, last = ops.selective_scan(**d, return_final_state=True)
+    y = ops.selective_scan_step(**{k: d[k][:, 0] for k in ("u", "dt", "B", "C", "z")}, A=d["A"], D=d["D"], dt_bias=d["dt_bias"], state=d["initial_state"])
+    _close("y", y, whole[:, 0].double(), 4 + 32)
+    _close("state", d["initial_state"], last.double(), 4 + 16)
+
+
 # ---- sizes that one launch does not hold ----------------------------------------------------------------------------------
 
 def _conv_reference(x, weight, bias, first=None, lengths=None):
