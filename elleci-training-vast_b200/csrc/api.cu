@@ -733,7 +733,7 @@ int el_block_norm_backward(const el_block_norm_t* a, el_stream_t stream) {
     if ((rc = require_sm100()) != EL_OK) return rc;
     if (a->width == 0) return EL_OK;
     const size_t need = block_norm_backward_workspace_bytes(*a);
-    if (a->rows > 0 && (!a->h || !a->y || !a->post_weight || !a->pre_weight || !a->rstd || !a->dh || !a->dy_in || !a->workspace)) return EL_ERR_NULL_PTR;
+    if (a->rows > 0 && (!a->h || !a->y || !a->post_weight || !a->pre_weight || !a->rstd || (need > 0 && !a->workspace))) return EL_ERR_NULL_PTR;
     if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
     return launch_block_norm_backward(*a, (cudaStream_t)stream);

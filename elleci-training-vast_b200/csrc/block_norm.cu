@@ -289,7 +289,7 @@ block_norm_backward_kernel(const el_block_norm_t a, float* __restrict__ partial)
         if (a.gate) out(a.dgate, m, hn);
         out(a.dy_in, m, dt);
     }
-    if (mine) {
+    if (mine && partial) {
 #pragma unroll
         for (int q = 0; q < 3; ++q) put<float, V, ALIGNED>(partial + ((long long)blockIdx.x * 3 + q) * K + k, K - k, stride, sums[q]);
     }
@@ -378,11 +378,12 @@ block_norm_backward_wide_kernel(const el_block_norm_t a, float* __restrict__ par
             }
             add_to(2, c, ds);
             add_to(0, c, dw);
-            put<T, 8, ALIGNED>(static_cast<T*>(a.dh) + (long long)m * K + k, K - k, stride, d);
+            if (a.dh) put<T, 8, ALIGNED>(static_cast<T*>(a.dh) + (long long)m * K + k, K - k, stride, d);
             if (a.gate && a.dgate) put<T, 8, ALIGNED>(static_cast<T*>(a.dgate) + (long long)m * K + k, K - k, stride, hn);
-            put<T, 8, ALIGNED>(static_cast<T*>(a.dy_in) + (long long)m * K + k, K - k, stride, dn);
+            if (a.dy_in) put<T, 8, ALIGNED>(static_cast<T*>(a.dy_in) + (long long)m * K + k, K - k, stride, dn);
         }
     }
+    if (partial == nullptr) return;
     for (int c = 0; c < vecs; ++c) {
         const int k = norm_column<ALIGNED>(c);
         if (k >= K) continue;
@@ -423,7 +424,11 @@ static int norm_backward_blocks(const el_block_norm_t& a) {
     if (a.width > NORM_HELD || a.width == 0) return norm_blocks(a.rows, 1);
     return norm_blocks(a.rows, (a.dtype == EL_F32 ? NORM_THREADS<float> : NORM_THREADS<__half>) / norm_held_threads(a));
 }
-size_t block_norm_backward_workspace_bytes(const el_block_norm_t& a) { return (size_t)norm_backward_blocks(a) * 3 * a.width * sizeof(float); }
+static bool norm_wants_sums(const el_block_norm_t& a) { return a.dpost_weight || a.dpre_weight || a.dscale; }
+size_t block_norm_backward_workspace_bytes(const el_block_norm_t& a) {
+    if (!norm_wants_sums(a) && (a.dh || a.dy_in || a.dgate)) return 0;
+    return (size_t)norm_backward_blocks(a) * 3 * a.width * sizeof(float);
+}
 
 static bool norm_aligned(const el_block_norm_t& a) {
     if (a.width % 8 != 0) return false;
@@ -477,7 +482,7 @@ int launch_block_norm(const el_block_norm_t& a, cudaStream_t st) {
 
 int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st) {
     const int blocks = norm_backward_blocks(a);
-    float* partial = static_cast<float*>(a.workspace);
+    float* partial = norm_wants_sums(a) ? static_cast<float*>(a.workspace) : nullptr;
     if (blocks > 0) {
         const int rc = norm_variant(a, [&](auto t, auto al) {
             using T = decltype(t);
@@ -497,7 +502,7 @@ int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st) {
         });
         if (rc != EL_OK) return rc;
     }
-    if (!a.dpost_weight && !a.dpre_weight && !a.dscale) return EL_OK;
+    if (!norm_wants_sums(a)) return EL_OK;
     return launch_column_sums(partial, blocks, 3 * a.width, NormSums{a.dpost_weight, a.dpre_weight, a.dscale, a.width}, st);
 }
 

@@ -1005,7 +1005,8 @@ PyObject* block_norm(PyObject* const* a) {
     return tuple_of(wrap(out), wrap(normed), wrap_or_none(rstd));
 }
 
-// block_norm_backward(h, y, post_weight, pre_weight, gate, scale, eps, rstd, dh_out, dnormed) -> (dh, dy, dpost_weight, dpre_weight, dgate, dscale)
+// block_norm_backward(h, y, post_weight, pre_weight, gate, scale, eps, rstd, dh_out, dnormed, wanted) -> (dh, dy, dpost_weight, dpre_weight, dgate,
+// dscale), `wanted`: bits 0 .. 5 in this order
 PyObject* block_norm_backward(PyObject* const* a) {
     no_tangent("block_norm_backward", a, {0, 1, 2, 3, 4, 5, 8, 9});
     NormCall k;
@@ -1019,10 +1020,14 @@ PyObject* block_norm_backward(PyObject* const* a) {
     Rows dh_out, dn;
     if (!is_none(a[8])) dh_out = norm_rows(a[8], "dh_out", shaped);
     if (!is_none(a[9])) dn = norm_rows(a[9], "dnormed", shaped);
-    Tensor dh = new_empty(h, shaped.sizes(), h.scalar_type()), dy = new_empty(h, shaped.sizes(), h.scalar_type()), dg, ds;
-    Tensor dw1 = new_empty(h, {K}, at::kFloat), dw2 = new_empty(h, {K}, at::kFloat);
-    if (k.g.t.defined()) dg = new_empty(h, shaped.sizes(), h.scalar_type());
-    if (k.scale.defined()) ds = new_empty(h, {K}, at::kFloat);
+    const int want = (int)int_arg(a[10]);
+    Tensor dh, dy, dw1, dw2, dg, ds;
+    if (want & 1) dh = new_empty(h, shaped.sizes(), h.scalar_type());
+    if (want & 2) dy = new_empty(h, shaped.sizes(), h.scalar_type());
+    if (want & 4) dw1 = new_empty(h, {K}, at::kFloat);
+    if (want & 8) dw2 = new_empty(h, {K}, at::kFloat);
+    if ((want & 16) && k.g.t.defined()) dg = new_empty(h, shaped.sizes(), h.scalar_type());
+    if ((want & 32) && k.scale.defined()) ds = new_empty(h, {K}, at::kFloat);
     c.rstd = ptr<float>(rstd);
     if (dh_out.t.defined()) {
         c.dh_out = ptr(dh_out.t);
@@ -1042,7 +1047,7 @@ PyObject* block_norm_backward(PyObject* const* a) {
     Tensor ws = scratch(h, c.workspace_bytes);
     c.workspace = ptr(ws);
     call("el_block_norm_backward", g_lib.el_block_norm_backward, &c, stream_on(h));
-    return tuple_of(wrap(dh), wrap(dy), wrap(dw1), wrap(dw2), wrap_or_none(dg), wrap_or_none(ds));
+    return tuple_of(wrap_or_none(dh), wrap_or_none(dy), wrap_or_none(dw1), wrap_or_none(dw2), wrap_or_none(dg), wrap_or_none(ds));
 }
 
 // ---- module -------------------------------------------------------------------------------------------------------------
@@ -1086,7 +1091,7 @@ PyMethodDef methods[] = {
     EL_ENTRY(rmsnorm_backward, 4), EL_ENTRY(swiglu_quantize_rows, 5), EL_ENTRY(swiglu_backward, 6), EL_ENTRY(prelinear_rows, 4),
     EL_ENTRY(gemm_fwd, 7), EL_ENTRY(gemm_dx, 8), EL_ENTRY(dw_hysteresis, 11), EL_ENTRY(weight_update, 13), EL_ENTRY(linear_decode, 8), EL_ENTRY(set_hooks, 4),
     EL_ENTRY(causal_conv, 7), EL_ENTRY(causal_conv_backward, 9), EL_ENTRY(causal_conv_step, 6), EL_ENTRY(selective_scan, 13),
-    EL_ENTRY(selective_scan_backward, 15), EL_ENTRY(selective_scan_step, 11), EL_ENTRY(block_norm, 8), EL_ENTRY(block_norm_backward, 10),
+    EL_ENTRY(selective_scan_backward, 15), EL_ENTRY(selective_scan_step, 11), EL_ENTRY(block_norm, 8), EL_ENTRY(block_norm_backward, 11),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "elleci_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

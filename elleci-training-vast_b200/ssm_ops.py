@@ -156,7 +156,7 @@ class _BlockNorm(Function):
         if dh_out is None and dnormed is None:
             return (None,) * 7
         dh, dy, dw1, dw2, dgate, dscale = host_ops().block_norm_backward(h, y, post_weight, pre_weight, gate, scale, ctx.eps, rstd,
-                                                                         dh_out, dnormed)
+                                                                         dh_out, dnormed, _bits(ctx.needs_input_grad[:6]))
         return dh, dy, dw1, dw2, dgate, dscale, None
 
 

@@ -502,7 +502,8 @@ EL_API int el_selective_scan_step(const el_scan_t* args, el_stream_t stream);
  *   normed = pre_weight * h_out / rms(h_out)                              (of h_out before it is rounded to the dtype)
  * with rms(v) = sqrt(mean v^2 + eps).  ld_*: row pitches of the inputs.  rstd [rows, 2] receives 1/rms of y and of h_out (NULL when no
  * gradient is wanted).  el_block_norm_backward writes dh, dy_in (the gradient of y), dgate, dscale, dpost_weight, dpre_weight
- * (dgate with gate, dscale with scale) from dh_out and dnormed (either may be NULL), and reads h, y, gate and rstd again.
+ * (dgate with gate, dscale with scale; each may be NULL) from dh_out and dnormed (either may be NULL), and reads h, y, gate and rstd again.
+ * Its workspace size is that of the gradients that the struct names, or of all of them where it names none.
  * Width up to 16384. */
 typedef struct el_block_norm_t {
     int dtype, rows, width;

@@ -334,3 +334,31 @@ def test_relative_error_of_step_sizes(ops):
     want = F.softplus(x.double(), threshold=1e9)
     off = (y[0, 0].double().cpu() - want).abs()
     assert bool((off <= want * (7.3e-8 * x.double().abs() + 2.0 ** -22 + 4.1e-7) + 2 * 2.0 ** -149).all()), float((off / want).max())
+
+
+# ---- gradients that nobody asked for ----------------------------------------------------------------------------------------
+
+def _peak(f):
+    """Bytes that a call takes beyond what was there before it."""
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    result = f()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - before, result
+
+
+@pytest.mark.parametrize("K", [2048, 8192])
+def test_norm_backward_forms_what_is_wanted(ops, K):
+    """A frozen norm over one input that has a gradient: one output, no partial sums; and the same bits as beside all others."""
+    t, da, db = _norm_case(512, K, torch.bfloat16, True, True)
+    gpu = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    douts = (da.to(DEV), db.to(DEV))
+    whole = dict(zip(gpu, torch.autograd.grad(ops.block_norm(**gpu), list(gpu.values()), douts)))
+    for k in gpu:
+        alone = {j: v.detach().requires_grad_(j == k) for j, v in gpu.items()}
+        outs = ops.block_norm(**alone)
+        bytes_, (g,) = _peak(lambda: torch.autograd.grad(outs, alone[k], douts))
+        assert torch.equal(g, whole[k]), k
+        if g.dim() == 2:
+            assert bytes_ <= g.numel() * 2 + 4096, (k, bytes_)
