@@ -469,7 +469,7 @@ template <typename S> __device__ __forceinline__ void bc_sums(float (&v)[8], flo
 }
 
 // LOCAL: the gradient of the state at the chunk's start from zeros at its end, and the sum of delta.
-// partial_bc [blocks of a group][2][batch][length][groups][states]; partial_a [batch][chunks][channels][states + 2]: dA, dD, dbias.
+// partial_bc [blocks of a group][2][batch][length][groups][states], or NULL where neither dB nor dC is wanted; partial_a [batch][chunks][channels][states + 2]: dA, dD, dbias.
 template <typename T, typename S, bool LOCAL>
 __global__ void __launch_bounds__(32 * BACK_WARPS, S::BACK_PER_SM / BACK_WARPS)
 selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool aligned, bool aligned_bc, float* __restrict__ partial_bc,
@@ -536,8 +536,9 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     // dB and dC: this block's row of the partial sums, for thread's value (token, B or C, state)
     const long long bc_all = (long long)a.batch * a.length * a.groups * N;
     float* bc = LOCAL ? nullptr : partial_bc + 2 * block * bc_all + ((long long)p.b * a.length * a.groups + p.g) * N;
+    const int bc_end = partial_bc ? end : 0;                  // formed, but kept nowhere, if not wanted: a question per tile costs 1 % of all calls
     auto store_bc = [&](int t, int m, int n, float v) {
-        if (n < N && t < end) bc[m * bc_all + (long long)t * a.groups * N + n] = v;
+        if (n < N && t < bc_end) bc[m * bc_all + (long long)t * a.groups * N + n] = v;
     };
 
     Quad<T> u[PAIRS], u_next[PAIRS], dt_next[PAIRS], z_next[PAIRS], dy_next[PAIRS], b_next[BCS], c_next[BCS];
@@ -596,7 +597,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             if (ddt) store_quad<T>(ddt + (long long)t * a.channels, valid, aligned, zero);
             if (dz) store_quad<T>(dz + (long long)t * a.channels, valid, aligned, zero);
         }
-        for (int t = begin + n_tiles * KEEP; t < end; ++t)
+        for (int t = begin + n_tiles * KEEP; t < bc_end; ++t)
             for (int i = threadIdx.x; i < 2 * S::NS; i += 32 * BACK_WARPS) store_bc(t, i / S::NS, i % S::NS, 0.0f);
     }
     if (n_tiles > 0) fetch(begin + (n_tiles - 1) * KEEP);
@@ -923,14 +924,18 @@ size_t selective_scan_workspace_bytes(const el_scan_t& a) {
 }
 
 // Backward's workspace: partial sums of dB and dC, of dA, dD and dbias, and the chunks' states.
+// dB and dC, the larger part, have no room where neither is wanted; a struct that names no gradient yet asks for all of them.
 struct ScanBackwardPlan { ScanSplit split; long long blocks; float *bc, *a; size_t floats; };
+static bool scan_wants_bc(const el_scan_t& a) {
+    return a.dB || a.dC || !(a.du || a.ddt || a.dz || a.dA || a.dD || a.ddt_bias || a.d_initial_state);
+}
 template <typename S> static ScanBackwardPlan scan_backward_plan(const el_scan_t& a, float* ws) {
     ScanBackwardPlan p;
     p.blocks = parts_of(a, S::CW * BACK_WARPS);
     p.split = scan_split(a, parts_of(a, S::CW), S::BACK_PER_SM, S::BACK_PER_SM * 3 / 4, nullptr);
     const size_t per_group = (a.channels / a.groups + S::CW * BACK_WARPS - 1) / (S::CW * BACK_WARPS);
-    const size_t n_bc = 2 * per_group * a.batch * a.length * a.groups * a.states, n_a = (size_t)a.batch * p.split.chunks * a.channels * (a.states + 2);
-    p.bc = ws;
+    const size_t n_bc = scan_wants_bc(a) ? 2 * per_group * a.batch * a.length * a.groups * a.states : 0, n_a = (size_t)a.batch * p.split.chunks * a.channels * (a.states + 2);
+    p.bc = n_bc ? ws : nullptr;
     p.a = ws + n_bc;
     p.split.states = p.a + n_a;
     p.split.deltas = p.split.states + (size_t)a.batch * p.split.chunks * a.channels * a.states;

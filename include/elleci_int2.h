@@ -453,7 +453,8 @@ EL_API int el_causal_conv_step(const el_conv_t* args, el_stream_t stream);
  * `checkpoints` (el_selective_scan_checkpoint_bytes; NULL when no gradient is wanted) receives the states that the backward pass
  * starts from and has to reach it unchanged.
  * el_selective_scan_backward writes du, ddt, dz (with z), dB, dC [batch, length, groups, states], dA, dD (with D), ddt_bias (with dt_bias) and
- * d_initial_state (each may be NULL) from dy and d_final_state (either may be NULL).  All sums have a fixed order.
+ * d_initial_state (each may be NULL) from dy and d_final_state (either may be NULL).  All sums have a fixed order.  Its workspace size is that of
+ * the gradients that the struct names, or of all of them where it names none.
  * el_selective_scan_step: one token for every sequence, as el_causal_conv_step. */
 typedef struct el_scan_t {
     int dtype, batch, length, channels, groups, states, softplus;

@@ -339,13 +339,13 @@ def test_relative_error_of_step_sizes(ops):
 # ---- gradients that nobody asked for ----------------------------------------------------------------------------------------
 
 def _peak(f):
-    """Bytes that a call takes beyond what was there before it."""
+    """Bytes that a call asks for beyond what was there before it."""
     torch.cuda.synchronize()
     torch.cuda.reset_peak_memory_stats()
-    before = torch.cuda.memory_allocated()
+    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
     result = f()
     torch.cuda.synchronize()
-    return torch.cuda.max_memory_allocated() - before, result
+    return torch.cuda.memory_stats()["requested_bytes.all.peak"] - before, result
 
 
 @pytest.mark.parametrize("K", [2048, 8192])
@@ -362,3 +362,21 @@ def test_norm_backward_forms_what_is_wanted(ops, K):
         assert torch.equal(g, whole[k]), k
         if g.dim() == 2:
             assert bytes_ <= g.numel() * 2 + 4096, (k, bytes_)
+
+
+def test_scan_backward_keeps_no_room_for_what_is_not_wanted(pkg, ops):
+    """B and C without a gradient: the partial sums of dB and dC, 2 x 8 blocks of channels x batch x length x states floats here, have no place."""
+    t, _, dy, _ = _scan_case(2, 200, 1024, 16, 1, torch.float32)
+    gpu = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    dy = dy.to(DEV)
+    whole = dict(zip(gpu, torch.autograd.grad(ops.selective_scan(**gpu), list(gpu.values()), dy)))
+    partial = 2 * 8 * 2 * 200 * 16 * 4
+    sizes = {}
+    for k in gpu:
+        alone = {j: v.detach().requires_grad_(j == k) for j, v in gpu.items()}
+        y = ops.selective_scan(**alone)
+        sizes[k], (g,) = _peak(lambda: torch.autograd.grad(y, alone[k], dy))
+        assert torch.equal(g, whole[k]), k
+        sizes[k] -= g.numel() * 4
+    assert abs(sizes["B"] - sizes["A"] - partial) <= 4096 and abs(sizes["C"] - sizes["B"]) <= 4096
+    assert all(abs(v - sizes["A"]) <= 4096 for k, v in sizes.items() if k not in "BC"), sizes
