@@ -698,9 +698,8 @@ int el_selective_scan_backward(const el_scan_t* a, el_stream_t stream) {
     int rc = check_scan(a);
     if (rc != EL_OK) return rc;
     if ((rc = require_sm100()) != EL_OK) return rc;
-    if (a->channels == 0) return EL_OK;
     const size_t need = selective_scan_backward_workspace_bytes(*a);
-    if (!a->A || (a->length > 0 && a->batch > 0 && (!a->u || !a->dt || !a->B || !a->C || !a->checkpoints)) || (need > 0 && !a->workspace))
+    if ((a->channels > 0 && !a->A) || (a->length > 0 && a->batch > 0 && a->channels > 0 && (!a->u || !a->dt || !a->B || !a->C || !a->checkpoints)) || (need > 0 && !a->workspace))
         return EL_ERR_NULL_PTR;
     if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;

@@ -1020,18 +1020,18 @@ int launch_selective_scan_backward(const el_scan_t& a, cudaStream_t st) {
             const ScanBackwardPlan p = scan_backward_plan<S>(a, static_cast<float*>(a.workspace));
             if (p.blocks > (1ll << 31) - 1) return (int)EL_ERR_TOO_LARGE;
             int rc = EL_OK;
-            if (a.batch > 0) {
+            if (p.blocks > 0) {                               // else all sums are empty: zeros
                 if (p.split.chunks > 1) rc = launch_scan_backward_pass<T, S, true>(a, p, st);
                 if (rc == EL_OK) rc = launch_scan_backward_pass<T, S, false>(a, p, st);
             }
             if (rc != EL_OK) return rc;
             const long long all = (long long)a.batch * a.length * a.groups * a.states, cols = (long long)a.channels * (a.states + 2);
             if ((a.dB || a.dC) && all > 0) {
-                scan_bc_sums_kernel<T><<<(unsigned)((2 * all + 255) / 256), 256, 0, st>>>(p.bc, (int)(p.blocks / (a.batch * a.groups)), all,
+                scan_bc_sums_kernel<T><<<(unsigned)((2 * all + 255) / 256), 256, 0, st>>>(p.bc, (int)(p.blocks / ((long long)a.batch * a.groups)), all,
                                                                                          static_cast<T*>(a.dB), static_cast<T*>(a.dC));
                 if ((rc = check_launch()) != EL_OK) return rc;
             }
-            if (a.dA || a.dD || a.ddt_bias)
+            if ((a.dA || a.dD || a.ddt_bias) && cols > 0)
                 scan_a_sums_kernel<<<(unsigned)((cols + 255) / 256), 256, 0, st>>>(p.a, a.batch * p.split.chunks, a.channels, a.states, a.dA, a.dD,
                                                                                  a.ddt_bias);
             return check_launch();

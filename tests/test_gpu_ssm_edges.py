@@ -380,3 +380,19 @@ def test_scan_backward_keeps_no_room_for_what_is_not_wanted(pkg, ops):
         sizes[k] -= g.numel() * 4
     assert abs(sizes["B"] - sizes["A"] - partial) <= 4096 and abs(sizes["C"] - sizes["B"]) <= 4096
     assert all(abs(v - sizes["A"]) <= 4096 for k, v in sizes.items() if k not in "BC"), sizes
+
+
+# ---- nothing to add up ------------------------------------------------------------------------------------------------------
+
+def test_gradients_of_no_channels_are_zeros(ops):
+    """dB and dC are sums over the channels: of none of them, zeros, whatever the memory held before."""
+    t, *_ = _scan_case(2, 9, 8, 4, 2, torch.float32)
+    gpu = {k: (v[..., :0] if k in ("u", "dt", "z", "D", "dt_bias") else v[:0] if k == "A" else v[:, :0] if k == "initial_state" else v).to(DEV).requires_grad_(True)
+           for k, v in t.items()}
+    y, s = ops.selective_scan(**gpu, return_final_state=True)
+    assert y.shape == (2, 9, 0) and s.shape == (2, 0, 4)
+    for _ in range(2):
+        junk = [torch.full((2, 9, 2, 4), NAN, device=DEV) for _ in range(8)]
+        del junk
+        for k, g in zip(gpu, torch.autograd.grad((y, s), list(gpu.values()), (torch.zeros_like(y), torch.zeros_like(s)), retain_graph=True)):
+            assert g.shape == gpu[k].shape and not g.any(), k
