@@ -612,7 +612,7 @@ PyObject* linear_decode(PyObject* const* a) {
 // ---- between the projections of a Mamba block ----------------------------------------------------------------------------
 // Activations of one dtype, channel-last; a tensor whose channels are contiguous is read in place, whatever its other strides.
 
-// `o` as a tensor on x's device with x's dtype and the given sizes, its last dimension contiguous; empty sizes: any
+// `o` as a tensor on x's device with x's dtype and the given sizes, its last dimension contiguous
 Tensor tokens_arg(PyObject* o, const char* name, const Tensor& x, at::IntArrayRef sizes) {
     const Tensor& t = cuda_arg(o, name);
     if (t.device() != x.device()) raise(std::string(name) + " is on another device");

@@ -536,9 +536,9 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
     // dB and dC: this block's row of the partial sums, for thread's value (token, B or C, state)
     const long long bc_all = (long long)a.batch * a.length * a.groups * N;
     float* bc = LOCAL ? nullptr : partial_bc + 2 * block * bc_all + ((long long)p.b * a.length * a.groups + p.g) * N;
-    const int bc_end = partial_bc ? end : 0;                  // formed, but kept nowhere, if not wanted: a question per tile costs 1 % of all calls
+    const int bc_stop = partial_bc ? stop : 0;                // formed, but kept nowhere, if not wanted: a question per tile costs 1 % of all calls
     auto store_bc = [&](int t, int m, int n, float v) {
-        if (n < N && t < bc_end) bc[m * bc_all + (long long)t * a.groups * N + n] = v;
+        if (n < N) bc[m * bc_all + (long long)t * a.groups * N + n] = v;
     };
 
     Quad<T> u[PAIRS], u_next[PAIRS], dt_next[PAIRS], z_next[PAIRS], dy_next[PAIRS], b_next[BCS], c_next[BCS];
@@ -597,7 +597,8 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
             if (ddt) store_quad<T>(ddt + (long long)t * a.channels, valid, aligned, zero);
             if (dz) store_quad<T>(dz + (long long)t * a.channels, valid, aligned, zero);
         }
-        for (int t = begin + n_tiles * KEEP; t < bc_end; ++t)
+        const int bc_end = partial_bc ? end : 0;
+        for (int t = max(begin, stop); t < bc_end; ++t)
             for (int i = threadIdx.x; i < 2 * S::NS; i += 32 * BACK_WARPS) store_bc(t, i / S::NS, i % S::NS, 0.0f);
     }
     if (n_tiles > 0) fetch(begin + (n_tiles - 1) * KEEP);
@@ -719,7 +720,7 @@ selective_scan_backward_kernel(const el_scan_t a, const ScanSplit split, bool al
 #pragma unroll
             for (int w = 0; w < BACK_WARPS; ++w) v += reinterpret_cast<const float*>(tiles[w].bc[k & 1])[i];
             const int t = t0 + i / (2 * S::NS);
-            store_bc(t, i / S::NS & 1, i % S::NS, t < stop ? v : 0.0f);      // of padding: zero times a state that may not be finite
+            if (t < bc_stop) store_bc(t, i / S::NS & 1, i % S::NS, v);        // not padding's: zero times a state that may not be finite
         }
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {

@@ -155,8 +155,10 @@ class _BlockNorm(Function):
         h, y, post_weight, pre_weight, gate, scale, rstd = ctx.saved_tensors
         if dh_out is None and dnormed is None:
             return (None,) * 7
+        need = ctx.needs_input_grad
+        wanted = need[0] | need[1] << 1 | need[2] << 2 | need[3] << 3 | need[4] << 4 | need[5] << 5
         dh, dy, dw1, dw2, dgate, dscale = host_ops().block_norm_backward(h, y, post_weight, pre_weight, gate, scale, ctx.eps, rstd,
-                                                                         dh_out, dnormed, _bits(ctx.needs_input_grad[:6]))
+                                                                         dh_out, dnormed, wanted)
         return dh, dy, dw1, dw2, dgate, dscale, None
 
 
