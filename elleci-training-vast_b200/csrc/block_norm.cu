@@ -180,7 +180,7 @@ block_norm_kernel(const el_block_norm_t a) {
 
 // Backward, rows of up to 4096 columns: a row's values stay in registers, one vector of 16 bytes a thread, and so do the column sums of a block's
 // rows, which go to `partial` [blocks][3][width]: dw1, dw2, ds.  The next row is on asynchronous copies into the threads' own slots in shared
-// memory (one row ahead; two or three gain nothing); rows that no vector copy takes are fetched into registers.  4096 x 4096, bfloat16 67 us, float32 98.
+// memory (one row ahead; two or three gain nothing); rows that no vector copy takes are fetched into registers.  4096 x 4096, bfloat16 67 us, float32 95.
 template <typename T> constexpr int NORM_V = 16 / sizeof(T);
 template <typename T> constexpr int NORM_THREADS = sizeof(T) == 2 ? 512 : 1024;        // of an SM: what its registers take
 template <typename T> struct NormGrads { Vec<T, NORM_V<T>> v[5]; };              // dnormed, y, h, gate, dh_out

@@ -5,8 +5,8 @@
 //
 // A thread owns a vector of channels and walks over a strip of tokens with the last W-1 inputs (backward: and W dpre) in registers, so
 // every input is read once but for the W-1 tokens at a strip's ends.  Floor: memory, one read and one write per value
-// (backward two and one).  4 x 1024 tokens of 8192 channels: forward 33 us in bfloat16 (floor 20), 48 in float32 (41); backward 68 (31) and 83 (61): the
-// 16-bit types are bound by instructions and latencies, not by bytes.
+// (backward two and one).  4 x 1024 tokens of 8192 channels: forward 33 us in bfloat16 (floor 20), 49 in float32 (41); backward 68 (31) and 84 (61): in
+// 16-bit types no unit is full, a copy, an address step and a store of 8 bytes carry two operands each.
 #include "mamba_common.cuh"
 
 namespace el {

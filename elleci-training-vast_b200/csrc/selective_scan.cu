@@ -10,7 +10,7 @@
 // Floor: the exponentials.  16 states are 16 of them per token and channel (backward: twice), softplus and SiLU four more special functions, at
 // 16 a clock and SM; the memory traffic of a bfloat16 call (forward 8 bytes per token and channel) takes less than a third of that time.  What binds
 // beside them: wavefronts of shared memory, 19 per token and 16 channels forward, 76 backward, each worth a clock of the SM.  4 x 1024 tokens of
-// 8192 channels, 16 states, bfloat16: forward 245 us (floor 144), backward 871.
+// 8192 channels, 16 states, bfloat16: forward 246 us (floor 144), backward 874.
 #include "mamba_common.cuh"
 
 namespace el {
@@ -38,7 +38,7 @@ __device__ __forceinline__ int live_tokens(const el_scan_t& a, int b) { return a
 
 // The lanes of a warp over the states and channels of its tile.  4 states x 2 channels a lane: B and C are read once for two channels, and 16
 // channels a warp are still 512 warps for a layer of 8192.  Forward, 4096 tokens of 8192 channels / 4 x 1024 tokens, 16 states, bfloat16, when the
-// shapes were compared: this 349 / 251 us (319 / 245 now); 4 channels a lane 567 / 289; 2 states a lane 464 / 435.
+// shapes were compared: this 349 / 251 us (319 / 246 now); 4 channels a lane 567 / 289; 2 states a lane 464 / 435.
 template <int NS_>
 struct Shape {
     static constexpr int NS = NS_, SPL = 4, CPL = 2;
@@ -889,7 +889,7 @@ static long long parts_of(const el_scan_t& a, int width) {     // pieces of that
 // its own (half of a forward pass again, a quarter of a backward pass), then, from the states that those give, for the outputs.  As many chunks as the
 // SMs take at once (`slots` warps each): one more would be a second round.  Below `enough` warps an SM, as measured, 16 states, us:
 //   forward (slots 8, enough 3)    16384 x 2048 channels 0.9 warps an SM: 9 chunks 417, 10 chunks 568;  4096 x 8192 3.5: whole 343, 2 chunks 464
-//   backward (slots 16, enough 12) 4096 x 8192 channels 3.5: whole 3459, 4 chunks 1138;  4 x 1024 x 8192 13.8: whole 915, 2 chunks 1263 (1089 and 871 now)
+//   backward (slots 16, enough 12) 4096 x 8192 channels 3.5: whole 3459, 4 chunks 1138;  4 x 1024 x 8192 13.8: whole 915, 2 chunks 1263 (1093 and 874 now)
 static ScanSplit scan_split(const el_scan_t& a, long long warps, int slots, int enough, float* states) {
     int sms = 148;
     device_sm_count(&sms);
