@@ -49,7 +49,7 @@ typedef void* el_stream_t;
 #define EL_ERR_CUDA              -5   /* a CUDA runtime call failed; see el_last_cuda_error() */
 #define EL_ERR_DEVICE            -6   /* the current device is not an sm_100 part */
 #define EL_ERR_DRIVER            -7   /* the driver refused a tensor-map descriptor */
-#define EL_ERR_TOO_LARGE         -8   /* a size exceeds the fixed capacity of the entry point (el_linear_decode_static) */
+#define EL_ERR_TOO_LARGE         -8   /* a size exceeds the fixed capacity of the entry point (el_linear_decode_static; sequences of more than 2^31 - 65536 tokens) */
 
 /* ---- element types of floating-point / output buffers ------------------------------------------------ */
 #define EL_F16  0
@@ -411,7 +411,7 @@ EL_API int el_linear_decode_static(const void* x, int x_dtype, const uint8_t* W_
  * its element type; bases and strides of 16 bytes are read faster.
  * `lengths` [batch] (NULL: all sequences have `length` tokens): tokens from lengths[b] on are padding.  They are not read, their outputs and
  * gradients are zeros and they leave the state as it is; a sequence of length 0 keeps its initial state.  Values outside
- * 0 .. length are clamped.
+ * 0 .. length are clamped.  Sequences have up to 2^31 - 65536 tokens; a longer one returns EL_ERR_TOO_LARGE.
  * Outside the reference's INT2 path: its block has them as tensor operations (core/mamba/mamba2.py). */
 
 /* Depthwise causal convolution over the last `width` (2 .. 4) tokens of each channel, with bias and SiLU:
