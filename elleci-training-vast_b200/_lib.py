@@ -87,6 +87,16 @@ SIGNATURES = {
     "el_block_norm": [_vp, _vp],
     "el_block_norm_backward": [_vp, _vp],
     "el_block_norm_backward_workspace_bytes": [_vp],
+    # so do the operators of latent attention
+    "el_rotary": [_vp, _vp],
+    "el_latent_attention": [_vp, _vp],
+    "el_latent_attention_lse_bytes": [_vp],
+    "el_latent_attention_backward": [_vp, _vp],
+    "el_latent_attention_backward_workspace_bytes": [_vp],
+    "el_latent_cache_write": [_vp, _vp],
+    "el_latent_cache_read": [_vp, _vp],
+    "el_latent_attention_step": [_vp, _vp],
+    "el_latent_attention_step_workspace_bytes": [_vp],
 }
 
 

@@ -86,6 +86,16 @@ size_t block_norm_backward_workspace_bytes(const el_block_norm_t& a);
 int launch_block_norm(const el_block_norm_t& a, cudaStream_t st);
 int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st);
 
+int launch_rotary(const el_rotary_t& a, cudaStream_t st);
+size_t attention_lse_bytes(const el_attention_t& a);
+size_t attention_backward_workspace_bytes(const el_attention_t& a);
+int launch_attention(const el_attention_t& a, cudaStream_t st);
+int launch_attention_backward(const el_attention_t& a, cudaStream_t st);
+int launch_latent_cache_write(el_latent_cache_t a, cudaStream_t st);
+int launch_latent_cache_read(const el_latent_cache_t& a, cudaStream_t st);
+size_t latent_step_workspace_bytes(const el_latent_step_t& a);
+int launch_latent_step(const el_latent_step_t& a, cudaStream_t st);
+
 static thread_local int g_last_cuda_error = 0;
 
 int record_cuda_error(cudaError_t e) {
@@ -736,6 +746,121 @@ int el_block_norm_backward(const el_block_norm_t* a, el_stream_t stream) {
     if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
     return launch_block_norm_backward(*a, (cudaStream_t)stream);
+}
+
+// ---- latent attention ---------------------------------------------------------------------------------------------------------
+
+int el_rotary(const el_rotary_t* a, el_stream_t stream) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->heads < 0 || a->dim < 0 || a->table_rows < 0) return EL_ERR_INVALID_ARG;
+    if (a->dim % 2 != 0) return EL_ERR_UNSUPPORTED_SHAPE;
+    int rc = require_sm100();
+    if (rc != EL_OK) return rc;
+    if (a->batch == 0 || a->length == 0 || a->heads == 0 || a->dim == 0) return EL_OK;
+    if (a->table_rows == 0) return EL_ERR_UNSUPPORTED_SHAPE;
+    if (!a->x || !a->table || !a->y) return EL_ERR_NULL_PTR;
+    return launch_rotary(*a, (cudaStream_t)stream);
+}
+
+static int check_attention(const el_attention_t* a) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->keys < 0 || a->heads < 0 || a->key_dim < 0 || a->rot_dim < 0 || a->value_dim < 0)
+        return EL_ERR_INVALID_ARG;
+    if ((long long)a->key_dim + a->rot_dim > 256 || a->value_dim > 256) return EL_ERR_UNSUPPORTED_SHAPE;
+    // a block for every 64 rows of every head, counted in 31 bits
+    const long long rows = (a->length > a->keys ? a->length : a->keys) + 127LL;
+    if (a->length > 0x7FFFFF00 || a->keys > 0x7FFFFF00 || (double)(rows / 64 + 1) * a->batch * a->heads > 2147483647.0) return EL_ERR_TOO_LARGE;
+    return EL_OK;
+}
+
+size_t el_latent_attention_lse_bytes(const el_attention_t* a) { return check_attention(a) == EL_OK ? attention_lse_bytes(*a) : 0; }
+size_t el_latent_attention_backward_workspace_bytes(const el_attention_t* a) { return check_attention(a) == EL_OK ? attention_backward_workspace_bytes(*a) : 0; }
+
+int el_latent_attention(const el_attention_t* a, el_stream_t stream) {
+    int rc = check_attention(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->length == 0 || a->heads == 0) return EL_OK;
+    if (a->value_dim > 0 && !a->out) return EL_ERR_NULL_PTR;
+    if ((a->key_dim > 0 && !a->q) || (a->rot_dim > 0 && !a->q_rot)) return EL_ERR_NULL_PTR;
+    if (a->keys > 0 && ((a->key_dim > 0 && !a->k) || (a->value_dim > 0 && !a->v) || (a->rot_dim > 0 && !a->k_rot))) return EL_ERR_NULL_PTR;
+    return launch_attention(*a, (cudaStream_t)stream);
+}
+
+int el_latent_attention_backward(const el_attention_t* a, el_stream_t stream) {
+    int rc = check_attention(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->heads == 0) return EL_OK;
+    const size_t need = attention_backward_workspace_bytes(*a);
+    if (need > 0 && !a->workspace) return EL_ERR_NULL_PTR;
+    if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
+    if (a->length > 0 && (!a->lse || (a->value_dim > 0 && (!a->out || !a->dout)) || (a->key_dim > 0 && !a->q) || (a->rot_dim > 0 && !a->q_rot))) return EL_ERR_NULL_PTR;
+    if (a->keys > 0 && ((a->key_dim > 0 && !a->k) || (a->value_dim > 0 && !a->v) || (a->rot_dim > 0 && !a->k_rot))) return EL_ERR_NULL_PTR;
+    return launch_attention_backward(*a, (cudaStream_t)stream);
+}
+
+static int check_cache(const el_latent_cache_t* a) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->rank < 0 || a->rot_dim < 0 || a->pages < 0 || a->page_size < 0 || a->pages_per_sequence < 0 ||
+        a->table_rows < 0)
+        return EL_ERR_INVALID_ARG;
+    if (a->rank == 0 || a->rank % 16 != 0 || a->rank > 512 || a->rot_dim > 64 || (a->table && a->rot_dim % 2 != 0) || (a->table && a->table_rows == 0) || a->page_size == 0)
+        return EL_ERR_UNSUPPORTED_SHAPE;
+    if ((long long)a->batch * a->length > 0x3FFFFFFFFLL) return EL_ERR_TOO_LARGE;
+    if (reinterpret_cast<uintptr_t>(a->latents) % 16 != 0) return EL_ERR_ALIGNMENT;
+    return EL_OK;
+}
+
+int el_latent_cache_write(const el_latent_cache_t* a, el_stream_t stream) {
+    int rc = check_cache(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->length == 0 || a->pages_per_sequence == 0 || a->pages == 0) return EL_OK;
+    if (!a->latents || !a->absmax || !a->block_table || !a->x || (a->rot_dim > 0 && (!a->cache_keys || !a->k_rot))) return EL_ERR_NULL_PTR;
+    return launch_latent_cache_write(*a, (cudaStream_t)stream);
+}
+
+int el_latent_cache_read(const el_latent_cache_t* a, el_stream_t stream) {
+    int rc = check_cache(a);
+    if (rc != EL_OK) return rc;
+    if (a->out_dtype >= 0 && !float_dtype(a->out_dtype)) return EL_ERR_INVALID_ARG;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->length == 0) return EL_OK;
+    if ((a->pages > 0 && (!a->latents || !a->absmax || (a->rot_dim > 0 && !a->cache_keys))) || (a->pages_per_sequence > 0 && !a->block_table) || !a->out ||
+        (a->out_dtype < 0 && !a->out_absmax) || (a->rot_dim > 0 && !a->out_keys))
+        return EL_ERR_NULL_PTR;
+    if (reinterpret_cast<uintptr_t>(a->out) % 16 != 0 || reinterpret_cast<uintptr_t>(a->out_keys) % 16 != 0) return EL_ERR_ALIGNMENT;
+    return launch_latent_cache_read(*a, (cudaStream_t)stream);
+}
+
+static int check_step(const el_latent_step_t* a) {
+    if (!a) return EL_ERR_NULL_PTR;
+    if (!float_dtype(a->dtype) || a->batch < 0 || a->heads < 0 || a->key_dim < 0 || a->rot_dim < 0 || a->value_dim < 0 || a->rank < 0 || a->pages < 0 || a->page_size < 0 ||
+        a->pages_per_sequence < 0 || a->table_rows < 0)
+        return EL_ERR_INVALID_ARG;
+    if (a->rank == 0 || a->rank % 16 != 0 || a->rank > 512 || a->rot_dim > 64 || a->key_dim > 256 || a->value_dim > 256 || (a->table && a->rot_dim % 2 != 0) ||
+        (a->table && a->table_rows == 0) || a->page_size == 0)
+        return EL_ERR_UNSUPPORTED_SHAPE;
+    if (a->batch > 65535 || a->heads > 1024) return EL_ERR_TOO_LARGE;
+    if (reinterpret_cast<uintptr_t>(a->latents) % 16 != 0 || reinterpret_cast<uintptr_t>(a->W_packed) % 4 != 0) return EL_ERR_ALIGNMENT;
+    return EL_OK;
+}
+
+size_t el_latent_attention_step_workspace_bytes(const el_latent_step_t* a) { return check_step(a) == EL_OK ? latent_step_workspace_bytes(*a) : 0; }
+
+int el_latent_attention_step(const el_latent_step_t* a, el_stream_t stream) {
+    int rc = check_step(a);
+    if (rc != EL_OK) return rc;
+    if ((rc = require_sm100()) != EL_OK) return rc;
+    if (a->batch == 0 || a->heads == 0 || a->value_dim == 0) return EL_OK;
+    if (!a->out || !a->lengths || !a->W_packed || (a->key_dim > 0 && !a->q) || (a->rot_dim > 0 && !a->q_rot)) return EL_ERR_NULL_PTR;
+    if ((a->pages > 0 && (!a->latents || !a->absmax || (a->rot_dim > 0 && !a->cache_keys))) || (a->pages_per_sequence > 0 && !a->block_table)) return EL_ERR_NULL_PTR;
+    if (!a->workspace) return EL_ERR_NULL_PTR;
+    if (a->workspace_bytes < latent_step_workspace_bytes(*a)) return EL_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return EL_ERR_ALIGNMENT;
+    return launch_latent_step(*a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -19,6 +19,7 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
 #include <cstdlib>
 #include <vector>
 
@@ -41,7 +42,10 @@ PyObject* g_check_status = nullptr;     // int2_tc_ops.check_device_status(devic
     X(el_causal_conv) X(el_causal_conv_backward) X(el_causal_conv_backward_workspace_bytes) X(el_causal_conv_step)        \
     X(el_selective_scan) X(el_selective_scan_checkpoint_bytes) X(el_selective_scan_workspace_bytes)                       \
     X(el_selective_scan_backward) X(el_selective_scan_backward_workspace_bytes) X(el_selective_scan_step)                 \
-    X(el_block_norm) X(el_block_norm_backward) X(el_block_norm_backward_workspace_bytes)
+    X(el_block_norm) X(el_block_norm_backward) X(el_block_norm_backward_workspace_bytes)                                  \
+    X(el_rotary) X(el_latent_attention) X(el_latent_attention_lse_bytes) X(el_latent_attention_backward)                  \
+    X(el_latent_attention_backward_workspace_bytes) X(el_latent_cache_write) X(el_latent_cache_read)                      \
+    X(el_latent_attention_step) X(el_latent_attention_step_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
     EL_FUNCTIONS(X)
@@ -1050,6 +1054,408 @@ PyObject* block_norm_backward(PyObject* const* a) {
     return tuple_of(wrap_or_none(dh), wrap_or_none(dy), wrap_or_none(dw1), wrap_or_none(dw2), wrap_or_none(dg), wrap_or_none(ds));
 }
 
+// ---- latent attention ---------------------------------------------------------------------------------------------------
+// `o` with its last dimension contiguous and no dimension of a stride of 0 or less but those of size 1 (an expanded tensor is copied: its rows are
+// read as rows of a tensor map)
+Tensor attention_arg(PyObject* o, const char* name, const Tensor& x, at::IntArrayRef sizes) {
+    Tensor t = tokens_arg(o, name, x, sizes);
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) == 0) return t.contiguous();
+    return t;
+}
+// int64 values are clamped to 0 .. most before they are narrowed
+Tensor indices_arg(PyObject* o, const char* name, const Tensor& x, at::IntArrayRef sizes, int64_t most) {
+    if (is_none(o)) return Tensor();
+    const Tensor& t = cuda_arg(o, name);
+    if (t.device() != x.device()) raise(std::string(name) + " is on another device");
+    if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) raise(std::string(name) + " must be int32 or int64");
+    if (t.sizes() != sizes) {
+        std::string want;
+        for (auto s : sizes) want += (want.empty() ? "" : ", ") + std::to_string(s);
+        raise(std::string(name) + " must have shape [" + want + "]");
+    }
+    return (t.scalar_type() == at::kLong ? t.clamp(-1, most).to(at::kInt) : t).contiguous();
+}
+Tensor table_arg(PyObject* o, const Tensor& x, int64_t dim) {
+    const Tensor& t = cuda_arg(o, "table");
+    if (t.device() != x.device()) raise("table is on another device");
+    EL_REQUIRE(t.scalar_type() == at::kFloat, "table must be Float");
+    if (t.dim() != 2 || t.size(0) < 1 || t.size(1) != dim) raise("table must have shape [positions, " + std::to_string(dim) + "] with at least one position");
+    return t.contiguous();
+}
+
+// rotary(x, table, positions, neighbours, inverse) -> y
+PyObject* rotary(PyObject* const* a) {
+    no_tangent("rotary", a, {0, 1});
+    const Tensor& x4 = cuda_arg(a[0], "x");
+    EL_REQUIRE(float_type(x4.scalar_type()), "x must be float16, bfloat16 or float32");
+    EL_REQUIRE(x4.dim() == 3 || x4.dim() == 4, "x must be [batch, length, (heads,) dim]");
+    EL_REQUIRE(x4.size(-1) % 2 == 0, "the rotated dimension must be even");
+    const c10::cuda::CUDAGuard device(x4.device());
+    Tensor x = tokens_arg(a[0], "x", x4, x4.sizes()), table = table_arg(a[1], x, x.size(-1)), positions;
+    el_rotary_t c = {};
+    if (!is_none(a[2])) {
+        const Tensor& p = cuda_arg(a[2], "positions");
+        c.position_each = p.dim() == 2;
+        positions = c.position_each ? indices_arg(a[2], "positions", x, {x.size(0), x.size(1)}, table.size(0)) : indices_arg(a[2], "positions", x, {x.size(0)}, INT32_MAX);
+    }
+    Tensor y = new_empty(x, x4.sizes(), x.scalar_type());
+    const bool heads = x.dim() == 4;
+    c.dtype = code_of(x.scalar_type());
+    c.batch = int_size(x.size(0));
+    c.length = int_size(x.size(1));
+    c.heads = heads ? int_size(x.size(2)) : 1;
+    c.dim = int_size(x.size(-1));
+    c.table_rows = int_size(table.size(0));
+    c.neighbours = int_arg(a[3]) != 0;
+    c.inverse = int_arg(a[4]) != 0;
+    c.x = ptr(x);
+    c.x_stride_b = stride_of(x, 0);
+    c.x_stride_t = stride_of(x, 1);
+    c.x_stride_h = heads ? stride_of(x, 2) : 0;
+    c.table = ptr<float>(table);
+    c.positions = ptr<int32_t>(positions);
+    c.y = ptr(y);
+    call("el_rotary", g_lib.el_rotary, &c, stream_on(x));
+    return wrap(y);
+}
+
+struct AttentionCall {
+    el_attention_t c = {};
+    std::vector<Tensor> keep;
+    Tensor q;
+    int64_t B = 0, T = 0, S = 0, H = 0, D = 0, R = 0, V = 0;
+};
+// q [batch, length, heads, key_dim], kv [batch, keys, heads * (key_dim + value_dim)], q_rot, k_rot, causal, scale (None: 1 / sqrt of the key's channels),
+// lengths, key_lengths
+void attention_call(AttentionCall& k, PyObject* const* a) {
+    const Tensor &q = cuda_arg(a[0], "q"), &kv = cuda_arg(a[1], "kv");
+    EL_REQUIRE(float_type(q.scalar_type()), "q must be float16, bfloat16 or float32");
+    EL_REQUIRE(q.dim() == 4, "q must be [batch, length, heads, key_dim]");
+    EL_REQUIRE(kv.dim() == 3, "kv must be [batch, keys, heads * (key_dim + value_dim)]");
+    k.B = q.size(0);
+    k.T = q.size(1);
+    k.S = kv.size(1);
+    k.H = q.size(2);
+    k.D = q.size(3);
+    EL_REQUIRE(k.H >= 1, "q must have at least one head");
+    EL_REQUIRE(kv.size(2) % k.H == 0 && kv.size(2) / k.H >= k.D, "kv's channels must be heads * (key_dim + value_dim)");
+    k.V = kv.size(2) / k.H - k.D;
+    EL_REQUIRE(is_none(a[2]) == is_none(a[3]), "q_rot and k_rot come together");
+    k.q = attention_arg(a[0], "q", q, q.sizes());
+    Tensor pair = attention_arg(a[1], "kv", q, {k.B, k.S, kv.size(2)}), qr, kr;
+    if (!is_none(a[2])) {
+        const Tensor& r = cuda_arg(a[2], "q_rot");
+        EL_REQUIRE(r.dim() == 4, "q_rot must be [batch, length, heads, rot_dim]");
+        k.R = r.size(3);
+        qr = attention_arg(a[2], "q_rot", q, {k.B, k.T, k.H, k.R});
+        kr = attention_arg(a[3], "k_rot", q, {k.B, k.S, k.R});
+    }
+    EL_REQUIRE(k.D + k.R >= 1 && k.D + k.R <= 256, "keys of 1 to 256 channels are supported");
+    EL_REQUIRE(k.V <= 256, "values of up to 256 channels are supported");
+    el_attention_t& c = k.c;
+    c.dtype = code_of(q.scalar_type());
+    c.batch = int_size(k.B);
+    c.length = int_size(k.T);
+    c.keys = int_size(k.S);
+    c.heads = int_size(k.H);
+    c.key_dim = (int)k.D;
+    c.rot_dim = (int)k.R;
+    c.value_dim = (int)k.V;
+    c.causal = int_arg(a[4]) != 0;
+    c.scale = is_none(a[5]) ? (float)(1.0 / std::sqrt((double)(k.D + k.R))) : (float)float_arg(a[5]);
+    Tensor lengths = lengths_arg(a[6], q, k.B, k.T), key_lengths = indices_arg(a[7], "key_lengths", q, {k.B}, k.S);
+    if (!key_lengths.defined() && k.S == k.T) key_lengths = lengths;
+    const int e = (int)q.element_size();
+    c.q = ptr(k.q);
+    c.q_stride_b = stride_of(k.q, 0);
+    c.q_stride_t = stride_of(k.q, 1);
+    c.q_stride_h = stride_of(k.q, 2);
+    c.k = ptr(pair);
+    c.k_stride_b = c.v_stride_b = stride_of(pair, 0);
+    c.k_stride_t = c.v_stride_t = stride_of(pair, 1);
+    c.k_stride_h = k.D;
+    c.v = c.k ? static_cast<const char*>(c.k) + k.H * k.D * e : nullptr;
+    c.v_stride_h = k.V;
+    if (qr.defined()) {
+        c.q_rot = ptr(qr);
+        c.q_rot_stride_b = stride_of(qr, 0);
+        c.q_rot_stride_t = stride_of(qr, 1);
+        c.q_rot_stride_h = stride_of(qr, 2);
+        c.k_rot = ptr(kr);
+        c.k_rot_stride_b = stride_of(kr, 0);
+        c.k_rot_stride_t = stride_of(kr, 1);
+    }
+    c.lengths = ptr<int32_t>(lengths);
+    c.key_lengths = ptr<int32_t>(key_lengths);
+    c.dev_status = status_word(q);
+    k.keep = {pair, qr, kr, lengths, key_lengths};
+}
+
+// latent_attention(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, log sums wanted) -> (out, log sums or None)
+PyObject* latent_attention(PyObject* const* a) {
+    no_tangent("latent_attention", a, {0, 1, 2, 3});
+    AttentionCall k;
+    attention_call(k, a);
+    const c10::cuda::CUDAGuard device(k.q.device());
+    Tensor out = new_empty(k.q, {k.B, k.T, k.H, k.V}, k.q.scalar_type()), lse;
+    if (int_arg(a[8])) lse = new_empty(k.q, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&k.c) / sizeof(float))}, at::kFloat);
+    k.c.out = ptr(out);
+    k.c.lse = ptr<float>(lse);
+    call("el_latent_attention", g_lib.el_latent_attention, &k.c, stream_on(k.q));
+    maybe_check(k.q);
+    return tuple_of(wrap(out), wrap_or_none(lse));
+}
+
+// latent_attention_backward(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, out, log sums, dout, wanted) -> (dq, dkv, dq_rot, dk_rot), `wanted`: bits
+// 0 .. 3 in this order
+PyObject* latent_attention_backward(PyObject* const* a) {
+    no_tangent("latent_attention_backward", a, {0, 1, 2, 3, 8, 10});
+    AttentionCall k;
+    attention_call(k, a);
+    const Tensor& q = k.q;
+    const c10::cuda::CUDAGuard device(q.device());
+    el_attention_t& c = k.c;
+    Tensor out = dense_arg(a[8], "out", q, q.scalar_type(), {k.B, k.T, k.H, k.V});
+    Tensor lse = dense_arg(a[9], "lse", q, at::kFloat, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&c) / sizeof(float))});
+    Tensor dout = attention_arg(a[10], "dout", q, out.sizes());
+    const int want = (int)int_arg(a[11]);
+    const auto io = q.scalar_type();
+    Tensor dq, dkv, dqr, dkr;
+    if (want & 1) dq = new_empty(q, {k.B, k.T, k.H, k.D}, io);
+    if (want & 2) dkv = new_empty(q, {k.B, k.S, k.H * (k.D + k.V)}, io);
+    if ((want & 4) && k.R) dqr = new_empty(q, {k.B, k.T, k.H, k.R}, io);
+    if ((want & 8) && k.R) dkr = new_empty(q, {k.B, k.S, k.R}, io);
+    c.out = ptr(out);
+    c.lse = ptr<float>(lse);
+    c.dout = ptr(dout);
+    c.dout_stride_b = stride_of(dout, 0);
+    c.dout_stride_t = stride_of(dout, 1);
+    c.dout_stride_h = stride_of(dout, 2);
+    c.dq = ptr(dq);
+    c.dq_rot = ptr(dqr);
+    c.dk_rot = ptr(dkr);
+    if (dkv.defined()) {
+        const int64_t row = k.H * (k.D + k.V);
+        c.dk = ptr(dkv);
+        c.dv = c.dk ? static_cast<char*>(c.dk) + k.H * k.D * (int64_t)q.element_size() : nullptr;
+        c.dk_stride_b = c.dv_stride_b = k.S * row;
+        c.dk_stride_t = c.dv_stride_t = row;
+        c.dk_stride_h = k.D;
+        c.dv_stride_h = k.V;
+    }
+    c.workspace_bytes = g_lib.el_latent_attention_backward_workspace_bytes(&c);
+    Tensor ws = scratch(q, c.workspace_bytes);
+    c.workspace = ptr(ws);
+    call("el_latent_attention_backward", g_lib.el_latent_attention_backward, &c, stream_on(q));
+    maybe_check(q);
+    return tuple_of(wrap_or_none(dq), wrap_or_none(dkv), wrap_or_none(dqr), wrap_or_none(dkr));
+}
+
+struct CacheCall {
+    el_latent_cache_t c = {};
+    std::vector<Tensor> keep;
+    Tensor latents;
+};
+// a pool: latents [pages, page_size, rank] int8, absmax [pages, page_size], keys [pages, page_size, rot_dim] or None
+void pool_args(PyObject* const* a, Tensor& latents, Tensor& absmax, Tensor& keys) {
+    latents = cuda_arg(a[0], "latents");
+    EL_REQUIRE(latents.scalar_type() == at::kChar && latents.dim() == 3, "latents must be int8 [pages, page_size, rank]");
+    EL_REQUIRE(latents.size(1) >= 1, "pages must hold at least one token");
+    EL_REQUIRE(latents.size(2) >= 16 && latents.size(2) <= 512 && latents.size(2) % 16 == 0, "ranks that are multiples of 16 up to 512 are supported");
+    absmax = cuda_arg(a[1], "absmax");
+    EL_REQUIRE(absmax.device() == latents.device(), "absmax is on another device");
+    EL_REQUIRE(absmax.scalar_type() == at::kFloat && absmax.dim() == 2 && absmax.size(0) == latents.size(0) && absmax.size(1) == latents.size(1), "absmax must be Float [pages, page_size]");
+    if (!is_none(a[2])) {
+        keys = cuda_arg(a[2], "keys");
+        EL_REQUIRE(keys.device() == latents.device(), "keys is on another device");
+        EL_REQUIRE(float_type(keys.scalar_type()) && keys.dim() == 3 && keys.size(0) == latents.size(0) && keys.size(1) == latents.size(1),
+                   "keys must be float16, bfloat16 or float32 [pages, page_size, rot_dim]");
+        EL_REQUIRE(keys.size(2) <= 64, "rotated parts of up to 64 channels are supported");
+    }
+    // written in place and read by rows: a copy would be of no use
+    EL_REQUIRE(latents.is_contiguous() && absmax.is_contiguous() && (!keys.defined() || keys.is_contiguous()), "the cache's tensors must be contiguous");
+    EL_REQUIRE(reinterpret_cast<uintptr_t>(latents.data_ptr()) % 16 == 0, "latents must lie on 16 bytes");
+}
+Tensor block_table_arg(PyObject* o, const Tensor& x, int64_t batch) {
+    const Tensor& t = cuda_arg(o, "block_table");
+    if (t.device() != x.device()) raise("block_table is on another device");
+    EL_REQUIRE(t.scalar_type() == at::kInt && t.dim() == 2, "block_table must be int32 [batch, pages of a sequence]");
+    EL_REQUIRE(batch < 0 || t.size(0) == batch, "block_table must have one row per sequence");
+    return t.contiguous();
+}
+// latents, absmax, keys, block_table
+void cache_call(CacheCall& k, PyObject* const* a, int64_t batch) {
+    Tensor absmax, keys;
+    pool_args(a, k.latents, absmax, keys);
+    Tensor blocks = block_table_arg(a[3], k.latents, batch);
+    el_latent_cache_t& c = k.c;
+    c.dtype = keys.defined() ? code_of(keys.scalar_type()) : EL_BF16;
+    c.batch = int_size(blocks.size(0));
+    c.rank = (int)k.latents.size(2);
+    c.rot_dim = keys.defined() ? (int)keys.size(2) : 0;
+    c.pages = int_size(k.latents.size(0));
+    c.page_size = int_size(k.latents.size(1));
+    c.pages_per_sequence = int_size(blocks.size(1));
+    c.latents = ptr<int8_t>(k.latents);
+    c.absmax = ptr<float>(absmax);
+    c.cache_keys = ptr(keys);
+    c.block_table = ptr<int32_t>(blocks);
+    c.out_dtype = -1;
+    k.keep = {absmax, keys, blocks};
+}
+
+// latent_cache_write(latents, absmax, keys, block_table, x, norm_weight, k_rot, table, starts, lengths, norm eps, quantiser's eps, neighbours)
+PyObject* latent_cache_write(PyObject* const* a) {
+    no_gradient("latent_cache_write", a, {4, 5, 6, 7});
+    no_tangent("latent_cache_write", a, {4, 5, 6, 7});
+    const Tensor& x0 = cuda_arg(a[4], "latent");
+    EL_REQUIRE(float_type(x0.scalar_type()), "latent must be float16, bfloat16 or float32");
+    EL_REQUIRE(x0.dim() == 3, "latent must be [batch, length, rank]");
+    CacheCall k;
+    cache_call(k, a, x0.size(0));
+    const c10::cuda::CUDAGuard device(k.latents.device());
+    EL_REQUIRE(x0.device() == k.latents.device(), "latent is on another device");
+    el_latent_cache_t& c = k.c;
+    Tensor x = tokens_arg(a[4], "latent", x0, {x0.size(0), x0.size(1), c.rank}), w = maybe_dense(a[5], "norm_weight", x0, at::kFloat, {c.rank}), kr, table;
+    EL_REQUIRE(is_none(a[6]) == is_none(a[2]), "k_rot and the cache's keys come together");
+    if (!is_none(a[6])) {
+        EL_REQUIRE(k.keep[1].scalar_type() == x0.scalar_type(), "the cache's keys have another dtype than the activations");
+        kr = tokens_arg(a[6], "k_rot", x0, {x0.size(0), x0.size(1), c.rot_dim});
+    }
+    if (!is_none(a[7])) {
+        EL_REQUIRE(kr.defined(), "a table needs k_rot");
+        EL_REQUIRE(c.rot_dim % 2 == 0, "the rotated dimension must be even");
+        table = table_arg(a[7], x0, c.rot_dim);
+        c.table_rows = int_size(table.size(0));
+    }
+    Tensor starts = indices_arg(a[8], "starts", x0, {x0.size(0)}, INT32_MAX), lengths = lengths_arg(a[9], x0, x0.size(0), x0.size(1));
+    c.dtype = code_of(x0.scalar_type());
+    c.length = int_size(x0.size(1));
+    c.neighbours = int_arg(a[12]) != 0;
+    c.norm_eps = (float)float_arg(a[10]);
+    c.quant_eps = (float)float_arg(a[11]);
+    EL_REQUIRE(c.norm_eps >= 0.0f && c.quant_eps > 0.0f, "eps must not be negative");
+    c.x = ptr(x);
+    c.x_stride_b = stride_of(x, 0);
+    c.x_stride_t = stride_of(x, 1);
+    c.norm_weight = ptr<float>(w);
+    if (kr.defined()) {
+        c.k_rot = ptr(kr);
+        c.k_rot_stride_b = stride_of(kr, 0);
+        c.k_rot_stride_t = stride_of(kr, 1);
+    }
+    c.table = ptr<float>(table);
+    c.starts = ptr<int32_t>(starts);
+    c.lengths = ptr<int32_t>(lengths);
+    call("el_latent_cache_write", g_lib.el_latent_cache_write, &c, stream_on(x));
+    written(k.latents);
+    written(k.keep[0]);
+    if (k.keep[1].defined()) written(k.keep[1]);
+    return none();
+}
+
+// latent_cache_read(latents, absmax, keys, block_table, length, starts, lengths, dtype or None) -> (rows [batch * length, rank], absmax [batch * length], keys or
+// None), or with a dtype (values [batch, length, rank], keys or None)
+PyObject* latent_cache_read(PyObject* const* a) {
+    CacheCall k;
+    cache_call(k, a, -1);
+    const c10::cuda::CUDAGuard device(k.latents.device());
+    el_latent_cache_t& c = k.c;
+    const int64_t B = c.batch, L = int_arg(a[4]);
+    EL_REQUIRE(L >= 0, "length must not be negative");
+    c.length = int_size(L);
+    Tensor starts = indices_arg(a[5], "starts", k.latents, {B}, INT32_MAX), lengths = lengths_arg(a[6], k.latents, B, L), out, top, keys;
+    c.starts = ptr<int32_t>(starts);
+    c.lengths = ptr<int32_t>(lengths);
+    const bool values = !is_none(a[7]);
+    if (values) {
+        const auto dt = dtype_arg(a[7]);
+        EL_REQUIRE(float_type(dt), "dtype must be float16, bfloat16 or float32");
+        c.out_dtype = code_of(dt);
+        out = new_empty(k.latents, {B, L, c.rank}, dt);
+    } else {
+        out = new_empty(k.latents, {B * L, c.rank}, at::kChar);
+        top = new_empty(k.latents, {B * L}, at::kFloat);
+    }
+    if (c.rot_dim) keys = new_empty(k.latents, {B, L, c.rot_dim}, k.keep[1].scalar_type());
+    c.out = ptr(out);
+    c.out_absmax = ptr<float>(top);
+    c.out_keys = ptr(keys);
+    call("el_latent_cache_read", g_lib.el_latent_cache_read, &c, stream_on(k.latents));
+    return values ? tuple_of(wrap(out), wrap_or_none(keys)) : tuple_of(wrap(out), wrap(top), wrap_or_none(keys));
+}
+
+// latent_attention_step(latents, absmax, keys, block_table, q, W_packed, gamma, lengths, value_dim, q_rot, table, scale or None, neighbours) -> out
+PyObject* latent_attention_step(PyObject* const* a) {
+    no_gradient("latent_attention_step", a, {4, 9, 10});
+    no_tangent("latent_attention_step", a, {4, 9, 10});
+    const Tensor& q0 = cuda_arg(a[4], "q");
+    EL_REQUIRE(float_type(q0.scalar_type()), "q must be float16, bfloat16 or float32");
+    EL_REQUIRE(q0.dim() == 3, "q must be [batch, heads, key_dim]");
+    Tensor latents, absmax, keys;
+    pool_args(a, latents, absmax, keys);
+    const c10::cuda::CUDAGuard device(latents.device());
+    EL_REQUIRE(q0.device() == latents.device(), "q is on another device");
+    const int64_t B = q0.size(0), H = q0.size(1), D = q0.size(2), V = int_arg(a[8]), R = latents.size(2), P = keys.defined() ? keys.size(2) : 0;
+    EL_REQUIRE(D <= 256 && V >= 0 && V <= 256, "keys and values of up to 256 channels are supported");
+    EL_REQUIRE(B <= 65535 && H <= 1024, "up to 65535 sequences and 1024 heads are supported");
+    Tensor blocks = block_table_arg(a[3], q0, B), q = tokens_arg(a[4], "q", q0, q0.sizes()), qr, table;
+    Tensor W = dense_arg(a[5], "W_packed", q0, at::kByte, {H * (D + V), R / 4});
+    EL_REQUIRE(reinterpret_cast<uintptr_t>(W.data_ptr()) % 4 == 0, "W_packed must lie on 4 bytes");
+    EL_REQUIRE(!is_none(a[7]), "lengths must be a CUDA tensor");
+    Tensor lengths = indices_arg(a[7], "lengths", q0, {B}, blocks.size(1) * latents.size(1));
+    EL_REQUIRE(is_none(a[9]) == (P == 0), "q_rot and the cache's keys come together");
+    if (P) {
+        EL_REQUIRE(keys.scalar_type() == q0.scalar_type(), "the cache's keys have another dtype than the activations");
+        qr = tokens_arg(a[9], "q_rot", q0, {B, H, P});
+    }
+    el_latent_step_t c = {};
+    if (!is_none(a[10])) {
+        EL_REQUIRE(P, "a table needs q_rot");
+        EL_REQUIRE(P % 2 == 0, "the rotated dimension must be even");
+        table = table_arg(a[10], q0, P);
+        c.table_rows = int_size(table.size(0));
+    }
+    c.dtype = code_of(q0.scalar_type());
+    c.batch = int_size(B);
+    c.heads = int_size(H);
+    c.key_dim = (int)D;
+    c.rot_dim = (int)P;
+    c.value_dim = (int)V;
+    c.rank = (int)R;
+    c.pages = int_size(latents.size(0));
+    c.page_size = int_size(latents.size(1));
+    c.pages_per_sequence = int_size(blocks.size(1));
+    c.neighbours = int_arg(a[12]) != 0;
+    c.scale = is_none(a[11]) ? (float)(1.0 / std::sqrt((double)(D + P > 0 ? D + P : 1))) : (float)float_arg(a[11]);
+    c.gamma = (float)float_arg(a[6]);
+    c.q = ptr(q);
+    c.q_stride_b = stride_of(q, 0);
+    c.q_stride_h = stride_of(q, 1);
+    if (qr.defined()) {
+        c.q_rot = ptr(qr);
+        c.q_rot_stride_b = stride_of(qr, 0);
+        c.q_rot_stride_h = stride_of(qr, 1);
+    }
+    c.W_packed = ptr<uint8_t>(W);
+    c.table = ptr<float>(table);
+    c.latents = ptr<int8_t>(latents);
+    c.absmax = ptr<float>(absmax);
+    c.cache_keys = ptr(keys);
+    c.block_table = ptr<int32_t>(blocks);
+    c.lengths = ptr<int32_t>(lengths);
+    c.dev_status = status_word(q);
+    Tensor out = new_empty(q, {B, H, V}, q.scalar_type());
+    c.out = ptr(out);
+    c.workspace_bytes = g_lib.el_latent_attention_step_workspace_bytes(&c);
+    Tensor ws = scratch(q, c.workspace_bytes);
+    c.workspace = ptr(ws);
+    call("el_latent_attention_step", g_lib.el_latent_attention_step, &c, stream_on(q));
+    maybe_check(q);
+    return wrap(out);
+}
+
 // ---- module -------------------------------------------------------------------------------------------------------------
 template <PyObject* (*F)(PyObject* const*), int NARGS>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -1092,6 +1498,8 @@ PyMethodDef methods[] = {
     EL_ENTRY(gemm_fwd, 7), EL_ENTRY(gemm_dx, 8), EL_ENTRY(dw_hysteresis, 11), EL_ENTRY(weight_update, 13), EL_ENTRY(linear_decode, 8), EL_ENTRY(set_hooks, 4),
     EL_ENTRY(causal_conv, 7), EL_ENTRY(causal_conv_backward, 9), EL_ENTRY(causal_conv_step, 6), EL_ENTRY(selective_scan, 13),
     EL_ENTRY(selective_scan_backward, 15), EL_ENTRY(selective_scan_step, 11), EL_ENTRY(block_norm, 8), EL_ENTRY(block_norm_backward, 11),
+    EL_ENTRY(rotary, 5), EL_ENTRY(latent_attention, 9), EL_ENTRY(latent_attention_backward, 12), EL_ENTRY(latent_cache_write, 13), EL_ENTRY(latent_cache_read, 8),
+    EL_ENTRY(latent_attention_step, 13),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "elleci_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,400 @@
+// Attention in the expanded form of latent attention, forward and backward, for every type and head size up to 256: float32 on the CUDA cores.
+//
+//   s[i,j] = scale * (q[i] . k[j] + q_rot[i] . k_rot[j]),  p[i,:] = softmax of s[i,:] over the keys that query i sees,  out[i] = sum_j p[i,j] v[j]
+//   dv[j] = sum_i p[i,j] dout[i],  ds[i,j] = p[i,j] (dout[i] . v[j] - delta[i]) scale,  delta[i] = dout[i] . out[i]
+//   dq[i] = sum_j ds[i,j] k[j],  dk[j] = sum_i ds[i,j] q[i]  (the rotated parts alike; dk_rot is the sum over the heads)
+//
+// The forward pass keeps lse[i] = log2(sum_j 2^(s[i,j] log2 e)), from which the backward kernels form p again (+inf for a query that sees nothing:
+// p = 0).  The tcgen05 kernels (latent_attention_tc.cu) take 16-bit types whose head sizes are multiples of 16; this file's take float32
+// and the other sizes.  A block holds 64 rows (queries, or keys for dk and dv) and walks over tiles of the other side.  Bound: shared-memory reads,
+// 8 for 16 multiply-adds.
+#include "latent_common.cuh"
+
+namespace el {
+
+int launch_attention_tc(const el_attention_t& a, cudaStream_t st);
+int launch_attention_backward_tc(const el_attention_t& a, const float* delta, float* rot_parts, cudaStream_t st);
+bool attention_tc_takes(const el_attention_t& a, bool backward);
+
+using namespace latent;
+
+namespace {
+
+constexpr int ROWS = 64;              // rows that a block holds
+constexpr int THREADS = 256;
+constexpr int MOST_DIM = 256;         // channels of a key (both parts) and of a value
+
+// rows `first` .. of a matrix of two parts (content, rotated) into dst [rows][pitch], zeros from row `valid` on
+template <typename T>
+__device__ void load_rows(float* dst, int pitch, int rows, const T* x, long long stride, int dim, const T* rot, long long rot_stride, int rot_dim, int first, int valid) {
+    const int all = dim + rot_dim;
+    for (int i = threadIdx.x; i < rows * all; i += THREADS) {
+        const int r = i / all, c = i - r * all;
+        float v = 0.0f;
+        if (first + r < valid) v = c < dim ? to_float(x[(first + r) * stride + c]) : to_float(rot[(first + r) * rot_stride + c - dim]);
+        dst[r * pitch + c] = v;
+    }
+}
+
+template <typename T> struct Heads {       // one head of one sequence
+    const T *q, *q_rot, *k, *k_rot, *v;
+    __device__ Heads(const el_attention_t& a, int b, int h) {
+        q = static_cast<const T*>(a.q) + b * a.q_stride_b + h * a.q_stride_h;
+        q_rot = static_cast<const T*>(a.q_rot) + b * a.q_rot_stride_b + h * a.q_rot_stride_h;
+        k = static_cast<const T*>(a.k) + b * a.k_stride_b + h * a.k_stride_h;
+        k_rot = static_cast<const T*>(a.k_rot) + b * a.k_rot_stride_b;
+        v = static_cast<const T*>(a.v) + b * a.v_stride_b + h * a.v_stride_h;
+    }
+};
+
+// A thread holds rows 4 ty .. 4 ty + 3; columns of the score tile and of the output are tx + 16 n.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_rows_kernel(const el_attention_t a) {
+    extern __shared__ float sm[];
+    const int D = a.key_dim + a.rot_dim, V = a.value_dim, DP = D | 1, VP = V | 1;
+    float* Q = sm;
+    float* K = Q + ROWS * DP;
+    float* Vs = K + ROWS * DP;
+    float* P = Vs + ROWS * VP;                      // [64][65]
+    const Place at(a);                              // the longest rows first
+    const int b = at.batch, h = at.head, i0 = ((int)(lse_pitch(a.length) / ROWS) - 1 - at.tile) * ROWS;
+    const Sequence seq(a, b);
+    const Heads<T> in(a, b, h);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const float to_log2 = a.scale * mamba::LOG2E;
+    load_rows<T>(Q, DP, ROWS, in.q, a.q_stride_t, a.key_dim, in.q_rot, a.q_rot_stride_t, a.rot_dim, i0, seq.queries);
+    float top[4], sum[4], o[4][MOST_DIM / 16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        top[r] = -INFINITY;
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < MOST_DIM / 16; ++c) o[r][c] = 0.0f;
+    }
+    const int end = seq.key_end(i0 + ROWS);
+    for (int j0 = 0; j0 < end; j0 += ROWS) {
+        __syncthreads();
+        load_rows<T>(K, DP, ROWS, in.k, a.k_stride_t, a.key_dim, in.k_rot, a.k_rot_stride_t, a.rot_dim, j0, seq.keys);
+        load_rows<T>(Vs, VP, ROWS, in.v, a.v_stride_t, V, in.v, 0, 0, j0, seq.keys);
+        __syncthreads();
+        float s[4][4] = {};
+        for (int d = 0; d < D; ++d) {
+            float x[4], y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = Q[(4 * ty + r) * DP + d];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = K[(tx + 16 * c) * DP + d];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[r][c] = fmaf(x[r], y[c], s[r][c]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = i0 + 4 * ty + r;
+            float m = top[r];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                s[r][c] = seq.sees(i, j0 + tx + 16 * c) ? s[r][c] * to_log2 : -INFINITY;
+                m = mamba::max_nan(m, s[r][c]);
+            }
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) m = mamba::max_nan(m, __shfl_xor_sync(0xffffffffu, m, w));
+            const float from = m == -INFINITY ? 0.0f : m, old = exp2_neg(top[r] - from);
+            top[r] = m;
+            float t = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float p = exp2_neg(s[r][c] - from);
+                t += p;
+                P[(4 * ty + r) * 65 + tx + 16 * c] = p;
+            }
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
+            sum[r] = fmaf(sum[r], old, t);
+#pragma unroll
+            for (int c = 0; c < MOST_DIM / 16; ++c) o[r][c] *= old;
+        }
+        __syncwarp();                               // a row of P is written and read by the same half warp
+        const int n = seq.keys - j0 < ROWS ? seq.keys - j0 : ROWS;
+        for (int j = 0; j < n; ++j) {
+            float p[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[r] = P[(4 * ty + r) * 65 + j];
+#pragma unroll
+            for (int c = 0; c < MOST_DIM / 16; ++c) {
+                if (16 * c >= V) break;
+                const float v = tx + 16 * c < V ? Vs[j * VP + tx + 16 * c] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r][c] = fmaf(p[r], v, o[r][c]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int i = i0 + 4 * ty + r;
+        const bool empty = top[r] == -INFINITY;      // also the padding
+        const float inv = 1.0f / sum[r];
+        if (a.lse && tx == 0) a.lse[((long long)b * a.heads + h) * lse_pitch(a.length) + i] = empty ? INFINITY : top[r] + log2f(sum[r]);
+        if (i >= a.length) continue;
+        T* out = static_cast<T*>(a.out) + (((long long)b * a.length + i) * a.heads + h) * V;
+#pragma unroll
+        for (int c = 0; c < MOST_DIM / 16; ++c)
+            if (tx + 16 * c < V) out[tx + 16 * c] = mamba::from_float<T>(empty ? 0.0f : o[r][c] * inv);
+    }
+}
+
+// delta[b,h,i] = dout[i] . out[i], zeros for padding.  A warp takes a row.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_delta_kernel(const el_attention_t a, float* __restrict__ delta) {
+    const long long pitch = lse_pitch(a.length), row = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+    if (row >= a.batch * (long long)a.heads * pitch) return;
+    const long long i = row % pitch, bh = row / pitch;
+    const int b = (int)(bh / a.heads), h = (int)(bh - (long long)b * a.heads), lane = threadIdx.x & 31;
+    float s = 0.0f;
+    if (i < length_of(a.lengths, b, a.length, a.length)) {
+        const T* o = static_cast<const T*>(a.out) + ((b * (long long)a.length + i) * a.heads + h) * a.value_dim;
+        const T* g = static_cast<const T*>(a.dout) + b * a.dout_stride_b + i * a.dout_stride_t + h * a.dout_stride_h;
+        for (int c = lane; c < a.value_dim; c += 32) s = fmaf(to_float(o[c]), to_float(g[c]), s);
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    if (lane == 0) delta[row] = s;
+}
+
+// KEYS: the block holds 64 keys, walks over the queries and forms dk and dv; otherwise it holds 64 queries, walks over the keys and forms dq.
+// The held side's two matrices (k and v, or q and dout) are A1 and A2, the other side's B1 and B2: s = A1 B1', dp = A2 B2'.
+template <typename T, bool KEYS>
+__global__ void __launch_bounds__(THREADS) attention_backward_rows_kernel(const el_attention_t a, const float* __restrict__ delta, float* __restrict__ rot_parts) {
+    constexpr int STEP = 32;
+    extern __shared__ float sm[];
+    const int D = a.key_dim + a.rot_dim, V = a.value_dim, DP = D | 1, VP = V | 1;
+    float* A1 = sm;
+    float* A2 = A1 + ROWS * DP;
+    float* B1 = A2 + ROWS * VP;
+    float* B2 = B1 + STEP * DP;
+    float* P = B2 + STEP * VP;                      // [64][33]
+    float* G = P + ROWS * 33;
+    const Place at(a);
+    const int b = at.batch, h = at.head, r0 = at.tile * ROWS;
+    const Sequence seq(a, b);
+    const Heads<T> in(a, b, h);
+    const T* g = static_cast<const T*>(a.dout) + b * a.dout_stride_b + h * a.dout_stride_h;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const float to_log2 = a.scale * mamba::LOG2E;
+    const long long stats = ((long long)b * a.heads + h) * lse_pitch(a.length);
+    if (KEYS) {
+        load_rows<T>(A1, DP, ROWS, in.k, a.k_stride_t, a.key_dim, in.k_rot, a.k_rot_stride_t, a.rot_dim, r0, seq.keys);
+        load_rows<T>(A2, VP, ROWS, in.v, a.v_stride_t, V, in.v, 0, 0, r0, seq.keys);
+    } else {
+        load_rows<T>(A1, DP, ROWS, in.q, a.q_stride_t, a.key_dim, in.q_rot, a.q_rot_stride_t, a.rot_dim, r0, seq.queries);
+        load_rows<T>(A2, VP, ROWS, g, a.dout_stride_t, V, g, 0, 0, r0, seq.queries);
+    }
+    float d1[4][MOST_DIM / 16], d2[4][KEYS ? MOST_DIM / 16 : 1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int c = 0; c < MOST_DIM / 16; ++c) d1[r][c] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < (KEYS ? MOST_DIM / 16 : 1); ++c) d2[r][c] = 0.0f;
+    }
+    const int begin = KEYS ? (r0 < seq.keys ? seq.query_begin(r0) / STEP * STEP : seq.queries) : 0, end = KEYS ? seq.queries : seq.key_end(r0 + ROWS);
+    for (int c0 = begin; c0 < end; c0 += STEP) {
+        __syncthreads();
+        if (KEYS) {
+            load_rows<T>(B1, DP, STEP, in.q, a.q_stride_t, a.key_dim, in.q_rot, a.q_rot_stride_t, a.rot_dim, c0, seq.queries);
+            load_rows<T>(B2, VP, STEP, g, a.dout_stride_t, V, g, 0, 0, c0, seq.queries);
+        } else {
+            load_rows<T>(B1, DP, STEP, in.k, a.k_stride_t, a.key_dim, in.k_rot, a.k_rot_stride_t, a.rot_dim, c0, seq.keys);
+            load_rows<T>(B2, VP, STEP, in.v, a.v_stride_t, V, in.v, 0, 0, c0, seq.keys);
+        }
+        __syncthreads();
+        float s[4][2] = {}, dp[4][2] = {};
+        for (int d = 0; d < D; ++d) {
+            const float y0 = B1[tx * DP + d], y1 = B1[(tx + 16) * DP + d];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float x = A1[(4 * ty + r) * DP + d];
+                s[r][0] = fmaf(x, y0, s[r][0]);
+                s[r][1] = fmaf(x, y1, s[r][1]);
+            }
+        }
+        for (int d = 0; d < V; ++d) {
+            const float y0 = B2[tx * VP + d], y1 = B2[(tx + 16) * VP + d];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float x = A2[(4 * ty + r) * VP + d];
+                dp[r][0] = fmaf(x, y0, dp[r][0]);
+                dp[r][1] = fmaf(x, y1, dp[r][1]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int row = r0 + 4 * ty + r, col = c0 + tx + 16 * c, i = KEYS ? col : row, j = KEYS ? row : col;
+                float p = 0.0f, ds = 0.0f;
+                if (seq.sees(i, j)) {
+                    p = exp2_neg(fmaf(s[r][c], to_log2, -a.lse[stats + i]));
+                    ds = p * (dp[r][c] - delta[stats + i]) * a.scale;
+                }
+                if (KEYS) P[(4 * ty + r) * 33 + tx + 16 * c] = p;
+                G[(4 * ty + r) * 33 + tx + 16 * c] = ds;
+            }
+        __syncwarp();
+        for (int c = 0; c < STEP; ++c) {
+            float x[4], y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = G[(4 * ty + r) * 33 + c];
+                y[r] = KEYS ? P[(4 * ty + r) * 33 + c] : 0.0f;
+            }
+#pragma unroll
+            for (int n = 0; n < MOST_DIM / 16; ++n) {
+                if (16 * n >= D) break;
+                const float z = tx + 16 * n < D ? B1[c * DP + tx + 16 * n] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) d1[r][n] = fmaf(x[r], z, d1[r][n]);
+            }
+            if (KEYS) {
+#pragma unroll
+                for (int n = 0; n < (KEYS ? MOST_DIM / 16 : 1); ++n) {
+                    if (16 * n >= V) break;
+                    const float z = tx + 16 * n < V ? B2[c * VP + tx + 16 * n] : 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) d2[r][n] = fmaf(y[r], z, d2[r][n]);
+                }
+            }
+        }
+    }
+    const int all = KEYS ? a.keys : a.length, live = KEYS ? seq.keys : seq.queries;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const long long row = r0 + 4 * ty + r;
+        if (row >= all) continue;
+#pragma unroll
+        for (int n = 0; n < MOST_DIM / 16; ++n) {
+            const int c = tx + 16 * n;
+            if (c >= D) continue;
+            const float v = row < live ? d1[r][n] : 0.0f;
+            if (KEYS) {
+                if (c < a.key_dim) {
+                    if (a.dk) static_cast<T*>(a.dk)[b * a.dk_stride_b + row * a.dk_stride_t + h * a.dk_stride_h + c] = mamba::from_float<T>(v);
+                } else if (rot_parts) {
+                    rot_parts[((b * (long long)a.heads + h) * a.keys + row) * a.rot_dim + c - a.key_dim] = v;
+                }
+            } else {
+                const long long to = (b * (long long)a.length + row) * a.heads + h;
+                if (c < a.key_dim) {
+                    if (a.dq) static_cast<T*>(a.dq)[to * a.key_dim + c] = mamba::from_float<T>(v);
+                } else if (a.dq_rot) {
+                    static_cast<T*>(a.dq_rot)[to * a.rot_dim + c - a.key_dim] = mamba::from_float<T>(v);
+                }
+            }
+        }
+        if (KEYS && a.dv) {
+#pragma unroll
+            for (int n = 0; n < (KEYS ? MOST_DIM / 16 : 1); ++n) {
+                const int c = tx + 16 * n;
+                if (c < V) static_cast<T*>(a.dv)[b * a.dv_stride_b + row * a.dv_stride_t + h * a.dv_stride_h + c] = mamba::from_float<T>(row < live ? d2[r][n] : 0.0f);
+            }
+        }
+    }
+}
+
+// dk_rot[b,j,c] = sum over the heads of parts[b,h,j,c], in their order
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_rot_sum_kernel(const float* __restrict__ parts, T* __restrict__ out, int heads, long long per_head, long long n) {
+    const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
+    if (i >= n) return;
+    const long long b = i / per_head, at = i - b * per_head;
+    const float* p = parts + b * heads * per_head + at;
+    float s = 0.0f;
+#pragma unroll 4
+    for (int h = 0; h < heads; ++h) s += p[h * per_head];
+    out[i] = mamba::from_float<T>(s);
+}
+
+template <typename F> int of_type(int dtype, F f) {
+    switch (dtype) {
+        case EL_F16: return f(__half());
+        case EL_BF16: return f(__nv_bfloat16());
+        default: return f(float());
+    }
+}
+
+template <typename K> int allow_shared(K kernel, int bytes, DeviceOnce& once) {
+    int dev = 0;
+    EL_CUDA_TRY(cudaGetDevice(&dev));
+    if (!once.is_done(dev)) {
+        EL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        once.mark(dev);
+    }
+    return EL_OK;
+}
+
+int forward_bytes(int D, int V) { return 4 * (2 * ROWS * (D | 1) + ROWS * (V | 1) + ROWS * 65); }
+int backward_bytes(int D, int V) { return 4 * ((ROWS + 32) * ((D | 1) + (V | 1)) + 2 * ROWS * 33); }
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+size_t delta_bytes(const el_attention_t& a) { return align16((size_t)a.batch * a.heads * lse_pitch(a.length) * 4); }
+
+}  // namespace
+
+size_t attention_lse_bytes(const el_attention_t& a) { return (size_t)a.batch * a.heads * lse_pitch(a.length) * 4; }
+size_t attention_backward_workspace_bytes(const el_attention_t& a) {
+    return delta_bytes(a) + (a.dk_rot ? align16((size_t)a.batch * a.heads * a.keys * a.rot_dim * 4) : 0);
+}
+
+int launch_attention(const el_attention_t& a, cudaStream_t st) {
+    if (attention_tc_takes(a, false)) return launch_attention_tc(a, st);
+    return of_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        static DeviceOnce once;
+        const int rc = allow_shared(attention_rows_kernel<T>, forward_bytes(MOST_DIM, MOST_DIM), once);
+        if (rc != EL_OK) return rc;
+        // every row of the padded log sums is written
+        attention_rows_kernel<T><<<blocks_of(a, (int)lse_pitch(a.length), ROWS), THREADS, forward_bytes(a.key_dim + a.rot_dim, a.value_dim), st>>>(a);
+        return check_launch();
+    });
+}
+
+int launch_attention_backward(const el_attention_t& a, cudaStream_t st) {
+    float* delta = static_cast<float*>(a.workspace);
+    float* rot_parts = a.dk_rot ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + delta_bytes(a)) : nullptr;
+    return of_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        if (a.length > 0) {
+            const long long rows = (long long)a.batch * a.heads * lse_pitch(a.length);
+            attention_delta_kernel<T><<<(unsigned)((rows + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, st>>>(a, delta);
+            int rc = check_launch();
+            if (rc != EL_OK) return rc;
+        }
+        int rc = EL_OK;
+        if (attention_tc_takes(a, true)) {
+            rc = launch_attention_backward_tc(a, delta, rot_parts, st);
+            if (rc != EL_OK) return rc;
+        } else {
+            const int bytes = backward_bytes(a.key_dim + a.rot_dim, a.value_dim);
+            static DeviceOnce once[2];
+            if ((a.dk || a.dv || a.dk_rot) && a.keys > 0) {
+                rc = allow_shared(attention_backward_rows_kernel<T, true>, backward_bytes(MOST_DIM, MOST_DIM), once[0]);
+                if (rc != EL_OK) return rc;
+                attention_backward_rows_kernel<T, true><<<blocks_of(a, a.keys, ROWS), THREADS, bytes, st>>>(a, delta, rot_parts);
+                if ((rc = check_launch()) != EL_OK) return rc;
+            }
+            if ((a.dq || a.dq_rot) && a.length > 0) {
+                rc = allow_shared(attention_backward_rows_kernel<T, false>, backward_bytes(MOST_DIM, MOST_DIM), once[1]);
+                if (rc != EL_OK) return rc;
+                attention_backward_rows_kernel<T, false><<<blocks_of(a, a.length, ROWS), THREADS, bytes, st>>>(a, delta, rot_parts);
+                if ((rc = check_launch()) != EL_OK) return rc;
+            }
+        }
+        if (!a.dk_rot || a.keys == 0) return rc;
+        const long long per_head = (long long)a.keys * a.rot_dim, n = a.batch * per_head;
+        attention_rot_sum_kernel<T><<<(unsigned)((n + THREADS - 1) / THREADS), THREADS, 0, st>>>(rot_parts, static_cast<T*>(a.dk_rot), a.heads, per_head, n);
+        return check_launch();
+    });
+}
+
+}  // namespace el

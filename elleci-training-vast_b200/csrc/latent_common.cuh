@@ -1,0 +1,58 @@
+// Shared device helpers of the operators of latent attention (latent_attention.cu, latent_attention_tc.cu, latent_cache.cu, latent_step.cu).
+#pragma once
+#include "mamba_common.cuh"
+
+namespace el {
+namespace latent {
+
+// a length from device memory (or `all` where there is none), clamped to 0 .. most
+__device__ __forceinline__ int length_of(const int32_t* lengths, int b, int all, int most) {
+    const int n = lengths ? lengths[b] : all;
+    return n < 0 ? 0 : n > most ? most : n;
+}
+
+// The rows of one sequence in an attention: query i (of `queries`) sees key j (of `keys`) if j <= i + shift.  Without causality the shift lets
+// every query see every key.
+struct Sequence {
+    int queries, keys;
+    long long shift;
+    __device__ __forceinline__ Sequence(const el_attention_t& a, int b) {
+        queries = length_of(a.lengths, b, a.length, a.length);
+        keys = length_of(a.key_lengths, b, a.keys, a.keys);
+        shift = a.causal ? (long long)keys - queries : (long long)keys;
+    }
+    __device__ __forceinline__ bool sees(int i, int j) const { return i < queries && j < keys && j <= i + shift; }
+    // keys that some query of i0 .. i1 - 1 sees: 0 .. end - 1
+    __device__ __forceinline__ int key_end(int i1) const {
+        const int last = (i1 < queries ? i1 : queries) - 1;
+        if (last < 0) return 0;
+        const long long e = last + shift + 1;
+        return e < 0 ? 0 : e > keys ? keys : (int)e;
+    }
+    // the first query that sees key j
+    __device__ __forceinline__ int query_begin(int j) const {
+        const long long i = j - shift;
+        return i < 0 ? 0 : i > queries ? queries : (int)i;
+    }
+};
+
+constexpr int LSE_PAD = 128;          // the rows of a log-sum array are padded to a multiple of this
+__host__ __device__ inline long long lse_pitch(int length) { return ((long long)length + LSE_PAD - 1) / LSE_PAD * LSE_PAD; }
+
+// A block's tile, sequence and head: all heads of all sequences take their first tiles first.
+struct Place {
+    int tile, batch, head;
+    __device__ __forceinline__ Place(const el_attention_t& a) {
+        const unsigned pairs = (unsigned)a.batch * a.heads, t = blockIdx.x / pairs, bh = blockIdx.x - t * pairs;
+        tile = (int)t;
+        batch = (int)(bh / a.heads);
+        head = (int)(bh - (unsigned)batch * a.heads);
+    }
+};
+inline unsigned blocks_of(const el_attention_t& a, int rows, int tile) { return (unsigned)((rows + (long long)tile - 1) / tile * a.batch * a.heads); }
+
+// 2^x where x <= 0 or -inf (0 then)
+__device__ __forceinline__ float exp2_neg(float x) { return mamba::ex2(x); }
+
+}  // namespace latent
+}  // namespace el

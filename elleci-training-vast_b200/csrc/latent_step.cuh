@@ -1,0 +1,76 @@
+// What the kernels of a step against the cache of latent vectors share (latent_step.cu, latent_step_tc.cu): the division of all sequences' tokens
+// among blocks, and the layout of what a block leaves.
+//
+// The sequences' tiles of STEP_TILE tokens lie one after another, N in all; worker w of G <= N takes tiles w N / G .. (w + 1) N / G - 1, which may be
+// parts of several sequences.  Every worker has the same share whatever the lengths are.  What worker w found in sequence b (each head's largest
+// score, its sum and its weighted latent vectors) goes to slot w + b: from one part of a worker to its next b grows, and where one worker ends inside a
+// sequence the next one begins there, so no two parts share a slot.
+#pragma once
+#include "latent_common.cuh"
+
+namespace el {
+namespace latent {
+
+constexpr int STEP_TILE = 64;
+
+__device__ __forceinline__ int step_tokens(const el_latent_step_t& a, int b) {
+    return length_of(a.lengths, b, 0, (int)min((long long)a.pages_per_sequence * a.page_size, 0x7fffff00LL));
+}
+__device__ __forceinline__ int step_tiles(const el_latent_step_t& a, int b) { return (step_tokens(a, b) + STEP_TILE - 1) / STEP_TILE; }
+
+// Tiles of all sequences before sequence `upto`; called by a whole warp.
+__device__ __forceinline__ long long step_tiles_before(const el_latent_step_t& a, int upto) {
+    long long n = 0;
+    for (int b = threadIdx.x & 31; b < upto; b += 32) n += step_tiles(a, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+}
+// The sequence that tile `t` (of all) belongs to and the tiles before that sequence; called by a whole warp, t < all tiles.
+__device__ __forceinline__ void step_find(const el_latent_step_t& a, long long t, int& seq, long long& before) {
+    const int lane = threadIdx.x & 31;
+    before = 0;
+    for (int b0 = 0;; b0 += 32) {
+        const int n = b0 + lane < a.batch ? step_tiles(a, b0 + lane) : 0;
+        long long upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + upto > t);
+        if (past || b0 + 32 >= a.batch) {
+            const int l = past ? __ffs(past) - 1 : 31;
+            seq = b0 + l;
+            before += __shfl_sync(0xffffffffu, upto - n, l);
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+// workers with something to do: of as many as there are tiles, or fewer, none is without one
+__device__ __forceinline__ int step_active(int workers, long long tiles) { return tiles < workers ? (int)tiles : workers; }
+// the worker that has tile t
+__device__ __forceinline__ int step_worker(long long t, int workers, long long tiles) { return (int)(((t + 1) * workers - 1) / tiles); }
+
+// A slot: for each head its largest score and its sum, then the heads' latent vectors.
+struct StepParts {
+    float* base;
+    int heads, rank;
+    __device__ __forceinline__ float* stats(long long slot) const { return base + slot * heads * (2LL + rank); }
+    __device__ __forceinline__ float* vectors(long long slot) const { return stats(slot) + 2 * heads; }
+};
+
+// The query of one head against latent vectors: [rank + rot_dim], scaled so that scores are exponents of 2.
+inline size_t step_query_bytes(const el_latent_step_t& a, int element) {
+    return ((size_t)a.batch * a.heads * (a.rank + a.rot_dim) * element + 255) / 256 * 256;
+}
+
+// the pool's row of position p of sequence b, or -1
+__device__ __forceinline__ long long step_row(const el_latent_step_t& a, int b, int p) {
+    const int page = a.block_table[(long long)b * a.pages_per_sequence + p / a.page_size];
+    return page < 0 || page >= a.pages ? -1 : (long long)page * a.page_size + p % a.page_size;
+}
+
+}  // namespace latent
+}  // namespace el

@@ -538,6 +538,128 @@ EL_API int el_block_norm(const el_block_norm_t* args, el_stream_t stream);
 EL_API size_t el_block_norm_backward_workspace_bytes(const el_block_norm_t* args);
 EL_API int el_block_norm_backward(const el_block_norm_t* args, el_stream_t stream);
 
+/* ---- latent attention ----------------------------------------------------------------------------------- */
+
+/* Attention whose keys and values come from one latent vector a token: an INT2 layer (the up projection) makes every head's key and value of it.  Part of
+ * a key may be rotated by its position instead; that part is one for all heads.  Types and strides as for the Mamba block's operators.  Outside the
+ * reference's INT2 path: its block calls torch's attention (model/common/mla.py). */
+
+/* Rotation by position: y = x with the pairs (x[i], x[i + dim/2]) (neighbours 0) or (x[2i], x[2i+1]) (neighbours 1) turned by the angles of the token's
+ * position.  table [table_rows, dim]: a row holds the dim/2 cosines, then the sines.  positions: [batch] the position of a sequence's first token, or with
+ * position_each [batch, length], or NULL (token t is at t); positions outside the table are clamped to it.  inverse: turned back, which is the gradient. */
+typedef struct el_rotary_t {
+    int dtype, batch, length, heads, dim, table_rows, neighbours, inverse, position_each;
+    const void* x;                      /* [batch, length, heads, dim] */
+    long long x_stride_b, x_stride_t, x_stride_h;
+    const float* table;
+    const int32_t* positions;
+    void* y;                            /* [batch, length, heads, dim] */
+} el_rotary_t;
+EL_API int el_rotary(const el_rotary_t* args, el_stream_t stream);
+
+/* The expanded form, for training and prompts:
+ *   s[i,j] = scale * (q[i,h] . k[j,h] + q_rot[i,h] . k_rot[j]),  out[i,h] = sum_j softmax_j(s[i,j]) v[j,h]
+ * over the keys that query i sees: of a sequence with m = lengths[b] queries and n = key_lengths[b] keys those below n and, with `causal`, up to
+ * i + n - m (its queries are its last tokens).  A query that sees no key, and padding, has the output 0.  key_dim + rot_dim and value_dim up to
+ * 256; rot_dim 0 for none.  lse (el_latent_attention_lse_bytes; NULL when no gradient is wanted) is what the backward pass needs beside the inputs and out.
+ * el_latent_attention_backward writes dq, dq_rot, dk, dv, dk_rot (each may be NULL) from dout; all sums have a fixed order.  dk and dv have strides of
+ * their own, so that they can be parts of one tensor.  16-bit types whose three head sizes are multiples of 16 up to 128, 64 and 128 with strides and bases on
+ * 16 bytes run on the tensor cores, which take probabilities and their gradients rounded to the type (float32 sums); the others run in float32.
+ * Padding is not read; an infinity or NaN in a token's own key or value reaches the queries of its tile, also those that do not see it. */
+typedef struct el_attention_t {
+    int dtype, batch, length, keys, heads, key_dim, rot_dim, value_dim, causal;
+    float scale;
+    const void* q;                      /* [batch, length, heads, key_dim] */
+    long long q_stride_b, q_stride_t, q_stride_h;
+    const void* q_rot;                  /* [batch, length, heads, rot_dim] */
+    long long q_rot_stride_b, q_rot_stride_t, q_rot_stride_h;
+    const void* k;                      /* [batch, keys, heads, key_dim] */
+    long long k_stride_b, k_stride_t, k_stride_h;
+    const void* v;                      /* [batch, keys, heads, value_dim] */
+    long long v_stride_b, v_stride_t, v_stride_h;
+    const void* k_rot;                  /* [batch, keys, rot_dim] */
+    long long k_rot_stride_b, k_rot_stride_t;
+    const int32_t* lengths;             /* [batch] or NULL: all `length` */
+    const int32_t* key_lengths;         /* [batch] or NULL: all `keys` */
+    void* out;                          /* [batch, length, heads, value_dim] */
+    float* lse;
+    const void* dout;
+    long long dout_stride_b, dout_stride_t, dout_stride_h;
+    void* dq;                           /* dense, as q */
+    void* dq_rot;                       /* dense, as q_rot */
+    void* dk;
+    long long dk_stride_b, dk_stride_t, dk_stride_h;
+    void* dv;
+    long long dv_stride_b, dv_stride_t, dv_stride_h;
+    void* dk_rot;                       /* dense, as k_rot */
+    void* workspace;                    /* backward: el_latent_attention_backward_workspace_bytes, 16-byte aligned */
+    size_t workspace_bytes;
+    int32_t* dev_status;
+} el_attention_t;
+EL_API size_t el_latent_attention_lse_bytes(const el_attention_t* args);
+EL_API int el_latent_attention(const el_attention_t* args, el_stream_t stream);
+EL_API size_t el_latent_attention_backward_workspace_bytes(const el_attention_t* args);
+EL_API int el_latent_attention_backward(const el_attention_t* args, el_stream_t stream);
+
+/* The cache of latent vectors: a pool of `pages` pages of page_size tokens.  A token is an int8 row [rank] and its largest magnitude (value = row * absmax /
+ * 127: what the up projection's own quantiser makes of it, so el_gemm_fwd takes rows that were read back as they are) and a rotated key part [rot_dim] of type
+ * dtype.  rank: a multiple of 16 up to 512; rot_dim up to 64, even where a table is given.  Position p of sequence b is token p % page_size of page
+ * block_table[b][p / page_size]; positions beyond the table and entries outside the pool are not followed: nothing is written there, zeros are read.
+ * el_latent_cache_write: tokens x [batch, length, rank] (through the RMSNorm of el_rmsnorm_quantize_rows where norm_weight is given, same bits) and k_rot
+ * [batch, length, rot_dim] (rotated by table, NULL: as it is) to positions starts[b] (NULL: 0) + t, t < lengths[b].  Two tokens of a call
+ * must not share a place.
+ * el_latent_cache_read: positions starts[b] + t, t < lengths[b] (zeros from there on): out [batch, length, rank] int8 rows and out_absmax [batch, length]
+ * (out_dtype < 0), or values of out_dtype; out_keys [batch, length, rot_dim]. */
+typedef struct el_latent_cache_t {
+    int dtype, batch, length, rank, rot_dim, pages, page_size, pages_per_sequence, table_rows, neighbours, out_dtype;
+    int x_aligned;                      /* set by the library */
+    float norm_eps, quant_eps;
+    int8_t* latents;                    /* [pages, page_size, rank], 16-byte aligned */
+    float* absmax;                      /* [pages, page_size] */
+    void* cache_keys;                   /* [pages, page_size, rot_dim] */
+    const int32_t* block_table;         /* [batch, pages_per_sequence] */
+    const int32_t* starts;              /* [batch] or NULL */
+    const int32_t* lengths;             /* [batch] or NULL */
+    const void* x;
+    long long x_stride_b, x_stride_t;
+    const float* norm_weight;           /* [rank] or NULL */
+    const void* k_rot;
+    long long k_rot_stride_b, k_rot_stride_t;
+    const float* table;                 /* [table_rows, rot_dim] or NULL */
+    void* out;
+    float* out_absmax;
+    void* out_keys;
+} el_latent_cache_t;
+EL_API int el_latent_cache_write(const el_latent_cache_t* args, el_stream_t stream);
+EL_API int el_latent_cache_read(const el_latent_cache_t* args, el_stream_t stream);
+
+/* The absorbed form, for one token of every sequence against the cache, which already holds that token (position lengths[b] - 1):
+ *   out[b,h] = sum_j softmax_j(scale * (q[b,h] . k[j,h] + rotated q_rot[b,h] . key[j])) v[j,h],  j < lengths[b]
+ * with k and v those that the up projection W_packed [heads * (key_dim + value_dim), rank / 4] (all heads' keys, then all heads' values) with weight
+ * scale gamma would make of the cached rows; they are not formed.  lengths 0 gives 0; tokens of pages outside the pool are passed over.  q_rot is rotated by
+ * table (NULL: as it is).  key_dim and value_dim up to 256, W_packed on 4 bytes. */
+typedef struct el_latent_step_t {
+    int dtype, batch, heads, key_dim, rot_dim, value_dim, rank, pages, page_size, pages_per_sequence, table_rows, neighbours;
+    float scale, gamma;
+    const void* q;                      /* [batch, heads, key_dim] */
+    long long q_stride_b, q_stride_h;
+    const void* q_rot;                  /* [batch, heads, rot_dim] */
+    long long q_rot_stride_b, q_rot_stride_h;
+    const uint8_t* W_packed;
+    const float* table;                 /* [table_rows, rot_dim] or NULL */
+    const int8_t* latents;
+    const float* absmax;
+    const void* cache_keys;
+    const int32_t* block_table;
+    const int32_t* lengths;
+    void* out;                          /* [batch, heads, value_dim] */
+    void* workspace;                    /* el_latent_attention_step_workspace_bytes, 256-byte aligned */
+    size_t workspace_bytes;
+    int32_t* dev_status;
+} el_latent_step_t;
+EL_API size_t el_latent_attention_step_workspace_bytes(const el_latent_step_t* args);
+EL_API int el_latent_attention_step(const el_latent_step_t* args, el_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
