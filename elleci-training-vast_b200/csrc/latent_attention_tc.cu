@@ -1,6 +1,372 @@
-#include "latent_common.cuh"
+// The forward pass of latent attention's expanded form on the tensor cores (latent_attention.cu has the formulas): 16-bit types, head sizes that are
+// multiples of 16 up to 128 (content), 64 (rotated) and 128 (value).
+//
+// A block takes 256 queries of one head as two tiles of 128 rows, which share the keys' tiles of 128: while the softmax of one tile runs, the
+// tensor core works on the other.  Warps: 0-3 and 4-7 softmax of the two tiles (a thread owns a row), 8 issues the products, 9 the loads.
+//   S_i = Q_i K'   accumulator of 128 columns in tensor memory; the thread reads its row, forms p = 2^(s - reference) and writes it back as 16-bit
+//                  values over S_i, where it is the left factor of
+//   O_i += P_i V   whose sums stay in tensor memory.  The reference of a row follows its maximum only when that has grown by more than 2^8:
+//                  then the row of O_i is scaled.  P stays below 2^8, sums are float32.
+// Order of products: P_0 V, S_0 of the next keys, P_1 V, S_1 of the next keys.  Keys and values go through one ring of 16 KB chunks in the order in
+// which they are first used.
+#include "latent_tc.cuh"
+
 namespace el {
-bool attention_tc_takes(const el_attention_t&, bool) { return false; }
-int launch_attention_tc(const el_attention_t&, cudaStream_t) { return EL_ERR_UNSUPPORTED_SHAPE; }
-int launch_attention_backward_tc(const el_attention_t&, const float*, float*, cudaStream_t) { return EL_ERR_UNSUPPORTED_SHAPE; }
+
+using namespace tc;
+using namespace latent;
+
+namespace {
+
+constexpr int TILE = 128;                       // rows of a query tile, and keys of a tile
+constexpr int CHUNK = TILE * 128;               // bytes of 64 columns of a tile
+constexpr int MAX_SLOTS = 12;
+constexpr int WARP_MMA = 8, WARP_TMA = 9, THREADS = 320;
+constexpr float GROWTH = 8.0f;                  // exponent of 2 by which a row's maximum may outgrow its reference
+
+struct Plan {
+    int key_chunks, rot_chunks, value_chunks;   // of 64 columns
+    int slots;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQr, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmKr, const __grid_constant__ CUtensorMap tmV, const el_attention_t a, const Plan plan) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const int QC = plan.key_chunks + plan.rot_chunks, VC = plan.value_chunks, NS = plan.slots;
+    const uint32_t ring = base + 2 * QC * CHUNK;
+    uint8_t* ring_gen = gen + 2 * QC * CHUNK;
+    const uint32_t bars = ring + NS * CHUNK;
+    auto q_full = [&](int i) { return bars + 8u * i; };
+    auto s_full = [&](int i) { return bars + 8u * (2 + i); };
+    auto p_full = [&](int i) { return bars + 8u * (4 + i); };
+    auto o_full = [&](int i) { return bars + 8u * (6 + i); };
+    const uint32_t landed = bars + 8u * 8;
+    auto slot_full = [&](int s) { return bars + 8u * (9 + s); };
+    auto slot_empty = [&](int s) { return bars + 8u * (9 + MAX_SLOTS + s); };
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * CHUNK + 8 * (9 + 2 * MAX_SLOTS));
+
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const Place at(a);
+    const int pairs = (a.length + 2 * TILE - 1) / (2 * TILE), b = at.batch, h = at.head;
+    const int i0 = (pairs - 1 - at.tile) * 2 * TILE;            // the longest rows first
+    const Sequence seq(a, b);
+    // key tiles of the two query tiles
+    const int n0 = i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0, n1 = i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0;
+    const int n = n0 > n1 ? n0 : n1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full(i), 1);
+            mbar_init(s_full(i), 1);
+            mbar_init(p_full(i), 4);
+            mbar_init(o_full(i), 1);
+        }
+        mbar_init(landed, 1);
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(slot_full(s), 1);
+            mbar_init(slot_empty(s), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == WARP_MMA) tmem_alloc<512>(smem_u32((const void*)tmem_holder));
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const uint32_t S = tmem, O = tmem + 256;                    // S_i at 128 i, O_i at 256 + 128 i
+    int32_t* status = a.dev_status;
+
+    if (warp == WARP_TMA) {
+        // ================= loads =================
+        for (int i = 0; i < 2; ++i) {
+            if ((i == 0 ? n0 : n1) == 0) continue;
+            if (elect_one()) {
+                mbar_expect_tx(q_full(i), QC * CHUNK);
+                for (int c = 0; c < plan.key_chunks; ++c)
+                    tma_load_3d(base + (i * QC + c) * CHUNK, &tmQ, q_full(i), (int)(h * a.q_stride_h) + c * CHUNK_COLS, i0 + i * TILE, b);
+                if (plan.rot_chunks) tma_load_3d(base + (i * QC + plan.key_chunks) * CHUNK, &tmQr, q_full(i), (int)(h * a.q_rot_stride_h), i0 + i * TILE, b);
+            }
+            __syncwarp();
+        }
+        int s = 0;
+        uint32_t ph = 0, land = 0;
+        bool ok = true;
+        for (int j = 0; j < n && ok; ++j) {
+            // values behind the sequence's end may be anything, and zero times anything is not always zero: those rows are cleared
+            const int live = seq.keys - j * TILE;
+            const bool clear = live < TILE && j * TILE + live < a.keys;
+            for (int c = 0; c < QC + VC; ++c) {
+                if (!mbar_wait_warp(slot_empty(s), ph ^ 1u, status, 1)) { ok = false; break; }
+                const bool value = c >= QC, late = value && clear;
+                if (elect_one()) {
+                    const uint32_t dst = ring + s * CHUNK, bar = late ? landed : slot_full(s);
+                    mbar_expect_tx(bar, CHUNK);
+                    if (value) tma_load_3d(dst, &tmV, bar, (int)(h * a.v_stride_h) + (c - QC) * CHUNK_COLS, j * TILE, b);
+                    else if (c < plan.key_chunks) tma_load_3d(dst, &tmK, bar, (int)(h * a.k_stride_h) + c * CHUNK_COLS, j * TILE, b);
+                    else tma_load_3d(dst, &tmKr, bar, 0, j * TILE, b);
+                }
+                __syncwarp();
+                if (late) {
+                    if (!mbar_wait_warp(landed, land, status, 2)) { ok = false; break; }
+                    land ^= 1u;
+                    uint4* rows = reinterpret_cast<uint4*>(ring_gen + s * CHUNK);
+                    for (int k = live * 8 + lane; k < TILE * 8; k += 32) rows[k] = make_uint4(0u, 0u, 0u, 0u);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive(slot_full(s));
+                    __syncwarp();
+                }
+                if (++s == NS) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == WARP_MMA) {
+        // ================= products =================
+        const uint32_t i_s = idesc_f16<T>(0, 0, TILE);
+        const int key_steps = a.key_dim / 16, rot_steps = a.rot_dim / 16, V = a.value_dim;
+        bool ok = true;
+        // ring position of the first chunk of keys j: chunks are taken in order
+        auto slot_of = [&](int chunk) { return chunk % NS; };
+        auto phase_of = [&](int chunk) { return (uint32_t)(chunk / NS) & 1u; };
+        auto wait_chunks = [&](int first, int count) {
+            for (int c = first; c < first + count && ok; ++c) ok = mbar_wait_warp(slot_full(slot_of(c)), phase_of(c), status, 3);
+            tcgen05_fence_after();
+        };
+        auto release = [&](int first, int count) {
+            for (int c = first; c < first + count; ++c) umma_commit(slot_empty(slot_of(c)));
+        };
+        auto scores = [&](int i, int first) {                   // S_i = Q_i K'; one thread
+            for (int c = 0; c < QC; ++c) {
+                const uint32_t q = base + (i * QC + c) * CHUNK, k = ring + slot_of(first + c) * CHUNK;
+                const int steps = c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps;
+                for (int x = 0; x < steps; ++x) umma_f16(S + i * 128, make_desc(q + x * 32, 16), make_desc(k + x * 32, 16), i_s, (c | x) != 0);
+            }
+            umma_commit(s_full(i));
+        };
+        auto values = [&](int i, int first, bool more) {        // O_i += P_i V; one thread
+            const int s0 = slot_of(first);
+            if (VC == 1 || s0 + 1 < NS) {                       // the chunks lie side by side
+                const uint32_t id = idesc_f16<T>(0, 1, V);
+                for (int x = 0; x < TILE / 16; ++x) umma_f16_ts(O + i * 128, S + i * 128 + x * 8, make_desc(ring + s0 * CHUNK + x * 2048, CHUNK), id, more || x != 0);
+            } else {
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t id = idesc_f16<T>(0, 1, c == 0 ? 64 : V - 64), v = ring + slot_of(first + c) * CHUNK;
+                    for (int x = 0; x < TILE / 16; ++x) umma_f16_ts(O + i * 128 + c * 64, S + i * 128 + x * 8, make_desc(v + x * 2048, CHUNK), id, more || x != 0);
+                }
+            }
+            umma_commit(o_full(i));
+        };
+        if (n > 0) {
+            for (int i = 0; i < 2 && ok; ++i) {
+                if ((i == 0 ? n0 : n1) == 0) continue;
+                ok = mbar_wait_warp(q_full(i), 0, status, 4);
+                wait_chunks(0, QC);
+                if (ok && elect_one()) scores(i, 0);
+                __syncwarp();
+            }
+            if (ok && elect_one()) release(0, QC);
+            __syncwarp();
+        }
+        for (int j = 0; j < n && ok; ++j) {
+            const int v = j * (QC + VC) + QC, k = (j + 1) * (QC + VC);
+            for (int i = 0; i < 2 && ok; ++i) {
+                const int mine = i == 0 ? n0 : n1;
+                if (j >= mine) continue;
+                ok = mbar_wait_warp(p_full(i), (uint32_t)j & 1u, status, 5);
+                if (ok) wait_chunks(v, VC);
+                if (ok && elect_one()) values(i, v, j != 0);
+                __syncwarp();
+                if (j + 1 < mine && ok) {
+                    wait_chunks(k, QC);
+                    if (ok && elect_one()) scores(i, k);
+                    __syncwarp();
+                }
+            }
+            if (ok && elect_one()) {
+                release(v, VC);
+                if (j + 1 < n) release(k, QC);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ================= softmax =================
+        const int i = warp >> 2, mine = i == 0 ? n0 : n1, quarter = warp & 3;
+        const int row = i0 + i * TILE + quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t s_addr = S + i * 128 + lanes, o_addr = O + i * 128 + lanes;
+        const float by = a.scale * mamba::LOG2E;
+        // keys that this row sees: 0 .. sees - 1
+        long long sees = row < seq.queries ? row + seq.shift + 1 : 0;
+        sees = sees < 0 ? 0 : sees > seq.keys ? seq.keys : sees;
+        float ref = -INFINITY, sum = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < mine; ++j) {
+            if (!(ok = mbar_wait_warp(s_full(i), (uint32_t)j & 1u, status, 6))) break;
+            tcgen05_fence_after();
+            uint32_t v[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
+            tmem_ld_wait();
+            const int here = (int)sees - j * TILE;               // columns that the row sees
+            if (__any_sync(0xffffffffu, here < TILE)) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[c][k] = c * 32 + k < here ? v[c][k] : 0xff800000u;
+            }
+            float top[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                top[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+                for (int k = 1; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(v[c][k]));
+            }
+            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * by;
+            const bool grown = m > ref + GROWTH;                 // also a row's first finite maximum
+            if (__any_sync(0xffffffffu, grown)) {
+                const float to = grown ? m : ref, factor = grown && ref != -INFINITY ? exp2_neg(ref - m) : 1.0f;
+                if (j > 0) {
+                    if (!(ok = mbar_wait_warp(o_full(i), (uint32_t)(j - 1) & 1u, status, 7))) break;
+                    tcgen05_fence_after();
+                    for (int c = 0; c < a.value_dim; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_addr + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                        tmem_st16(o_addr + c, o);
+                    }
+                    tmem_st_wait();
+                }
+                sum *= factor;
+                ref = to;
+            }
+            const float from = ref == -INFINITY ? 0.0f : -ref;
+            const rowio::f32x2 by2 = rowio::pair(by, by), from2 = rowio::pair(from, from);
+            rowio::f32x2 part[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) part[c] = rowio::pair(0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                uint32_t p[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    const int e = 2 * k, cc = c + e / 32;
+                    const rowio::f32x2 x = rowio::fma2(rowio::pair(__uint_as_float(v[cc][e % 32]), __uint_as_float(v[cc][e % 32 + 1])), by2, from2);
+                    const float y0 = mamba::ex2(rowio::lo_of(x)), y1 = mamba::ex2(rowio::hi_of(x));
+                    part[k & 3] = rowio::add2(part[k & 3], rowio::pair(y0, y1));
+                    p[k] = pack_word<T>(y0, y1);
+                }
+                tmem_st32(s_addr + c * 16, p);
+            }
+            const rowio::f32x2 t = rowio::add2(rowio::add2(part[0], part[1]), rowio::add2(part[2], part[3]));
+            sum += rowio::lo_of(t) + rowio::hi_of(t);
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(i));
+        }
+        const bool empty = ref == -INFINITY && !(sum != sum);    // sees nothing; a NaN is no such row
+        const float inv = 1.0f / sum;
+        if (a.lse && row < lse_pitch(a.length))
+            a.lse[((long long)b * a.heads + h) * lse_pitch(a.length) + row] = empty ? INFINITY : ref + log2f(sum);
+        if (ok && mine > 0) ok = mbar_wait_warp(o_full(i), (uint32_t)(mine - 1) & 1u, status, 8);
+        tcgen05_fence_after();
+        if (ok) {
+            T* out = static_cast<T*>(a.out) + (((long long)b * a.length + row) * a.heads + h) * a.value_dim;
+            for (int c = 0; c < a.value_dim; c += 16) {
+                uint32_t o[16], w[8];
+                if (mine > 0) {
+                    tmem_ld16(o_addr + c, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    w[k] = mine == 0 || empty ? 0u : pack_word<T>(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
+                if (row < a.length) {
+                    *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+            }
+        }
+    }
+    if (status != nullptr && *reinterpret_cast<volatile int32_t*>(status) != 0) {
+        // a wait gave up somewhere: copies and products still in flight get time to land before their memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) { }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == WARP_MMA) {
+        tcgen05_fence_after();
+        tmem_free<512>(tmem);
+    }
 }
+
+Plan plan_of(const el_attention_t& a) {
+    Plan p;
+    p.key_chunks = (a.key_dim + 63) / 64;
+    p.rot_chunks = (a.rot_dim + 63) / 64;
+    p.value_chunks = (a.value_dim + 63) / 64;
+    const int room = (227 * 1024 - 2048) / CHUNK - 2 * (p.key_chunks + p.rot_chunks);
+    p.slots = room < MAX_SLOTS ? room : MAX_SLOTS;
+    return p;
+}
+int shared_bytes(const Plan& p) { return 1024 + (2 * (p.key_chunks + p.rot_chunks) + p.slots) * CHUNK + 8 * (9 + 2 * MAX_SLOTS) + 16; }
+
+bool map_takes(const void* base, long long stride_b, long long stride_t, long long stride_h, int heads) {
+    return stride_h >= 0 && (heads - 1) * stride_h < (1LL << 30) && reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride_b % 8 == 0 && stride_t % 8 == 0 && stride_h % 8 == 0;
+}
+
+template <typename T> int launch(const el_attention_t& a, const Plan& plan, const CUtensorMap* m, cudaStream_t st) {
+    static DeviceOnce once;
+    int dev = 0;
+    EL_CUDA_TRY(cudaGetDevice(&dev));
+    if (!once.is_done(dev)) {
+        EL_CUDA_TRY(cudaFuncSetAttribute(attention_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        once.mark(dev);
+    }
+    attention_tc_kernel<T><<<blocks_of(a, a.length, 2 * TILE), THREADS, shared_bytes(plan), st>>>(m[0], m[1], m[2], m[3], m[4], a, plan);
+    return check_launch();
+}
+
+}  // namespace
+
+// Whether the tensor-core kernels take the call.  Scales that are not positive would turn maxima into minima.
+bool attention_tc_takes(const el_attention_t& a, bool backward) {
+    if (a.dtype == EL_F32 || a.key_dim % 16 || a.rot_dim % 16 || a.value_dim % 16 || a.key_dim < 16 || a.key_dim > 128 || a.rot_dim > 64 || a.value_dim < 16 || a.value_dim > 128)
+        return false;
+    if (a.length == 0 || a.keys == 0 || !(a.scale > 0.0f && a.scale < 1e30f)) return false;
+    if (!map_takes(a.q, a.q_stride_b, a.q_stride_t, a.q_stride_h, a.heads) || !map_takes(a.k, a.k_stride_b, a.k_stride_t, a.k_stride_h, a.heads) ||
+        !map_takes(a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h, a.heads) || reinterpret_cast<uintptr_t>(a.out) % 16)
+        return false;
+    if (a.rot_dim && (!map_takes(a.q_rot, a.q_rot_stride_b, a.q_rot_stride_t, a.q_rot_stride_h, a.heads) || !map_takes(a.k_rot, a.k_rot_stride_b, a.k_rot_stride_t, 0, 1))) return false;
+    return !backward;
+}
+
+int attention_maps(const el_attention_t& a, CUtensorMap m[5], int query_rows, int key_rows) {
+    int rc = make_map_tokens(&m[0], a.q, (a.heads - 1) * a.q_stride_h + a.key_dim, a.length, a.q_stride_t, a.batch, a.q_stride_b, query_rows);
+    if (rc == EL_OK) rc = make_map_tokens(&m[2], a.k, (a.heads - 1) * a.k_stride_h + a.key_dim, a.keys, a.k_stride_t, a.batch, a.k_stride_b, key_rows);
+    if (rc == EL_OK) rc = make_map_tokens(&m[4], a.v, (a.heads - 1) * a.v_stride_h + a.value_dim, a.keys, a.v_stride_t, a.batch, a.v_stride_b, key_rows);
+    m[1] = m[0];
+    m[3] = m[2];
+    if (rc == EL_OK && a.rot_dim) rc = make_map_tokens(&m[1], a.q_rot, (a.heads - 1) * a.q_rot_stride_h + a.rot_dim, a.length, a.q_rot_stride_t, a.batch, a.q_rot_stride_b, query_rows);
+    if (rc == EL_OK && a.rot_dim) rc = make_map_tokens(&m[3], a.k_rot, a.rot_dim, a.keys, a.k_rot_stride_t, a.batch, a.k_rot_stride_b, key_rows);
+    return rc;
+}
+
+int launch_attention_tc(const el_attention_t& a, cudaStream_t st) {
+    CUtensorMap m[5];
+    const int rc = attention_maps(a, m, TILE, TILE);
+    if (rc != EL_OK) return rc;
+    const Plan plan = plan_of(a);
+    return a.dtype == EL_F16 ? launch<__half>(a, plan, m, st) : launch<__nv_bfloat16>(a, plan, m, st);
+}
+
+int launch_attention_backward_tc(const el_attention_t&, const float*, float*, cudaStream_t) { return EL_ERR_UNSUPPORTED_SHAPE; }
+
+}  // namespace el

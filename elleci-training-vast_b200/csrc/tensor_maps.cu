@@ -61,6 +61,23 @@ int make_map_out(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows,
     return r == CUDA_SUCCESS ? EL_OK : EL_ERR_DRIVER;
 }
 
+// [batch, tokens, inner] of 2-byte elements with strides in elements; boxes of 64 columns x `rows` tokens of one sequence, swizzled by 128 bytes.  A
+// dimension of size 1 may have any stride.
+int make_map_tokens(CUtensorMap* m, const void* base, uint64_t inner, uint64_t tokens, uint64_t stride_t, uint64_t batch, uint64_t stride_b, uint32_t rows) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (fn == nullptr) return EL_ERR_DRIVER;
+    if (tokens == 1) stride_t = (inner + 7) / 8 * 8;
+    if (batch == 1) stride_b = tokens * stride_t;
+    if ((reinterpret_cast<uintptr_t>(base) & 15) != 0 || stride_t % 8 != 0 || stride_b % 8 != 0) return EL_ERR_ALIGNMENT;
+    cuuint64_t dims[3] = {inner, tokens, batch};
+    cuuint64_t strides[2] = {stride_t * 2, stride_b * 2};
+    cuuint32_t box[3] = {64, rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? EL_OK : EL_ERR_DRIVER;
+}
+
 }  // namespace tc
 
 // EL_OK if the tensor-core kernels take the problem: 16-byte aligned operands and pitches.
