@@ -345,7 +345,13 @@ bool attention_tc_takes(const el_attention_t& a, bool backward) {
         !map_takes(a.v, a.v_stride_b, a.v_stride_t, a.v_stride_h, a.heads) || reinterpret_cast<uintptr_t>(a.out) % 16)
         return false;
     if (a.rot_dim && (!map_takes(a.q_rot, a.q_rot_stride_b, a.q_rot_stride_t, a.q_rot_stride_h, a.heads) || !map_takes(a.k_rot, a.k_rot_stride_b, a.k_rot_stride_t, 0, 1))) return false;
-    return !backward;
+    if (!backward) return true;
+    if (!map_takes(a.dout, a.dout_stride_b, a.dout_stride_t, a.dout_stride_h, a.heads)) return false;
+    if (a.dk && !map_takes(a.dk, a.dk_stride_b, a.dk_stride_t, a.dk_stride_h, 1)) return false;
+    if (a.dv && !map_takes(a.dv, a.dv_stride_b, a.dv_stride_t, a.dv_stride_h, 1)) return false;
+    for (const void* p : {(const void*)a.dq, (const void*)a.dq_rot, (const void*)a.lse})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+    return true;
 }
 
 int attention_maps(const el_attention_t& a, CUtensorMap m[5], int query_rows, int key_rows) {
@@ -366,7 +372,5 @@ int launch_attention_tc(const el_attention_t& a, cudaStream_t st) {
     const Plan plan = plan_of(a);
     return a.dtype == EL_F16 ? launch<__half>(a, plan, m, st) : launch<__nv_bfloat16>(a, plan, m, st);
 }
-
-int launch_attention_backward_tc(const el_attention_t&, const float*, float*, cudaStream_t) { return EL_ERR_UNSUPPORTED_SHAPE; }
 
 }  // namespace el

@@ -1,0 +1,392 @@
+// The backward pass of latent attention's expanded form on the tensor cores (latent_attention.cu has the formulas, latent_attention_tc.cu the sizes).
+//
+// Two kernels of one shape: a block holds 128 rows of one side of one head and walks over tiles of 64 rows of the other side.
+//   KEYS   rows are keys:    S' = K Q',  dP' = V dO',  dV += P' dO,  dK += dS' Q
+//   else   rows are queries: S  = Q K',  dP  = dO V',                dQ += dS K
+// with A1, A2 the held matrices (K, V or Q, dO) and B1, B2 the others: S = A1 B1', dP = A2 B2', acc2 += P B2, acc1 += dS B1.  Every sum is formed by one
+// block in a fixed order, so no gradient depends on the order of blocks; that is worth forming S and dP twice (5 + 3 products instead of 5).
+//
+// Warps 0-7: a thread owns a row and half of a tile's columns; it forms p = 2^(s - lse) and ds = p (dp - delta) and writes both over S and dP as 16-bit
+// left factors.  The softmax scale is applied to the sums, so that ds, rounded, is not smaller than it has to be.  Warp 8 issues the products, 9 the loads.
+// While the threads work on a tile, the tensor core forms the next S (and dP, where tensor memory has room for two of them).
+#include "latent_tc.cuh"
+
+namespace el {
+
+using namespace tc;
+using namespace latent;
+
+int attention_maps(const el_attention_t& a, CUtensorMap m[5], int query_rows, int key_rows);
+
+namespace {
+
+constexpr int HELD = 128, STEP = 64;
+constexpr int HELD_CHUNK = HELD * 128, STEP_CHUNK = STEP * 128;      // bytes of 64 columns
+constexpr int WARP_MMA = 8, WARP_TMA = 9, THREADS = 320;
+constexpr int MAX_STAGES = 4;
+
+struct Plan {
+    int key_chunks, rot_chunks, value_chunks, stages;
+};
+
+template <typename T, bool KEYS>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmA1r, const __grid_constant__ CUtensorMap tmA2,
+                             const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB1r, const __grid_constant__ CUtensorMap tmB2,
+                             const el_attention_t a, const float* __restrict__ delta, float* __restrict__ rot_parts, const Plan plan) {
+    constexpr int DP_BUFFERS = KEYS ? 1 : 2;                   // tensor memory: acc1 192, acc2 128, S 2 x 64, dP 64 or 2 x 64
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const int QC = plan.key_chunks + plan.rot_chunks, VC = plan.value_chunks, NS = plan.stages;
+    const int held_bytes = (QC + VC) * HELD_CHUNK, stage_bytes = (QC + VC) * STEP_CHUNK;
+    const uint32_t ring = base + held_bytes, stats = ring + NS * stage_bytes, bars = stats + NS * 2 * STEP * 4;
+    uint8_t* ring_gen = gen + held_bytes;
+    const float* stats_gen = reinterpret_cast<const float*>(ring_gen + NS * stage_bytes);
+    const uint32_t a_full = bars, landed = bars + 8, done = bars + 16;
+    auto s_full = [&](int i) { return bars + 8u * (3 + i); };
+    auto dp_full = [&](int i) { return bars + 8u * (5 + i); };
+    auto p_full = [&](int i) { return bars + 8u * (7 + i); };
+    auto ds_full = [&](int i) { return bars + 8u * (9 + i); };
+    auto full = [&](int s) { return bars + 8u * (11 + s); };
+    auto empty = [&](int s) { return bars + 8u * (11 + MAX_STAGES + s); };
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * (stage_bytes + 2 * STEP * 4) + 8 * (11 + 2 * MAX_STAGES));
+
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const Place at(a);
+    const int all = KEYS ? a.keys : a.length, other = KEYS ? a.length : a.keys, tiles = (all + HELD - 1) / HELD;
+    const int b = at.batch, h = at.head, r0 = (KEYS ? at.tile : tiles - 1 - at.tile) * HELD;     // the longest rows first
+    const Sequence seq(a, b);
+    const int live = KEYS ? seq.keys : seq.queries, other_live = KEYS ? seq.queries : seq.keys;
+    int begin = 0, end = 0;
+    if (r0 < live) {
+        begin = KEYS ? seq.query_begin(r0) / STEP * STEP : 0;
+        end = KEYS ? seq.queries : seq.key_end(r0 + HELD);
+    }
+    const int n = end > begin ? (end - begin + STEP - 1) / STEP : 0;
+    const long long stat_row = ((long long)b * a.heads + h) * lse_pitch(a.length);
+
+    if (threadIdx.x == 0) {
+        mbar_init(a_full, 1);
+        mbar_init(landed, 1);
+        mbar_init(done, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full(i), 1);
+            mbar_init(dp_full(i), 1);
+            mbar_init(p_full(i), 8);
+            mbar_init(ds_full(i), 8);
+        }
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == WARP_MMA) tmem_alloc<512>(smem_u32((const void*)tmem_holder));
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const uint32_t ACC1 = tmem, ACC2 = tmem + 192, S = KEYS ? tmem + 320 : tmem + 192, DP = S + 128;      // S_i at 64 i, dP_i at 64 i
+    int32_t* status = a.dev_status;
+
+    if (warp == WARP_TMA) {
+        // ================= loads =================
+        const int qh = (int)(h * a.q_stride_h), qrh = (int)(h * a.q_rot_stride_h), kh = (int)(h * a.k_stride_h), vh = (int)(h * a.v_stride_h), gh = (int)(h * a.dout_stride_h);
+        const int x1 = KEYS ? kh : qh, x1r = KEYS ? 0 : qrh, x2 = KEYS ? vh : gh, y1 = KEYS ? qh : kh, y1r = KEYS ? qrh : 0, y2 = KEYS ? gh : vh;
+        if (n > 0 && elect_one()) {
+            mbar_expect_tx(a_full, held_bytes);
+            for (int c = 0; c < plan.key_chunks; ++c) tma_load_3d(base + c * HELD_CHUNK, &tmA1, a_full, x1 + c * CHUNK_COLS, r0, b);
+            if (plan.rot_chunks) tma_load_3d(base + plan.key_chunks * HELD_CHUNK, &tmA1r, a_full, x1r, r0, b);
+            for (int c = 0; c < VC; ++c) tma_load_3d(base + (QC + c) * HELD_CHUNK, &tmA2, a_full, x2 + c * CHUNK_COLS, r0, b);
+        }
+        __syncwarp();
+        int s = 0;
+        uint32_t ph = 0;
+        for (int j = 0; j < n; ++j) {
+            if (!mbar_wait_warp(empty(s), ph ^ 1u, status, 1)) break;
+            const int c0 = begin + j * STEP, rows = other_live - c0;
+            // rows behind the sequence's end may be anything, and zero times anything is not always zero: they are cleared
+            const bool late = rows < STEP && c0 + rows < other;
+            const uint32_t dst = ring + s * stage_bytes, bar = late ? landed : full(s);
+            if (elect_one()) {
+                mbar_expect_tx(bar, stage_bytes + (KEYS ? 2 * STEP * 4 : 0));
+                for (int c = 0; c < plan.key_chunks; ++c) tma_load_3d(dst + c * STEP_CHUNK, &tmB1, bar, y1 + c * CHUNK_COLS, c0, b);
+                if (plan.rot_chunks) tma_load_3d(dst + plan.key_chunks * STEP_CHUNK, &tmB1r, bar, y1r, c0, b);
+                for (int c = 0; c < VC; ++c) tma_load_3d(dst + (QC + c) * STEP_CHUNK, &tmB2, bar, y2 + c * CHUNK_COLS, c0, b);
+                if (KEYS) {
+                    bulk_load(stats + s * 2 * STEP * 4, a.lse + stat_row + c0, STEP * 4, bar);
+                    bulk_load(stats + s * 2 * STEP * 4 + STEP * 4, delta + stat_row + c0, STEP * 4, bar);
+                }
+            }
+            __syncwarp();
+            if (late) {
+                if (!mbar_wait_warp(landed, 0, status, 2)) break;            // the last tile only
+                for (int c = 0; c < QC + VC; ++c) {
+                    uint4* chunk = reinterpret_cast<uint4*>(ring_gen + s * stage_bytes + c * STEP_CHUNK);
+                    for (int k = rows * 8 + lane; k < STEP * 8; k += 32) chunk[k] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(full(s));
+                __syncwarp();
+            }
+            if (++s == NS) { s = 0; ph ^= 1u; }
+        }
+    } else if (warp == WARP_MMA) {
+        // ================= products =================
+        const int key_steps = a.key_dim / 16, rot_steps = a.rot_dim / 16, value_steps = a.value_dim / 16, D = a.key_dim, R = a.rot_dim, V = a.value_dim;
+        const uint32_t i_s = idesc_f16<T>(0, 0, STEP), i_v = idesc_f16<T>(0, 1, V);
+        const bool joined = R == 0 || D % 64 == 0;               // acc1's columns are the chunks' columns, one after another
+        const uint32_t i_1 = idesc_f16<T>(0, 1, joined ? D + R : D), i_r = idesc_f16<T>(0, 1, R);
+        auto stage = [&](int j) { return ring + (j % NS) * stage_bytes; };
+        auto scores = [&](int j) {
+            for (int c = 0; c < QC; ++c) {
+                const uint32_t x = base + c * HELD_CHUNK, y = stage(j) + c * STEP_CHUNK;
+                const int steps = c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps;
+                for (int k = 0; k < steps; ++k) umma_f16(S + (j & 1) * 64, make_desc(x + k * 32, 16), make_desc(y + k * 32, 16), i_s, (c | k) != 0);
+            }
+            umma_commit(s_full(j & 1));
+        };
+        auto grads = [&](int j) {
+            const int buf = DP_BUFFERS == 2 ? j & 1 : 0;
+            for (int k = 0; k < value_steps; ++k)
+                umma_f16(DP + buf * 64, make_desc(base + (QC + k / 4) * HELD_CHUNK + k % 4 * 32, 16), make_desc(stage(j) + (QC + k / 4) * STEP_CHUNK + k % 4 * 32, 16), i_s, k != 0);
+            umma_commit(dp_full(buf));
+        };
+        auto left = [&](int k) { return k < 2 ? k * 8 : 32 + (k - 2) * 8; };      // the two halves of the threads write their factors over their own columns
+        bool ok = n > 0 && mbar_wait_warp(a_full, 0, status, 3) && mbar_wait_warp(full(0), 0, status, 3);
+        tcgen05_fence_after();
+        if (ok && elect_one()) {
+            scores(0);
+            grads(0);
+        }
+        __syncwarp();
+        for (int j = 0; j < n && ok; ++j) {
+            if (j + 1 < n) {
+                ok = mbar_wait_warp(full((j + 1) % NS), (uint32_t)((j + 1) / NS) & 1u, status, 4);
+                tcgen05_fence_after();
+                if (ok && elect_one()) {
+                    scores(j + 1);
+                    if (DP_BUFFERS == 2) grads(j + 1);
+                }
+                __syncwarp();
+            }
+            if (KEYS && ok) {
+                ok = mbar_wait_warp(p_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 5);
+                tcgen05_fence_after();
+                if (ok && elect_one())
+                    for (int k = 0; k < 4; ++k) umma_f16_ts(ACC2, S + (j & 1) * 64 + left(k), make_desc(stage(j) + QC * STEP_CHUNK + k * 2048, STEP_CHUNK), i_v, (j | k) != 0);
+                __syncwarp();
+            }
+            if (!ok) break;
+            ok = mbar_wait_warp(ds_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6);
+            tcgen05_fence_after();
+            if (ok && elect_one()) {
+                const uint32_t f = DP + (DP_BUFFERS == 2 ? j & 1 : 0) * 64;
+                for (int k = 0; k < 4; ++k) {
+                    umma_f16_ts(ACC1, f + left(k), make_desc(stage(j) + k * 2048, STEP_CHUNK), i_1, (j | k) != 0);
+                    if (!joined) umma_f16_ts(ACC1 + D, f + left(k), make_desc(stage(j) + plan.key_chunks * STEP_CHUNK + k * 2048, STEP_CHUNK), i_r, (j | k) != 0);
+                }
+                umma_commit(empty(j % NS));
+                if (DP_BUFFERS == 1 && j + 1 < n) grads(j + 1);
+                if (j + 1 == n) umma_commit(done);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ================= probabilities and their gradients =================
+        const int half = warp >> 2, quarter = warp & 3, row = r0 + quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16, cols = half * 32;
+        const float by = a.scale * mamba::LOG2E;
+        const rowio::f32x2 by2 = rowio::pair(by, by);
+        float lse = INFINITY, del = 0.0f;
+        if (!KEYS && row < seq.queries) {
+            lse = a.lse[stat_row + row];
+            del = delta[stat_row + row];
+        }
+        // columns (of all) that the row meets: first .. last - 1
+        long long first = 0, last = 0;
+        if (row < live) {
+            first = KEYS ? seq.query_begin(row) : 0;
+            last = KEYS ? seq.queries : row + seq.shift + 1;
+            if (!KEYS && last > seq.keys) last = seq.keys;
+        }
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int c0 = begin + j * STEP + cols, buf = j & 1, dbuf = DP_BUFFERS == 2 ? buf : 0;
+            const uint32_t dph = DP_BUFFERS == 2 ? (uint32_t)(j >> 1) & 1u : (uint32_t)j & 1u;
+            const float* st = stats_gen + (j % NS) * 2 * STEP + cols;
+            if (!(ok = mbar_wait_warp(s_full(buf), (uint32_t)(j >> 1) & 1u, status, 7))) break;
+            tcgen05_fence_after();
+            uint32_t s[32], w[16];
+            tmem_ld32(S + buf * 64 + lanes + cols, s);
+            tmem_ld_wait();
+            // what a bulk copy brought is visible to who has waited for it: a phase that the product's issuer has already seen
+            if (KEYS && !(ok = mbar_wait_warp(full(j % NS), (uint32_t)(j / NS) & 1u, status, 8))) break;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+                float4 l = make_float4(lse, lse, lse, lse);
+                if (KEYS) l = *reinterpret_cast<const float4*>(st + k);
+                const rowio::f32x2 x = rowio::fma2(rowio::pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), by2, rowio::pair(-l.x, -l.y));
+                const rowio::f32x2 y = rowio::fma2(rowio::pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), by2, rowio::pair(-l.z, -l.w));
+                s[k] = __float_as_uint(mamba::ex2(rowio::lo_of(x)));
+                s[k + 1] = __float_as_uint(mamba::ex2(rowio::hi_of(x)));
+                s[k + 2] = __float_as_uint(mamba::ex2(rowio::lo_of(y)));
+                s[k + 3] = __float_as_uint(mamba::ex2(rowio::hi_of(y)));
+            }
+            const int lo = (int)(first - c0 < 0 ? 0 : first - c0 > 32 ? 32 : first - c0), hi = (int)(last - c0 < 0 ? 0 : last - c0 > 32 ? 32 : last - c0);
+            const bool partial = __any_sync(0xffffffffu, lo > 0 || hi < 32);
+            if (partial) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) s[k] = k >= lo && k < hi ? s[k] : 0u;
+            }
+            if (KEYS) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+                tmem_st16(S + buf * 64 + lanes + cols, w);
+                tmem_st_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(buf));
+            }
+            if (!(ok = mbar_wait_warp(dp_full(dbuf), dph, status, 9))) break;
+            tcgen05_fence_after();
+            uint32_t g[32];
+            tmem_ld32(DP + dbuf * 64 + lanes + cols, g);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+                float4 d = make_float4(del, del, del, del);
+                if (KEYS) d = *reinterpret_cast<const float4*>(st + STEP + k);
+                const rowio::f32x2 x = rowio::mul2(rowio::pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                                                   rowio::add2(rowio::pair(__uint_as_float(g[k]), __uint_as_float(g[k + 1])), rowio::pair(-d.x, -d.y)));
+                const rowio::f32x2 y = rowio::mul2(rowio::pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])),
+                                                   rowio::add2(rowio::pair(__uint_as_float(g[k + 2]), __uint_as_float(g[k + 3])), rowio::pair(-d.z, -d.w)));
+                g[k] = __float_as_uint(rowio::lo_of(x));
+                g[k + 1] = __float_as_uint(rowio::hi_of(x));
+                g[k + 2] = __float_as_uint(rowio::lo_of(y));
+                g[k + 3] = __float_as_uint(rowio::hi_of(y));
+            }
+            if (partial) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) g[k] = k >= lo && k < hi ? g[k] : 0u;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(g[2 * k]), __uint_as_float(g[2 * k + 1]));
+            tmem_st16(DP + dbuf * 64 + lanes + cols, w);
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ds_full(buf));
+        }
+        if (ok && n > 0) ok = mbar_wait_warp(done, 0, status, 10);
+        tcgen05_fence_after();
+        if (ok) {
+            // 16 columns at a time, the two halves of the threads in turn
+            auto columns = [&](uint32_t acc, int c, float scale, float (&v)[16]) {
+                uint32_t o[16];
+                if (n > 0) {
+                    tmem_ld16(acc + lanes + c, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = n > 0 && row < live ? __uint_as_float(o[k]) * scale : 0.0f;
+            };
+            auto put = [&](T* p, const float (&v)[16]) {
+                *reinterpret_cast<uint4*>(p) = make_uint4(pack_word<T>(v[0], v[1]), pack_word<T>(v[2], v[3]), pack_word<T>(v[4], v[5]), pack_word<T>(v[6], v[7]));
+                *reinterpret_cast<uint4*>(p + 8) = make_uint4(pack_word<T>(v[8], v[9]), pack_word<T>(v[10], v[11]), pack_word<T>(v[12], v[13]), pack_word<T>(v[14], v[15]));
+            };
+            const long long at_q = ((long long)b * a.length + row) * a.heads + h;
+            T* to = KEYS ? (a.dk ? static_cast<T*>(a.dk) + b * a.dk_stride_b + row * a.dk_stride_t + h * a.dk_stride_h : nullptr)
+                         : (a.dq ? static_cast<T*>(a.dq) + at_q * a.key_dim : nullptr);
+            float v[16];
+            for (int c = half * 16; c < a.key_dim; c += 32) {
+                columns(ACC1, c, a.scale, v);
+                if (row < all && to) put(to + c, v);
+            }
+            for (int c = half * 16; c < a.rot_dim; c += 32) {
+                columns(ACC1, a.key_dim + c, a.scale, v);
+                if (row < all && KEYS && rot_parts) {
+                    float4* p = reinterpret_cast<float4*>(rot_parts + (((long long)b * a.heads + h) * a.keys + row) * a.rot_dim + c);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) p[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                } else if (row < all && !KEYS && a.dq_rot) {
+                    put(static_cast<T*>(a.dq_rot) + at_q * a.rot_dim + c, v);
+                }
+            }
+            if (KEYS && a.dv) {
+                T* dv = static_cast<T*>(a.dv) + b * a.dv_stride_b + row * a.dv_stride_t + h * a.dv_stride_h;
+                for (int c = half * 16; c < a.value_dim; c += 32) {
+                    columns(ACC2, c, 1.0f, v);
+                    if (row < all) put(dv + c, v);
+                }
+            }
+        }
+    }
+    if (status != nullptr && *reinterpret_cast<volatile int32_t*>(status) != 0) {
+        // a wait gave up somewhere: copies and products still in flight get time to land before their memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) { }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == WARP_MMA) {
+        tcgen05_fence_after();
+        tmem_free<512>(tmem);
+    }
+}
+
+Plan plan_of(const el_attention_t& a) {
+    Plan p;
+    p.key_chunks = (a.key_dim + 63) / 64;
+    p.rot_chunks = (a.rot_dim + 63) / 64;
+    p.value_chunks = (a.value_dim + 63) / 64;
+    const int chunks = p.key_chunks + p.rot_chunks + p.value_chunks;
+    const int room = (227 * 1024 - 2048 - chunks * HELD_CHUNK) / (chunks * STEP_CHUNK + 2 * STEP * 4);
+    p.stages = room < MAX_STAGES ? room : MAX_STAGES;
+    return p;
+}
+int shared_bytes(const Plan& p) {
+    const int chunks = p.key_chunks + p.rot_chunks + p.value_chunks;
+    return 1024 + chunks * HELD_CHUNK + p.stages * (chunks * STEP_CHUNK + 2 * STEP * 4) + 8 * (11 + 2 * MAX_STAGES) + 16;
+}
+
+template <typename T, bool KEYS>
+int launch(const el_attention_t& a, const CUtensorMap* held, const CUtensorMap* step, const float* delta, float* rot_parts, cudaStream_t st) {
+    static DeviceOnce once;
+    int dev = 0;
+    EL_CUDA_TRY(cudaGetDevice(&dev));
+    if (!once.is_done(dev)) {
+        EL_CUDA_TRY(cudaFuncSetAttribute(attention_backward_tc_kernel<T, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        once.mark(dev);
+    }
+    const Plan plan = plan_of(a);
+    attention_backward_tc_kernel<T, KEYS><<<blocks_of(a, KEYS ? a.keys : a.length, HELD), THREADS, shared_bytes(plan), st>>>(
+        held[0], held[1], held[2], step[0], step[1], step[2], a, delta, rot_parts, plan);
+    return check_launch();
+}
+
+}  // namespace
+
+int launch_attention_backward_tc(const el_attention_t& a, const float* delta, float* rot_parts, cudaStream_t st) {
+    CUtensorMap m[5], g;                                         // q, q_rot, k, k_rot, v and dout
+    auto run = [&](auto t, auto keys) {
+        using T = decltype(t);
+        constexpr bool KEYS = decltype(keys)::value;
+        const int query_rows = KEYS ? STEP : HELD, key_rows = KEYS ? HELD : STEP;
+        int rc = attention_maps(a, m, query_rows, key_rows);
+        if (rc == EL_OK) rc = make_map_tokens(&g, a.dout, (a.heads - 1) * a.dout_stride_h + a.value_dim, a.length, a.dout_stride_t, a.batch, a.dout_stride_b, query_rows);
+        if (rc != EL_OK) return rc;
+        const CUtensorMap by_key[3] = {m[2], m[3], m[4]}, by_query[3] = {m[0], m[1], g};
+        return KEYS ? launch<T, true>(a, by_key, by_query, delta, rot_parts, st) : launch<T, false>(a, by_query, by_key, delta, rot_parts, st);
+    };
+    auto typed = [&](auto keys) { return a.dtype == EL_F16 ? run(__half(), keys) : run(__nv_bfloat16(), keys); };
+    int rc = EL_OK;
+    if (a.dk || a.dv || rot_parts) rc = typed(std::true_type());
+    if (rc == EL_OK && (a.dq || a.dq_rot)) rc = typed(std::false_type());
+    return rc;
+}
+
+}  // namespace el
