@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libelleci_int2.so")
-SOURCES = ["api.cu", "pack_quant.cu", "hysteresis.cu", "gemm_simple.cu", "gemm_skinny.cu", "tensor_maps.cu", "gemm_dw.cu", "gemm_wt.cu", "decode_static.cu", "gemv_small.cu", "gemv_mma.cu", "rmsnorm.cu", "swiglu.cu", "peer_sync.cu", "causal_conv.cu", "selective_scan.cu", "block_norm.cu", "latent_attention.cu", "latent_attention_tc.cu", "latent_backward_tc.cu", "latent_cache.cu", "latent_step.cu"]
+SOURCES = ["api.cu", "pack_quant.cu", "hysteresis.cu", "gemm_simple.cu", "gemm_skinny.cu", "tensor_maps.cu", "gemm_dw.cu", "gemm_wt.cu", "decode_static.cu", "gemv_small.cu", "gemv_mma.cu", "rmsnorm.cu", "swiglu.cu", "peer_sync.cu", "causal_conv.cu", "selective_scan.cu", "block_norm.cu", "latent_attention.cu", "latent_attention_tc.cu", "latent_backward_tc.cu", "latent_cache.cu", "latent_step.cu", "latent_step_tc.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-fmad=false",                       # the integer state must not depend on fused multiply-adds

@@ -9,10 +9,15 @@
 //   join    out[h] = gamma W_v[h] (sum over the parts of 2^(max' - max) o[h]) / (sum of p)
 //
 // Three launches: query, scores and sums of the workers' parts (latent_step.cuh says how tokens are divided), join.  The kernel of this file
-// holds everything in float32 and takes float32 activations; latent_step_tc.cu takes 16-bit ones.
+// holds everything in float32; latent_step_tc.cu takes 16-bit activations.
 #include "latent_step.cuh"
 
 namespace el {
+
+bool latent_step_tc_takes(const el_latent_step_t& a);
+int latent_step_tc_groups(const el_latent_step_t& a);
+int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const float* steps, const void* rotated, const latent::StepParts& parts, int workers,
+                          cudaStream_t st);
 
 using namespace latent;
 
@@ -27,10 +32,12 @@ constexpr int MOST_RANK = 512, MOST_ROT = 64;
 __device__ __forceinline__ float weight_of(uint32_t w, int i) { return (float)decode2(w >> (2 * i)); }
 
 // u and w of one head for PER sequences.  Thread (x, y): column words x of the weights (16 columns each), rows y, y + 8 ..
-template <typename T, typename Q, int PER>
-__global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_step_t a, Q* __restrict__ query) {
+// DIGITS: for the tensor cores, u as two 8-bit digits of 1 / 32512 of its largest magnitude (digits [.., 2, rank padded to 32], steps) and w as T [.., 64].
+template <typename T, bool DIGITS, int PER>
+__global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_step_t a, float* __restrict__ query, int8_t* __restrict__ digits, float* __restrict__ steps, T* __restrict__ rotated) {
     __shared__ float q[PER][256];
     __shared__ float part[WARPS][32][17];
+    __shared__ float most[WARPS];
     const int h = blockIdx.x, b0 = blockIdx.y * PER, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int words = a.rank / 16, width = a.rank + a.rot_dim;
     const float by = a.scale * mamba::LOG2E;
@@ -63,17 +70,49 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[warp][lane][i] = sum[n][i];
         __syncthreads();
-        Q* out = query + ((long long)(b0 + n) * a.heads + h) * width;
-        for (int c = threadIdx.x; c < a.rank; c += THREADS) {
-            float s = 0.0f;
+        const long long bh = (long long)(b0 + n) * a.heads + h;
+        float* out = query + bh * width;
+        float u[MOST_RANK / THREADS], top = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) s += part[w][c / 16][c % 16];
-            out[c] = mamba::from_float<Q>(s * (a.gamma * by));
+        for (int i = 0; i < MOST_RANK / THREADS; ++i) {
+            const int c = threadIdx.x + i * THREADS;
+            u[i] = 0.0f;
+            if (c < a.rank) {
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) u[i] += part[w][c / 16][c % 16];
+                u[i] *= a.gamma * by;
+                if (!DIGITS) out[c] = u[i];
+            }
+            top = mamba::max_nan(top, fabsf(u[i]));
         }
+        if constexpr (DIGITS) {
+            const int rp = (a.rank + 31) / 32 * 32;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) top = mamba::max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
+            if (lane == 0) most[warp] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = mamba::max_nan(top, most[w]);
+            const float step = top * (1.0f / 32512.0f), inv = step > 0.0f ? 32512.0f / top : 0.0f;
+            if (threadIdx.x == 0) steps[bh] = step;                  // a NaN or infinity makes the scores NaN
+#pragma unroll
+            for (int i = 0; i < MOST_RANK / THREADS; ++i) {
+                const int c = threadIdx.x + i * THREADS;
+                if (c >= rp) continue;
+                const int v = __float2int_rn(u[i] * inv), hi = (v + 128) >> 8;
+                digits[bh * 2 * rp + c] = (int8_t)hi;
+                digits[bh * 2 * rp + rp + c] = (int8_t)(v - hi * 256);
+            }
+            for (int c = a.rot_dim + threadIdx.x; c < 64; c += THREADS) rotated[bh * 64 + c] = mamba::from_float<T>(0.0f);
+        }
+        auto put = [&](int c, float v) {
+            if constexpr (DIGITS) rotated[bh * 64 + c] = mamba::from_float<T>(v);
+            else out[a.rank + c] = v;
+        };
         if (a.rot_dim == 0) continue;
         const T* x = static_cast<const T*>(a.q_rot) + (b0 + n) * a.q_rot_stride_b + h * a.q_rot_stride_h;
         if (!a.table) {
-            for (int c = threadIdx.x; c < a.rot_dim; c += THREADS) out[a.rank + c] = mamba::from_float<Q>(to_float(x[c]) * by);
+            for (int c = threadIdx.x; c < a.rot_dim; c += THREADS) put(c, to_float(x[c]) * by);
             continue;
         }
         const int half = a.rot_dim / 2, at = step_tokens(a, b0 + n) - 1;      // the token itself is the cache's last one
@@ -81,8 +120,8 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
         for (int c = threadIdx.x; c < half; c += THREADS) {
             const int i0 = a.neighbours ? 2 * c : c, i1 = a.neighbours ? 2 * c + 1 : c + half;
             const float u = to_float(x[i0]), v = to_float(x[i1]), co = cs[c], si = cs[c + half];
-            out[a.rank + i0] = mamba::from_float<Q>(fmaf(u, co, -__fmul_rn(v, si)) * by);
-            out[a.rank + i1] = mamba::from_float<Q>(fmaf(v, co, __fmul_rn(u, si)) * by);
+            put(i0, fmaf(u, co, -__fmul_rn(v, si)) * by);
+            put(i1, fmaf(v, co, __fmul_rn(u, si)) * by);
         }
     }
 }
@@ -253,42 +292,64 @@ template <typename F> int of_type(int dtype, F f) {
     }
 }
 
-// Blocks that share the tokens: two for every SM, but no more than there can be tiles.
-int step_workers(const el_latent_step_t& a) {
+// Blocks that share the tokens: one for every SM, but no more than there can be tiles.
+int step_workers(const el_latent_step_t& a, int groups) {
     int sms = 148;
     device_sm_count(&sms);
     const long long tiles = (((long long)a.pages_per_sequence * a.page_size + STEP_TILE - 1) / STEP_TILE) * a.batch;
-    return (int)(tiles < sms ? tiles : sms);
+    const int most = sms / groups > 0 ? sms / groups : 1;
+    return (int)(tiles < most ? tiles : most);
 }
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+size_t digits_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * a.heads * 2 * ((a.rank + 31) / 32 * 32)); }
+size_t steps_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * a.heads * 4); }
+size_t rotated_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * a.heads * 64 * 2); }
+size_t query_bytes(const el_latent_step_t& a) {
+    return latent_step_tc_takes(a) ? digits_bytes(a) + steps_bytes(a) + rotated_bytes(a) : align256((size_t)a.batch * a.heads * (a.rank + a.rot_dim) * 4);
+}
+int groups_of(const el_latent_step_t& a) { return latent_step_tc_takes(a) ? latent_step_tc_groups(a) : 1; }
 
 }  // namespace
 
 size_t latent_step_workspace_bytes(const el_latent_step_t& a) {
-    return step_query_bytes(a, 4) + (size_t)(step_workers(a) + a.batch) * a.heads * (2 + (size_t)a.rank) * 4;
+    return query_bytes(a) + (size_t)(step_workers(a, groups_of(a)) + a.batch) * a.heads * (2 + (size_t)a.rank) * 4;
 }
 
 int launch_latent_step(const el_latent_step_t& a, cudaStream_t st) {
-    const int workers = step_workers(a);
-    float* query = static_cast<float*>(a.workspace);
-    const StepParts parts{reinterpret_cast<float*>(static_cast<char*>(a.workspace) + step_query_bytes(a, 4)), a.heads, a.rank};
+    const int workers = step_workers(a, groups_of(a));
+    char* ws = static_cast<char*>(a.workspace);
+    const StepParts parts{reinterpret_cast<float*>(ws + query_bytes(a)), a.heads, a.rank};
+    constexpr int PER = 4;
+    const dim3 grid(a.heads, (a.batch + PER - 1) / PER);
     return of_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        constexpr int PER = 4;
-        step_query_kernel<T, float, PER><<<dim3(a.heads, (a.batch + PER - 1) / PER), THREADS, 0, st>>>(a, query);
-        int rc = check_launch();
-        if (rc != EL_OK) return rc;
-        if (workers > 0) {
-            static DeviceOnce once;
-            int dev = 0;
-            constexpr int most = 4 * (32 * (MOST_RANK + MOST_ROT + 1) + GROUP * (MOST_RANK + MOST_ROT));
-            EL_CUDA_TRY(cudaGetDevice(&dev));
-            if (!once.is_done(dev)) {
-                EL_CUDA_TRY(cudaFuncSetAttribute(step_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-                once.mark(dev);
-            }
-            step_rows_kernel<T><<<dim3(workers, (a.heads + GROUP - 1) / GROUP), THREADS, most, st>>>(a, query, parts, workers);
+        int rc = EL_OK;
+        if (latent_step_tc_takes(a)) {
+            int8_t* digits = reinterpret_cast<int8_t*>(ws);
+            float* steps = reinterpret_cast<float*>(ws + digits_bytes(a));
+            T* rotated = reinterpret_cast<T*>(ws + digits_bytes(a) + steps_bytes(a));
+            step_query_kernel<T, true, PER><<<grid, THREADS, 0, st>>>(a, nullptr, digits, steps, rotated);
             if ((rc = check_launch()) != EL_OK) return rc;
+            if (workers > 0) rc = launch_latent_step_tc(a, digits, steps, rotated, parts, workers, st);
+        } else {
+            float* query = reinterpret_cast<float*>(ws);
+            step_query_kernel<T, false, PER><<<grid, THREADS, 0, st>>>(a, query, nullptr, nullptr, nullptr);
+            if ((rc = check_launch()) != EL_OK) return rc;
+            if (workers > 0) {
+                static DeviceOnce once;
+                int dev = 0;
+                constexpr int most = 4 * (32 * (MOST_RANK + MOST_ROT + 1) + GROUP * (MOST_RANK + MOST_ROT));
+                EL_CUDA_TRY(cudaGetDevice(&dev));
+                if (!once.is_done(dev)) {
+                    EL_CUDA_TRY(cudaFuncSetAttribute(step_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+                    once.mark(dev);
+                }
+                step_rows_kernel<T><<<dim3(workers, (a.heads + GROUP - 1) / GROUP), THREADS, most, st>>>(a, query, parts, workers);
+                rc = check_launch();
+            }
         }
+        if (rc != EL_OK) return rc;
         step_join_kernel<T><<<(unsigned)(a.batch * a.heads), THREADS, 0, st>>>(a, parts, workers);
         return check_launch();
     });

@@ -11,7 +11,7 @@
 namespace el {
 namespace latent {
 
-constexpr int STEP_TILE = 64;
+constexpr int STEP_TILE = 32;
 
 __device__ __forceinline__ int step_tokens(const el_latent_step_t& a, int b) {
     return length_of(a.lengths, b, 0, (int)min((long long)a.pages_per_sequence * a.page_size, 0x7fffff00LL));
@@ -60,11 +60,6 @@ struct StepParts {
     __device__ __forceinline__ float* stats(long long slot) const { return base + slot * heads * (2LL + rank); }
     __device__ __forceinline__ float* vectors(long long slot) const { return stats(slot) + 2 * heads; }
 };
-
-// The query of one head against latent vectors: [rank + rot_dim], scaled so that scores are exponents of 2.
-inline size_t step_query_bytes(const el_latent_step_t& a, int element) {
-    return ((size_t)a.batch * a.heads * (a.rank + a.rot_dim) * element + 255) / 256 * 256;
-}
 
 // the pool's row of position p of sequence b, or -1
 __device__ __forceinline__ long long step_row(const el_latent_step_t& a, int b, int p) {

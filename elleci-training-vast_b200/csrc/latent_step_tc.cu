@@ -1,0 +1,474 @@
+// The absorbed form for 16-bit activations on the tensor cores (latent_step.cu has the formulas and the launches around it).
+//
+// The cached rows are int8 already, so they go to the tensor cores as they are (kind::i8, exact int32 sums) and nothing is dequantised: what multiplies
+// them is split into two 8-bit digits instead, x = step * (256 hi + lo), 16 bits of a row's largest magnitude.  One copy of a tile of tokens in
+// shared memory serves both products:
+//   scores   S [128 tokens x 2 heads' digits] = rows (K-major: tokens by latent channels) * query digits;  with the rotated part in 16-bit floats beside it
+//            s[j,h] = absmax[j] / 127 * step[h] * (256 S_hi + S_lo) + key[j] . w[h]
+//   sums     O [latent channels x 2 heads' digits] = rows (MN-major: the same bytes, read as channels by tokens) * digits of p[j,h] absmax[j] / largest absmax
+// p = 2^(s - m) with m the running maximum of the head, so p <= 1 and a digit step is 2^-15 of the largest weight that a token of the tile can have: finer
+// than bfloat16's 2^-8 of each weight where weights matter.  The tiles' int32 sums are added up in float32 registers, scaled when m grows.
+//
+// Warps 0-7: thread t of each half is token t of the tile and takes 16 heads' scores; then two of the four blocks of 128 latent channels, a thread a channel.
+// The sums of a tile are taken while the tensor core forms the next tile's scores.  Warp 8 issues the products.  Warps
+// 9 and 10 load, each every other tile: 16-byte asynchronous copies of a token's row from wherever its page lies.
+// Bound: memory; a tile of 128 tokens of rank 512 and 64 rotated channels is 82 KB, 3400 cycles of an SM's share of the HBM, and 1100 of its tensor core.
+#include "latent_step.cuh"
+#include "latent_tc.cuh"
+
+namespace el {
+
+using namespace tc;
+using namespace latent;
+
+namespace {
+
+constexpr int TOKENS = 128, CHUNK = TOKENS * 128;      // a tile; 128 bytes of every token
+constexpr int WARP_MMA = 8, WARP_LOAD = 9, THREADS = 11 * 32;
+constexpr float STEPS = 32512.0f;                      // 127 * 256: the largest value of two digits whose high one is at most 127
+constexpr float MAGIC = 12582912.0f;                   // 1.5 * 2^23: adding it rounds to an integer, whose low bits are the sum's
+
+struct Shape {
+    int chunks, hp, groups;                            // 128-byte chunks of a row; heads of a group, padded to 16 or 32
+    __host__ __device__ int n() const { return 2 * hp; }
+};
+
+// Digits of the integers i < 2^15 in magnitude: the low one is the integer's low byte as a signed number, the high one what is left.
+__device__ __forceinline__ uint32_t high_digit(int v) { return (uint32_t)((v + 128) >> 8) & 0xFFu; }
+__device__ __forceinline__ uint32_t low_digit(int v) { return (uint32_t)v & 0xFFu; }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pair_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); }
+
+// The parts of a worker's range: sequence after sequence, tile after tile.
+struct Walk {
+    const el_latent_step_t& a;
+    long long t, last, before;
+    int b;
+    int p0, p1;                                        // positions of the current part
+    __device__ Walk(const el_latent_step_t& args, long long first, long long end) : a(args), t(first), last(end) { step_find(a, first, b, before); open(); }
+    __device__ __forceinline__ void open() {
+        while (t < last) {
+            const int n = step_tokens(a, b), here = (n + STEP_TILE - 1) / STEP_TILE;
+            if (here > 0) {
+                const long long stop = before + here < last ? before + here : last;
+                p0 = (int)(t - before) * STEP_TILE;
+                const long long e = (stop - before) * STEP_TILE;
+                p1 = (int)(e < n ? e : n);
+                return;
+            }
+            ++b;
+        }
+    }
+    __device__ __forceinline__ bool more() const { return t < last; }
+    __device__ __forceinline__ int tiles() const { return (p1 - p0 + TOKENS - 1) / TOKENS; }
+    __device__ __forceinline__ void next() {
+        const int here = step_tiles(a, b);
+        t = before + here < last ? before + here : last;
+        before += here;
+        ++b;
+        open();
+    }
+};
+
+// Reduces 16 values over a warp by maximum (or sum): lane l has the result of value l % 16.
+template <bool MAX> __device__ __forceinline__ float reduce16(const float (&v)[16]) {
+    const int lane = threadIdx.x & 31;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = v[i];
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const float give = up ? x[i] : x[i + w], keep = up ? x[i + w] : x[i];
+            const float got = __shfl_xor_sync(0xffffffffu, give, w);
+            x[i] = MAX ? mamba::max_nan(keep, got) : keep + got;
+        }
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, x[0], 16);
+    return MAX ? mamba::max_nan(x[0], other) : x[0] + other;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+step_tc_kernel(const el_latent_step_t a, const int8_t* __restrict__ digits, const float* __restrict__ steps, const T* __restrict__ rotated, const StepParts parts,
+               int workers, const Shape shape) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const int R = a.rank, P = a.rot_dim, HP = shape.hp, N = shape.n(), KC = shape.chunks, rp = (R + 31) / 32 * 32;
+    const int key_bytes = P ? CHUNK : 0, stage_bytes = KC * CHUNK + key_bytes;
+    // two stages [rows][keys]; query digits [chunks][N rows][128]; w [HP rows][128]; p digits [tokens][128]
+    const uint32_t q_at = base + 2 * stage_bytes, w_at = q_at + KC * N * 128, p_at = w_at + (P ? HP * 128 : 0);
+    uint8_t* tail = gen + (p_at - base) + CHUNK;
+    float* scale_of = reinterpret_cast<float*>(tail);                       // [2][128]
+    uint32_t* seen = reinterpret_cast<uint32_t*>(tail + 1024);              // [2][4]
+    float* step_of = reinterpret_cast<float*>(tail + 1088);                 // [2][32], by part
+    float* factor = reinterpret_cast<float*>(tail + 1344);                  // [2][32], by tile
+    float* weight = reinterpret_cast<float*>(tail + 1600);                  // [2], by tile
+    float* wmax = reinterpret_cast<float*>(tail + 1632);                    // [2 halves][2][4 warps][16 heads]
+    float* smax = reinterpret_cast<float*>(tail + 2656);                    // [2 halves][2][4 warps]
+    float* wsum = reinterpret_cast<float*>(tail + 2720);                    // [2 halves][4 warps][16 heads]
+    const uint32_t bars = p_at + CHUNK + 3232;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (2 + s); };
+    auto s_full = [&](int s) { return bars + 8u * (4 + s); };
+    const uint32_t p_full = bars + 48, o_full = bars + 56, q_empty = bars + 64;
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(tail + 3232 + 72);
+
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const int w = blockIdx.x / shape.groups, group = blockIdx.x - w * shape.groups, h0 = group * 32;
+    int32_t* status = a.dev_status;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+            mbar_init(s_full(s), 1);
+        }
+        mbar_init(p_full, 8);
+        mbar_init(o_full, 1);
+        mbar_init(q_empty, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == WARP_MMA) tmem_alloc<512>(smem_u32((const void*)tmem_holder));
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    const uint32_t O = tmem, S = tmem + 256;                                // O of chunk c at 64 c; S of tile g at 128 (g & 1), its rotated part 64 further
+
+    const long long tiles = step_tiles_before(a, a.batch);
+    workers = step_active(workers, tiles);
+    const long long first = w < workers ? w * tiles / workers : 0, last = w < workers ? (w + 1) * tiles / workers : 0;
+
+    if (warp >= WARP_LOAD) {
+        // ================= loads =================
+        const int mine = warp - WARP_LOAD;                                            // every other tile
+        int g = 0, part = 0;
+        bool ok = true;
+        if (first < last) {
+            for (Walk k(a, first, last); k.more() && ok; k.next(), ++part) {
+                const int count = k.tiles();
+                for (int i = 0; i < count && ok; ++i, ++g) {
+                    if ((g & 1) != mine) continue;
+                    const uint32_t at = base + mine * stage_bytes;
+                    const int p = k.p0 + i * TOKENS;
+                    long long row[4];
+                    float sc[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int pos = p + q * 32 + lane;
+                        row[q] = pos < k.p1 ? step_row(a, k.b, pos) : -1;
+                        sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
+                    }
+                    if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+#pragma unroll 8
+                        for (int t = 0; t < 32; ++t) {
+                            const long long r = __shfl_sync(0xffffffffu, row[q], t);
+                            const int to = q * 32 + t;
+                            if (lane * 16 < R && r >= 0)
+                                copy16(at + (lane >> 3) * CHUNK + to * 128 + (((lane & 7) ^ (to & 7)) << 4), a.latents + r * R + lane * 16, true);
+                        }
+                        if (P) {
+                            const int pieces = (P + 15) / 16 * 2;                     // of 8 channels, zeros behind the last
+#pragma unroll 4
+                            for (int t = 0; t < 32; t += 4) {
+                                const int tt = t + (lane >> 3), c = lane & 7, to = q * 32 + tt;
+                                const long long r = __shfl_sync(0xffffffffu, row[q], tt);
+                                if (c < pieces) {
+                                    const bool there = r >= 0 && c * 8 < P;
+                                    copy16(at + KC * CHUNK + to * 128 + ((c ^ (to & 7)) << 4), there ? static_cast<const T*>(a.cache_keys) + r * P + c * 8 : a.cache_keys, there);
+                                }
+                            }
+                        }
+                        scale_of[mine * 128 + q * 32 + lane] = __fdiv_rn(sc[q], 127.0f);
+                        const uint32_t have = __ballot_sync(0xffffffffu, row[q] >= 0);
+                        if (lane == 0) seen[mine * 4 + q] = have;
+                    }
+                    if (i == 0) {                                                     // the part's query
+                        if (part > 0 && !mbar_wait_warp(q_empty, (uint32_t)(part - 1) & 1u, status, 2)) { ok = false; break; }
+                        const long long bh = (long long)k.b * a.heads + h0;
+                        for (int r = 0; r < N; ++r) {
+                            const int h = r % HP, digit = r / HP;
+                            const bool there = h0 + h < a.heads;
+                            const int8_t* src = digits + ((bh + (there ? h : 0)) * 2 + digit) * rp + lane * 16;
+                            if (lane * 16 < rp) copy16(q_at + (lane >> 3) * N * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4), there ? src : digits, there);
+                        }
+                        if (P) {
+                            for (int r = 0; r < HP; r += 4) {
+                                const int h = r + (lane >> 3), c = lane & 7;
+                                const bool there = h0 + h < a.heads;
+                                copy16(w_at + h * 128 + ((c ^ (h & 7)) << 4), there ? rotated + (bh + h) * 64 + c * 8 : rotated, there);
+                            }
+                        }
+                        step_of[(part & 1) * 32 + lane] = h0 + lane < a.heads ? steps[bh + lane] : 0.0f;
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full(mine));
+                }
+            }
+        }
+    } else if (warp == WARP_MMA) {
+        // ================= products =================
+        const uint32_t i_s = make_idesc(0, 0, N), i_o = make_idesc(1, 1, N), i_r = idesc_f16<T>(0, 0, HP);
+        const int key_steps = rp / 32, rot_steps = (P + 15) / 16;
+        auto scores = [&](int g) {
+            const uint32_t at = base + (g & 1) * stage_bytes, to = S + (g & 1) * 128;
+            for (int k = 0; k < key_steps; ++k) {
+                const int c = k >> 2, x = (k & 3) * 32;
+                umma_i8(to, make_desc(at + c * CHUNK + x, 16), make_desc(q_at + c * N * 128 + x, 16), i_s, k != 0);
+            }
+            for (int k = 0; k < rot_steps; ++k) umma_f16(to + 64, make_desc(at + KC * CHUNK + k * 32, 16), make_desc(w_at + k * 32, 16), i_r, k != 0);
+            umma_commit(s_full(g & 1));
+        };
+        auto sums = [&](int g) {
+            const uint32_t at = base + (g & 1) * stage_bytes;
+            for (int c = 0; c < KC; ++c)
+                for (int k = 0; k < TOKENS / 32; ++k) umma_i8(O + c * 64, make_desc(at + c * CHUNK + k * 4096, CHUNK), make_desc(p_at + k * 4096, CHUNK), i_o, k != 0);
+            umma_commit(o_full);
+            umma_commit(empty(g & 1));
+        };
+        bool ok = true;
+        int g = 0;                                                                    // scores issued
+        auto issue_scores = [&](bool ends_part) {
+            ok = ok && mbar_wait_warp(full(g & 1), (uint32_t)(g >> 1) & 1u, status, 3);
+            tcgen05_fence_after();
+            if (ok && elect_one()) {
+                scores(g);
+                if (ends_part) umma_commit(q_empty);
+            }
+            __syncwarp();
+            ++g;
+        };
+        auto issue_sums = [&](int j) {
+            // the threads that made the digits have also taken the sums of the tile before
+            ok = ok && mbar_wait_warp(p_full, (uint32_t)j & 1u, status, 4);
+            tcgen05_fence_after();
+            if (ok && elect_one()) sums(j);
+            __syncwarp();
+        };
+        if (first < last) {
+            for (Walk k(a, first, last); k.more() && ok; k.next()) {
+                const int count = k.tiles();
+                for (int i = 0; i < count && ok; ++i) {
+                    if (g > 0) issue_sums(g - 1);
+                    issue_scores(i + 1 == count);
+                }
+            }
+            if (ok && g > 0) issue_sums(g - 1);
+        }
+    } else if (first < last) {
+        // ================= softmax and sums =================
+        const int half = warp >> 2, quarter = warp & 3, token = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const bool scoring = half * 16 < HP;                                          // 16 heads have one half
+        float acc[2][32];                                                             // channels of chunks 2 half, 2 half + 1; heads
+        float top[16], sum[16];
+        bool ok = true;
+        int g = 0, part = 0;
+
+        auto softmax = [&](int j) {
+            if (!(ok = mbar_wait_warp(s_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6) && mbar_wait_warp(full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6))) return;
+            tcgen05_fence_after();
+            float s[16];
+            const float sc = scale_of[(j & 1) * 128 + token];
+            const bool here = (seen[(j & 1) * 4 + quarter] >> lane) & 1u;
+            if (scoring) {
+                uint32_t hi[16], lo[16], r[16];
+                const uint32_t at = S + (j & 1) * 128 + lanes + half * 16;
+                tmem_ld16(at, hi);
+                tmem_ld16(at + HP, lo);
+                if (P) tmem_ld16(at + 64, r);
+                tmem_ld_wait();
+                const float* st = step_of + (part & 1) * 32 + half * 16;
+#pragma unroll
+                for (int h = 0; h < 16; ++h) {
+                    const float x = (float)((int)(hi[h] * 256u) + (int)lo[h]) * (sc * st[h]);
+                    s[h] = here ? (P ? x + __uint_as_float(r[h]) : x) : -INFINITY;
+                }
+                const float m = reduce16<true>(s);
+                if (lane < 16) wmax[((half * 2 + (j & 1)) * 4 + quarter) * 16 + lane] = m;
+            }
+            float big = here ? sc : 0.0f;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+            if (lane == 0) smax[(half * 2 + (j & 1)) * 4 + quarter] = big;
+            pair_barrier(half);
+            const float4 b4 = *reinterpret_cast<const float4*>(smax + (half * 2 + (j & 1)) * 4);
+            big = fmaxf(fmaxf(b4.x, b4.y), fmaxf(b4.z, b4.w));
+            const float ratio = big > 0.0f ? sc / big * STEPS : 0.0f;
+            if (scoring) {                               // the products of the tile before have read its digits: its sums were taken
+                uint32_t dh[4] = {}, dl[4] = {};
+                const float* wm = wmax + (half * 2 + (j & 1)) * 64;
+                float f[16];
+                bool moved = false;
+#pragma unroll
+                for (int h = 0; h < 16; ++h) {
+                    const float m = mamba::max_nan(mamba::max_nan(mamba::max_nan(wm[h], wm[16 + h]), mamba::max_nan(wm[32 + h], wm[48 + h])), top[h]);
+                    moved = moved || m != top[h];
+                    f[h] = top[h];
+                    top[h] = m;
+                }
+                if (moved) {                                                          // the same for all threads of the half
+#pragma unroll
+                    for (int h = 0; h < 16; ++h) {
+                        f[h] = f[h] == -INFINITY ? 0.0f : exp2_neg(f[h] - top[h]);
+                        sum[h] *= f[h];
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 16; ++h) {
+                    const float e = here ? exp2_neg(s[h] - top[h]) : 0.0f;
+                    sum[h] += e;
+                    const int v = __float_as_int(fmaf(e, ratio, MAGIC)) - __float_as_int(MAGIC);
+                    dh[h / 4] |= high_digit(v) << (8 * (h & 3));
+                    dl[h / 4] |= low_digit(v) << (8 * (h & 3));
+                }
+                uint8_t* p = gen + (p_at - base) + token * 128;
+                *reinterpret_cast<uint4*>(p + ((half ^ (token & 7)) << 4)) = make_uint4(dh[0], dh[1], dh[2], dh[3]);
+                *reinterpret_cast<uint4*>(p + ((HP / 16 + half) ^ (token & 7)) * 16) = make_uint4(dl[0], dl[1], dl[2], dl[3]);
+                if (token == 0) {
+#pragma unroll
+                    for (int h = 0; h < 16; ++h) factor[(j & 1) * 32 + half * 16 + h] = moved ? f[h] : 1.0f;
+                }
+            }
+            if (token == 0 && half == 0) weight[j & 1] = big / STEPS;
+            fence_async_smem();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full);
+        };
+        auto gather = [&](int j) {
+            if (!(ok = mbar_wait_warp(o_full, (uint32_t)j & 1u, status, 8))) return;
+            // factors and weights of both halves' threads, which have all arrived at the barrier that the products waited for
+            if (!(ok = mbar_wait_warp(p_full, (uint32_t)j & 1u, status, 8))) return;
+            tcgen05_fence_after();
+            const float by = weight[j & 1];
+            const float* f = factor + (j & 1) * 32;
+            const rowio::f32x2 magic = rowio::pair(-MAGIC, -MAGIC), hi_by = rowio::pair(256.0f * by, 256.0f * by), lo_by = rowio::pair(by, by);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if ((2 * half + c) * 128 >= R) break;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    if (hh * 16 >= HP) break;
+                    uint32_t hi[16], lo[16];
+                    const uint32_t at = O + (2 * half + c) * 64 + lanes + hh * 16;
+                    tmem_ld16(at, hi);
+                    tmem_ld16(at + HP, lo);
+                    tmem_ld_wait();
+                    // sums of a tile's digits are below 2^22: adding them to the bits of 1.5 * 2^23 makes floats of them
+#pragma unroll
+                    for (int h = 0; h < 16; h += 2) {
+                        const rowio::f32x2 x = rowio::add2(rowio::pair(__int_as_float((int)hi[h] + __float_as_int(MAGIC)), __int_as_float((int)hi[h + 1] + __float_as_int(MAGIC))), magic);
+                        const rowio::f32x2 y = rowio::add2(rowio::pair(__int_as_float((int)lo[h] + __float_as_int(MAGIC)), __int_as_float((int)lo[h + 1] + __float_as_int(MAGIC))), magic);
+                        const float2 fs = *reinterpret_cast<const float2*>(f + hh * 16 + h);
+                        rowio::f32x2 o = rowio::fma2(x, hi_by, rowio::mul2(rowio::pair(acc[c][hh * 16 + h], acc[c][hh * 16 + h + 1]), rowio::pair(fs.x, fs.y)));
+                        o = rowio::fma2(y, lo_by, o);
+                        acc[c][hh * 16 + h] = rowio::lo_of(o);
+                        acc[c][hh * 16 + h + 1] = rowio::hi_of(o);
+                    }
+                }
+            }
+            tcgen05_fence_before();
+        };
+
+        for (Walk k(a, first, last); k.more() && ok; k.next(), ++part) {
+#pragma unroll
+            for (int h = 0; h < 16; ++h) {
+                top[h] = -INFINITY;
+                sum[h] = 0.0f;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int h = 0; h < 32; ++h) acc[c][h] = 0.0f;
+            const int count = k.tiles();
+            for (int i = 0; i < count && ok; ++i, ++g) {
+                if (i > 0) gather(g - 1);
+                if (ok) softmax(g);
+            }
+            if (!ok) break;
+            gather(g - 1);
+            if (!ok) break;
+            // ---- the part's result ----
+            const long long slot = (long long)w + k.b;
+            if (scoring) {
+                const float s = reduce16<false>(sum);
+                if (lane < 16) wsum[(half * 4 + quarter) * 16 + lane] = s;
+            }
+            pair_barrier(half);
+            if (scoring && token < 16 && h0 + half * 16 + token < a.heads) {
+                float m = top[0];
+#pragma unroll
+                for (int h = 1; h < 16; ++h) m = token == h ? top[h] : m;
+                const float* ws = wsum + half * 64 + token;
+                float* st = parts.stats(slot) + 2 * (h0 + half * 16 + token);
+                st[0] = m;
+                st[1] = (ws[0] + ws[16]) + (ws[32] + ws[48]);
+            }
+            pair_barrier(half);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int r = (2 * half + c) * 128 + token;
+                if (r >= R) continue;
+                float* out = parts.vectors(slot) + (long long)h0 * R + r;
+#pragma unroll
+                for (int h = 0; h < 32; ++h)
+                    if (h < HP && h0 + h < a.heads) out[(long long)h * R] = acc[c][h];
+            }
+        }
+    }
+    if (status != nullptr && *reinterpret_cast<volatile int32_t*>(status) != 0) {
+        // a wait gave up somewhere: copies and products still in flight get time to land before their memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) { }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == WARP_MMA) {
+        tcgen05_fence_after();
+        tmem_free<512>(tmem);
+    }
+}
+
+Shape shape_of(const el_latent_step_t& a) { return Shape{(a.rank + 127) / 128, a.heads <= 16 ? 16 : 32, (a.heads + 31) / 32}; }
+int shared_bytes(const el_latent_step_t& a, const Shape& s) {
+    const int stage = s.chunks * CHUNK + (a.rot_dim ? CHUNK : 0);
+    return 1024 + 2 * stage + s.chunks * s.n() * 128 + (a.rot_dim ? s.hp * 128 : 0) + CHUNK + 3232 + 96;
+}
+
+}  // namespace
+
+bool latent_step_tc_takes(const el_latent_step_t& a) {
+    return a.dtype != EL_F32 && a.rot_dim % 8 == 0 && reinterpret_cast<uintptr_t>(a.cache_keys) % 16 == 0 && (long long)a.batch * a.heads < (1 << 24);
+}
+int latent_step_tc_groups(const el_latent_step_t& a) { return shape_of(a).groups; }
+
+int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const float* steps, const void* rotated, const StepParts& parts, int workers, cudaStream_t st) {
+    const Shape shape = shape_of(a);
+    auto run = [&](auto t) {
+        using T = decltype(t);
+        static DeviceOnce once;
+        int dev = 0;
+        EL_CUDA_TRY(cudaGetDevice(&dev));
+        if (!once.is_done(dev)) {
+            EL_CUDA_TRY(cudaFuncSetAttribute(step_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+            once.mark(dev);
+        }
+        step_tc_kernel<T><<<workers * shape.groups, THREADS, shared_bytes(a, shape), st>>>(a, digits, steps, static_cast<const T*>(rotated), parts, workers, shape);
+        return check_launch();
+    };
+    return a.dtype == EL_F16 ? run(__half()) : run(__nv_bfloat16());
+}
+
+}  // namespace el
