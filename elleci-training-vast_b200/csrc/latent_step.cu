@@ -27,20 +27,49 @@ constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int GROUP = 32;             // heads of a block
 constexpr int MOST_RANK = 512, MOST_ROT = 64;
+constexpr float STEPS = 32512.0f;     // 127 * 256: the largest value of two digits whose high one is at most 127
 
-// four 2-bit codes as float: 0 -> -1, 1 -> 0, 2 -> 1, 3 -> 0
-__device__ __forceinline__ float weight_of(uint32_t w, int i) { return (float)decode2(w >> (2 * i)); }
+// Two neighbouring 2-bit codes (the low four bits of x) as two 16-bit floats: 0 -> -1, 1 -> 0, 2 -> 1, 3 -> 0, by a byte permutation of their tables.
+template <typename T> __device__ __forceinline__ uint32_t weight_pair(uint32_t first, uint32_t second) {
+    constexpr uint32_t high = std::is_same<T, __half>::value ? 0x003C00BCu : 0x003F00BFu, low = std::is_same<T, __half>::value ? 0u : 0x00800080u;
+    return prmt(high, low, first * 0x11u + (second * 0x1100u + 0x0404u));
+}
+// d += a b on the warp: a 16 x 16 (rows lane / 4 and 8 more), b 16 x 8 of T, sums in float32.  The products here are small next to what is read for them.
+template <typename T> __device__ __forceinline__ void warp_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
-// u and w of one head for PER sequences.  Thread (x, y): column words x of the weights (16 columns each), rows y, y + 8 ..
-// DIGITS: for the tensor cores, u as two 8-bit digits of 1 / 32512 of its largest magnitude (digits [.., 2, rank padded to 32], steps) and w as T [.., 64].
-template <typename T, bool DIGITS, int PER>
-__global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_step_t a, float* __restrict__ query, int8_t* __restrict__ digits, float* __restrict__ steps, T* __restrict__ rotated) {
+// w of one head of one sequence: put(c, value) for every rotated channel, by a block's threads
+template <typename T, typename F> __device__ __forceinline__ void rotated_query(const el_latent_step_t& a, int b, int h, int first, int step, F put) {
+    const float by = a.scale * mamba::LOG2E;
+    const T* x = static_cast<const T*>(a.q_rot) + b * a.q_rot_stride_b + h * a.q_rot_stride_h;
+    if (!a.table) {
+        for (int c = first; c < a.rot_dim; c += step) put(c, to_float(x[c]) * by);
+        return;
+    }
+    const int half = a.rot_dim / 2, at = step_tokens(a, b) - 1;               // the token itself is the cache's last one
+    const float* cs = a.table + (long long)(at < 0 ? 0 : at >= a.table_rows ? a.table_rows - 1 : at) * a.rot_dim;
+    for (int c = first; c < half; c += step) {
+        const int i0 = a.neighbours ? 2 * c : c, i1 = a.neighbours ? 2 * c + 1 : c + half;
+        const float u = to_float(x[i0]), v = to_float(x[i1]), co = cs[c], si = cs[c + half];
+        put(i0, fmaf(u, co, -__fmul_rn(v, si)) * by);
+        put(i1, fmaf(v, co, __fmul_rn(u, si)) * by);
+    }
+}
+
+// u and w of one head for 4 sequences, in float32.  Thread (x, y): column words x of the weights (16 columns each), rows y, y + 8 ..
+template <typename T>
+__global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_step_t a, float* __restrict__ query) {
+    constexpr int PER = 4;
     __shared__ float q[PER][256];
     __shared__ float part[WARPS][32][17];
-    __shared__ float most[WARPS];
     const int h = blockIdx.x, b0 = blockIdx.y * PER, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int words = a.rank / 16, width = a.rank + a.rot_dim;
-    const float by = a.scale * mamba::LOG2E;
     for (int i = threadIdx.x; i < PER * a.key_dim; i += THREADS) {
         const int n = i / a.key_dim, d = i - n * a.key_dim;
         q[n][d] = b0 + n < a.batch ? to_float(static_cast<const T*>(a.q)[(b0 + n) * a.q_stride_b + h * a.q_stride_h + d]) : 0.0f;
@@ -49,12 +78,11 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
     float sum[PER][16] = {};
     if (lane < words) {
         const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed + (long long)h * a.key_dim * (a.rank / 4)) + lane;
-#pragma unroll 4
         for (int d = warp; d < a.key_dim; d += WARPS) {
             const uint32_t w = W[(long long)d * words];
             float f[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = weight_of(w, i);
+            for (int i = 0; i < 16; ++i) f[i] = (float)decode2(w >> (2 * i));
 #pragma unroll
             for (int n = 0; n < PER; ++n) {
                 const float v = q[n][d];
@@ -70,60 +98,100 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
 #pragma unroll
         for (int i = 0; i < 16; ++i) part[warp][lane][i] = sum[n][i];
         __syncthreads();
-        const long long bh = (long long)(b0 + n) * a.heads + h;
-        float* out = query + bh * width;
-        float u[MOST_RANK / THREADS], top = 0.0f;
+        float* out = query + ((long long)(b0 + n) * a.heads + h) * width;
+        for (int c = threadIdx.x; c < a.rank; c += THREADS) {
+            float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < MOST_RANK / THREADS; ++i) {
-            const int c = threadIdx.x + i * THREADS;
-            u[i] = 0.0f;
-            if (c < a.rank) {
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) u[i] += part[w][c / 16][c % 16];
-                u[i] *= a.gamma * by;
-                if (!DIGITS) out[c] = u[i];
-            }
-            top = mamba::max_nan(top, fabsf(u[i]));
+            for (int w = 0; w < WARPS; ++w) s += part[w][c / 16][c % 16];
+            out[c] = s * (a.gamma * a.scale * mamba::LOG2E);
         }
-        if constexpr (DIGITS) {
-            const int rp = (a.rank + 31) / 32 * 32;
+        if (a.rot_dim) rotated_query<T>(a, b0 + n, h, threadIdx.x, THREADS, [&](int c, float v) { out[a.rank + c] = v; });
+    }
+}
+
+// u and w for the tensor cores: of one head, 128 columns of u for 64 sequences.  u = gamma scale log2(e) q W is held in two 8-bit digits of 1 / 32512 of
+// gamma scale log2(e) sum |q|, which it cannot exceed whatever the weights are: no block has to know another's columns.  (For weights of
+// random signs that is 3 to 4 times the largest u, 14 bits of it.)  digits [batch, heads, 2, rank padded to 32], steps [batch, heads], w [batch, heads, 64].
+// A warp takes 16 columns, which are one word of every row of the weights.
+constexpr int QUERY_ROWS = 64, QUERY_COLS = 128;
+template <typename T>
+__global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_latent_step_t a, int8_t* __restrict__ digits, float* __restrict__ steps, T* __restrict__ rotated) {
+    __shared__ T q[QUERY_ROWS][256 + 8];
+    __shared__ uint32_t W[256][WARPS + 1];
+    __shared__ float most[QUERY_ROWS];
+    const int h = blockIdx.x, c0 = blockIdx.y * QUERY_COLS, b0 = blockIdx.z * QUERY_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nb = min(QUERY_ROWS, a.batch - b0), D = a.key_dim, DP = (D + 15) / 16 * 16, words = a.rank / 16, rp = (a.rank + 31) / 32 * 32;
+    const float by = a.gamma * a.scale * mamba::LOG2E;
+    for (int i = threadIdx.x; i < DP * WARPS; i += THREADS) {
+        const int d = i / WARPS, w = i - d * WARPS;
+        W[d][w] = d < D && c0 / 16 + w < words ? reinterpret_cast<const uint32_t*>(a.W_packed)[((long long)h * D + d) * words + c0 / 16 + w] : 0x55555555u;
+    }
+    const int rows = (nb + 15) / 16 * 16;
+    for (int i = threadIdx.x; i < rows * DP; i += THREADS) {
+        const int n = i / DP, d = i - n * DP;
+        q[n][d] = n < nb && d < D ? static_cast<const T*>(a.q)[(b0 + n) * a.q_stride_b + h * a.q_stride_h + d] : mamba::from_float<T>(0.0f);
+    }
+    __syncthreads();
+    for (int n = warp; n < nb; n += WARPS) {
+        float s = 0.0f;
+        for (int d = lane; d < D; d += 32) s += fabsf(to_float(q[n][d]));
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) top = mamba::max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
-            if (lane == 0) most[warp] = top;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) top = mamba::max_nan(top, most[w]);
-            const float step = top * (1.0f / 32512.0f), inv = step > 0.0f ? 32512.0f / top : 0.0f;
-            if (threadIdx.x == 0) steps[bh] = step;                  // a NaN or infinity makes the scores NaN
-#pragma unroll
-            for (int i = 0; i < MOST_RANK / THREADS; ++i) {
-                const int c = threadIdx.x + i * THREADS;
-                if (c >= rp) continue;
-                const int v = __float2int_rn(u[i] * inv), hi = (v + 128) >> 8;
-                digits[bh * 2 * rp + c] = (int8_t)hi;
-                digits[bh * 2 * rp + rp + c] = (int8_t)(v - hi * 256);
-            }
-            for (int c = a.rot_dim + threadIdx.x; c < 64; c += THREADS) rotated[bh * 64 + c] = mamba::from_float<T>(0.0f);
-        }
-        auto put = [&](int c, float v) {
-            if constexpr (DIGITS) rotated[bh * 64 + c] = mamba::from_float<T>(v);
-            else out[a.rank + c] = v;
-        };
-        if (a.rot_dim == 0) continue;
-        const T* x = static_cast<const T*>(a.q_rot) + (b0 + n) * a.q_rot_stride_b + h * a.q_rot_stride_h;
-        if (!a.table) {
-            for (int c = threadIdx.x; c < a.rot_dim; c += THREADS) put(c, to_float(x[c]) * by);
-            continue;
-        }
-        const int half = a.rot_dim / 2, at = step_tokens(a, b0 + n) - 1;      // the token itself is the cache's last one
-        const float* cs = a.table + (long long)(at < 0 ? 0 : at >= a.table_rows ? a.table_rows - 1 : at) * a.rot_dim;
-        for (int c = threadIdx.x; c < half; c += THREADS) {
-            const int i0 = a.neighbours ? 2 * c : c, i1 = a.neighbours ? 2 * c + 1 : c + half;
-            const float u = to_float(x[i0]), v = to_float(x[i1]), co = cs[c], si = cs[c + half];
-            put(i0, fmaf(u, co, -__fmul_rn(v, si)) * by);
-            put(i1, fmaf(v, co, __fmul_rn(u, si)) * by);
+        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        if (lane == 0) {
+            most[n] = s > 0.0f ? STEPS / s : 0.0f;
+            if (c0 == 0) steps[(long long)(b0 + n) * a.heads + h] = by * s * (1.0f / STEPS);      // a NaN or infinity makes the scores NaN
         }
     }
+    if (c0 == 0 && a.rot_dim) {
+        for (int n = warp; n < nb; n += WARPS) {
+            T* out = rotated + ((long long)(b0 + n) * a.heads + h) * 64;
+            rotated_query<T>(a, b0 + n, h, lane, 32, [&](int c, float v) { out[c] = mamba::from_float<T>(v); });
+            for (int c = a.rot_dim + lane; c < 64; c += 32) out[c] = mamba::from_float<T>(0.0f);
+        }
+    }
+    float sum[QUERY_ROWS / 16][2][4] = {};
+    const int r = lane >> 2, k2 = (lane & 3) * 2;
+    for (int k = 0; k < DP; k += 16) {
+        const uint32_t w0 = W[k + k2][warp], w1 = W[k + k2 + 1][warp], w2 = W[k + k2 + 8][warp], w3 = W[k + k2 + 9][warp];
+        uint32_t b[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int at = 2 * (t * 8 + r);
+            b[t][0] = weight_pair<T>((w0 >> at) & 3u, (w1 >> at) & 3u);
+            b[t][1] = weight_pair<T>((w2 >> at) & 3u, (w3 >> at) & 3u);
+        }
+#pragma unroll
+        for (int m = 0; m < QUERY_ROWS / 16; ++m) {
+            if (m * 16 >= nb) break;
+            const uint32_t x[4] = {*reinterpret_cast<const uint32_t*>(&q[m * 16 + r][k + k2]), *reinterpret_cast<const uint32_t*>(&q[m * 16 + r + 8][k + k2]),
+                                   *reinterpret_cast<const uint32_t*>(&q[m * 16 + r][k + k2 + 8]), *reinterpret_cast<const uint32_t*>(&q[m * 16 + r + 8][k + k2 + 8])};
+            warp_mma<T>(sum[m][0], x, b[0][0], b[0][1]);
+            warp_mma<T>(sum[m][1], x, b[1][0], b[1][1]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < QUERY_ROWS / 16; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int n = m * 16 + r + 8 * i;
+            if (n >= nb) continue;
+            const float inv = most[n];
+            int8_t* out = digits + ((long long)(b0 + n) * a.heads + h) * 2 * rp;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int c = c0 + warp * 16 + t * 8 + k2;
+                if (c >= rp) continue;
+                int v[2], hi[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    v[e] = min(max(__float2int_rn(sum[m][t][2 * i + e] * inv), -(int)STEPS), (int)STEPS);
+                    hi[e] = (v[e] + 128) >> 8;
+                }
+                *reinterpret_cast<char2*>(out + c) = make_char2((signed char)hi[0], (signed char)hi[1]);
+                *reinterpret_cast<char2*>(out + rp + c) = make_char2((signed char)(v[0] - hi[0] * 256), (signed char)(v[1] - hi[1] * 256));
+            }
+        }
 }
 
 // A block takes 32 heads of a worker's tokens, 32 at a time; a warp takes 4 heads: a lane is a token for the scores, a column in every 32 for the sums.
@@ -235,52 +303,112 @@ __global__ void __launch_bounds__(THREADS) step_rows_kernel(const el_latent_step
     }
 }
 
-// A block joins the parts of one head of one sequence and takes the result through the head's value rows.
+// A block joins the parts of one head of up to 16 sequences and takes the results through the head's value rows.  Sequences are spread over the 16
+// warps; where there are fewer, several warps share a sequence's parts.  The product with the value rows runs on the warps' matrix instructions, the float32
+// vectors split into two bfloat16 terms (16 bits of each), three for float32 outputs.
+constexpr int JOIN_THREADS = 512, JOIN_ROWS = 16, JOIN_PITCH = MOST_RANK + 8;
+template <typename T> constexpr int JOIN_TERMS = sizeof(T) == 4 ? 3 : 2;
+template <typename T> constexpr int JOIN_BYTES = JOIN_ROWS * MOST_RANK * 4 + JOIN_TERMS<T> * JOIN_ROWS * JOIN_PITCH * 2;
+
 template <typename T>
-__global__ void __launch_bounds__(THREADS) step_join_kernel(const el_latent_step_t a, const StepParts parts, int workers) {
-    __shared__ float o[MOST_RANK];
-    __shared__ int range[2];
-    const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.rank;
-    if (warp == 0) {
-        const long long tiles = step_tiles_before(a, a.batch), before = step_tiles_before(a, b);
-        const int here = step_tiles(a, b);
-        workers = step_active(workers, tiles);
-        if (lane == 0) {
-            range[0] = here ? step_worker(before, workers, tiles) : 0;
-            range[1] = here ? step_worker(before + here - 1, workers, tiles) : -1;
+__global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent_step_t a, const StepParts parts, int workers) {
+    extern __shared__ float4 join_smem[];
+    float* o = reinterpret_cast<float*>(join_smem);                                            // [16 warps][512]
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(o + JOIN_ROWS * MOST_RANK);        // [terms][16 sequences][JOIN_PITCH]
+    const int h = blockIdx.x, b0 = blockIdx.y * JOIN_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.rank;
+    const int nb = min(JOIN_ROWS, a.batch - b0);
+    int spread = 1;                                  // sequences side by side, a power of two; 16 / spread warps share one
+    while (spread < nb) spread *= 2;
+    const int shares = 16 / spread, share = warp / spread, b = b0 + warp % spread;
+    float acc[MOST_RANK / 32] = {};
+    if (warp % spread < nb) {
+        long long tiles = 0, before = 0;
+        int here = 0;
+        for (int x = lane; x < a.batch; x += 32) {
+            const int n = step_tiles(a, x);
+            tiles += n;
+            before += x < b ? n : 0;
+            here += x == b ? n : 0;
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            tiles += __shfl_xor_sync(0xffffffffu, tiles, x);
+            before += __shfl_xor_sync(0xffffffffu, before, x);
+            here += __shfl_xor_sync(0xffffffffu, here, x);
+        }
+        if (here > 0) {
+            const int active = step_active(workers, tiles), w0 = step_worker(before, active, tiles), w1 = step_worker(before + here - 1, active, tiles);
+            float top = -INFINITY, sum = 0.0f;
+            for (int w = w0 + lane; w <= w1; w += 32) top = mamba::max_nan(top, parts.stats((long long)w + b)[2 * h]);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) top = mamba::max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float from = top == -INFINITY ? 0.0f : top;
+            for (int w = w0 + lane; w <= w1; w += 32) {
+                const float2 st = *reinterpret_cast<const float2*>(parts.stats((long long)w + b) + 2 * h);
+                sum = fmaf(exp2_neg(st.x - from), st.y, sum);
+            }
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            const float by = top == -INFINITY ? 0.0f : a.gamma / sum;
+            // 32 of this warp's parts at a time: lane l has the factor of the l-th
+            for (int p = w0 + share; p <= w1; p += 32 * shares) {
+                const int mine = p + lane * shares, count = min(32, (w1 - p) / shares + 1);
+                const float f = mine <= w1 ? exp2_neg(parts.stats((long long)mine + b)[2 * h] - from) * by : 0.0f;
+#pragma unroll 4
+                for (int i = 0; i < count; ++i) {
+                    const float x = __shfl_sync(0xffffffffu, f, i);
+                    const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + i * shares + b) + (long long)h * R);
+#pragma unroll
+                    for (int c = 0; c < MOST_RANK / 128; ++c) {
+                        if ((c * 32 + lane) * 4 >= R) continue;
+                        const float4 y = v[c * 32 + lane];
+                        acc[4 * c] = fmaf(x, y.x, acc[4 * c]);
+                        acc[4 * c + 1] = fmaf(x, y.y, acc[4 * c + 1]);
+                        acc[4 * c + 2] = fmaf(x, y.z, acc[4 * c + 2]);
+                        acc[4 * c + 3] = fmaf(x, y.w, acc[4 * c + 3]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < MOST_RANK / 128; ++c)
+        reinterpret_cast<float4*>(o + warp * MOST_RANK)[c * 32 + lane] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < JOIN_ROWS * R; i += JOIN_THREADS) {
+        const int n = i / R, c = i - n * R;
+        float v = 0.0f;
+        if (n < nb)
+            for (int s = 0; s < shares; ++s) v += o[(s * spread + n) * MOST_RANK + c];
+#pragma unroll
+        for (int t = 0; t < JOIN_TERMS<T>; ++t) {
+            const __nv_bfloat16 x = __float2bfloat16_rn(v);
+            terms[(t * JOIN_ROWS + n) * JOIN_PITCH + c] = x;
+            v -= __bfloat162float(x);
         }
     }
     __syncthreads();
-    const int w0 = range[0], w1 = range[1];
-    float top = -INFINITY, sum = 0.0f;
-    for (int w = w0; w <= w1; ++w) top = mamba::max_nan(top, parts.stats((long long)w + b)[2 * h]);
-    for (int w = w0; w <= w1; ++w) {
-        const float m = parts.stats((long long)w + b)[2 * h];
-        if (m != -INFINITY) sum += exp2_neg(m - top) * parts.stats((long long)w + b)[2 * h + 1];
-    }
-    const float by = top == -INFINITY ? 0.0f : a.gamma / sum;
-    for (int c = threadIdx.x; c < R; c += THREADS) {
-        float s = 0.0f;
-        for (int w = w0; w <= w1; ++w) {
-            const float m = parts.stats((long long)w + b)[2 * h];
-            if (m != -INFINITY) s = fmaf(exp2_neg(m - top), parts.vectors((long long)w + b)[(long long)h * R + c], s);
-        }
-        o[c] = s * by;
-    }
-    __syncthreads();
-    const int words = R / 16;
-    const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim) * (R / 4));
-    T* out = static_cast<T*>(a.out) + ((long long)b * a.heads + h) * a.value_dim;
-    for (int v = warp; v < a.value_dim; v += WARPS) {
-        float s = 0.0f;
-        if (lane < words) {
-            const uint32_t w = W[(long long)v * words + lane];
+    const int words = R / 16, r = lane >> 2, k2 = (lane & 3) * 2;
+    const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim) * words;
+    for (int v0 = warp * 8; v0 < a.value_dim; v0 += 128) {
+        float d[4] = {};
+#pragma unroll 4
+        for (int k = 0; k < words; ++k) {
+            const uint32_t w = (v0 + r < a.value_dim ? W[(long long)(v0 + r) * words + k] : 0x55555555u) >> (2 * k2);
+            const uint32_t x0 = weight_pair<__nv_bfloat16>(w & 3u, (w >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((w >> 16) & 3u, (w >> 18) & 3u);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s = fmaf(weight_of(w, i), o[lane * 16 + i], s);
+            for (int t = JOIN_TERMS<T> - 1; t >= 0; --t) {
+                const __nv_bfloat16* p = terms + (t * JOIN_ROWS + r) * JOIN_PITCH + k * 16 + k2;
+                const uint32_t x[4] = {*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH), *reinterpret_cast<const uint32_t*>(p + 8),
+                                       *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH + 8)};
+                warp_mma<__nv_bfloat16>(d, x, x0, x1);
+            }
         }
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        if (lane == 0) out[v] = mamba::from_float<T>(s);
+        for (int i = 0; i < 4; ++i) {
+            const int n = r + 8 * (i >> 1), v = v0 + k2 + (i & 1);
+            if (n < nb && v < a.value_dim) static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v] = mamba::from_float<T>(d[i]);
+        }
     }
 }
 
@@ -290,6 +418,16 @@ template <typename F> int of_type(int dtype, F f) {
         case EL_BF16: return f(__nv_bfloat16());
         default: return f(float());
     }
+}
+
+template <typename K> int allow_shared(K kernel, int bytes, DeviceOnce& once) {
+    int dev = 0;
+    EL_CUDA_TRY(cudaGetDevice(&dev));
+    if (!once.is_done(dev)) {
+        EL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        once.mark(dev);
+    }
+    return EL_OK;
 }
 
 // Blocks that share the tokens: one for every SM, but no more than there can be tiles.
@@ -319,38 +457,33 @@ size_t latent_step_workspace_bytes(const el_latent_step_t& a) {
 int launch_latent_step(const el_latent_step_t& a, cudaStream_t st) {
     const int workers = step_workers(a, groups_of(a));
     char* ws = static_cast<char*>(a.workspace);
-    const StepParts parts{reinterpret_cast<float*>(ws + query_bytes(a)), a.heads, a.rank};
-    constexpr int PER = 4;
-    const dim3 grid(a.heads, (a.batch + PER - 1) / PER);
+    float* vectors = reinterpret_cast<float*>(ws + query_bytes(a));
+    const StepParts parts{vectors, vectors + (size_t)(workers + a.batch) * a.heads * a.rank, a.heads, a.rank};
     return of_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         int rc = EL_OK;
-        if (latent_step_tc_takes(a)) {
+        if (!latent_step_tc_takes(a)) {
+            float* query = reinterpret_cast<float*>(ws);
+            step_query_kernel<T><<<dim3(a.heads, (a.batch + 3) / 4), THREADS, 0, st>>>(a, query);
+            constexpr int bytes = 4 * (32 * (MOST_RANK + MOST_ROT + 1) + GROUP * (MOST_RANK + MOST_ROT));
+            static DeviceOnce once;
+            if ((rc = check_launch()) == EL_OK) rc = allow_shared(step_rows_kernel<T>, bytes, once);
+            if (rc == EL_OK && workers > 0) {
+                step_rows_kernel<T><<<dim3(workers, (a.heads + GROUP - 1) / GROUP), THREADS, bytes, st>>>(a, query, parts, workers);
+                rc = check_launch();
+            }
+        } else if constexpr (!std::is_same<T, float>::value) {
             int8_t* digits = reinterpret_cast<int8_t*>(ws);
             float* steps = reinterpret_cast<float*>(ws + digits_bytes(a));
             T* rotated = reinterpret_cast<T*>(ws + digits_bytes(a) + steps_bytes(a));
-            step_query_kernel<T, true, PER><<<grid, THREADS, 0, st>>>(a, nullptr, digits, steps, rotated);
-            if ((rc = check_launch()) != EL_OK) return rc;
-            if (workers > 0) rc = launch_latent_step_tc(a, digits, steps, rotated, parts, workers, st);
-        } else {
-            float* query = reinterpret_cast<float*>(ws);
-            step_query_kernel<T, false, PER><<<grid, THREADS, 0, st>>>(a, query, nullptr, nullptr, nullptr);
-            if ((rc = check_launch()) != EL_OK) return rc;
-            if (workers > 0) {
-                static DeviceOnce once;
-                int dev = 0;
-                constexpr int most = 4 * (32 * (MOST_RANK + MOST_ROT + 1) + GROUP * (MOST_RANK + MOST_ROT));
-                EL_CUDA_TRY(cudaGetDevice(&dev));
-                if (!once.is_done(dev)) {
-                    EL_CUDA_TRY(cudaFuncSetAttribute(step_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-                    once.mark(dev);
-                }
-                step_rows_kernel<T><<<dim3(workers, (a.heads + GROUP - 1) / GROUP), THREADS, most, st>>>(a, query, parts, workers);
-                rc = check_launch();
-            }
+            const dim3 grid(a.heads, (a.rank + QUERY_COLS - 1) / QUERY_COLS, (a.batch + QUERY_ROWS - 1) / QUERY_ROWS);
+            step_query_digits_kernel<T><<<grid, THREADS, 0, st>>>(a, digits, steps, rotated);
+            if ((rc = check_launch()) == EL_OK && workers > 0) rc = launch_latent_step_tc(a, digits, steps, rotated, parts, workers, st);
         }
         if (rc != EL_OK) return rc;
-        step_join_kernel<T><<<(unsigned)(a.batch * a.heads), THREADS, 0, st>>>(a, parts, workers);
+        static DeviceOnce once;
+        if ((rc = allow_shared(step_join_kernel<T>, JOIN_BYTES<T>, once)) != EL_OK) return rc;
+        step_join_kernel<T><<<dim3(a.heads, (a.batch + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, JOIN_BYTES<T>, st>>>(a, parts, workers);
         return check_launch();
     });
 }

@@ -53,12 +53,12 @@ __device__ __forceinline__ int step_active(int workers, long long tiles) { retur
 // the worker that has tile t
 __device__ __forceinline__ int step_worker(long long t, int workers, long long tiles) { return (int)(((t + 1) * workers - 1) / tiles); }
 
-// A slot: for each head its largest score and its sum, then the heads' latent vectors.
+// A slot: for each head its largest score and its sum, and its latent vector.
 struct StepParts {
-    float* base;
+    float *vectors_at, *stats_at;
     int heads, rank;
-    __device__ __forceinline__ float* stats(long long slot) const { return base + slot * heads * (2LL + rank); }
-    __device__ __forceinline__ float* vectors(long long slot) const { return stats(slot) + 2 * heads; }
+    __device__ __forceinline__ float* vectors(long long slot) const { return vectors_at + slot * heads * rank; }
+    __device__ __forceinline__ float* stats(long long slot) const { return stats_at + slot * heads * 2; }
 };
 
 // the pool's row of position p of sequence b, or -1

@@ -11,12 +11,17 @@
 //
 // Warps 0-7: thread t of each half is token t of the tile and takes 16 heads' scores; then two of the four blocks of 128 latent channels, a thread a channel.
 // The sums of a tile are taken while the tensor core forms the next tile's scores.  Warp 8 issues the products.  Warps
-// 9 and 10 load, each every other tile: 16-byte asynchronous copies of a token's row from wherever its page lies.
+// 9 and 10 load, each every other tile: by tensor maps where pages are multiples of 8 tokens (a box lies in one page), otherwise by 16-byte
+// asynchronous copies of each token's row.
 // Bound: memory; a tile of 128 tokens of rank 512 and 64 rotated channels is 82 KB, 3400 cycles of an SM's share of the HBM, and 1100 of its tensor core.
 #include "latent_step.cuh"
 #include "latent_tc.cuh"
 
 namespace el {
+
+namespace tc {
+int make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes);
+}
 
 using namespace tc;
 using namespace latent;
@@ -30,6 +35,7 @@ constexpr float MAGIC = 12582912.0f;                   // 1.5 * 2^23: adding it 
 
 struct Shape {
     int chunks, hp, groups;                            // 128-byte chunks of a row; heads of a group, padded to 16 or 32
+    int box;                                           // tokens of a tensor map's box, which lie in one page; 0: no tensor maps
     __host__ __device__ int n() const { return 2 * hp; }
 };
 
@@ -39,6 +45,10 @@ __device__ __forceinline__ uint32_t low_digit(int v) { return (uint32_t)v & 0xFF
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// bytes that a barrier's phase waits for, without an arrival
+__device__ __forceinline__ void mbar_expect_tx_only(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void pair_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); }
 
@@ -95,7 +105,7 @@ template <bool MAX> __device__ __forceinline__ float reduce16(const float (&v)[1
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1)
-step_tc_kernel(const el_latent_step_t a, const int8_t* __restrict__ digits, const float* __restrict__ steps, const T* __restrict__ rotated, const StepParts parts,
+step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant__ CUtensorMap tmKeys, const el_latent_step_t a, const int8_t* __restrict__ digits, const float* __restrict__ steps, const T* __restrict__ rotated, const StepParts parts,
                int workers, const Shape shape) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -160,34 +170,61 @@ step_tc_kernel(const el_latent_step_t a, const int8_t* __restrict__ digits, cons
                     const int p = k.p0 + i * TOKENS;
                     long long row[4];
                     float sc[4];
+                    if (shape.box) {                                                  // lane l looks up box l
+                        const int pos = p + lane * shape.box;
+                        const long long start = lane * shape.box < TOKENS && pos < k.p1 ? step_row(a, k.b, pos) : -1;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int pos = p + q * 32 + lane;
-                        row[q] = pos < k.p1 ? step_row(a, k.b, pos) : -1;
-                        sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
-                    }
-                    if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-#pragma unroll 8
-                        for (int t = 0; t < 32; ++t) {
-                            const long long r = __shfl_sync(0xffffffffu, row[q], t);
-                            const int to = q * 32 + t;
-                            if (lane * 16 < R && r >= 0)
-                                copy16(at + (lane >> 3) * CHUNK + to * 128 + (((lane & 7) ^ (to & 7)) << 4), a.latents + r * R + lane * 16, true);
+                        for (int q = 0; q < 4; ++q) {
+                            const int to = q * 32 + lane;
+                            const long long r = __shfl_sync(0xffffffffu, start, to / shape.box);
+                            row[q] = r >= 0 && p + to < k.p1 ? r + to % shape.box : -1;
+                            sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
                         }
-                        if (P) {
-                            const int pieces = (P + 15) / 16 * 2;                     // of 8 channels, zeros behind the last
+                        if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
+                        const unsigned there = __ballot_sync(0xffffffffu, start >= 0);
+                        if (elect_one()) mbar_expect_tx_only(full(mine), __popc(there) * shape.box * 128 * (KC + (P ? 1 : 0)));
+                        __syncwarp();
+                        for (int x = 0; x < TOKENS / shape.box; ++x) {
+                            const int r = __shfl_sync(0xffffffffu, (int)start, x);
+                            if (r >= 0 && elect_one()) {
+                                for (int c = 0; c < KC; ++c) tma_load_2d(at + c * CHUNK + x * shape.box * 128, &tmRows, full(mine), c * 128, r);
+                                if (P) tma_load_2d(at + KC * CHUNK + x * shape.box * 128, &tmKeys, full(mine), 0, r);
+                            }
+                            __syncwarp();
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int pos = p + q * 32 + lane;
+                            row[q] = pos < k.p1 ? step_row(a, k.b, pos) : -1;
+                            sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
+                        }
+                        if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+#pragma unroll 8
+                            for (int t = 0; t < 32; ++t) {
+                                const long long r = __shfl_sync(0xffffffffu, row[q], t);
+                                const int to = q * 32 + t;
+                                if (lane * 16 < R && r >= 0)
+                                    copy16(at + (lane >> 3) * CHUNK + to * 128 + (((lane & 7) ^ (to & 7)) << 4), a.latents + r * R + lane * 16, true);
+                            }
+                            if (P) {
+                                const int pieces = (P + 15) / 16 * 2;                 // of 8 channels, zeros behind the last
 #pragma unroll 4
-                            for (int t = 0; t < 32; t += 4) {
-                                const int tt = t + (lane >> 3), c = lane & 7, to = q * 32 + tt;
-                                const long long r = __shfl_sync(0xffffffffu, row[q], tt);
-                                if (c < pieces) {
-                                    const bool there = r >= 0 && c * 8 < P;
-                                    copy16(at + KC * CHUNK + to * 128 + ((c ^ (to & 7)) << 4), there ? static_cast<const T*>(a.cache_keys) + r * P + c * 8 : a.cache_keys, there);
+                                for (int t = 0; t < 32; t += 4) {
+                                    const int tt = t + (lane >> 3), c = lane & 7, to = q * 32 + tt;
+                                    const long long r = __shfl_sync(0xffffffffu, row[q], tt);
+                                    if (c < pieces) {
+                                        const bool there = r >= 0 && c * 8 < P;
+                                        copy16(at + KC * CHUNK + to * 128 + ((c ^ (to & 7)) << 4), there ? static_cast<const T*>(a.cache_keys) + r * P + c * 8 : a.cache_keys, there);
+                                    }
                                 }
                             }
                         }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
                         scale_of[mine * 128 + q * 32 + lane] = __fdiv_rn(sc[q], 127.0f);
                         const uint32_t have = __ballot_sync(0xffffffffu, row[q] >= 0);
                         if (lane == 0) seen[mine * 4 + q] = have;
@@ -441,7 +478,14 @@ step_tc_kernel(const el_latent_step_t a, const int8_t* __restrict__ digits, cons
     }
 }
 
-Shape shape_of(const el_latent_step_t& a) { return Shape{(a.rank + 127) / 128, a.heads <= 16 ? 16 : 32, (a.heads + 31) / 32}; }
+// Parts begin at multiples of STEP_TILE, so boxes of up to that many tokens do not cross pages that they divide.
+int box_of(const el_latent_step_t& a) {
+    int g = STEP_TILE;
+    while (g > 1 && a.page_size % g) g /= 2;
+    // (a tensor map's rows are counted in 31 bits)
+    return g >= 8 && a.pages > 0 && (long long)a.pages * a.page_size < (1LL << 31) ? g : 0;
+}
+Shape shape_of(const el_latent_step_t& a) { return Shape{(a.rank + 127) / 128, a.heads <= 16 ? 16 : 32, (a.heads + 31) / 32, box_of(a)}; }
 int shared_bytes(const el_latent_step_t& a, const Shape& s) {
     const int stage = s.chunks * CHUNK + (a.rot_dim ? CHUNK : 0);
     return 1024 + 2 * stage + s.chunks * s.n() * 128 + (a.rot_dim ? s.hp * 128 : 0) + CHUNK + 3232 + 96;
@@ -455,7 +499,14 @@ bool latent_step_tc_takes(const el_latent_step_t& a) {
 int latent_step_tc_groups(const el_latent_step_t& a) { return shape_of(a).groups; }
 
 int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const float* steps, const void* rotated, const StepParts& parts, int workers, cudaStream_t st) {
-    const Shape shape = shape_of(a);
+    Shape shape = shape_of(a);
+    CUtensorMap rows = {}, keys = {};
+    if (shape.box) {
+        const uint64_t tokens = (uint64_t)a.pages * a.page_size;
+        int rc = make_map(&rows, a.latents, a.rank, tokens, a.rank, 128, shape.box, 128);
+        if (rc == EL_OK && a.rot_dim) rc = make_map(&keys, a.cache_keys, a.rot_dim * 2, tokens, a.rot_dim * 2, 128, shape.box, 128);
+        if (rc != EL_OK) return rc;
+    }
     auto run = [&](auto t) {
         using T = decltype(t);
         static DeviceOnce once;
@@ -465,7 +516,7 @@ int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const
             EL_CUDA_TRY(cudaFuncSetAttribute(step_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
             once.mark(dev);
         }
-        step_tc_kernel<T><<<workers * shape.groups, THREADS, shared_bytes(a, shape), st>>>(a, digits, steps, static_cast<const T*>(rotated), parts, workers, shape);
+        step_tc_kernel<T><<<workers * shape.groups, THREADS, shared_bytes(a, shape), st>>>(rows, keys, a, digits, steps, static_cast<const T*>(rotated), parts, workers, shape);
         return check_launch();
     };
     return a.dtype == EL_F16 ? run(__half()) : run(__nv_bfloat16());

@@ -101,7 +101,7 @@ def attention(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, dtype, d
 
 
 def cached(latents, absmax, keys, block_table, n):
-    """(values [n, rank], keys [n, rot] or None, truth values of what has a page) of positions 0 .. n - 1 of one sequence; block_table its row."""
+    """(values [n, rank], keys [n, rot] or None, truth values of what has a page, rows of the pool) of positions 0 .. n - 1 of one sequence; block_table its row."""
     pages, page, rank = latents.shape
     at = torch.arange(n)
     entry = block_table.long()[at // page]
@@ -109,7 +109,7 @@ def cached(latents, absmax, keys, block_table, n):
     row = torch.where(here, entry, 0) * page + at % page
     value = latents.reshape(-1, rank)[row].double() * (absmax.reshape(-1)[row].double() / 127)[:, None]
     k = None if keys is None else keys.reshape(-1, keys.shape[-1])[row].double()
-    return value, k, here
+    return value, k, here, row
 
 
 def step(q, W, gamma, latents, absmax, keys, block_table, lengths, value_dim, q_rot, table, scale, dtype, neighbours=False):
@@ -123,14 +123,15 @@ def step(q, W, gamma, latents, absmax, keys, block_table, lengths, value_dim, q_
     out, bound = torch.zeros(B, H, value_dim, dtype=torch.float64), torch.zeros(B, H, value_dim, dtype=torch.float64)
     for b in range(B):
         n = int(lengths[b].clamp(0, most))
-        c, k, here = cached(latents, absmax, keys, block_table[b], n)
+        c, k, here, rows = cached(latents, absmax, keys, block_table[b], n)
         if not bool(here.any()):
             continue
         u = torch.einsum("hd,hdr->hr", q[b].double(), Wk)
         u_abs = torch.einsum("hd,hdr->hr", q[b].double().abs(), Wk.abs())
         z, size = u @ c.T, u.abs() @ c.abs().T
-        # u is rounded as a factor, and is a sum of D terms before that
-        off = (unit * u.abs() + E * (D + 4) * u_abs) @ c.abs().T + tiny * math.sqrt(rank) * c.abs().sum(-1)
+        # u is rounded as a factor: relative to itself, or to half a 32512th of the sum of |q| that bounds it; it is a sum of D terms before that
+        step_of = (q[b].double().abs().sum(-1, keepdim=True) * abs(gamma) / (2 * 32512) if dtype != torch.float32 else 0.0) + unit * u.abs()
+        off = (step_of + E * (D + 4) * u_abs) @ c.abs().T + tiny * math.sqrt(rank) * c.abs().sum(-1)
         if R:
             w = q_rot[b].double() if table is None else rotate(q_rot[b].double(), table, torch.full((H,), n - 1).clamp(max=table.shape[0] - 1), neighbours)
             z = z + w @ k.T
@@ -140,9 +141,14 @@ def step(q, W, gamma, latents, absmax, keys, block_table, lengths, value_dim, q_
         off = ((off + E * (rank + R + 8) * size) * abs(scale)).amax(-1, keepdim=True)
         p = _probabilities(z, here.expand(H, -1))
         rel = 2 * off + 4 * 2.0 ** -22 + 4 * (n + 8) * E + unit
-        # probabilities are rounded together with their token's scale; the parts' sums are float32
+        # probabilities are rounded together with their token's scale, relative to themselves, or to half a 32512th of the largest probability times the
+        # largest scale (of the tile; here of all); the parts' sums are float32
         o, o_abs = p @ c, p @ c.abs()
         o_off = o_abs * (rel + n * E) + tiny * c.abs().sum(0)
+        if dtype != torch.float32:
+            scale_of = absmax.reshape(-1)[rows[here]].double() / 127
+            ints = latents.reshape(-1, rank)[rows[here]].double().abs().sum(0)
+            o_off = o_off + p.amax(-1, keepdim=True) * float(scale_of.max()) * ints * (1 + 1e-3) / (2 * 32512)
         out[b] = torch.einsum("hr,hvr->hv", o, Wv)
         bound[b] = torch.einsum("hr,hvr->hv", o_off + (rank + 4) * E * o_abs, Wv.abs()) + unit * out[b].abs() + tiny
     return out, bound

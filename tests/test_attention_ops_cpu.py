@@ -107,7 +107,7 @@ def test_reference_step_is_the_expanded_form():
     latents, absmax = torch.randint(-128, 128, (4, page, rank), generator=g).to(torch.int8), torch.rand(4, page, generator=g)
     blocks, W, q = torch.tensor([[2, 0, 3]]), torch.randint(-1, 2, (H * (D + V), rank), generator=g), torch.randn(B, H, D, generator=g)
     out, _ = R.step(q, W, 0.3, latents, absmax, None, blocks, torch.tensor([n]), V, None, None, None, torch.float32)
-    c, _, here = R.cached(latents, absmax, None, blocks[0], n)
+    c, _, here, _ = R.cached(latents, absmax, None, blocks[0], n)
     assert here.all()
     kv = (c @ W.double().T * 0.3)[None]
     value, _ = R.attention(q[:, None], kv, None, None, True, None, None, None, torch.float32)
