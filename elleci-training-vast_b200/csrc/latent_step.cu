@@ -15,9 +15,7 @@
 namespace el {
 
 bool latent_step_tc_takes(const el_latent_step_t& a);
-int latent_step_tc_groups(const el_latent_step_t& a);
-int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const float* steps, const void* rotated, const latent::StepParts& parts, int workers,
-                          cudaStream_t st);
+int launch_latent_step_tc(const el_latent_step_t& a, const uint8_t* images, const float* steps, const latent::StepParts& parts, int workers, cudaStream_t st);
 
 using namespace latent;
 
@@ -44,22 +42,21 @@ template <typename T> __device__ __forceinline__ void warp_mma(float (&d)[4], co
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// w of one head of one sequence: put(c, value) for every rotated channel, by a block's threads
-template <typename T, typename F> __device__ __forceinline__ void rotated_query(const el_latent_step_t& a, int b, int h, int first, int step, F put) {
+// pair c (of rot_dim / 2) of w of one head of one sequence: put(channel, value)
+template <typename T, typename F> __device__ __forceinline__ void rotated_query(const el_latent_step_t& a, int b, int h, int c, F put) {
     const float by = a.scale * mamba::LOG2E;
     const T* x = static_cast<const T*>(a.q_rot) + b * a.q_rot_stride_b + h * a.q_rot_stride_h;
-    if (!a.table) {
-        for (int c = first; c < a.rot_dim; c += step) put(c, to_float(x[c]) * by);
-        return;
+    const int half = a.rot_dim / 2, i0 = a.neighbours ? 2 * c : c, i1 = a.neighbours ? 2 * c + 1 : c + half;
+    float u = to_float(x[i0]), v = to_float(x[i1]);
+    if (a.table) {
+        const int at = step_tokens(a, b) - 1;        // the token itself is the cache's last one
+        const float* cs = a.table + (long long)(at < 0 ? 0 : at >= a.table_rows ? a.table_rows - 1 : at) * a.rot_dim;
+        const float co = cs[c], si = cs[c + half], t = fmaf(u, co, -__fmul_rn(v, si));
+        v = fmaf(v, co, __fmul_rn(u, si));
+        u = t;
     }
-    const int half = a.rot_dim / 2, at = step_tokens(a, b) - 1;               // the token itself is the cache's last one
-    const float* cs = a.table + (long long)(at < 0 ? 0 : at >= a.table_rows ? a.table_rows - 1 : at) * a.rot_dim;
-    for (int c = first; c < half; c += step) {
-        const int i0 = a.neighbours ? 2 * c : c, i1 = a.neighbours ? 2 * c + 1 : c + half;
-        const float u = to_float(x[i0]), v = to_float(x[i1]), co = cs[c], si = cs[c + half];
-        put(i0, fmaf(u, co, -__fmul_rn(v, si)) * by);
-        put(i1, fmaf(v, co, __fmul_rn(u, si)) * by);
-    }
+    put(i0, u * by);
+    put(i1, v * by);
 }
 
 // u and w of one head for 4 sequences, in float32.  Thread (x, y): column words x of the weights (16 columns each), rows y, y + 8 ..
@@ -105,31 +102,56 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
             for (int w = 0; w < WARPS; ++w) s += part[w][c / 16][c % 16];
             out[c] = s * (a.gamma * a.scale * mamba::LOG2E);
         }
-        if (a.rot_dim) rotated_query<T>(a, b0 + n, h, threadIdx.x, THREADS, [&](int c, float v) { out[a.rank + c] = v; });
+        auto put = [&](int c, float v) { out[a.rank + c] = v; };
+        for (int c = threadIdx.x; c < a.rot_dim / 2; c += THREADS) rotated_query<T>(a, b0 + n, h, c, put);
+        // an odd last channel has no partner and is not turned (there is no table then)
+        if (a.rot_dim % 2 && threadIdx.x == 0)
+            put(a.rot_dim - 1, to_float(static_cast<const T*>(a.q_rot)[(b0 + n) * a.q_rot_stride_b + h * a.q_rot_stride_h + a.rot_dim - 1]) * a.scale * mamba::LOG2E);
     }
 }
 
-// u and w for the tensor cores: of one head, 128 columns of u for 64 sequences.  u = gamma scale log2(e) q W is held in two 8-bit digits of 1 / 32512 of
-// gamma scale log2(e) sum |q|, which it cannot exceed whatever the weights are: no block has to know another's columns.  (For weights of
-// random signs that is 3 to 4 times the largest u, 14 bits of it.)  digits [batch, heads, 2, rank padded to 32], steps [batch, heads], w [batch, heads, 64].
-// A warp takes 16 columns, which are one word of every row of the weights.
+// u and w for the tensor cores: of one head, 128 columns of u for 64 sequences, into the images of latent_step.cuh.  u = gamma scale log2(e) q W is held in
+// two 8-bit digits of 1 / 32512 of gamma scale log2(e) sum |q|, which it cannot exceed whatever the weights are: no block has to know another's columns.
+// (For weights of random signs that is 3 to 4 times the largest u, 14 bits of it.)  steps [batch, groups, 32].  A warp takes 16 columns, which are one
+// word of every row of the weights.
 constexpr int QUERY_ROWS = 64, QUERY_COLS = 128;
 template <typename T>
-__global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_latent_step_t a, int8_t* __restrict__ digits, float* __restrict__ steps, T* __restrict__ rotated) {
-    __shared__ T q[QUERY_ROWS][256 + 8];
+__global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_latent_step_t a, uint8_t* __restrict__ images, float* __restrict__ steps, const bool vectors) {
+    __shared__ __align__(16) T q[QUERY_ROWS][256 + 8];
     __shared__ uint32_t W[256][WARPS + 1];
     __shared__ float most[QUERY_ROWS];
+    const StepImage image(a);
+    asm volatile("griddepcontrol.launch_dependents;");
     const int h = blockIdx.x, c0 = blockIdx.y * QUERY_COLS, b0 = blockIdx.z * QUERY_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int nb = min(QUERY_ROWS, a.batch - b0), D = a.key_dim, DP = (D + 15) / 16 * 16, words = a.rank / 16, rp = (a.rank + 31) / 32 * 32;
+    const int nb = min(QUERY_ROWS, a.batch - b0), D = h < a.heads ? a.key_dim : 0, DP = (D + 15) / 16 * 16, words = a.rank / 16, rp = (a.rank + 31) / 32 * 32;
+    const int group = h / 32, hg = h % 32;
     const float by = a.gamma * a.scale * mamba::LOG2E;
     for (int i = threadIdx.x; i < DP * WARPS; i += THREADS) {
-        const int d = i / WARPS, w = i - d * WARPS;
+        const int d = i / WARPS, w = i % WARPS;
         W[d][w] = d < D && c0 / 16 + w < words ? reinterpret_cast<const uint32_t*>(a.W_packed)[((long long)h * D + d) * words + c0 / 16 + w] : 0x55555555u;
     }
     const int rows = (nb + 15) / 16 * 16;
-    for (int i = threadIdx.x; i < rows * DP; i += THREADS) {
-        const int n = i / DP, d = i - n * DP;
-        q[n][d] = n < nb && d < D ? static_cast<const T*>(a.q)[(b0 + n) * a.q_stride_b + h * a.q_stride_h + d] : mamba::from_float<T>(0.0f);
+    if (vectors) {                                   // rows of 8 values on 16 bytes
+        const int per = DP / 8;
+        for (int n = threadIdx.x / 32; n < rows; n += WARPS)
+            if (lane < per)
+                *reinterpret_cast<uint4*>(&q[n][lane * 8]) = n < nb && lane * 8 < D ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (b0 + n) * a.q_stride_b + h * a.q_stride_h + lane * 8)
+                                                                                    : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        for (int n = threadIdx.x / 32; n < rows; n += WARPS)
+            for (int d = lane; d < DP; d += 32) q[n][d] = n < nb && d < D ? static_cast<const T*>(a.q)[(b0 + n) * a.q_stride_b + h * a.q_stride_h + d] : mamba::from_float<T>(0.0f);
+    }
+    if (a.rot_dim) {                                 // the column blocks share the rows
+        const int pairs = 32;                        // of the 64 places of w; those behind rot_dim are zeros
+        for (int i = blockIdx.y * THREADS + threadIdx.x; i < nb * pairs; i += gridDim.y * THREADS) {
+            const int n = i / pairs, c = i % pairs, half = a.rot_dim / 2;
+            uint8_t* out = images + ((long long)(b0 + n) * image.groups + group) * image.bytes();
+            auto put = [&](int x, float v) { *reinterpret_cast<T*>(out + image.w(2 * x, hg)) = mamba::from_float<T>(v); };
+            if (h < a.heads && c < half) rotated_query<T>(a, b0 + n, h, c, put);
+            for (int x = a.rot_dim + c; x < 64; x += pairs) put(x, 0.0f);
+            if (h >= a.heads)
+                for (int x = c; x < a.rot_dim; x += pairs) put(x, 0.0f);
+        }
     }
     __syncthreads();
     for (int n = warp; n < nb; n += WARPS) {
@@ -139,14 +161,7 @@ __global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_lat
         for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
         if (lane == 0) {
             most[n] = s > 0.0f ? STEPS / s : 0.0f;
-            if (c0 == 0) steps[(long long)(b0 + n) * a.heads + h] = by * s * (1.0f / STEPS);      // a NaN or infinity makes the scores NaN
-        }
-    }
-    if (c0 == 0 && a.rot_dim) {
-        for (int n = warp; n < nb; n += WARPS) {
-            T* out = rotated + ((long long)(b0 + n) * a.heads + h) * 64;
-            rotated_query<T>(a, b0 + n, h, lane, 32, [&](int c, float v) { out[c] = mamba::from_float<T>(v); });
-            for (int c = a.rot_dim + lane; c < 64; c += 32) out[c] = mamba::from_float<T>(0.0f);
+            if (c0 == 0) steps[((long long)(b0 + n) * image.groups + group) * 32 + hg] = by * s * (1.0f / STEPS);      // a NaN or infinity makes the scores NaN
         }
     }
     float sum[QUERY_ROWS / 16][2][4] = {};
@@ -177,7 +192,7 @@ __global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_lat
             const int n = m * 16 + r + 8 * i;
             if (n >= nb) continue;
             const float inv = most[n];
-            int8_t* out = digits + ((long long)(b0 + n) * a.heads + h) * 2 * rp;
+            uint8_t* out = images + ((long long)(b0 + n) * image.groups + group) * image.bytes();
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int c = c0 + warp * 16 + t * 8 + k2;
@@ -188,8 +203,8 @@ __global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_lat
                     v[e] = min(max(__float2int_rn(sum[m][t][2 * i + e] * inv), -(int)STEPS), (int)STEPS);
                     hi[e] = (v[e] + 128) >> 8;
                 }
-                *reinterpret_cast<char2*>(out + c) = make_char2((signed char)hi[0], (signed char)hi[1]);
-                *reinterpret_cast<char2*>(out + rp + c) = make_char2((signed char)(v[0] - hi[0] * 256), (signed char)(v[1] - hi[1] * 256));
+                *reinterpret_cast<char2*>(out + image.digit(c, 0, hg)) = make_char2((signed char)hi[0], (signed char)hi[1]);
+                *reinterpret_cast<char2*>(out + image.digit(c, 1, hg)) = make_char2((signed char)(v[0] - hi[0] * 256), (signed char)(v[1] - hi[1] * 256));
             }
         }
 }
@@ -205,7 +220,7 @@ __global__ void __launch_bounds__(THREADS) step_rows_kernel(const el_latent_step
     __shared__ float scale_of[TILE];
     __shared__ int seen[TILE];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h0 = blockIdx.y * GROUP, w = blockIdx.x;
-    const long long tiles = step_tiles_before(a, a.batch);
+    const long long tiles = step_all_tiles(a);
     workers = step_active(workers, tiles);
     if (w >= workers) return;
     const long long first = w * tiles / workers, last = (w + 1) * tiles / workers;
@@ -320,10 +335,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
     int spread = 1;                                  // sequences side by side, a power of two; 16 / spread warps share one
     while (spread < nb) spread *= 2;
     const int shares = 16 / spread, share = warp / spread, b = b0 + warp % spread;
+    // the weights of the warp's first eight value rows, before anything that the kernels before leave is there
+    const int words = R / 16, r = lane >> 2, k2 = (lane & 3) * 2;
+    const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim) * words;
+    uint32_t first[MOST_RANK / 16];
+#pragma unroll
+    for (int k = 0; k < MOST_RANK / 16; ++k) first[k] = k < words && warp * 8 + r < a.value_dim ? W[(long long)(warp * 8 + r) * words + k] : 0x55555555u;
     float acc[MOST_RANK / 32] = {};
+    int w0 = 0, w1 = -1;
     if (warp % spread < nb) {
         long long tiles = 0, before = 0;
         int here = 0;
+#pragma unroll 4
         for (int x = lane; x < a.batch; x += 32) {
             const int n = step_tiles(a, x);
             tiles += n;
@@ -337,36 +360,46 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
             here += __shfl_xor_sync(0xffffffffu, here, x);
         }
         if (here > 0) {
-            const int active = step_active(workers, tiles), w0 = step_worker(before, active, tiles), w1 = step_worker(before + here - 1, active, tiles);
-            float top = -INFINITY, sum = 0.0f;
-            for (int w = w0 + lane; w <= w1; w += 32) top = mamba::max_nan(top, parts.stats((long long)w + b)[2 * h]);
+            const int active = step_active(workers, tiles);
+            w0 = step_worker(before, active, tiles);
+            w1 = step_worker(before + here - 1, active, tiles);
+        }
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (w0 <= w1) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll 5
+        for (int w = w0 + lane; w <= w1; w += 32) {
+            const float2 st = *reinterpret_cast<const float2*>(parts.stats((long long)w + b) + 2 * h);
+            const float m = mamba::max_nan(top, st.x), from = m == -INFINITY ? 0.0f : m;
+            sum = fmaf(sum, exp2_neg(top - from), exp2_neg(st.x - from) * st.y);
+            top = m;
+        }
+        float all = top;
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) top = mamba::max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float from = top == -INFINITY ? 0.0f : top;
-            for (int w = w0 + lane; w <= w1; w += 32) {
-                const float2 st = *reinterpret_cast<const float2*>(parts.stats((long long)w + b) + 2 * h);
-                sum = fmaf(exp2_neg(st.x - from), st.y, sum);
-            }
+        for (int x = 16; x > 0; x >>= 1) all = mamba::max_nan(all, __shfl_xor_sync(0xffffffffu, all, x));
+        const float from = all == -INFINITY ? 0.0f : all;
+        sum *= exp2_neg(top - from);
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            const float by = top == -INFINITY ? 0.0f : a.gamma / sum;
-            // 32 of this warp's parts at a time: lane l has the factor of the l-th
-            for (int p = w0 + share; p <= w1; p += 32 * shares) {
-                const int mine = p + lane * shares, count = min(32, (w1 - p) / shares + 1);
-                const float f = mine <= w1 ? exp2_neg(parts.stats((long long)mine + b)[2 * h] - from) * by : 0.0f;
+        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const float by = all == -INFINITY ? 0.0f : a.gamma / sum;
+        // 32 of this warp's parts at a time: lane l has the factor of the l-th
+        for (int p = w0 + share; p <= w1; p += 32 * shares) {
+            const int mine = p + lane * shares, count = min(32, (w1 - p) / shares + 1);
+            const float f = mine <= w1 ? exp2_neg(parts.stats((long long)mine + b)[2 * h] - from) * by : 0.0f;
+            const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + b) + (long long)h * R) + lane;
+            const long long step = (long long)shares * a.heads * (R / 4);
 #pragma unroll 4
-                for (int i = 0; i < count; ++i) {
-                    const float x = __shfl_sync(0xffffffffu, f, i);
-                    const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + i * shares + b) + (long long)h * R);
+            for (int i = 0; i < count; ++i) {
+                const float x = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
-                    for (int c = 0; c < MOST_RANK / 128; ++c) {
-                        if ((c * 32 + lane) * 4 >= R) continue;
-                        const float4 y = v[c * 32 + lane];
-                        acc[4 * c] = fmaf(x, y.x, acc[4 * c]);
-                        acc[4 * c + 1] = fmaf(x, y.y, acc[4 * c + 1]);
-                        acc[4 * c + 2] = fmaf(x, y.z, acc[4 * c + 2]);
-                        acc[4 * c + 3] = fmaf(x, y.w, acc[4 * c + 3]);
-                    }
+                for (int c = 0; c < MOST_RANK / 128; ++c) {
+                    if ((c * 32 + lane) * 4 >= R) continue;
+                    const float4 y = v[i * step + c * 32];
+                    acc[4 * c] = fmaf(x, y.x, acc[4 * c]);
+                    acc[4 * c + 1] = fmaf(x, y.y, acc[4 * c + 1]);
+                    acc[4 * c + 2] = fmaf(x, y.z, acc[4 * c + 2]);
+                    acc[4 * c + 3] = fmaf(x, y.w, acc[4 * c + 3]);
                 }
             }
         }
@@ -375,26 +408,25 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
     for (int c = 0; c < MOST_RANK / 128; ++c)
         reinterpret_cast<float4*>(o + warp * MOST_RANK)[c * 32 + lane] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
     __syncthreads();
-    for (int i = threadIdx.x; i < JOIN_ROWS * R; i += JOIN_THREADS) {
-        const int n = i / R, c = i - n * R;
-        float v = 0.0f;
-        if (n < nb)
-            for (int s = 0; s < shares; ++s) v += o[(s * spread + n) * MOST_RANK + c];
+    for (int n = warp; n < JOIN_ROWS; n += JOIN_THREADS / 32)
+        for (int c = lane; c < R; c += 32) {
+            float v = 0.0f;
+            if (n < nb)
+                for (int s = 0; s < shares; ++s) v += o[(s * spread + n) * MOST_RANK + c];
 #pragma unroll
-        for (int t = 0; t < JOIN_TERMS<T>; ++t) {
-            const __nv_bfloat16 x = __float2bfloat16_rn(v);
-            terms[(t * JOIN_ROWS + n) * JOIN_PITCH + c] = x;
-            v -= __bfloat162float(x);
+            for (int t = 0; t < JOIN_TERMS<T>; ++t) {
+                const __nv_bfloat16 x = __float2bfloat16_rn(v);
+                terms[(t * JOIN_ROWS + n) * JOIN_PITCH + c] = x;
+                v -= __bfloat162float(x);
+            }
         }
-    }
     __syncthreads();
-    const int words = R / 16, r = lane >> 2, k2 = (lane & 3) * 2;
-    const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim) * words;
     for (int v0 = warp * 8; v0 < a.value_dim; v0 += 128) {
         float d[4] = {};
-#pragma unroll 4
-        for (int k = 0; k < words; ++k) {
-            const uint32_t w = (v0 + r < a.value_dim ? W[(long long)(v0 + r) * words + k] : 0x55555555u) >> (2 * k2);
+#pragma unroll
+        for (int k = 0; k < MOST_RANK / 16; ++k) {
+            if (k >= words) break;
+            const uint32_t w = first[k] >> (2 * k2);
             const uint32_t x0 = weight_pair<__nv_bfloat16>(w & 3u, (w >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((w >> 16) & 3u, (w >> 18) & 3u);
 #pragma unroll
             for (int t = JOIN_TERMS<T> - 1; t >= 0; --t) {
@@ -409,7 +441,27 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
             const int n = r + 8 * (i >> 1), v = v0 + k2 + (i & 1);
             if (n < nb && v < a.value_dim) static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v] = mamba::from_float<T>(d[i]);
         }
+        if (v0 + 128 < a.value_dim) {                // value heads beyond 128 channels
+#pragma unroll
+            for (int k = 0; k < MOST_RANK / 16; ++k) first[k] = k < words && v0 + 128 + r < a.value_dim ? W[(long long)(v0 + 128 + r) * words + k] : 0x55555555u;
+        }
     }
+}
+
+// A launch that may begin before the one in front of it has ended; what that one leaves is read behind griddepcontrol.wait.
+template <typename K, typename... A> int launch_dependent(K kernel, dim3 grid, int threads, int bytes, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    EL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return check_launch();
 }
 
 template <typename F> int of_type(int dtype, F f) {
@@ -440,13 +492,11 @@ int step_workers(const el_latent_step_t& a, int groups) {
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-size_t digits_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * a.heads * 2 * ((a.rank + 31) / 32 * 32)); }
-size_t steps_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * a.heads * 4); }
-size_t rotated_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * a.heads * 64 * 2); }
+size_t images_bytes(const el_latent_step_t& a) { return align256((size_t)a.batch * StepImage(a).groups * StepImage(a).bytes()); }
 size_t query_bytes(const el_latent_step_t& a) {
-    return latent_step_tc_takes(a) ? digits_bytes(a) + steps_bytes(a) + rotated_bytes(a) : align256((size_t)a.batch * a.heads * (a.rank + a.rot_dim) * 4);
+    return latent_step_tc_takes(a) ? images_bytes(a) + align256((size_t)a.batch * StepImage(a).groups * 32 * 4) : align256((size_t)a.batch * a.heads * (a.rank + a.rot_dim) * 4);
 }
-int groups_of(const el_latent_step_t& a) { return latent_step_tc_takes(a) ? latent_step_tc_groups(a) : 1; }
+int groups_of(const el_latent_step_t& a) { return latent_step_tc_takes(a) ? StepImage(a).groups : 1; }
 
 }  // namespace
 
@@ -473,18 +523,18 @@ int launch_latent_step(const el_latent_step_t& a, cudaStream_t st) {
                 rc = check_launch();
             }
         } else if constexpr (!std::is_same<T, float>::value) {
-            int8_t* digits = reinterpret_cast<int8_t*>(ws);
-            float* steps = reinterpret_cast<float*>(ws + digits_bytes(a));
-            T* rotated = reinterpret_cast<T*>(ws + digits_bytes(a) + steps_bytes(a));
-            const dim3 grid(a.heads, (a.rank + QUERY_COLS - 1) / QUERY_COLS, (a.batch + QUERY_ROWS - 1) / QUERY_ROWS);
-            step_query_digits_kernel<T><<<grid, THREADS, 0, st>>>(a, digits, steps, rotated);
-            if ((rc = check_launch()) == EL_OK && workers > 0) rc = launch_latent_step_tc(a, digits, steps, rotated, parts, workers, st);
+            uint8_t* images = reinterpret_cast<uint8_t*>(ws);
+            float* steps = reinterpret_cast<float*>(ws + images_bytes(a));
+            const StepImage image(a);
+            const bool vectors = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride_b % 8 == 0 && a.q_stride_h % 8 == 0 && a.key_dim % 8 == 0;
+            const dim3 grid((image.groups - 1) * 32 + image.hp, (a.rank + QUERY_COLS - 1) / QUERY_COLS, (a.batch + QUERY_ROWS - 1) / QUERY_ROWS);
+            step_query_digits_kernel<T><<<grid, THREADS, 0, st>>>(a, images, steps, vectors);
+            if ((rc = check_launch()) == EL_OK && workers > 0) rc = launch_latent_step_tc(a, images, steps, parts, workers, st);
         }
         if (rc != EL_OK) return rc;
         static DeviceOnce once;
         if ((rc = allow_shared(step_join_kernel<T>, JOIN_BYTES<T>, once)) != EL_OK) return rc;
-        step_join_kernel<T><<<dim3(a.heads, (a.batch + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, JOIN_BYTES<T>, st>>>(a, parts, workers);
-        return check_launch();
+        return launch_dependent(step_join_kernel<T>, dim3(a.heads, (a.batch + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, JOIN_BYTES<T>, st, a, parts, workers);
     });
 }
 

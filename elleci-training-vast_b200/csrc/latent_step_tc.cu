@@ -10,7 +10,7 @@
 // than bfloat16's 2^-8 of each weight where weights matter.  The tiles' int32 sums are added up in float32 registers, scaled when m grows.
 //
 // Warps 0-7: thread t of each half is token t of the tile and takes 16 heads' scores; then two of the four blocks of 128 latent channels, a thread a channel.
-// The sums of a tile are taken while the tensor core forms the next tile's scores.  Warp 8 issues the products.  Warps
+// The sums of a tile are taken after the next tile's scores, so that the tensor core has work meanwhile.  Warp 8 issues the products.  Warps
 // 9 and 10 load, each every other tile: by tensor maps where pages are multiples of 8 tokens (a box lies in one page), otherwise by 16-byte
 // asynchronous copies of each token's row.
 // Bound: memory; a tile of 128 tokens of rank 512 and 64 rotated channels is 82 KB, 3400 cycles of an SM's share of the HBM, and 1100 of its tensor core.
@@ -33,24 +33,27 @@ constexpr int WARP_MMA = 8, WARP_LOAD = 9, THREADS = 11 * 32;
 constexpr float STEPS = 32512.0f;                      // 127 * 256: the largest value of two digits whose high one is at most 127
 constexpr float MAGIC = 12582912.0f;                   // 1.5 * 2^23: adding it rounds to an integer, whose low bits are the sum's
 
-struct Shape {
-    int chunks, hp, groups;                            // 128-byte chunks of a row; heads of a group, padded to 16 or 32
-    int box;                                           // tokens of a tensor map's box, which lie in one page; 0: no tensor maps
-    __host__ __device__ int n() const { return 2 * hp; }
-};
-
-// Digits of the integers i < 2^15 in magnitude: the low one is the integer's low byte as a signed number, the high one what is left.
-__device__ __forceinline__ uint32_t high_digit(int v) { return (uint32_t)((v + 128) >> 8) & 0xFFu; }
-__device__ __forceinline__ uint32_t low_digit(int v) { return (uint32_t)v & 0xFFu; }
-
+// bytes i of four words as one word
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t sel) { return prmt(prmt(a, b, sel), prmt(c, d, sel), 0x5410u); }
+// the largest value of a warp's lanes, NaN if there is one
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+// whether a barrier's phase has ended, without waiting for it (mbar_try may wait for a while)
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 // bytes that a barrier's phase waits for, without an arrival
 __device__ __forceinline__ void mbar_expect_tx_only(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void pair_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory"); }
 
 // The parts of a worker's range: sequence after sequence, tile after tile.
 struct Walk {
@@ -83,8 +86,8 @@ struct Walk {
     }
 };
 
-// Reduces 16 values over a warp by maximum (or sum): lane l has the result of value l % 16.
-template <bool MAX> __device__ __forceinline__ float reduce16(const float (&v)[16]) {
+// Sums 16 values over a warp: lane l has the sum of value l % 16.
+__device__ __forceinline__ float reduce16(const float (&v)[16]) {
     const int lane = threadIdx.x & 31;
     float x[16];
 #pragma unroll
@@ -93,27 +96,23 @@ template <bool MAX> __device__ __forceinline__ float reduce16(const float (&v)[1
     for (int w = 8; w > 0; w >>= 1) {
         const bool up = lane & w;
 #pragma unroll
-        for (int i = 0; i < w; ++i) {
-            const float give = up ? x[i] : x[i + w], keep = up ? x[i + w] : x[i];
-            const float got = __shfl_xor_sync(0xffffffffu, give, w);
-            x[i] = MAX ? mamba::max_nan(keep, got) : keep + got;
-        }
+        for (int i = 0; i < w; ++i) x[i] = (up ? x[i + w] : x[i]) + __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + w], w);
     }
-    const float other = __shfl_xor_sync(0xffffffffu, x[0], 16);
-    return MAX ? mamba::max_nan(x[0], other) : x[0] + other;
+    return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 16);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1)
-step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant__ CUtensorMap tmKeys, const el_latent_step_t a, const int8_t* __restrict__ digits, const float* __restrict__ steps, const T* __restrict__ rotated, const StepParts parts,
-               int workers, const Shape shape) {
+step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant__ CUtensorMap tmKeys, const el_latent_step_t a, const uint8_t* __restrict__ images,
+               const float* __restrict__ steps, const StepParts parts, int workers, const int box) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const int R = a.rank, P = a.rot_dim, HP = shape.hp, N = shape.n(), KC = shape.chunks, rp = (R + 31) / 32 * 32;
-    const int key_bytes = P ? CHUNK : 0, stage_bytes = KC * CHUNK + key_bytes;
-    // two stages [rows][keys]; query digits [chunks][N rows][128]; w [HP rows][128]; p digits [tokens][128]
-    const uint32_t q_at = base + 2 * stage_bytes, w_at = q_at + KC * N * 128, p_at = w_at + (P ? HP * 128 : 0);
+    const StepImage image(a);
+    const int R = a.rank, P = a.rot_dim, HP = image.hp, N = 2 * HP, KC = image.chunks, key_steps = (R + 31) / 32, rot_steps = (P + 15) / 16;
+    const int stage_bytes = (KC + (P ? 1 : 0)) * CHUNK;
+    // two stages [rows][keys]; the query's image; p digits [tokens][128]
+    const uint32_t q_at = base + 2 * stage_bytes, w_at = q_at + image.w_at(), p_at = q_at + image.bytes();
     uint8_t* tail = gen + (p_at - base) + CHUNK;
     float* scale_of = reinterpret_cast<float*>(tail);                       // [2][128]
     uint32_t* seen = reinterpret_cast<uint32_t*>(tail + 1024);              // [2][4]
@@ -123,36 +122,45 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
     float* wmax = reinterpret_cast<float*>(tail + 1632);                    // [2 halves][2][4 warps][16 heads]
     float* smax = reinterpret_cast<float*>(tail + 2656);                    // [2 halves][2][4 warps]
     float* wsum = reinterpret_cast<float*>(tail + 2720);                    // [2 halves][4 warps][16 heads]
-    const uint32_t bars = p_at + CHUNK + 3232;
+    float* heads_of = reinterpret_cast<float*>(tail + 3232);                // [8 warps][2][16 heads]: maxima and factors for the warp's own lanes
+    const uint32_t bars = p_at + CHUNK + 4256;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (2 + s); };
     auto s_full = [&](int s) { return bars + 8u * (4 + s); };
-    const uint32_t p_full = bars + 48, o_full = bars + 56, q_empty = bars + 64;
-    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(tail + 3232 + 72);
+    const uint32_t p_full = bars + 48, o_full = bars + 56, o_empty = bars + 64, q_empty = bars + 72;
+    auto half_at = [&](int half) { return bars + 80u + 8u * half; };
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(tail + 4256 + 96);
 
     const int warp = warp_index(), lane = threadIdx.x & 31;
-    const int w = blockIdx.x / shape.groups, group = blockIdx.x - w * shape.groups, h0 = group * 32;
+    const int w = blockIdx.x / image.groups, group = blockIdx.x - w * image.groups, h0 = group * 32;
     int32_t* status = a.dev_status;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
             mbar_init(s_full(s), 1);
+            mbar_init(half_at(s), 4);
         }
         mbar_init(p_full, 8);
         mbar_init(o_full, 1);
+        mbar_init(o_empty, 8);
         mbar_init(q_empty, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
     if (warp == WARP_MMA) tmem_alloc<512>(smem_u32((const void*)tmem_holder));
+    if (box && warp == WARP_LOAD && elect_one()) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmRows) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmKeys) : "memory");
+    }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem = *tmem_holder;
     const uint32_t O = tmem, S = tmem + 256;                                // O of chunk c at 64 c; S of tile g at 128 (g & 1), its rotated part 64 further
 
-    const long long tiles = step_tiles_before(a, a.batch);
+    asm volatile("griddepcontrol.launch_dependents;");
+    const long long tiles = step_all_tiles(a);
     workers = step_active(workers, tiles);
     const long long first = w < workers ? w * tiles / workers : 0, last = w < workers ? (w + 1) * tiles / workers : 0;
 
@@ -170,25 +178,25 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                     const int p = k.p0 + i * TOKENS;
                     long long row[4];
                     float sc[4];
-                    if (shape.box) {                                                  // lane l looks up box l
-                        const int pos = p + lane * shape.box;
-                        const long long start = lane * shape.box < TOKENS && pos < k.p1 ? step_row(a, k.b, pos) : -1;
+                    if (box) {                                                  // lane l looks up box l
+                        const int pos = p + lane * box;
+                        const long long start = lane * box < TOKENS && pos < k.p1 ? step_row(a, k.b, pos) : -1;
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const int to = q * 32 + lane;
-                            const long long r = __shfl_sync(0xffffffffu, start, to / shape.box);
-                            row[q] = r >= 0 && p + to < k.p1 ? r + to % shape.box : -1;
+                            const long long r = __shfl_sync(0xffffffffu, start, to / box);
+                            row[q] = r >= 0 && p + to < k.p1 ? r + to % box : -1;
                             sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
                         }
                         if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
                         const unsigned there = __ballot_sync(0xffffffffu, start >= 0);
-                        if (elect_one()) mbar_expect_tx_only(full(mine), __popc(there) * shape.box * 128 * (KC + (P ? 1 : 0)));
+                        if (elect_one()) mbar_expect_tx_only(full(mine), __popc(there) * box * 128 * (KC + (P ? 1 : 0)) + (i == 0 ? image.bytes() : 0));
                         __syncwarp();
-                        for (int x = 0; x < TOKENS / shape.box; ++x) {
+                        for (int x = 0; x < TOKENS / box; ++x) {
                             const int r = __shfl_sync(0xffffffffu, (int)start, x);
                             if (r >= 0 && elect_one()) {
-                                for (int c = 0; c < KC; ++c) tma_load_2d(at + c * CHUNK + x * shape.box * 128, &tmRows, full(mine), c * 128, r);
-                                if (P) tma_load_2d(at + KC * CHUNK + x * shape.box * 128, &tmKeys, full(mine), 0, r);
+                                for (int c = 0; c < KC; ++c) tma_load_2d(at + c * CHUNK + x * box * 128, &tmRows, full(mine), c * 128, r);
+                                if (P) tma_load_2d(at + KC * CHUNK + x * box * 128, &tmKeys, full(mine), 0, r);
                             }
                             __syncwarp();
                         }
@@ -231,21 +239,14 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                     }
                     if (i == 0) {                                                     // the part's query
                         if (part > 0 && !mbar_wait_warp(q_empty, (uint32_t)(part - 1) & 1u, status, 2)) { ok = false; break; }
-                        const long long bh = (long long)k.b * a.heads + h0;
-                        for (int r = 0; r < N; ++r) {
-                            const int h = r % HP, digit = r / HP;
-                            const bool there = h0 + h < a.heads;
-                            const int8_t* src = digits + ((bh + (there ? h : 0)) * 2 + digit) * rp + lane * 16;
-                            if (lane * 16 < rp) copy16(q_at + (lane >> 3) * N * 128 + r * 128 + (((lane & 7) ^ (r & 7)) << 4), there ? src : digits, there);
+                        griddep_wait();                                               // the kernel in front made it
+                        const long long bg = (long long)k.b * image.groups + group;
+                        if (elect_one()) {
+                            if (!box) mbar_expect_tx_only(full(mine), image.bytes());
+                            bulk_load(q_at, images + bg * image.bytes(), image.bytes(), full(mine));
                         }
-                        if (P) {
-                            for (int r = 0; r < HP; r += 4) {
-                                const int h = r + (lane >> 3), c = lane & 7;
-                                const bool there = h0 + h < a.heads;
-                                copy16(w_at + h * 128 + ((c ^ (h & 7)) << 4), there ? rotated + (bh + h) * 64 + c * 8 : rotated, there);
-                            }
-                        }
-                        step_of[(part & 1) * 32 + lane] = h0 + lane < a.heads ? steps[bh + lane] : 0.0f;
+                        __syncwarp();
+                        step_of[(part & 1) * 32 + lane] = lane < HP ? steps[bg * 32 + lane] : 0.0f;
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     fence_async_smem();
@@ -257,7 +258,6 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
     } else if (warp == WARP_MMA) {
         // ================= products =================
         const uint32_t i_s = make_idesc(0, 0, N), i_o = make_idesc(1, 1, N), i_r = idesc_f16<T>(0, 0, HP);
-        const int key_steps = rp / 32, rot_steps = (P + 15) / 16;
         auto scores = [&](int g) {
             const uint32_t at = base + (g & 1) * stage_bytes, to = S + (g & 1) * 128;
             for (int k = 0; k < key_steps; ++k) {
@@ -270,38 +270,53 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
         auto sums = [&](int g) {
             const uint32_t at = base + (g & 1) * stage_bytes;
             for (int c = 0; c < KC; ++c)
+#pragma unroll
                 for (int k = 0; k < TOKENS / 32; ++k) umma_i8(O + c * 64, make_desc(at + c * CHUNK + k * 4096, CHUNK), make_desc(p_at + k * 4096, CHUNK), i_o, k != 0);
             umma_commit(o_full);
             umma_commit(empty(g & 1));
         };
-        bool ok = true;
-        int g = 0;                                                                    // scores issued
-        auto issue_scores = [&](bool ends_part) {
-            ok = ok && mbar_wait_warp(full(g & 1), (uint32_t)(g >> 1) & 1u, status, 3);
-            tcgen05_fence_after();
-            if (ok && elect_one()) {
-                scores(g);
-                if (ends_part) umma_commit(q_empty);
-            }
-            __syncwarp();
-            ++g;
-        };
-        auto issue_sums = [&](int j) {
-            // the threads that made the digits have also taken the sums of the tile before
-            ok = ok && mbar_wait_warp(p_full, (uint32_t)j & 1u, status, 4);
-            tcgen05_fence_after();
-            if (ok && elect_one()) sums(j);
-            __syncwarp();
-        };
         if (first < last) {
-            for (Walk k(a, first, last); k.more() && ok; k.next()) {
-                const int count = k.tiles();
-                for (int i = 0; i < count && ok; ++i) {
-                    if (g > 0) issue_sums(g - 1);
-                    issue_scores(i + 1 == count);
+            // Scores of a tile as soon as it is there and the threads have read those of two tiles before; sums of a tile as soon as its digits are there and the
+            // sums before have been taken.  Whichever is ready goes first.
+            Walk k(a, first, last);
+            int g = 0, left = k.tiles(), done = 0, total = -1;                        // scores issued, tiles of the part without them, sums issued
+            long long since = clock64();
+            while (true) {
+                bool moved = false;
+                if (total < 0 && g < done + 2 && __all_sync(0xffffffffu, mbar_test(full(g & 1), (uint32_t)(g >> 1) & 1u))) {
+                    tcgen05_fence_after();
+                    --left;
+                    if (elect_one()) {
+                        scores(g);
+                        if (left == 0) umma_commit(q_empty);
+                    }
+                    __syncwarp();
+                    ++g;
+                    if (left == 0) {
+                        k.next();
+                        if (k.more()) left = k.tiles();
+                        else total = g;
+                    }
+                    moved = true;
+                }
+                if (done < g && __all_sync(0xffffffffu, mbar_test(p_full, (uint32_t)done & 1u)) &&
+                    (done == 0 || __all_sync(0xffffffffu, mbar_test(o_empty, (uint32_t)(done - 1) & 1u)))) {
+                    tcgen05_fence_after();
+                    if (elect_one()) sums(done);
+                    __syncwarp();
+                    ++done;
+                    moved = true;
+                }
+                if (done == total) break;
+                const long long now = clock64();
+                if (moved) since = now;
+                const bool lost = now - since > WAIT_LIMIT_CYCLES ||
+                                  (now - since > (1 << 22) && status != nullptr && *reinterpret_cast<volatile int32_t*>(status) != 0);
+                if (__any_sync(0xffffffffu, lost)) {
+                    if (status != nullptr) atomicCAS(status, 0, 3);
+                    break;
                 }
             }
-            if (ok && g > 0) issue_sums(g - 1);
         }
     } else if (first < last) {
         // ================= softmax and sums =================
@@ -309,9 +324,18 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const bool scoring = half * 16 < HP;                                          // 16 heads have one half
         float acc[2][32];                                                             // channels of chunks 2 half, 2 half + 1; heads
-        float top[16], sum[16];
+        float top = -INFINITY, sum[16];                                               // of head lane % 16; of all
         bool ok = true;
         int g = 0, part = 0;
+        uint32_t met = 0;
+        // The four warps of a half meet.  (A bar.sync would wait for good for a warp whose bounded wait gave up.)
+        auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(half_at(half));
+            ok = mbar_wait_warp(half_at(half), met & 1u, status, 9);
+            ++met;
+            return ok;
+        };
 
         auto softmax = [&](int j) {
             if (!(ok = mbar_wait_warp(s_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6) && mbar_wait_warp(full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6))) return;
@@ -319,64 +343,95 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
             float s[16];
             const float sc = scale_of[(j & 1) * 128 + token];
             const bool here = (seen[(j & 1) * 4 + quarter] >> lane) & 1u;
+            float* wm = wmax + (half * 2 + (j & 1)) * 64;
+            float* sm = smax + (half * 2 + (j & 1)) * 4;
             if (scoring) {
-                uint32_t hi[16], lo[16], r[16];
+                uint32_t hi[16], lo[16];
                 const uint32_t at = S + (j & 1) * 128 + lanes + half * 16;
                 tmem_ld16(at, hi);
                 tmem_ld16(at + HP, lo);
-                if (P) tmem_ld16(at + 64, r);
                 tmem_ld_wait();
-                const float* st = step_of + (part & 1) * 32 + half * 16;
+                const float4* st = reinterpret_cast<const float4*>(step_of + (part & 1) * 32 + half * 16);
+#pragma unroll
+                for (int h = 0; h < 16; h += 4) {
+                    const float4 x = st[h / 4];
+                    s[h] = (float)(int)(hi[h] * 256u + lo[h]) * (sc * x.x);
+                    s[h + 1] = (float)(int)(hi[h + 1] * 256u + lo[h + 1]) * (sc * x.y);
+                    s[h + 2] = (float)(int)(hi[h + 2] * 256u + lo[h + 2]) * (sc * x.z);
+                    s[h + 3] = (float)(int)(hi[h + 3] * 256u + lo[h + 3]) * (sc * x.w);
+                }
+                if (P) {
+                    tmem_ld16(at + 64, hi);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 16; ++h) s[h] += __uint_as_float(hi[h]);
+                }
+                float most = 0.0f;                                                    // lane l keeps head l's
 #pragma unroll
                 for (int h = 0; h < 16; ++h) {
-                    const float x = (float)((int)(hi[h] * 256u) + (int)lo[h]) * (sc * st[h]);
-                    s[h] = here ? (P ? x + __uint_as_float(r[h]) : x) : -INFINITY;
+                    s[h] = here ? s[h] : -INFINITY;
+                    const float m = warp_max(s[h]);
+                    most = lane == h ? m : most;
                 }
-                const float m = reduce16<true>(s);
-                if (lane < 16) wmax[((half * 2 + (j & 1)) * 4 + quarter) * 16 + lane] = m;
+                if (lane < 16) wm[quarter * 16 + lane] = most;
             }
-            float big = here ? sc : 0.0f;
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-            if (lane == 0) smax[(half * 2 + (j & 1)) * 4 + quarter] = big;
-            pair_barrier(half);
-            const float4 b4 = *reinterpret_cast<const float4*>(smax + (half * 2 + (j & 1)) * 4);
+            float big = warp_max(here ? sc : 0.0f);
+            if (lane == 0) sm[quarter] = big;
+            if (!meet()) return;
+            const float4 b4 = *reinterpret_cast<const float4*>(sm);
             big = fmaxf(fmaxf(b4.x, b4.y), fmaxf(b4.z, b4.w));
-            const float ratio = big > 0.0f ? sc / big * STEPS : 0.0f;
-            if (scoring) {                               // the products of the tile before have read its digits: its sums were taken
-                uint32_t dh[4] = {}, dl[4] = {};
-                const float* wm = wmax + (half * 2 + (j & 1)) * 64;
-                float f[16];
-                bool moved = false;
+            const float ratio = big > 0.0f ? sc * (STEPS / big) : 0.0f;
+            float scale = 1.0f;
+            uint32_t dh[4], dl[4];
+            if (scoring) {
+                // lane l (and l + 16) has head l's running maximum; every thread needs all of them
+                const int h0 = lane & 15;
+                const float m = mamba::max_nan(mamba::max_nan(mamba::max_nan(wm[h0], wm[16 + h0]), mamba::max_nan(wm[32 + h0], wm[48 + h0])), top);
+                const bool moved = __any_sync(0xffffffffu, m != top);                // the same for all warps of the half
+                float* own = heads_of + warp * 32;
+                const float f = m == top ? 1.0f : top == -INFINITY ? 0.0f : exp2_neg(top - m);
+                own[h0] = m;
+                if (moved) own[16 + h0] = f;
+                top = m;
+                __syncwarp();
+                if (moved) {
 #pragma unroll
-                for (int h = 0; h < 16; ++h) {
-                    const float m = mamba::max_nan(mamba::max_nan(mamba::max_nan(wm[h], wm[16 + h]), mamba::max_nan(wm[32 + h], wm[48 + h])), top[h]);
-                    moved = moved || m != top[h];
-                    f[h] = top[h];
-                    top[h] = m;
-                }
-                if (moved) {                                                          // the same for all threads of the half
-#pragma unroll
-                    for (int h = 0; h < 16; ++h) {
-                        f[h] = f[h] == -INFINITY ? 0.0f : exp2_neg(f[h] - top[h]);
-                        sum[h] *= f[h];
+                    for (int h = 0; h < 16; h += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(own + 16 + h);
+                        sum[h] *= x.x;
+                        sum[h + 1] *= x.y;
+                        sum[h + 2] *= x.z;
+                        sum[h + 3] *= x.w;
                     }
                 }
+                scale = f;
+                uint32_t v[16];
 #pragma unroll
-                for (int h = 0; h < 16; ++h) {
-                    const float e = here ? exp2_neg(s[h] - top[h]) : 0.0f;
-                    sum[h] += e;
-                    const int v = __float_as_int(fmaf(e, ratio, MAGIC)) - __float_as_int(MAGIC);
-                    dh[h / 4] |= high_digit(v) << (8 * (h & 3));
-                    dl[h / 4] |= low_digit(v) << (8 * (h & 3));
+                for (int h = 0; h < 16; h += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(own + h);
+                    const float t[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = here ? exp2_neg(s[h + e] - t[e]) : 0.0f;
+                        sum[h + e] += y;
+                        v[h + e] = __float_as_uint(fmaf(y, ratio, MAGIC));            // the integer is its low 16 bits: MAGIC's are zeros
+                    }
                 }
+                __syncwarp();                                                         // `own` is free again
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    dl[h] = bytes_of(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3], 0x0040u);
+                    dh[h] = bytes_of(v[4 * h] + 128u, v[4 * h + 1] + 128u, v[4 * h + 2] + 128u, v[4 * h + 3] + 128u, 0x0051u);
+                }
+            }
+            // The products of the tile before have read its digits, and were issued after all warps took the sums of the tile before that one: the digits, and the
+            // factors of two tiles before, may be overwritten.  (Both phases are still the barriers' last ones: the next cannot end without this warp.)
+            if (j > 0 && !(ok = mbar_wait_warp(o_full, (uint32_t)(j - 1) & 1u, status, 7) && mbar_wait_warp(p_full, (uint32_t)(j - 1) & 1u, status, 7))) return;
+            if (scoring) {
+                if (quarter == 0 && lane < 16) factor[(j & 1) * 32 + half * 16 + lane] = scale;
                 uint8_t* p = gen + (p_at - base) + token * 128;
                 *reinterpret_cast<uint4*>(p + ((half ^ (token & 7)) << 4)) = make_uint4(dh[0], dh[1], dh[2], dh[3]);
                 *reinterpret_cast<uint4*>(p + ((HP / 16 + half) ^ (token & 7)) * 16) = make_uint4(dl[0], dl[1], dl[2], dl[3]);
-                if (token == 0) {
-#pragma unroll
-                    for (int h = 0; h < 16; ++h) factor[(j & 1) * 32 + half * 16 + h] = moved ? f[h] : 1.0f;
-                }
             }
             if (token == 0 && half == 0) weight[j & 1] = big / STEPS;
             fence_async_smem();
@@ -384,10 +439,11 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full);
         };
-        auto gather = [&](int j) {
+        // Called behind softmax(j + 1), which has waited for p_full of tile j (by now that barrier may be a phase further), or for the part's last tile.
+        auto gather = [&](int j, bool last_of_part) {
             if (!(ok = mbar_wait_warp(o_full, (uint32_t)j & 1u, status, 8))) return;
-            // factors and weights of both halves' threads, which have all arrived at the barrier that the products waited for
-            if (!(ok = mbar_wait_warp(p_full, (uint32_t)j & 1u, status, 8))) return;
+            // factors and weights come from both halves' threads, which have all arrived at this barrier
+            if (last_of_part && !(ok = mbar_wait_warp(p_full, (uint32_t)j & 1u, status, 8))) return;
             tcgen05_fence_after();
             const float by = weight[j & 1];
             const float* f = factor + (j & 1) * 32;
@@ -417,43 +473,40 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                 }
             }
             tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty);
         };
 
         for (Walk k(a, first, last); k.more() && ok; k.next(), ++part) {
+            top = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < 16; ++h) {
-                top[h] = -INFINITY;
-                sum[h] = 0.0f;
-            }
+            for (int h = 0; h < 16; ++h) sum[h] = 0.0f;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int h = 0; h < 32; ++h) acc[c][h] = 0.0f;
             const int count = k.tiles();
             for (int i = 0; i < count && ok; ++i, ++g) {
-                if (i > 0) gather(g - 1);
-                if (ok) softmax(g);
+                softmax(g);
+                if (ok && i > 0) gather(g - 1, false);
             }
             if (!ok) break;
-            gather(g - 1);
+            gather(g - 1, true);
             if (!ok) break;
             // ---- the part's result ----
             const long long slot = (long long)w + k.b;
             if (scoring) {
-                const float s = reduce16<false>(sum);
+                const float s = reduce16(sum);
                 if (lane < 16) wsum[(half * 4 + quarter) * 16 + lane] = s;
             }
-            pair_barrier(half);
+            if (!meet()) break;
             if (scoring && token < 16 && h0 + half * 16 + token < a.heads) {
-                float m = top[0];
-#pragma unroll
-                for (int h = 1; h < 16; ++h) m = token == h ? top[h] : m;
                 const float* ws = wsum + half * 64 + token;
                 float* st = parts.stats(slot) + 2 * (h0 + half * 16 + token);
-                st[0] = m;
+                st[0] = top;
                 st[1] = (ws[0] + ws[16]) + (ws[32] + ws[48]);
             }
-            pair_barrier(half);
+            if (!meet()) break;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int r = (2 * half + c) * 128 + token;
@@ -485,26 +538,22 @@ int box_of(const el_latent_step_t& a) {
     // (a tensor map's rows are counted in 31 bits)
     return g >= 8 && a.pages > 0 && (long long)a.pages * a.page_size < (1LL << 31) ? g : 0;
 }
-Shape shape_of(const el_latent_step_t& a) { return Shape{(a.rank + 127) / 128, a.heads <= 16 ? 16 : 32, (a.heads + 31) / 32, box_of(a)}; }
-int shared_bytes(const el_latent_step_t& a, const Shape& s) {
-    const int stage = s.chunks * CHUNK + (a.rot_dim ? CHUNK : 0);
-    return 1024 + 2 * stage + s.chunks * s.n() * 128 + (a.rot_dim ? s.hp * 128 : 0) + CHUNK + 3232 + 96;
-}
+int shared_bytes(const el_latent_step_t& a, const StepImage& image) { return 1024 + 2 * (image.chunks + (a.rot_dim ? 1 : 0)) * CHUNK + image.bytes() + CHUNK + 4256 + 112; }
 
 }  // namespace
 
 bool latent_step_tc_takes(const el_latent_step_t& a) {
     return a.dtype != EL_F32 && a.rot_dim % 8 == 0 && reinterpret_cast<uintptr_t>(a.cache_keys) % 16 == 0 && (long long)a.batch * a.heads < (1 << 24);
 }
-int latent_step_tc_groups(const el_latent_step_t& a) { return shape_of(a).groups; }
 
-int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const float* steps, const void* rotated, const StepParts& parts, int workers, cudaStream_t st) {
-    Shape shape = shape_of(a);
+int launch_latent_step_tc(const el_latent_step_t& a, const uint8_t* images, const float* steps, const StepParts& parts, int workers, cudaStream_t st) {
+    const StepImage image(a);
+    const int box = box_of(a);
     CUtensorMap rows = {}, keys = {};
-    if (shape.box) {
+    if (box) {
         const uint64_t tokens = (uint64_t)a.pages * a.page_size;
-        int rc = make_map(&rows, a.latents, a.rank, tokens, a.rank, 128, shape.box, 128);
-        if (rc == EL_OK && a.rot_dim) rc = make_map(&keys, a.cache_keys, a.rot_dim * 2, tokens, a.rot_dim * 2, 128, shape.box, 128);
+        int rc = make_map(&rows, a.latents, a.rank, tokens, a.rank, 128, box, 128);
+        if (rc == EL_OK && a.rot_dim) rc = make_map(&keys, a.cache_keys, a.rot_dim * 2, tokens, a.rot_dim * 2, 128, box, 128);
         if (rc != EL_OK) return rc;
     }
     auto run = [&](auto t) {
@@ -516,7 +565,18 @@ int launch_latent_step_tc(const el_latent_step_t& a, const int8_t* digits, const
             EL_CUDA_TRY(cudaFuncSetAttribute(step_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
             once.mark(dev);
         }
-        step_tc_kernel<T><<<workers * shape.groups, THREADS, shared_bytes(a, shape), st>>>(rows, keys, a, digits, steps, static_cast<const T*>(rotated), parts, workers, shape);
+        cudaLaunchConfig_t cfg = {};
+        // may begin while the query's kernel still runs, and load; the query is read behind griddepcontrol.wait
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3(workers * image.groups);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = shared_bytes(a, image);
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        EL_CUDA_TRY(cudaLaunchKernelEx(&cfg, step_tc_kernel<T>, rows, keys, a, images, steps, parts, workers, box));
         return check_launch();
     };
     return a.dtype == EL_F16 ? run(__half()) : run(__nv_bfloat16());
