@@ -110,11 +110,11 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
     }
 }
 
-// u and w for the tensor cores: of one head, 128 columns of u for 64 sequences, into the images of latent_step.cuh.  u = gamma scale log2(e) q W is held in
+// u and w for the tensor cores: of one head, 128 columns of u for 16 sequences, into the images of latent_step.cuh.  u = gamma scale log2(e) q W is held in
 // two 8-bit digits of 1 / 32512 of gamma scale log2(e) sum |q|, which it cannot exceed whatever the weights are: no block has to know another's columns.
 // (For weights of random signs that is 3 to 4 times the largest u, 14 bits of it.)  steps [batch, groups, 32].  A warp takes 16 columns, which are one
 // word of every row of the weights.
-constexpr int QUERY_ROWS = 64, QUERY_COLS = 128;
+constexpr int QUERY_ROWS = 16, QUERY_COLS = 128;
 template <typename T>
 __global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_latent_step_t a, uint8_t* __restrict__ images, float* __restrict__ steps, const bool vectors) {
     __shared__ __align__(16) T q[QUERY_ROWS][256 + 8];
@@ -318,30 +318,49 @@ __global__ void __launch_bounds__(THREADS) step_rows_kernel(const el_latent_step
     }
 }
 
-// A block joins the parts of one head of up to 16 sequences and takes the results through the head's value rows.  Sequences are spread over the 16
-// warps; where there are fewer, several warps share a sequence's parts.  The product with the value rows runs on the warps' matrix instructions, the float32
-// vectors split into two bfloat16 terms (16 bits of each), three for float32 outputs.
-constexpr int JOIN_THREADS = 512, JOIN_ROWS = 16, JOIN_PITCH = MOST_RANK + 8;
-template <typename T> constexpr int JOIN_TERMS = sizeof(T) == 4 ? 3 : 2;
-template <typename T> constexpr int JOIN_BYTES = JOIN_ROWS * MOST_RANK * 4 + JOIN_TERMS<T> * JOIN_ROWS * JOIN_PITCH * 2;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// a word to the same place of shared memory in block `rank` of the cluster
+__device__ __forceinline__ void store_cluster(uint32_t addr, int rank, uint32_t v) {
+    asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, %1;\n\tst.shared::cluster.u32 [at], %2;\n\t}" ::"r"(addr), "r"(rank), "r"(v) : "memory");
+}
 
-template <typename T>
+// BLOCKS blocks (a cluster of four, or one) join the parts of one head of up to 16 sequences and take the results through the head's value rows: each block
+// joins its share of the latent channels, all write theirs into all blocks' shared memory, and each forms its share of the values.  Sequences are spread over
+// a block's 16 warps; where there are fewer, several warps share a sequence's parts, and the warps share the reduction of the product.  The product
+// runs on the warps' matrix instructions, the float32 vectors split into two bfloat16 terms (16 bits of each), three for float32 outputs.
+// Four blocks for up to 16 sequences, where each has many parts and there would be few blocks: 1 sequence of 32768 tokens, 32 heads: 22.5 us with one block, 15.6
+// with four; 64 sequences: 17.5 and 27.
+constexpr int JOIN_THREADS = 512, JOIN_WARPS = 16, JOIN_ROWS = 16, JOIN_PITCH = MOST_RANK + 8;
+template <typename T> constexpr int JOIN_TERMS = sizeof(T) == 4 ? 3 : 2;
+template <typename T, int BLOCKS> constexpr int JOIN_BYTES = JOIN_WARPS * (MOST_RANK / BLOCKS) * 4 + JOIN_TERMS<T> * JOIN_ROWS * JOIN_PITCH * 2;
+
+template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent_step_t a, const StepParts parts, int workers) {
+    constexpr int COLS = MOST_RANK / BLOCKS, WORDS = MOST_RANK / 16 / (BLOCKS == 1 ? 1 : 2);
     extern __shared__ float4 join_smem[];
-    float* o = reinterpret_cast<float*>(join_smem);                                            // [16 warps][512]
-    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(o + JOIN_ROWS * MOST_RANK);        // [terms][16 sequences][JOIN_PITCH]
-    const int h = blockIdx.x, b0 = blockIdx.y * JOIN_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.rank;
+    float* o = reinterpret_cast<float*>(join_smem);                                            // [16 warps][COLS]
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(o + JOIN_WARPS * COLS);            // [terms][16 sequences][JOIN_PITCH]
+    const int h = blockIdx.x / BLOCKS, quarter = blockIdx.x % BLOCKS, b0 = blockIdx.y * JOIN_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.rank;
     const int nb = min(JOIN_ROWS, a.batch - b0);
     int spread = 1;                                  // sequences side by side, a power of two; 16 / spread warps share one
     while (spread < nb) spread *= 2;
-    const int shares = 16 / spread, share = warp / spread, b = b0 + warp % spread;
-    // the weights of the warp's first eight value rows, before anything that the kernels before leave is there
-    const int words = R / 16, r = lane >> 2, k2 = (lane & 3) * 2;
-    const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim) * words;
-    uint32_t first[MOST_RANK / 16];
+    const int shares = JOIN_WARPS / spread, share = warp / spread, b = b0 + warp % spread;
+    const int c0 = quarter * COLS, cols = min(COLS, R - c0);                                   // this block's channels (none: 0 or less)
+    // the value rows of this block, eight for a warp at a time; warps that have the same ones take every `depth`-th word (16 channels) of them
+    const int words = R / 16, r = lane >> 2, k2 = (lane & 3) * 2, per = (a.value_dim + 8 * BLOCKS - 1) / (8 * BLOCKS) * 8, v_begin = quarter * per;
+    int groups = 1;                                  // of eight rows, a power of two and 16 at most
+    while (groups * 8 < per && groups < JOIN_WARPS) groups *= 2;
+    const int depth = JOIN_WARPS / groups, first = warp / groups;
+    uint32_t w[WORDS];                               // (four blocks have 64 value rows at most: depth is 2 or more)
+    auto load_weights = [&](int v0) {
+        const int row = v_begin + v0 + r;
+        const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim + row) * words;
 #pragma unroll
-    for (int k = 0; k < MOST_RANK / 16; ++k) first[k] = k < words && warp * 8 + r < a.value_dim ? W[(long long)(warp * 8 + r) * words + k] : 0x55555555u;
-    float acc[MOST_RANK / 32] = {};
+        for (int k = 0; k < WORDS; ++k) w[k] = v0 < per && row < a.value_dim && first + k * depth < words ? W[first + k * depth] : 0x55555555u;
+    };
+    load_weights((warp % groups) * 8);               // before anything that the kernels before leave is there
+    float acc[COLS / 32] = {};
     int w0 = 0, w1 = -1;
     if (warp % spread < nb) {
         long long tiles = 0, before = 0;
@@ -369,8 +388,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
     if (w0 <= w1) {
         float top = -INFINITY, sum = 0.0f;
 #pragma unroll 5
-        for (int w = w0 + lane; w <= w1; w += 32) {
-            const float2 st = *reinterpret_cast<const float2*>(parts.stats((long long)w + b) + 2 * h);
+        for (int p = w0 + lane; p <= w1; p += 32) {
+            const float2 st = *reinterpret_cast<const float2*>(parts.stats((long long)p + b) + 2 * h);
             const float m = mamba::max_nan(top, st.x), from = m == -INFINITY ? 0.0f : m;
             sum = fmaf(sum, exp2_neg(top - from), exp2_neg(st.x - from) * st.y);
             top = m;
@@ -385,16 +404,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
         const float by = all == -INFINITY ? 0.0f : a.gamma / sum;
         // 32 of this warp's parts at a time: lane l has the factor of the l-th
         for (int p = w0 + share; p <= w1; p += 32 * shares) {
-            const int mine = p + lane * shares, count = min(32, (w1 - p) / shares + 1);
-            const float f = mine <= w1 ? exp2_neg(parts.stats((long long)mine + b)[2 * h] - from) * by : 0.0f;
-            const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + b) + (long long)h * R) + lane;
+            const int own = p + lane * shares, count = min(32, (w1 - p) / shares + 1);
+            const float f = own <= w1 ? exp2_neg(parts.stats((long long)own + b)[2 * h] - from) * by : 0.0f;
+            const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + b) + (long long)h * R + c0) + lane;
             const long long step = (long long)shares * a.heads * (R / 4);
-#pragma unroll 4
+#pragma unroll (BLOCKS == 1 ? 4 : 8)
             for (int i = 0; i < count; ++i) {
                 const float x = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
-                for (int c = 0; c < MOST_RANK / 128; ++c) {
-                    if ((c * 32 + lane) * 4 >= R) continue;
+                for (int c = 0; c < COLS / 128; ++c) {
+                    if ((c * 32 + lane) * 4 >= cols) continue;
                     const float4 y = v[i * step + c * 32];
                     acc[4 * c] = fmaf(x, y.x, acc[4 * c]);
                     acc[4 * c + 1] = fmaf(x, y.y, acc[4 * c + 1]);
@@ -405,53 +424,91 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
         }
     }
 #pragma unroll
-    for (int c = 0; c < MOST_RANK / 128; ++c)
-        reinterpret_cast<float4*>(o + warp * MOST_RANK)[c * 32 + lane] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
-    __syncthreads();
-    for (int n = warp; n < JOIN_ROWS; n += JOIN_THREADS / 32)
-        for (int c = lane; c < R; c += 32) {
-            float v = 0.0f;
-            if (n < nb)
-                for (int s = 0; s < shares; ++s) v += o[(s * spread + n) * MOST_RANK + c];
-#pragma unroll
-            for (int t = 0; t < JOIN_TERMS<T>; ++t) {
-                const __nv_bfloat16 x = __float2bfloat16_rn(v);
-                terms[(t * JOIN_ROWS + n) * JOIN_PITCH + c] = x;
-                v -= __bfloat162float(x);
-            }
+    for (int c = 0; c < COLS / 128; ++c)
+        reinterpret_cast<float4*>(o + warp * COLS)[c * 32 + lane] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+    auto meet = [&]() {
+        if (BLOCKS > 1) {
+            cluster_arrive();
+            cluster_wait();
+        } else {
+            __syncthreads();
         }
-    __syncthreads();
-    for (int v0 = warp * 8; v0 < a.value_dim; v0 += 128) {
+    };
+    meet();                                          // the other blocks have begun, too: their shared memory may be written
+    for (int i = threadIdx.x; i < JOIN_ROWS * COLS / 2; i += JOIN_THREADS) {
+        const int n = i / (COLS / 2), c = i % (COLS / 2) * 2;
+        if (c >= cols) continue;
+        float2 v = make_float2(0.0f, 0.0f);
+        if (n < nb)
+            for (int s = 0; s < shares; ++s) {
+                const float2 x = *reinterpret_cast<const float2*>(o + (s * spread + n) * COLS + c);
+                v.x += x.x;
+                v.y += x.y;
+            }
+#pragma unroll
+        for (int t = 0; t < JOIN_TERMS<T>; ++t) {
+            const uint32_t x = pack_bf16x2(v.x, v.y);
+            __nv_bfloat16* to = terms + (t * JOIN_ROWS + n) * JOIN_PITCH + c0 + c;
+            if (BLOCKS > 1) {
+#pragma unroll
+                for (int q = 0; q < BLOCKS; ++q) store_cluster((uint32_t)__cvta_generic_to_shared(to), q, x);
+            } else {
+                *reinterpret_cast<uint32_t*>(to) = x;
+            }
+            v.x -= __uint_as_float(x << 16);
+            v.y -= __uint_as_float(x & 0xFFFF0000u);
+        }
+    }
+    meet();
+    for (int v0 = (warp % groups) * 8;; v0 += 128) {                                           // (more than 128 value rows: one block, depth 1)
         float d[4] = {};
 #pragma unroll
-        for (int k = 0; k < MOST_RANK / 16; ++k) {
-            if (k >= words) break;
-            const uint32_t w = first[k] >> (2 * k2);
-            const uint32_t x0 = weight_pair<__nv_bfloat16>(w & 3u, (w >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((w >> 16) & 3u, (w >> 18) & 3u);
+        for (int k = 0; k < WORDS; ++k) {
+            const int word = first + k * depth;
+            if (word >= words) break;
+            const uint32_t x = w[k] >> (2 * k2);
+            const uint32_t x0 = weight_pair<__nv_bfloat16>(x & 3u, (x >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((x >> 16) & 3u, (x >> 18) & 3u);
 #pragma unroll
             for (int t = JOIN_TERMS<T> - 1; t >= 0; --t) {
-                const __nv_bfloat16* p = terms + (t * JOIN_ROWS + r) * JOIN_PITCH + k * 16 + k2;
-                const uint32_t x[4] = {*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH), *reinterpret_cast<const uint32_t*>(p + 8),
+                const __nv_bfloat16* p = terms + (t * JOIN_ROWS + r) * JOIN_PITCH + word * 16 + k2;
+                const uint32_t y[4] = {*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH), *reinterpret_cast<const uint32_t*>(p + 8),
                                        *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH + 8)};
-                warp_mma<__nv_bfloat16>(d, x, x0, x1);
+                warp_mma<__nv_bfloat16>(d, y, x0, x1);
             }
+        }
+        if (depth > 1) {                             // the warps' shares of the reduction: [warp][16 sequences][8 rows]
+            *reinterpret_cast<float2*>(o + warp * 128 + r * 8 + k2) = make_float2(d[0], d[1]);
+            *reinterpret_cast<float2*>(o + warp * 128 + (r + 8) * 8 + k2) = make_float2(d[2], d[3]);
+            break;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int n = r + 8 * (i >> 1), v = v0 + k2 + (i & 1);
-            if (n < nb && v < a.value_dim) static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v] = mamba::from_float<T>(d[i]);
+            if (n < nb && v < per && v_begin + v < a.value_dim)
+                static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v_begin + v] = mamba::from_float<T>(d[i]);
         }
-        if (v0 + 128 < a.value_dim) {                // value heads beyond 128 channels
-#pragma unroll
-            for (int k = 0; k < MOST_RANK / 16; ++k) first[k] = k < words && v0 + 128 + r < a.value_dim ? W[(long long)(v0 + 128 + r) * words + k] : 0x55555555u;
-        }
+        if (v0 + 128 >= per) break;
+        load_weights(v0 + 128);
+    }
+    if (depth == 1) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < nb * per; i += JOIN_THREADS) {
+        const int n = i / per, v = i - n * per;
+        if (v_begin + v >= a.value_dim) continue;
+        float x = 0.0f;
+        for (int s = 0; s < depth; ++s) x += o[(s * groups + v / 8) * 128 + n * 8 + v % 8];
+        static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v_begin + v] = mamba::from_float<T>(x);
     }
 }
 
 // A launch that may begin before the one in front of it has ended; what that one leaves is read behind griddepcontrol.wait.
-template <typename K, typename... A> int launch_dependent(K kernel, dim3 grid, int threads, int bytes, cudaStream_t st, A... args) {
+template <typename K, typename... A> int launch_dependent(K kernel, dim3 grid, int cluster, int threads, int bytes, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = grid;
@@ -459,7 +516,7 @@ template <typename K, typename... A> int launch_dependent(K kernel, dim3 grid, i
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     EL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
     return check_launch();
 }
@@ -532,9 +589,15 @@ int launch_latent_step(const el_latent_step_t& a, cudaStream_t st) {
             if ((rc = check_launch()) == EL_OK && workers > 0) rc = launch_latent_step_tc(a, images, steps, parts, workers, st);
         }
         if (rc != EL_OK) return rc;
-        static DeviceOnce once;
-        if ((rc = allow_shared(step_join_kernel<T>, JOIN_BYTES<T>, once)) != EL_OK) return rc;
-        return launch_dependent(step_join_kernel<T>, dim3(a.heads, (a.batch + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, JOIN_BYTES<T>, st, a, parts, workers);
+        auto join = [&](auto blocks) {
+            constexpr int BLOCKS = decltype(blocks)::value;
+            static DeviceOnce once;
+            const int rc = allow_shared(step_join_kernel<T, BLOCKS>, JOIN_BYTES<T, BLOCKS>, once);
+            if (rc != EL_OK) return rc;
+            const dim3 grid(a.heads * BLOCKS, (a.batch + JOIN_ROWS - 1) / JOIN_ROWS);
+            return launch_dependent(step_join_kernel<T, BLOCKS>, grid, BLOCKS, JOIN_THREADS, JOIN_BYTES<T, BLOCKS>, st, a, parts, workers);
+        };
+        return a.batch <= JOIN_ROWS ? join(std::integral_constant<int, 4>()) : join(std::integral_constant<int, 1>());
     });
 }
 

@@ -101,6 +101,19 @@ __device__ __forceinline__ float reduce16(const float (&v)[16]) {
     return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 16);
 }
 
+__device__ __forceinline__ float reduce16max(const float (&v)[16]) {
+    const int lane = threadIdx.x & 31;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = v[i];
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int i = 0; i < w; ++i) x[i] = mamba::max_nan(up ? x[i + w] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + w], w));
+    }
+    return mamba::max_nan(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16));
+}
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1)
 step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant__ CUtensorMap tmKeys, const el_latent_step_t a, const uint8_t* __restrict__ images,
@@ -366,13 +379,9 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
 #pragma unroll
                     for (int h = 0; h < 16; ++h) s[h] += __uint_as_float(hi[h]);
                 }
-                float most = 0.0f;                                                    // lane l keeps head l's
 #pragma unroll
-                for (int h = 0; h < 16; ++h) {
-                    s[h] = here ? s[h] : -INFINITY;
-                    const float m = warp_max(s[h]);
-                    most = lane == h ? m : most;
-                }
+                for (int h = 0; h < 16; ++h) s[h] = here ? s[h] : -INFINITY;
+                const float most = reduce16max(s);
                 if (lane < 16) wm[quarter * 16 + lane] = most;
             }
             float big = warp_max(here ? sc : 0.0f);
