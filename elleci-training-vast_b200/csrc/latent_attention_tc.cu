@@ -55,7 +55,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int i0 = (pairs - 1 - at.tile) * 2 * TILE;            // the longest rows first
     const Sequence seq(a, b);
     // key tiles of the two query tiles
-    const int n0 = i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0, n1 = i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0;
+    const int n0 = uniform(i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0);
+    const int n1 = uniform(i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0);
     const int n = n0 > n1 ? n0 : n1;
 
     if (threadIdx.x == 0) {
@@ -77,7 +78,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *tmem_holder;
+    const uint32_t tmem = uniform(*tmem_holder);
     const uint32_t S = tmem, O = tmem + 256;                    // S_i at 128 i, O_i at 256 + 128 i
     int32_t* status = a.dev_status;
 
@@ -140,53 +141,61 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             for (int c = first; c < first + count; ++c) umma_commit(slot_empty(slot_of(c)));
         };
         auto scores = [&](int i, int first) {                   // S_i = Q_i K'; one thread
+            uint32_t q = desc_low(base + i * QC * CHUNK, 16);
+            int slot = slot_of(first);
+#pragma unroll 1
             for (int c = 0; c < QC; ++c) {
-                const uint32_t q = base + (i * QC + c) * CHUNK, k = ring + slot_of(first + c) * CHUNK;
-                const int steps = c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps;
-                for (int x = 0; x < steps; ++x) umma_f16(S + i * 128, make_desc(q + x * 32, 16), make_desc(k + x * 32, 16), i_s, (c | x) != 0);
+                umma_f16_chunk(S + i * 128, q, desc_low(ring + slot * CHUNK, 16), i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
+                q += CHUNK >> 4;
+                slot = slot + 1 == NS ? 0 : slot + 1;
             }
             umma_commit(s_full(i));
         };
         auto values = [&](int i, int first, bool more) {        // O_i += P_i V; one thread
-            const int s0 = slot_of(first);
-            if (VC == 1 || s0 + 1 < NS) {                       // the chunks lie side by side
-                const uint32_t id = idesc_f16<T>(0, 1, V);
-                for (int x = 0; x < TILE / 16; ++x) umma_f16_ts(O + i * 128, S + i * 128 + x * 8, make_desc(ring + s0 * CHUNK + x * 2048, CHUNK), id, more || x != 0);
-            } else {
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t id = idesc_f16<T>(0, 1, c == 0 ? 64 : V - 64), v = ring + slot_of(first + c) * CHUNK;
-                    for (int x = 0; x < TILE / 16; ++x) umma_f16_ts(O + i * 128 + c * 64, S + i * 128 + x * 8, make_desc(v + x * 2048, CHUNK), id, more || x != 0);
-                }
+            const int s0 = slot_of(first), parts = VC == 1 || s0 + 1 < NS ? 1 : 2;             // the chunks lie side by side, or the ring's end is between them
+#pragma unroll 1
+            for (int c = 0; c < parts; ++c) {
+                const uint32_t id = idesc_f16<T>(0, 1, parts == 1 ? V : c == 0 ? 64 : V - 64), v = desc_low(ring + (c == 0 ? s0 : 0) * CHUNK, CHUNK);
+                const uint32_t o = O + i * 128 + c * 64, p = S + i * 128;
+                umma_f16_ts(o, p, desc_of(v), id, more);
+#pragma unroll
+                for (int x = 1; x < TILE / 16; ++x) umma_f16_ts(o, p + x * 8, desc_of(v + x * 128), id, 1u);
             }
             umma_commit(o_full(i));
         };
         if (n > 0) {
-            for (int i = 0; i < 2 && ok; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 if ((i == 0 ? n0 : n1) == 0) continue;
-                ok = mbar_wait_warp(q_full(i), 0, status, 4);
+                ok = ok && mbar_wait_warp(q_full(i), 0, status, 4);
                 wait_chunks(0, QC);
-                if (ok && elect_one()) scores(i, 0);
+                if (!ok) break;
+                if (elect_one()) scores(i, 0);
                 __syncwarp();
             }
-            if (ok && elect_one()) release(0, QC);
-            __syncwarp();
+            if (ok) {
+                if (elect_one()) release(0, QC);
+                __syncwarp();
+            }
         }
         for (int j = 0; j < n && ok; ++j) {
             const int v = j * (QC + VC) + QC, k = (j + 1) * (QC + VC);
-            for (int i = 0; i < 2 && ok; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 const int mine = i == 0 ? n0 : n1;
                 if (j >= mine) continue;
-                ok = mbar_wait_warp(p_full(i), (uint32_t)j & 1u, status, 5);
+                ok = ok && mbar_wait_warp(p_full(i), (uint32_t)j & 1u, status, 5);
                 if (ok) wait_chunks(v, VC);
-                if (ok && elect_one()) values(i, v, j != 0);
+                if (!ok) break;
+                if (elect_one()) values(i, v, j != 0);
                 __syncwarp();
-                if (j + 1 < mine && ok) {
+                if (j + 1 < mine) {
                     wait_chunks(k, QC);
-                    if (ok && elect_one()) scores(i, k);
+                    if (!ok) break;
+                    if (elect_one()) scores(i, k);
                     __syncwarp();
                 }
             }
-            if (ok && elect_one()) {
+            if (!ok) break;
+            if (elect_one()) {
                 release(v, VC);
                 if (j + 1 < n) release(k, QC);
             }

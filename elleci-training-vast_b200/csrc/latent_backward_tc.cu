@@ -63,7 +63,8 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
         begin = KEYS ? seq.query_begin(r0) / STEP * STEP : 0;
         end = KEYS ? seq.queries : seq.key_end(r0 + HELD);
     }
-    const int n = end > begin ? (end - begin + STEP - 1) / STEP : 0;
+    begin = uniform(begin);
+    const int n = uniform(end > begin ? (end - begin + STEP - 1) / STEP : 0);
     const long long stat_row = ((long long)b * a.heads + h) * lse_pitch(a.length);
 
     if (threadIdx.x == 0) {
@@ -87,7 +88,7 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *tmem_holder;
+    const uint32_t tmem = uniform(*tmem_holder);
     const uint32_t ACC1 = tmem, ACC2 = tmem + 192, S = KEYS ? tmem + 320 : tmem + 192, DP = S + 128;      // S_i at 64 i, dP_i at 64 i
     int32_t* status = a.dev_status;
 
@@ -141,54 +142,69 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
         const bool joined = R == 0 || D % 64 == 0;               // acc1's columns are the chunks' columns, one after another
         const uint32_t i_1 = idesc_f16<T>(0, 1, joined ? D + R : D), i_r = idesc_f16<T>(0, 1, R);
         auto stage = [&](int j) { return ring + (j % NS) * stage_bytes; };
-        auto scores = [&](int j) {
+        auto scores = [&](int j) {                               // one thread, as the others
+            uint32_t x = desc_low(base, 16), y = desc_low(stage(j), 16);
+#pragma unroll 1
             for (int c = 0; c < QC; ++c) {
-                const uint32_t x = base + c * HELD_CHUNK, y = stage(j) + c * STEP_CHUNK;
-                const int steps = c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps;
-                for (int k = 0; k < steps; ++k) umma_f16(S + (j & 1) * 64, make_desc(x + k * 32, 16), make_desc(y + k * 32, 16), i_s, (c | k) != 0);
+                umma_f16_chunk(S + (j & 1) * 64, x, y, i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
+                x += HELD_CHUNK >> 4;
+                y += STEP_CHUNK >> 4;
             }
             umma_commit(s_full(j & 1));
         };
         auto grads = [&](int j) {
             const int buf = DP_BUFFERS == 2 ? j & 1 : 0;
-            for (int k = 0; k < value_steps; ++k)
-                umma_f16(DP + buf * 64, make_desc(base + (QC + k / 4) * HELD_CHUNK + k % 4 * 32, 16), make_desc(stage(j) + (QC + k / 4) * STEP_CHUNK + k % 4 * 32, 16), i_s, k != 0);
+            uint32_t x = desc_low(base + QC * HELD_CHUNK, 16), y = desc_low(stage(j) + QC * STEP_CHUNK, 16);
+#pragma unroll 1
+            for (int c = 0; c < VC; ++c) {
+                umma_f16_chunk(DP + buf * 64, x, y, i_s, c != 0, min(4, value_steps - 4 * c));
+                x += HELD_CHUNK >> 4;
+                y += STEP_CHUNK >> 4;
+            }
             umma_commit(dp_full(buf));
         };
-        auto left = [&](int k) { return k < 2 ? k * 8 : 32 + (k - 2) * 8; };      // the two halves of the threads write their factors over their own columns
+        // acc += left factors (over S or dP at `f`, each half of the threads over its own columns) times 64 rows of chunks at `rows`
+        auto sums = [&](uint32_t acc, uint32_t f, uint32_t rows, uint32_t idesc, bool more) {
+            const uint32_t y = desc_low(rows, STEP_CHUNK);
+            umma_f16_ts(acc, f, desc_of(y), idesc, more);
+            umma_f16_ts(acc, f + 8, desc_of(y + 128), idesc, 1u);
+            umma_f16_ts(acc, f + 32, desc_of(y + 256), idesc, 1u);
+            umma_f16_ts(acc, f + 40, desc_of(y + 384), idesc, 1u);
+        };
         bool ok = n > 0 && mbar_wait_warp(a_full, 0, status, 3) && mbar_wait_warp(full(0), 0, status, 3);
         tcgen05_fence_after();
-        if (ok && elect_one()) {
-            scores(0);
-            grads(0);
+        if (ok) {
+            if (elect_one()) {
+                scores(0);
+                grads(0);
+            }
+            __syncwarp();
         }
-        __syncwarp();
         for (int j = 0; j < n && ok; ++j) {
             if (j + 1 < n) {
                 ok = mbar_wait_warp(full((j + 1) % NS), (uint32_t)((j + 1) / NS) & 1u, status, 4);
                 tcgen05_fence_after();
-                if (ok && elect_one()) {
+                if (!ok) break;
+                if (elect_one()) {
                     scores(j + 1);
                     if (DP_BUFFERS == 2) grads(j + 1);
                 }
                 __syncwarp();
             }
-            if (KEYS && ok) {
+            if (KEYS) {
                 ok = mbar_wait_warp(p_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 5);
                 tcgen05_fence_after();
-                if (ok && elect_one())
-                    for (int k = 0; k < 4; ++k) umma_f16_ts(ACC2, S + (j & 1) * 64 + left(k), make_desc(stage(j) + QC * STEP_CHUNK + k * 2048, STEP_CHUNK), i_v, (j | k) != 0);
+                if (!ok) break;
+                if (elect_one()) sums(ACC2, S + (j & 1) * 64, stage(j) + QC * STEP_CHUNK, i_v, j != 0);
                 __syncwarp();
             }
-            if (!ok) break;
             ok = mbar_wait_warp(ds_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6);
             tcgen05_fence_after();
-            if (ok && elect_one()) {
+            if (!ok) break;
+            if (elect_one()) {
                 const uint32_t f = DP + (DP_BUFFERS == 2 ? j & 1 : 0) * 64;
-                for (int k = 0; k < 4; ++k) {
-                    umma_f16_ts(ACC1, f + left(k), make_desc(stage(j) + k * 2048, STEP_CHUNK), i_1, (j | k) != 0);
-                    if (!joined) umma_f16_ts(ACC1 + D, f + left(k), make_desc(stage(j) + plan.key_chunks * STEP_CHUNK + k * 2048, STEP_CHUNK), i_r, (j | k) != 0);
-                }
+                sums(ACC1, f, stage(j), i_1, j != 0);
+                if (!joined) sums(ACC1 + D, f, stage(j) + plan.key_chunks * STEP_CHUNK, i_r, j != 0);
                 umma_commit(empty(j % NS));
                 if (DP_BUFFERS == 1 && j + 1 < n) grads(j + 1);
                 if (j + 1 == n) umma_commit(done);

@@ -12,6 +12,16 @@ namespace tc {
 
 constexpr int CHUNK_COLS = 64;
 
+// The value of lane 0, in a form that the compiler knows to be the same for the whole warp.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Matrix descriptors by halves: the upper one is the same for all operands here (make_desc), the lower one is the address, which a step along the reduction
+// moves by a constant (2 for 32 bytes of a K-major row, 128 for 16 rows of an MN-major one).  One warp issues the products, an instruction every few
+// cycles: with descriptors built anew for every product it took 130 cycles for each, where a 128 x 128 x 16 product itself takes 64.
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) { return ((saddr & 0x3FFFFu) >> 4) | ((lbo_bytes >> 4) << 16); }
+__device__ __forceinline__ uint64_t desc_of(uint32_t low) { return ((uint64_t)DESC_HIGH << 32) | low; }
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -39,6 +49,17 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+// d += or = a b over `steps` (1 .. 4) steps of 16 along the reduction, both operands K-major chunks; one thread
+__device__ __forceinline__ void umma_f16_chunk(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate, int steps) {
+    umma_f16(d_tmem, desc_of(a_low), desc_of(b_low), idesc, accumulate);
+    if (steps == 4) {
+#pragma unroll
+        for (int x = 1; x < 4; ++x) umma_f16(d_tmem, desc_of(a_low + 2 * x), desc_of(b_low + 2 * x), idesc, 1u);
+        return;
+    }
+#pragma unroll 1
+    for (int x = 1; x < steps; ++x) umma_f16(d_tmem, desc_of(a_low + 2 * x), desc_of(b_low + 2 * x), idesc, 1u);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
