@@ -130,19 +130,30 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const uint32_t i_s = idesc_f16<T>(0, 0, TILE);
         const int key_steps = a.key_dim / 16, rot_steps = a.rot_dim / 16, V = a.value_dim;
         bool ok = true;
-        // ring position of the first chunk of keys j: chunks are taken in order
-        auto slot_of = [&](int chunk) { return chunk % NS; };
-        auto phase_of = [&](int chunk) { return (uint32_t)(chunk / NS) & 1u; };
-        auto wait_chunks = [&](int first, int count) {
-            for (int c = first; c < first + count && ok; ++c) ok = mbar_wait_warp(slot_full(slot_of(c)), phase_of(c), status, 3);
+        // a place in the ring, which chunks go through in order (counted, not divided: a division costs more than a product)
+        struct At {
+            int slot;
+            uint32_t phase;
+        };
+        auto after = [&](At x, int count) {
+            x.slot += count;
+            if (x.slot >= NS) {
+                x.slot -= NS;
+                x.phase ^= 1u;
+            }
+            return x;
+        };
+        auto wait_chunks = [&](At x, int count) {
+            for (int c = 0; c < count && ok; ++c, x = after(x, 1)) ok = mbar_wait_warp(slot_full(x.slot), x.phase, status, 3);
             tcgen05_fence_after();
         };
-        auto release = [&](int first, int count) {
-            for (int c = first; c < first + count; ++c) umma_commit(slot_empty(slot_of(c)));
+        auto release = [&](At x, int count) {
+#pragma unroll 1
+            for (int c = 0; c < count; ++c, x = after(x, 1)) umma_commit(slot_empty(x.slot));
         };
-        auto scores = [&](int i, int first) {                   // S_i = Q_i K'; one thread
+        auto scores = [&](int i, At first) {                    // S_i = Q_i K'; one thread
             uint32_t q = desc_low(base + i * QC * CHUNK, 16);
-            int slot = slot_of(first);
+            int slot = first.slot;
 #pragma unroll 1
             for (int c = 0; c < QC; ++c) {
                 umma_f16_chunk(S + i * 128, q, desc_low(ring + slot * CHUNK, 16), i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
@@ -151,8 +162,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             umma_commit(s_full(i));
         };
-        auto values = [&](int i, int first, bool more) {        // O_i += P_i V; one thread
-            const int s0 = slot_of(first), parts = VC == 1 || s0 + 1 < NS ? 1 : 2;             // the chunks lie side by side, or the ring's end is between them
+        auto values = [&](int i, At first, bool more) {         // O_i += P_i V; one thread
+            const int s0 = first.slot, parts = VC == 1 || s0 + 1 < NS ? 1 : 2;             // the chunks lie side by side, or the ring's end is between them
 #pragma unroll 1
             for (int c = 0; c < parts; ++c) {
                 const uint32_t id = idesc_f16<T>(0, 1, parts == 1 ? V : c == 0 ? 64 : V - 64), v = desc_low(ring + (c == 0 ? s0 : 0) * CHUNK, CHUNK);
@@ -163,22 +174,24 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             umma_commit(o_full(i));
         };
+        const At begin{0, 0};
+        At v = after(begin, QC);
         if (n > 0) {
             for (int i = 0; i < 2; ++i) {
                 if ((i == 0 ? n0 : n1) == 0) continue;
                 ok = ok && mbar_wait_warp(q_full(i), 0, status, 4);
-                wait_chunks(0, QC);
+                wait_chunks(begin, QC);
                 if (!ok) break;
-                if (elect_one()) scores(i, 0);
+                if (elect_one()) scores(i, begin);
                 __syncwarp();
             }
             if (ok) {
-                if (elect_one()) release(0, QC);
+                if (elect_one()) release(begin, QC);
                 __syncwarp();
             }
         }
         for (int j = 0; j < n && ok; ++j) {
-            const int v = j * (QC + VC) + QC, k = (j + 1) * (QC + VC);
+            const At k = after(v, VC);
             for (int i = 0; i < 2; ++i) {
                 const int mine = i == 0 ? n0 : n1;
                 if (j >= mine) continue;
@@ -200,6 +213,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                 if (j + 1 < n) release(k, QC);
             }
             __syncwarp();
+            v = after(k, QC);
         }
     } else {
         // ================= softmax =================

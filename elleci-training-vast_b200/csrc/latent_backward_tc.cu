@@ -141,9 +141,8 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
         const uint32_t i_s = idesc_f16<T>(0, 0, STEP), i_v = idesc_f16<T>(0, 1, V);
         const bool joined = R == 0 || D % 64 == 0;               // acc1's columns are the chunks' columns, one after another
         const uint32_t i_1 = idesc_f16<T>(0, 1, joined ? D + R : D), i_r = idesc_f16<T>(0, 1, R);
-        auto stage = [&](int j) { return ring + (j % NS) * stage_bytes; };
-        auto scores = [&](int j) {                               // one thread, as the others
-            uint32_t x = desc_low(base, 16), y = desc_low(stage(j), 16);
+        auto scores = [&](int j, uint32_t rows) {                // one thread, as the others
+            uint32_t x = desc_low(base, 16), y = desc_low(rows, 16);
 #pragma unroll 1
             for (int c = 0; c < QC; ++c) {
                 umma_f16_chunk(S + (j & 1) * 64, x, y, i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
@@ -152,9 +151,9 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
             }
             umma_commit(s_full(j & 1));
         };
-        auto grads = [&](int j) {
+        auto grads = [&](int j, uint32_t rows) {
             const int buf = DP_BUFFERS == 2 ? j & 1 : 0;
-            uint32_t x = desc_low(base + QC * HELD_CHUNK, 16), y = desc_low(stage(j) + QC * STEP_CHUNK, 16);
+            uint32_t x = desc_low(base + QC * HELD_CHUNK, 16), y = desc_low(rows + QC * STEP_CHUNK, 16);
 #pragma unroll 1
             for (int c = 0; c < VC; ++c) {
                 umma_f16_chunk(DP + buf * 64, x, y, i_s, c != 0, min(4, value_steps - 4 * c));
@@ -175,19 +174,22 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
         tcgen05_fence_after();
         if (ok) {
             if (elect_one()) {
-                scores(0);
-                grads(0);
+                scores(0, ring);
+                grads(0, ring);
             }
             __syncwarp();
         }
+        int slot = 0, next = NS == 1 ? 0 : 1;                    // stages of tiles j and j + 1
+        uint32_t next_phase = NS == 1 ? 1u : 0u;
         for (int j = 0; j < n && ok; ++j) {
+            const uint32_t rows = ring + slot * stage_bytes, next_rows = ring + next * stage_bytes;
             if (j + 1 < n) {
-                ok = mbar_wait_warp(full((j + 1) % NS), (uint32_t)((j + 1) / NS) & 1u, status, 4);
+                ok = mbar_wait_warp(full(next), next_phase, status, 4);
                 tcgen05_fence_after();
                 if (!ok) break;
                 if (elect_one()) {
-                    scores(j + 1);
-                    if (DP_BUFFERS == 2) grads(j + 1);
+                    scores(j + 1, next_rows);
+                    if (DP_BUFFERS == 2) grads(j + 1, next_rows);
                 }
                 __syncwarp();
             }
@@ -195,7 +197,7 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
                 ok = mbar_wait_warp(p_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 5);
                 tcgen05_fence_after();
                 if (!ok) break;
-                if (elect_one()) sums(ACC2, S + (j & 1) * 64, stage(j) + QC * STEP_CHUNK, i_v, j != 0);
+                if (elect_one()) sums(ACC2, S + (j & 1) * 64, rows + QC * STEP_CHUNK, i_v, j != 0);
                 __syncwarp();
             }
             ok = mbar_wait_warp(ds_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6);
@@ -203,13 +205,18 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
             if (!ok) break;
             if (elect_one()) {
                 const uint32_t f = DP + (DP_BUFFERS == 2 ? j & 1 : 0) * 64;
-                sums(ACC1, f, stage(j), i_1, j != 0);
-                if (!joined) sums(ACC1 + D, f, stage(j) + plan.key_chunks * STEP_CHUNK, i_r, j != 0);
-                umma_commit(empty(j % NS));
-                if (DP_BUFFERS == 1 && j + 1 < n) grads(j + 1);
+                sums(ACC1, f, rows, i_1, j != 0);
+                if (!joined) sums(ACC1 + D, f, rows + plan.key_chunks * STEP_CHUNK, i_r, j != 0);
+                umma_commit(empty(slot));
+                if (DP_BUFFERS == 1 && j + 1 < n) grads(j + 1, next_rows);
                 if (j + 1 == n) umma_commit(done);
             }
             __syncwarp();
+            slot = next;
+            if (++next == NS) {
+                next = 0;
+                next_phase ^= 1u;
+            }
         }
     } else {
         // ================= probabilities and their gradients =================
@@ -230,17 +237,19 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
             if (!KEYS && last > seq.keys) last = seq.keys;
         }
         bool ok = true;
+        int slot = 0;
+        uint32_t phase = 0;
         for (int j = 0; j < n; ++j) {
             const int c0 = begin + j * STEP + cols, buf = j & 1, dbuf = DP_BUFFERS == 2 ? buf : 0;
             const uint32_t dph = DP_BUFFERS == 2 ? (uint32_t)(j >> 1) & 1u : (uint32_t)j & 1u;
-            const float* st = stats_gen + (j % NS) * 2 * STEP + cols;
+            const float* st = stats_gen + slot * 2 * STEP + cols;
             if (!(ok = mbar_wait_warp(s_full(buf), (uint32_t)(j >> 1) & 1u, status, 7))) break;
             tcgen05_fence_after();
             uint32_t s[32], w[16];
             tmem_ld32(S + buf * 64 + lanes + cols, s);
             tmem_ld_wait();
             // what a bulk copy brought is visible to who has waited for it: a phase that the product's issuer has already seen
-            if (KEYS && !(ok = mbar_wait_warp(full(j % NS), (uint32_t)(j / NS) & 1u, status, 8))) break;
+            if (KEYS && !(ok = mbar_wait_warp(full(slot), phase, status, 8))) break;
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
                 float4 l = make_float4(lse, lse, lse, lse);
@@ -296,6 +305,10 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(ds_full(buf));
+            if (++slot == NS) {
+                slot = 0;
+                phase ^= 1u;
+            }
         }
         if (ok && n > 0) ok = mbar_wait_warp(done, 0, status, 10);
         tcgen05_fence_after();
