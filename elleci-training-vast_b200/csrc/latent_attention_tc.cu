@@ -45,7 +45,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     auto p_full = [&](int i) { return bars + 8u * (4 + i); };
     auto o_full = [&](int i) { return bars + 8u * (6 + i); };
     const uint32_t landed = bars + 8u * 8;
-    auto slot_full = [&](int s) { return bars + 8u * (9 + s); };
+    auto slot_full = [&](int s) { return bars + 8u * (9 + s); };          // of the chunks of one tile, at its first chunk's slot
     auto slot_empty = [&](int s) { return bars + 8u * (9 + MAX_SLOTS + s); };
     volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * CHUNK + 8 * (9 + 2 * MAX_SLOTS));
 
@@ -101,12 +101,15 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             // values behind the sequence's end may be anything, and zero times anything is not always zero: those rows are cleared
             const int live = seq.keys - j * TILE;
             const bool clear = live < TILE && j * TILE + live < a.keys;
+            int head = 0;
             for (int c = 0; c < QC + VC; ++c) {
                 if (!mbar_wait_warp(slot_empty(s), ph ^ 1u, status, 1)) { ok = false; break; }
                 const bool value = c >= QC, late = value && clear;
+                if (c == 0 || c == QC) head = s;
                 if (elect_one()) {
-                    const uint32_t dst = ring + s * CHUNK, bar = late ? landed : slot_full(s);
-                    mbar_expect_tx(bar, CHUNK);
+                    const uint32_t dst = ring + s * CHUNK, bar = late ? landed : slot_full(head);
+                    if (late) mbar_expect_tx(bar, CHUNK);
+                    else if (s == head) mbar_expect_tx(bar, (value ? VC : QC) * CHUNK);
                     if (value) tma_load_3d(dst, &tmV, bar, (int)(h * a.v_stride_h) + (c - QC) * CHUNK_COLS, j * TILE, b);
                     else if (c < plan.key_chunks) tma_load_3d(dst, &tmK, bar, (int)(h * a.k_stride_h) + c * CHUNK_COLS, j * TILE, b);
                     else tma_load_3d(dst, &tmKr, bar, 0, j * TILE, b);
@@ -119,7 +122,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     for (int k = live * 8 + lane; k < TILE * 8; k += 32) rows[k] = make_uint4(0u, 0u, 0u, 0u);
                     fence_async_smem();
                     __syncwarp();
-                    if (elect_one()) mbar_arrive(slot_full(s));
+                    if (c + 1 == QC + VC && elect_one()) mbar_arrive(slot_full(head));
                     __syncwarp();
                 }
                 if (++s == NS) { s = 0; ph ^= 1u; }
@@ -130,30 +133,21 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const uint32_t i_s = idesc_f16<T>(0, 0, TILE);
         const int key_steps = a.key_dim / 16, rot_steps = a.rot_dim / 16, V = a.value_dim;
         bool ok = true;
-        // a place in the ring, which chunks go through in order (counted, not divided: a division costs more than a product)
-        struct At {
-            int slot;
-            uint32_t phase;
-        };
-        auto after = [&](At x, int count) {
-            x.slot += count;
-            if (x.slot >= NS) {
-                x.slot -= NS;
-                x.phase ^= 1u;
-            }
-            return x;
-        };
-        auto wait_chunks = [&](At x, int count) {
-            for (int c = 0; c < count && ok; ++c, x = after(x, 1)) ok = mbar_wait_warp(slot_full(x.slot), x.phase, status, 3);
+        // A place in the ring, which chunks go through in order (counted, not divided: a division costs more than a product).
+        auto after = [&](int slot, int count) { return slot + count >= NS ? slot + count - NS : slot + count; };
+        uint32_t phases = 0;                                    // bit s: parity of slot s' next tile
+        auto wait_tile = [&](int slot) {
+            ok = ok && mbar_wait_warp(slot_full(slot), (phases >> slot) & 1u, status, 3);
+            phases ^= 1u << slot;
             tcgen05_fence_after();
         };
-        auto release = [&](At x, int count) {
+        auto release = [&](int slot, int count) {
 #pragma unroll 1
-            for (int c = 0; c < count; ++c, x = after(x, 1)) umma_commit(slot_empty(x.slot));
+            for (int c = 0; c < count; ++c, slot = after(slot, 1)) umma_commit(slot_empty(slot));
         };
-        auto scores = [&](int i, At first) {                    // S_i = Q_i K'; one thread
+        auto scores = [&](int i, int first) {                   // S_i = Q_i K'; one thread
             uint32_t q = desc_low(base + i * QC * CHUNK, 16);
-            int slot = first.slot;
+            int slot = first;
 #pragma unroll 1
             for (int c = 0; c < QC; ++c) {
                 umma_f16_chunk(S + i * 128, q, desc_low(ring + slot * CHUNK, 16), i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
@@ -162,8 +156,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             umma_commit(s_full(i));
         };
-        auto values = [&](int i, At first, bool more) {         // O_i += P_i V; one thread
-            const int s0 = first.slot, parts = VC == 1 || s0 + 1 < NS ? 1 : 2;             // the chunks lie side by side, or the ring's end is between them
+        auto values = [&](int i, int first, bool more) {        // O_i += P_i V; one thread
+            const int s0 = first, parts = VC == 1 || s0 + 1 < NS ? 1 : 2;             // the chunks lie side by side, or the ring's end is between them
 #pragma unroll 1
             for (int c = 0; c < parts; ++c) {
                 const uint32_t id = idesc_f16<T>(0, 1, parts == 1 ? V : c == 0 ? 64 : V - 64), v = desc_low(ring + (c == 0 ? s0 : 0) * CHUNK, CHUNK);
@@ -174,45 +168,51 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             umma_commit(o_full(i));
         };
-        const At begin{0, 0};
-        At v = after(begin, QC);
+        const int only = n0 == 0 ? 1 : 0;                       // the tile that waits for what both need: the first that there is
+        int v = QC;
         if (n > 0) {
             for (int i = 0; i < 2; ++i) {
                 if ((i == 0 ? n0 : n1) == 0) continue;
                 ok = ok && mbar_wait_warp(q_full(i), 0, status, 4);
-                wait_chunks(begin, QC);
+                if (i == only) wait_tile(0);
                 if (!ok) break;
-                if (elect_one()) scores(i, begin);
+                if (elect_one()) scores(i, 0);
                 __syncwarp();
             }
             if (ok) {
-                if (elect_one()) release(begin, QC);
+                if (elect_one()) release(0, QC);
                 __syncwarp();
             }
         }
         for (int j = 0; j < n && ok; ++j) {
-            const At k = after(v, VC);
+            const int k = after(v, VC);
+            bool have_v = false, have_k = false;
             for (int i = 0; i < 2; ++i) {
                 const int mine = i == 0 ? n0 : n1;
                 if (j >= mine) continue;
+                const bool last = i == 1 || j >= n1;            // nothing else reads the values; nor the next keys, if the other tile has no more
+                const bool last_k = i == 1 || j + 1 >= n1;
+                if (!have_v) wait_tile(v);
+                have_v = true;
                 ok = ok && mbar_wait_warp(p_full(i), (uint32_t)j & 1u, status, 5);
-                if (ok) wait_chunks(v, VC);
+                tcgen05_fence_after();
                 if (!ok) break;
-                if (elect_one()) values(i, v, j != 0);
+                if (elect_one()) {
+                    values(i, v, j != 0);
+                    if (last) release(v, VC);
+                }
                 __syncwarp();
                 if (j + 1 < mine) {
-                    wait_chunks(k, QC);
+                    if (!have_k) wait_tile(k);
+                    have_k = true;
                     if (!ok) break;
-                    if (elect_one()) scores(i, k);
+                    if (elect_one()) {
+                        scores(i, k);
+                        if (last_k) release(k, QC);
+                    }
                     __syncwarp();
                 }
             }
-            if (!ok) break;
-            if (elect_one()) {
-                release(v, VC);
-                if (j + 1 < n) release(k, QC);
-            }
-            __syncwarp();
             v = after(k, QC);
         }
     } else {
