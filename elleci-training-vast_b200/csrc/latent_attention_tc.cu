@@ -7,6 +7,8 @@
 //                  values over S_i, where it is the left factor of
 //   O_i += P_i V   whose sums stay in tensor memory.  The reference of a row follows its maximum only when that has grown by more than 2^8:
 //                  then the row of O_i is scaled.  P stays below 2^8, sums are float32.
+// As many blocks as SMs, which take every so many-th item (a pair of tiles of one head), the longest first: while a block's threads write an item's output, its
+// next item's queries and keys are on their way and their first products run.
 // Order of products: P_0 V, S_0 of the next keys, P_1 V, S_1 of the next keys.  Keys and values go through one ring of 16 KB chunks in the order in
 // which they are first used.
 #include "latent_tc.cuh"
@@ -21,7 +23,8 @@ namespace {
 constexpr int TILE = 128;                       // rows of a query tile, and keys of a tile
 constexpr int CHUNK = TILE * 128;               // bytes of 64 columns of a tile
 constexpr int MAX_SLOTS = 12;
-constexpr int WARP_MMA = 8, WARP_TMA = 9, THREADS = 320;
+constexpr int WARP_MMA = 8, WARP_TMA = 9, THREADS = 384;        // (warps 10 and 11 fill a group of four, for the split of registers)
+constexpr int REGS_SOFTMAX = 216, REGS_OTHER = 64;              // 256 x 216 + 128 x 64 of the launch's 384 x 168
 constexpr float GROWTH = 8.0f;                  // exponent of 2 by which a row's maximum may outgrow its reference
 
 struct Plan {
@@ -47,21 +50,36 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const uint32_t landed = bars + 8u * 8;
     auto slot_full = [&](int s) { return bars + 8u * (9 + s); };          // of the chunks of one tile, at its first chunk's slot
     auto slot_empty = [&](int s) { return bars + 8u * (9 + MAX_SLOTS + s); };
-    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * CHUNK + 8 * (9 + 2 * MAX_SLOTS));
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * CHUNK + 8 * (11 + 2 * MAX_SLOTS));
 
+    const uint32_t q_empty = slot_empty(MAX_SLOTS);             // two
     const int warp = warp_index(), lane = threadIdx.x & 31;
-    const Place at(a);
-    const int pairs = (a.length + 2 * TILE - 1) / (2 * TILE), b = at.batch, h = at.head;
-    const int i0 = (pairs - 1 - at.tile) * 2 * TILE;            // the longest rows first
-    const Sequence seq(a, b);
-    // key tiles of the two query tiles
-    const int n0 = uniform(i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0);
-    const int n1 = uniform(i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0);
-    const int n = n0 > n1 ? n0 : n1;
+    const int pairs = (a.length + 2 * TILE - 1) / (2 * TILE);
+    const unsigned items = (unsigned)pairs * a.batch * a.heads;
+    int32_t* status = a.dev_status;
+    // an item: its queries, and the key tiles of its two query tiles
+    struct Item {
+        int b, h, i0, n0, n1, n;
+        Sequence seq;
+        __device__ __forceinline__ Item(const el_attention_t& a, unsigned item, int pairs) : Item(a, Place(a, item), pairs) {}
+        __device__ __forceinline__ Item(const el_attention_t& a, const Place& at, int pairs) : b(at.batch), h(at.head), i0((pairs - 1 - at.tile) * 2 * TILE), seq(a, at.batch) {
+            n0 = uniform(i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0);
+            n1 = uniform(i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0);
+            n = n0 > n1 ? n0 : n1;
+        }
+    };
 
-    if (threadIdx.x == 0) {
+    if (warp == WARP_TMA && elect_one()) {
+        prefetch_map(&tmQ);
+        prefetch_map(&tmK);
+        prefetch_map(&tmV);
+        if (plan.rot_chunks) {
+            prefetch_map(&tmQr);
+            prefetch_map(&tmKr);
+        }
         for (int i = 0; i < 2; ++i) {
             mbar_init(q_full(i), 1);
+            mbar_init(q_empty + 8u * i, 1);
             mbar_init(s_full(i), 1);
             mbar_init(p_full(i), 4);
             mbar_init(o_full(i), 1);
@@ -80,54 +98,60 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tcgen05_fence_after();
     const uint32_t tmem = uniform(*tmem_holder);
     const uint32_t S = tmem, O = tmem + 256;                    // S_i at 128 i, O_i at 256 + 128 i
-    int32_t* status = a.dev_status;
 
+    if (warp >= WARP_MMA) fewer_registers<REGS_OTHER>();
     if (warp == WARP_TMA) {
         // ================= loads =================
-        for (int i = 0; i < 2; ++i) {
-            if ((i == 0 ? n0 : n1) == 0) continue;
-            if (elect_one()) {
-                mbar_expect_tx(q_full(i), QC * CHUNK);
-                for (int c = 0; c < plan.key_chunks; ++c)
-                    tma_load_3d(base + (i * QC + c) * CHUNK, &tmQ, q_full(i), (int)(h * a.q_stride_h) + c * CHUNK_COLS, i0 + i * TILE, b);
-                if (plan.rot_chunks) tma_load_3d(base + (i * QC + plan.key_chunks) * CHUNK, &tmQr, q_full(i), (int)(h * a.q_rot_stride_h), i0 + i * TILE, b);
-            }
-            __syncwarp();
-        }
         int s = 0;
-        uint32_t ph = 0, land = 0;
+        uint32_t ph = 0, land = 0, q_phase[2] = {1u, 1u};
         bool ok = true;
-        for (int j = 0; j < n && ok; ++j) {
-            // values behind the sequence's end may be anything, and zero times anything is not always zero: those rows are cleared
-            const int live = seq.keys - j * TILE;
-            const bool clear = live < TILE && j * TILE + live < a.keys;
-            int head = 0;
-            for (int c = 0; c < QC + VC; ++c) {
-                if (!mbar_wait_warp(slot_empty(s), ph ^ 1u, status, 1)) { ok = false; break; }
-                const bool value = c >= QC, late = value && clear;
-                if (c == 0 || c == QC) head = s;
+        each_item(items, [&](unsigned item) {
+            const Item it(a, item, pairs);
+            for (int i = 0; i < 2 && ok; ++i) {
+                if ((i == 0 ? it.n0 : it.n1) == 0) continue;
+                if (!mbar_wait_warp(q_empty + 8u * i, q_phase[i], status, 1)) { ok = false; break; }
+                q_phase[i] ^= 1u;
                 if (elect_one()) {
-                    const uint32_t dst = ring + s * CHUNK, bar = late ? landed : slot_full(head);
-                    if (late) mbar_expect_tx(bar, CHUNK);
-                    else if (s == head) mbar_expect_tx(bar, (value ? VC : QC) * CHUNK);
-                    if (value) tma_load_3d(dst, &tmV, bar, (int)(h * a.v_stride_h) + (c - QC) * CHUNK_COLS, j * TILE, b);
-                    else if (c < plan.key_chunks) tma_load_3d(dst, &tmK, bar, (int)(h * a.k_stride_h) + c * CHUNK_COLS, j * TILE, b);
-                    else tma_load_3d(dst, &tmKr, bar, 0, j * TILE, b);
+                    mbar_expect_tx(q_full(i), QC * CHUNK);
+                    for (int c = 0; c < plan.key_chunks; ++c)
+                        tma_load_3d(base + (i * QC + c) * CHUNK, &tmQ, q_full(i), (int)(it.h * a.q_stride_h) + c * CHUNK_COLS, it.i0 + i * TILE, it.b);
+                    if (plan.rot_chunks) tma_load_3d(base + (i * QC + plan.key_chunks) * CHUNK, &tmQr, q_full(i), (int)(it.h * a.q_rot_stride_h), it.i0 + i * TILE, it.b);
                 }
                 __syncwarp();
-                if (late) {
-                    if (!mbar_wait_warp(landed, land, status, 2)) { ok = false; break; }
-                    land ^= 1u;
-                    uint4* rows = reinterpret_cast<uint4*>(ring_gen + s * CHUNK);
-                    for (int k = live * 8 + lane; k < TILE * 8; k += 32) rows[k] = make_uint4(0u, 0u, 0u, 0u);
-                    fence_async_smem();
-                    __syncwarp();
-                    if (c + 1 == QC + VC && elect_one()) mbar_arrive(slot_full(head));
-                    __syncwarp();
-                }
-                if (++s == NS) { s = 0; ph ^= 1u; }
             }
-        }
+            for (int j = 0; j < it.n && ok; ++j) {
+                // values behind the sequence's end may be anything, and zero times anything is not always zero: those rows are cleared
+                const int live = it.seq.keys - j * TILE;
+                const bool clear = live < TILE && j * TILE + live < a.keys;
+                int head = 0;
+                for (int c = 0; c < QC + VC; ++c) {
+                    if (!mbar_wait_warp(slot_empty(s), ph ^ 1u, status, 1)) { ok = false; break; }
+                    const bool value = c >= QC, late = value && clear;
+                    if (c == 0 || c == QC) head = s;
+                    if (elect_one()) {
+                        const uint32_t dst = ring + s * CHUNK, bar = late ? landed : slot_full(head);
+                        if (late) mbar_expect_tx(bar, CHUNK);
+                        else if (s == head) mbar_expect_tx(bar, (value ? VC : QC) * CHUNK);
+                        if (value) tma_load_3d(dst, &tmV, bar, (int)(it.h * a.v_stride_h) + (c - QC) * CHUNK_COLS, j * TILE, it.b);
+                        else if (c < plan.key_chunks) tma_load_3d(dst, &tmK, bar, (int)(it.h * a.k_stride_h) + c * CHUNK_COLS, j * TILE, it.b);
+                        else tma_load_3d(dst, &tmKr, bar, 0, j * TILE, it.b);
+                    }
+                    __syncwarp();
+                    if (late) {
+                        if (!mbar_wait_warp(landed, land, status, 2)) { ok = false; break; }
+                        land ^= 1u;
+                        uint4* rows = reinterpret_cast<uint4*>(ring_gen + s * CHUNK);
+                        for (int k = live * 8 + lane; k < TILE * 8; k += 32) rows[k] = make_uint4(0u, 0u, 0u, 0u);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (c + 1 == QC + VC && elect_one()) mbar_arrive(slot_full(head));
+                        __syncwarp();
+                    }
+                    if (++s == NS) { s = 0; ph ^= 1u; }
+                }
+            }
+            return ok;
+        });
     } else if (warp == WARP_MMA) {
         // ================= products =================
         const uint32_t i_s = idesc_f16<T>(0, 0, TILE);
@@ -168,154 +192,176 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             umma_commit(o_full(i));
         };
-        const int only = n0 == 0 ? 1 : 0;                       // the tile that waits for what both need: the first that there is
-        int v = QC;
-        if (n > 0) {
+        int place = 0;                                          // of the next tile of keys or values
+        uint32_t q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};
+        each_item(items, [&](unsigned item) {
+            const Item it(a, item, pairs);
+            if (it.n == 0) return true;
+            const int only = it.n0 == 0 ? 1 : 0;                // the tile that waits for what both need: the first that there is
             for (int i = 0; i < 2; ++i) {
-                if ((i == 0 ? n0 : n1) == 0) continue;
-                ok = ok && mbar_wait_warp(q_full(i), 0, status, 4);
-                if (i == only) wait_tile(0);
-                if (!ok) break;
-                if (elect_one()) scores(i, 0);
-                __syncwarp();
-            }
-            if (ok) {
-                if (elect_one()) release(0, QC);
-                __syncwarp();
-            }
-        }
-        for (int j = 0; j < n && ok; ++j) {
-            const int k = after(v, VC);
-            bool have_v = false, have_k = false;
-            for (int i = 0; i < 2; ++i) {
-                const int mine = i == 0 ? n0 : n1;
-                if (j >= mine) continue;
-                const bool last = i == 1 || j >= n1;            // nothing else reads the values; nor the next keys, if the other tile has no more
-                const bool last_k = i == 1 || j + 1 >= n1;
-                if (!have_v) wait_tile(v);
-                have_v = true;
-                ok = ok && mbar_wait_warp(p_full(i), (uint32_t)j & 1u, status, 5);
-                tcgen05_fence_after();
+                const int mine = i == 0 ? it.n0 : it.n1;
+                if (mine == 0) continue;
+                ok = ok && mbar_wait_warp(q_full(i), q_phase[i], status, 4);
+                q_phase[i] ^= 1u;
+                if (i == only) wait_tile(place);
                 if (!ok) break;
                 if (elect_one()) {
-                    values(i, v, j != 0);
-                    if (last) release(v, VC);
+                    scores(i, place);
+                    if (mine == 1) umma_commit(q_empty + 8u * i);
+                    if (i == 1 || it.n1 == 0) release(place, QC);
                 }
                 __syncwarp();
-                if (j + 1 < mine) {
-                    if (!have_k) wait_tile(k);
-                    have_k = true;
+            }
+            int v = after(place, QC);
+            for (int j = 0; j < it.n && ok; ++j) {
+                const int k = after(v, VC);
+                bool have_v = false, have_k = false;
+                for (int i = 0; i < 2; ++i) {
+                    const int mine = i == 0 ? it.n0 : it.n1;
+                    if (j >= mine) continue;
+                    const bool last = i == 1 || j >= it.n1;     // nothing else reads the values; nor the next keys, if the other tile has no more
+                    const bool last_k = i == 1 || j + 1 >= it.n1;
+                    if (!have_v) wait_tile(v);
+                    have_v = true;
+                    ok = ok && mbar_wait_warp(p_full(i), p_phase[i], status, 5);
+                    p_phase[i] ^= 1u;
+                    tcgen05_fence_after();
                     if (!ok) break;
                     if (elect_one()) {
-                        scores(i, k);
-                        if (last_k) release(k, QC);
+                        values(i, v, j != 0);
+                        if (last) release(v, VC);
                     }
                     __syncwarp();
+                    if (j + 1 < mine) {
+                        if (!have_k) wait_tile(k);
+                        have_k = true;
+                        if (!ok) break;
+                        if (elect_one()) {
+                            scores(i, k);
+                            if (j + 2 == mine) umma_commit(q_empty + 8u * i);
+                            if (last_k) release(k, QC);
+                        }
+                        __syncwarp();
+                    }
                 }
+                place = k;
+                v = after(k, QC);
             }
-            v = after(k, QC);
-        }
-    } else {
+            return ok;
+        });
+    } else if (warp < WARP_MMA) {
         // ================= softmax =================
-        const int i = warp >> 2, mine = i == 0 ? n0 : n1, quarter = warp & 3;
-        const int row = i0 + i * TILE + quarter * 32 + lane;
+        more_registers<REGS_SOFTMAX>();
+        const int i = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = S + i * 128 + lanes, o_addr = O + i * 128 + lanes;
         const float by = a.scale * mamba::LOG2E;
-        // keys that this row sees: 0 .. sees - 1
-        long long sees = row < seq.queries ? row + seq.shift + 1 : 0;
-        sees = sees < 0 ? 0 : sees > seq.keys ? seq.keys : sees;
-        float ref = -INFINITY, sum = 0.0f;
         bool ok = true;
-        for (int j = 0; j < mine; ++j) {
-            if (!(ok = mbar_wait_warp(s_full(i), (uint32_t)j & 1u, status, 6))) break;
-            tcgen05_fence_after();
-            uint32_t v[4][32];
+        uint32_t phase = 0;                                     // of this tile's s_full; o_full of the tile before has the other one
+        each_item(items, [&](unsigned item) {
+            const Item it(a, item, pairs);
+            const int mine = i == 0 ? it.n0 : it.n1, row = it.i0 + i * TILE + quarter * 32 + lane;
+            // keys that this row sees: 0 .. sees - 1
+            long long sees = row < it.seq.queries ? row + it.seq.shift + 1 : 0;
+            sees = sees < 0 ? 0 : sees > it.seq.keys ? it.seq.keys : sees;
+            float ref = -INFINITY, sum = 0.0f;
+            for (int j = 0; j < mine; ++j, phase ^= 1u) {
+                if (!(ok = mbar_wait_warp(s_full(i), phase, status, 6))) break;
+                tcgen05_fence_after();
+                uint32_t v[4][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
-            tmem_ld_wait();
-            const int here = (int)sees - j * TILE;               // columns that the row sees
-            if (__any_sync(0xffffffffu, here < TILE)) {
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
+                tmem_ld_wait();
+                const int here = (int)sees - j * TILE;               // columns that the row sees
+                if (__any_sync(0xffffffffu, here < TILE)) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[c][k] = c * 32 + k < here ? v[c][k] : 0xff800000u;
-            }
-            float top[4];
+                        for (int k = 0; k < 32; ++k) v[c][k] = c * 32 + k < here ? v[c][k] : 0xff800000u;
+                }
+                float top[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                top[c] = __uint_as_float(v[c][0]);
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = __uint_as_float(v[c][0]);
 #pragma unroll
-                for (int k = 1; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(v[c][k]));
-            }
-            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * by;
-            const bool grown = m > ref + GROWTH;                 // also a row's first finite maximum
-            if (__any_sync(0xffffffffu, grown)) {
-                const float to = grown ? m : ref, factor = grown && ref != -INFINITY ? exp2_neg(ref - m) : 1.0f;
-                if (j > 0) {
-                    if (!(ok = mbar_wait_warp(o_full(i), (uint32_t)(j - 1) & 1u, status, 7))) break;
-                    tcgen05_fence_after();
-                    for (int c = 0; c < a.value_dim; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(o_addr + c, o);
-                        tmem_ld_wait();
+                    for (int k = 1; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(v[c][k]));
+                }
+                const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * by;
+                const bool grown = m > ref + GROWTH;                 // also a row's first finite maximum
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float to = grown ? m : ref, factor = grown && ref != -INFINITY ? exp2_neg(ref - m) : 1.0f;
+                    if (j > 0) {
+                        if (!(ok = mbar_wait_warp(o_full(i), phase ^ 1u, status, 7))) break;
+                        tcgen05_fence_after();
+                        for (int c = 0; c < a.value_dim; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + c, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                        tmem_st16(o_addr + c, o);
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                            tmem_st16(o_addr + c, o);
+                        }
+                        tmem_st_wait();
                     }
-                    tmem_st_wait();
+                    sum *= factor;
+                    ref = to;
                 }
-                sum *= factor;
-                ref = to;
-            }
-            const float from = ref == -INFINITY ? 0.0f : -ref;
-            const rowio::f32x2 by2 = rowio::pair(by, by), from2 = rowio::pair(from, from);
-            rowio::f32x2 part[4];
+                const float from = ref == -INFINITY ? 0.0f : -ref;
+                const rowio::f32x2 by2 = rowio::pair(by, by), from2 = rowio::pair(from, from);
+                rowio::f32x2 part[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) part[c] = rowio::pair(0.0f, 0.0f);
+                for (int c = 0; c < 4; ++c) part[c] = rowio::pair(0.0f, 0.0f);
 #pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-                uint32_t p[32];
+                for (int c = 0; c < 4; c += 2) {
+                    uint32_t p[32];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    const int e = 2 * k, cc = c + e / 32;
-                    const rowio::f32x2 x = rowio::fma2(rowio::pair(__uint_as_float(v[cc][e % 32]), __uint_as_float(v[cc][e % 32 + 1])), by2, from2);
-                    const float y0 = mamba::ex2(rowio::lo_of(x)), y1 = mamba::ex2(rowio::hi_of(x));
-                    part[k & 3] = rowio::add2(part[k & 3], rowio::pair(y0, y1));
-                    p[k] = pack_word<T>(y0, y1);
+                    for (int k = 0; k < 32; ++k) {
+                        const int e = 2 * k, cc = c + e / 32;
+                        const rowio::f32x2 x = rowio::fma2(rowio::pair(__uint_as_float(v[cc][e % 32]), __uint_as_float(v[cc][e % 32 + 1])), by2, from2);
+                        const float y0 = mamba::ex2(rowio::lo_of(x)), y1 = mamba::ex2(rowio::hi_of(x));
+                        part[k & 3] = rowio::add2(part[k & 3], rowio::pair(y0, y1));
+                        p[k] = pack_word<T>(y0, y1);
+                    }
+                    tmem_st32(s_addr + c * 16, p);
                 }
-                tmem_st32(s_addr + c * 16, p);
+                const rowio::f32x2 t = rowio::add2(rowio::add2(part[0], part[1]), rowio::add2(part[2], part[3]));
+                sum += rowio::lo_of(t) + rowio::hi_of(t);
+                tmem_st_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(i));
             }
-            const rowio::f32x2 t = rowio::add2(rowio::add2(part[0], part[1]), rowio::add2(part[2], part[3]));
-            sum += rowio::lo_of(t) + rowio::hi_of(t);
-            tmem_st_wait();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(i));
-        }
-        const bool empty = ref == -INFINITY && !(sum != sum);    // sees nothing; a NaN is no such row
-        const float inv = 1.0f / sum;
-        if (a.lse && row < lse_pitch(a.length))
-            a.lse[((long long)b * a.heads + h) * lse_pitch(a.length) + row] = empty ? INFINITY : ref + log2f(sum);
-        if (ok && mine > 0) ok = mbar_wait_warp(o_full(i), (uint32_t)(mine - 1) & 1u, status, 8);
-        tcgen05_fence_after();
-        if (ok) {
-            T* out = static_cast<T*>(a.out) + (((long long)b * a.length + row) * a.heads + h) * a.value_dim;
-            for (int c = 0; c < a.value_dim; c += 16) {
-                uint32_t o[16], w[8];
+            const bool empty = ref == -INFINITY && !(sum != sum);    // sees nothing; a NaN is no such row
+            const float inv = 1.0f / sum;
+            if (a.lse && row < lse_pitch(a.length))
+                a.lse[((long long)it.b * a.heads + it.h) * lse_pitch(a.length) + row] = empty ? INFINITY : ref + log2f(sum);
+            if (ok && mine > 0) ok = mbar_wait_warp(o_full(i), phase ^ 1u, status, 8);
+            if (!ok) return false;
+            tcgen05_fence_after();
+            // four lanes share the stores of their four rows
+            const int first = row & ~3;
+            T* out = static_cast<T*>(a.out) + (((long long)it.b * a.length + first) * a.heads + it.h) * a.value_dim + (lane & 3) * 8;
+            for (int c = 0; c < a.value_dim; c += 32) {
+                uint32_t o[32], w[16];
                 if (mine > 0) {
-                    tmem_ld16(o_addr + c, o);
+                    tmem_ld32(o_addr + c, o);
                     tmem_ld_wait();
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < 16; ++k)
                     w[k] = mine == 0 || empty ? 0u : pack_word<T>(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
-                if (row < a.length) {
-                    *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                transpose_rows(w);
+                if (c + (lane & 3) * 8 < a.value_dim) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (first + k < a.length)
+                            *reinterpret_cast<uint4*>(out + (long long)k * a.heads * a.value_dim + c) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
                 }
+                __syncwarp();
             }
-        }
+            tcgen05_fence_before();                             // the sums have been read: the next item's first product with values waits for these warps' factors
+            return true;
+        });
     }
     if (status != nullptr && *reinterpret_cast<volatile int32_t*>(status) != 0) {
         // a wait gave up somewhere: copies and products still in flight get time to land before their memory is released
@@ -339,7 +385,7 @@ Plan plan_of(const el_attention_t& a) {
     p.slots = room < MAX_SLOTS ? room : MAX_SLOTS;
     return p;
 }
-int shared_bytes(const Plan& p) { return 1024 + (2 * (p.key_chunks + p.rot_chunks) + p.slots) * CHUNK + 8 * (9 + 2 * MAX_SLOTS) + 16; }
+int shared_bytes(const Plan& p) { return 1024 + (2 * (p.key_chunks + p.rot_chunks) + p.slots) * CHUNK + 8 * (11 + 2 * MAX_SLOTS) + 16; }
 
 bool map_takes(const void* base, long long stride_b, long long stride_t, long long stride_h, int heads) {
     return stride_h >= 0 && (heads - 1) * stride_h < (1LL << 30) && reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride_b % 8 == 0 && stride_t % 8 == 0 && stride_h % 8 == 0;
@@ -353,7 +399,10 @@ template <typename T> int launch(const el_attention_t& a, const Plan& plan, cons
         EL_CUDA_TRY(cudaFuncSetAttribute(attention_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         once.mark(dev);
     }
-    attention_tc_kernel<T><<<blocks_of(a, a.length, 2 * TILE), THREADS, shared_bytes(plan), st>>>(m[0], m[1], m[2], m[3], m[4], a, plan);
+    int sms = 148;
+    device_sm_count(&sms);
+    const unsigned items = blocks_of(a, a.length, 2 * TILE);
+    attention_tc_kernel<T><<<items < (unsigned)sms ? items : sms, THREADS, shared_bytes(plan), st>>>(m[0], m[1], m[2], m[3], m[4], a, plan);
     return check_launch();
 }
 

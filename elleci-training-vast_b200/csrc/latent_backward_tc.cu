@@ -8,7 +8,8 @@
 //
 // Warps 0-7: a thread owns a row and half of a tile's columns; it forms p = 2^(s - lse) and ds = p (dp - delta) and writes both over S and dP as 16-bit
 // left factors.  The softmax scale is applied to the sums, so that ds, rounded, is not smaller than it has to be.  Warp 8 issues the products, 9 the loads.
-// While the threads work on a tile, the tensor core forms the next S (and dP, where tensor memory has room for two of them).
+// While the threads work on a tile, the tensor core forms the next S (and dP, where tensor memory has room for two of them).  As many blocks as SMs, which
+// take every so many-th item (128 rows of one head), the longest first; the next item's matrices load while a block finishes one.
 #include "latent_tc.cuh"
 
 namespace el {
@@ -43,32 +44,49 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
     const uint32_t ring = base + held_bytes, stats = ring + NS * stage_bytes, bars = stats + NS * 2 * STEP * 4;
     uint8_t* ring_gen = gen + held_bytes;
     const float* stats_gen = reinterpret_cast<const float*>(ring_gen + NS * stage_bytes);
-    const uint32_t a_full = bars, landed = bars + 8, done = bars + 16;
-    auto s_full = [&](int i) { return bars + 8u * (3 + i); };
-    auto dp_full = [&](int i) { return bars + 8u * (5 + i); };
-    auto p_full = [&](int i) { return bars + 8u * (7 + i); };
-    auto ds_full = [&](int i) { return bars + 8u * (9 + i); };
-    auto full = [&](int s) { return bars + 8u * (11 + s); };
-    auto empty = [&](int s) { return bars + 8u * (11 + MAX_STAGES + s); };
-    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * (stage_bytes + 2 * STEP * 4) + 8 * (11 + 2 * MAX_STAGES));
+    const uint32_t a_full = bars, a_empty = bars + 8, landed = bars + 16, done = bars + 24;
+    auto s_full = [&](int i) { return bars + 8u * (4 + i); };
+    auto dp_full = [&](int i) { return bars + 8u * (6 + i); };
+    auto p_full = [&](int i) { return bars + 8u * (8 + i); };
+    auto ds_full = [&](int i) { return bars + 8u * (10 + i); };
+    auto full = [&](int s) { return bars + 8u * (12 + s); };
+    auto empty = [&](int s) { return bars + 8u * (12 + MAX_STAGES + s); };
+    volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(ring_gen + NS * (stage_bytes + 2 * STEP * 4) + 8 * (12 + 2 * MAX_STAGES));
 
     const int warp = warp_index(), lane = threadIdx.x & 31;
-    const Place at(a);
     const int all = KEYS ? a.keys : a.length, other = KEYS ? a.length : a.keys, tiles = (all + HELD - 1) / HELD;
-    const int b = at.batch, h = at.head, r0 = (KEYS ? at.tile : tiles - 1 - at.tile) * HELD;     // the longest rows first
-    const Sequence seq(a, b);
-    const int live = KEYS ? seq.keys : seq.queries, other_live = KEYS ? seq.queries : seq.keys;
-    int begin = 0, end = 0;
-    if (r0 < live) {
-        begin = KEYS ? seq.query_begin(r0) / STEP * STEP : 0;
-        end = KEYS ? seq.queries : seq.key_end(r0 + HELD);
-    }
-    begin = uniform(begin);
-    const int n = uniform(end > begin ? (end - begin + STEP - 1) / STEP : 0);
-    const long long stat_row = ((long long)b * a.heads + h) * lse_pitch(a.length);
+    const unsigned items = (unsigned)tiles * a.batch * a.heads;
+    int32_t* status = a.dev_status;
+    // an item: its rows, and the tiles of the other side that they meet
+    struct Item {
+        int b, h, r0, live, other_live, begin, n;
+        Sequence seq;
+        __device__ __forceinline__ Item(const el_attention_t& a, unsigned item, int tiles) : Item(a, Place(a, item), tiles) {}
+        __device__ __forceinline__ Item(const el_attention_t& a, const Place& at, int tiles) : b(at.batch), h(at.head), r0((KEYS ? at.tile : tiles - 1 - at.tile) * HELD), seq(a, at.batch) {
+            live = KEYS ? seq.keys : seq.queries;
+            other_live = KEYS ? seq.queries : seq.keys;
+            int first = 0, end = 0;
+            if (r0 < live) {
+                first = KEYS ? seq.query_begin(r0) / STEP * STEP : 0;
+                end = KEYS ? seq.queries : seq.key_end(r0 + HELD);
+            }
+            begin = uniform(first);
+            n = uniform(end > first ? (end - first + STEP - 1) / STEP : 0);
+        }
+        __device__ __forceinline__ long long stat_row(const el_attention_t& a) const { return ((long long)b * a.heads + h) * lse_pitch(a.length); }
+    };
 
-    if (threadIdx.x == 0) {
+    if (warp == WARP_TMA && elect_one()) {
+        prefetch_map(&tmA1);
+        prefetch_map(&tmA2);
+        prefetch_map(&tmB1);
+        prefetch_map(&tmB2);
+        if (plan.rot_chunks) {
+            prefetch_map(&tmA1r);
+            prefetch_map(&tmB1r);
+        }
         mbar_init(a_full, 1);
+        mbar_init(a_empty, 1);
         mbar_init(landed, 1);
         mbar_init(done, 1);
         for (int i = 0; i < 2; ++i) {
@@ -90,69 +108,79 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
     tcgen05_fence_after();
     const uint32_t tmem = uniform(*tmem_holder);
     const uint32_t ACC1 = tmem, ACC2 = tmem + 192, S = KEYS ? tmem + 320 : tmem + 192, DP = S + 128;      // S_i at 64 i, dP_i at 64 i
-    int32_t* status = a.dev_status;
 
     if (warp == WARP_TMA) {
         // ================= loads =================
-        const int qh = (int)(h * a.q_stride_h), qrh = (int)(h * a.q_rot_stride_h), kh = (int)(h * a.k_stride_h), vh = (int)(h * a.v_stride_h), gh = (int)(h * a.dout_stride_h);
-        const int x1 = KEYS ? kh : qh, x1r = KEYS ? 0 : qrh, x2 = KEYS ? vh : gh, y1 = KEYS ? qh : kh, y1r = KEYS ? qrh : 0, y2 = KEYS ? gh : vh;
-        if (n > 0 && elect_one()) {
-            mbar_expect_tx(a_full, held_bytes);
-            for (int c = 0; c < plan.key_chunks; ++c) tma_load_3d(base + c * HELD_CHUNK, &tmA1, a_full, x1 + c * CHUNK_COLS, r0, b);
-            if (plan.rot_chunks) tma_load_3d(base + plan.key_chunks * HELD_CHUNK, &tmA1r, a_full, x1r, r0, b);
-            for (int c = 0; c < VC; ++c) tma_load_3d(base + (QC + c) * HELD_CHUNK, &tmA2, a_full, x2 + c * CHUNK_COLS, r0, b);
-        }
-        __syncwarp();
         int s = 0;
-        uint32_t ph = 0;
-        for (int j = 0; j < n; ++j) {
-            if (!mbar_wait_warp(empty(s), ph ^ 1u, status, 1)) break;
-            const int c0 = begin + j * STEP, rows = other_live - c0;
-            // rows behind the sequence's end may be anything, and zero times anything is not always zero: they are cleared
-            const bool late = rows < STEP && c0 + rows < other;
-            const uint32_t dst = ring + s * stage_bytes, bar = late ? landed : full(s);
+        uint32_t ph = 0, land = 0, a_phase = 1;
+        bool ok = true;
+        each_item(items, [&](unsigned item) {
+            const Item it(a, item, tiles);
+            if (it.n == 0) return true;
+            const int b = it.b, h = it.h;
+            const int qh = (int)(h * a.q_stride_h), qrh = (int)(h * a.q_rot_stride_h), kh = (int)(h * a.k_stride_h), vh = (int)(h * a.v_stride_h), gh = (int)(h * a.dout_stride_h);
+            const int x1 = KEYS ? kh : qh, x1r = KEYS ? 0 : qrh, x2 = KEYS ? vh : gh, y1 = KEYS ? qh : kh, y1r = KEYS ? qrh : 0, y2 = KEYS ? gh : vh;
+            if (!(ok = mbar_wait_warp(a_empty, a_phase, status, 1))) return false;
+            a_phase ^= 1u;
             if (elect_one()) {
-                mbar_expect_tx(bar, stage_bytes + (KEYS ? 2 * STEP * 4 : 0));
-                for (int c = 0; c < plan.key_chunks; ++c) tma_load_3d(dst + c * STEP_CHUNK, &tmB1, bar, y1 + c * CHUNK_COLS, c0, b);
-                if (plan.rot_chunks) tma_load_3d(dst + plan.key_chunks * STEP_CHUNK, &tmB1r, bar, y1r, c0, b);
-                for (int c = 0; c < VC; ++c) tma_load_3d(dst + (QC + c) * STEP_CHUNK, &tmB2, bar, y2 + c * CHUNK_COLS, c0, b);
-                if (KEYS) {
-                    bulk_load(stats + s * 2 * STEP * 4, a.lse + stat_row + c0, STEP * 4, bar);
-                    bulk_load(stats + s * 2 * STEP * 4 + STEP * 4, delta + stat_row + c0, STEP * 4, bar);
-                }
+                mbar_expect_tx(a_full, held_bytes);
+                for (int c = 0; c < plan.key_chunks; ++c) tma_load_3d(base + c * HELD_CHUNK, &tmA1, a_full, x1 + c * CHUNK_COLS, it.r0, b);
+                if (plan.rot_chunks) tma_load_3d(base + plan.key_chunks * HELD_CHUNK, &tmA1r, a_full, x1r, it.r0, b);
+                for (int c = 0; c < VC; ++c) tma_load_3d(base + (QC + c) * HELD_CHUNK, &tmA2, a_full, x2 + c * CHUNK_COLS, it.r0, b);
             }
             __syncwarp();
-            if (late) {
-                if (!mbar_wait_warp(landed, 0, status, 2)) break;            // the last tile only
-                for (int c = 0; c < QC + VC; ++c) {
-                    uint4* chunk = reinterpret_cast<uint4*>(ring_gen + s * stage_bytes + c * STEP_CHUNK);
-                    for (int k = rows * 8 + lane; k < STEP * 8; k += 32) chunk[k] = make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < it.n; ++j) {
+                if (!(ok = mbar_wait_warp(empty(s), ph ^ 1u, status, 1))) return false;
+                const int c0 = it.begin + j * STEP, rows = it.other_live - c0;
+                // rows behind the sequence's end may be anything, and zero times anything is not always zero: they are cleared
+                const bool late = rows < STEP && c0 + rows < other;
+                const uint32_t dst = ring + s * stage_bytes, bar = late ? landed : full(s);
+                if (elect_one()) {
+                    mbar_expect_tx(bar, stage_bytes + (KEYS ? 2 * STEP * 4 : 0));
+                    for (int c = 0; c < plan.key_chunks; ++c) tma_load_3d(dst + c * STEP_CHUNK, &tmB1, bar, y1 + c * CHUNK_COLS, c0, b);
+                    if (plan.rot_chunks) tma_load_3d(dst + plan.key_chunks * STEP_CHUNK, &tmB1r, bar, y1r, c0, b);
+                    for (int c = 0; c < VC; ++c) tma_load_3d(dst + (QC + c) * STEP_CHUNK, &tmB2, bar, y2 + c * CHUNK_COLS, c0, b);
+                    if (KEYS) {
+                        bulk_load(stats + s * 2 * STEP * 4, a.lse + it.stat_row(a) + c0, STEP * 4, bar);
+                        bulk_load(stats + s * 2 * STEP * 4 + STEP * 4, delta + it.stat_row(a) + c0, STEP * 4, bar);
+                    }
                 }
-                fence_async_smem();
                 __syncwarp();
-                if (elect_one()) mbar_arrive(full(s));
-                __syncwarp();
+                if (late) {
+                    if (!(ok = mbar_wait_warp(landed, land, status, 2))) return false;
+                    land ^= 1u;
+                    for (int c = 0; c < QC + VC; ++c) {
+                        uint4* chunk = reinterpret_cast<uint4*>(ring_gen + s * stage_bytes + c * STEP_CHUNK);
+                        for (int k = rows * 8 + lane; k < STEP * 8; k += 32) chunk[k] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive(full(s));
+                    __syncwarp();
+                }
+                if (++s == NS) { s = 0; ph ^= 1u; }
             }
-            if (++s == NS) { s = 0; ph ^= 1u; }
-        }
+            return true;
+        });
     } else if (warp == WARP_MMA) {
         // ================= products =================
         const int key_steps = a.key_dim / 16, rot_steps = a.rot_dim / 16, value_steps = a.value_dim / 16, D = a.key_dim, R = a.rot_dim, V = a.value_dim;
         const uint32_t i_s = idesc_f16<T>(0, 0, STEP), i_v = idesc_f16<T>(0, 1, V);
         const bool joined = R == 0 || D % 64 == 0;               // acc1's columns are the chunks' columns, one after another
         const uint32_t i_1 = idesc_f16<T>(0, 1, joined ? D + R : D), i_r = idesc_f16<T>(0, 1, R);
-        auto scores = [&](int j, uint32_t rows) {                // one thread, as the others
+        uint32_t t = 0;                                          // tiles so far: the parities of S, dP and their barriers go by it
+        auto scores = [&](uint32_t t, uint32_t rows) {           // one thread, as the others
             uint32_t x = desc_low(base, 16), y = desc_low(rows, 16);
 #pragma unroll 1
             for (int c = 0; c < QC; ++c) {
-                umma_f16_chunk(S + (j & 1) * 64, x, y, i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
+                umma_f16_chunk(S + (t & 1) * 64, x, y, i_s, c != 0, c < plan.key_chunks ? min(4, key_steps - 4 * c) : rot_steps);
                 x += HELD_CHUNK >> 4;
                 y += STEP_CHUNK >> 4;
             }
-            umma_commit(s_full(j & 1));
+            umma_commit(s_full(t & 1));
         };
-        auto grads = [&](int j, uint32_t rows) {
-            const int buf = DP_BUFFERS == 2 ? j & 1 : 0;
+        auto grads = [&](uint32_t t, uint32_t rows) {
+            const uint32_t buf = DP_BUFFERS == 2 ? t & 1 : 0;
             uint32_t x = desc_low(base + QC * HELD_CHUNK, 16), y = desc_low(rows + QC * STEP_CHUNK, 16);
 #pragma unroll 1
             for (int c = 0; c < VC; ++c) {
@@ -170,189 +198,222 @@ attention_backward_tc_kernel(const __grid_constant__ CUtensorMap tmA1, const __g
             umma_f16_ts(acc, f + 32, desc_of(y + 256), idesc, 1u);
             umma_f16_ts(acc, f + 40, desc_of(y + 384), idesc, 1u);
         };
-        bool ok = n > 0 && mbar_wait_warp(a_full, 0, status, 3) && mbar_wait_warp(full(0), 0, status, 3);
-        tcgen05_fence_after();
-        if (ok) {
-            if (elect_one()) {
-                scores(0, ring);
-                grads(0, ring);
-            }
-            __syncwarp();
-        }
-        int slot = 0, next = NS == 1 ? 0 : 1;                    // stages of tiles j and j + 1
-        uint32_t next_phase = NS == 1 ? 1u : 0u;
-        for (int j = 0; j < n && ok; ++j) {
-            const uint32_t rows = ring + slot * stage_bytes, next_rows = ring + next * stage_bytes;
-            if (j + 1 < n) {
-                ok = mbar_wait_warp(full(next), next_phase, status, 4);
-                tcgen05_fence_after();
-                if (!ok) break;
-                if (elect_one()) {
-                    scores(j + 1, next_rows);
-                    if (DP_BUFFERS == 2) grads(j + 1, next_rows);
-                }
-                __syncwarp();
-            }
-            if (KEYS) {
-                ok = mbar_wait_warp(p_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 5);
-                tcgen05_fence_after();
-                if (!ok) break;
-                if (elect_one()) sums(ACC2, S + (j & 1) * 64, rows + QC * STEP_CHUNK, i_v, j != 0);
-                __syncwarp();
-            }
-            ok = mbar_wait_warp(ds_full(j & 1), (uint32_t)(j >> 1) & 1u, status, 6);
-            tcgen05_fence_after();
-            if (!ok) break;
-            if (elect_one()) {
-                const uint32_t f = DP + (DP_BUFFERS == 2 ? j & 1 : 0) * 64;
-                sums(ACC1, f, rows, i_1, j != 0);
-                if (!joined) sums(ACC1 + D, f, rows + plan.key_chunks * STEP_CHUNK, i_r, j != 0);
-                umma_commit(empty(slot));
-                if (DP_BUFFERS == 1 && j + 1 < n) grads(j + 1, next_rows);
-                if (j + 1 == n) umma_commit(done);
-            }
-            __syncwarp();
-            slot = next;
+        bool ok = true;
+        int next = 0;                                            // the stage of the next tile
+        uint32_t next_phase = 0, a_phase = 0;
+        auto advance = [&]() {
             if (++next == NS) {
                 next = 0;
                 next_phase ^= 1u;
             }
-        }
+        };
+        each_item(items, [&](unsigned item) {
+            const Item it(a, item, tiles);
+            const int n = it.n;
+            if (n == 0) return true;
+            ok = mbar_wait_warp(a_full, a_phase, status, 3) && mbar_wait_warp(full(next), next_phase, status, 3);
+            a_phase ^= 1u;
+            tcgen05_fence_after();
+            if (!ok) return false;
+            int slot = next;
+            if (elect_one()) {
+                scores(t, ring + slot * stage_bytes);
+                grads(t, ring + slot * stage_bytes);
+                if (n == 1) umma_commit(a_empty);
+            }
+            __syncwarp();
+            advance();
+            for (int j = 0; j < n; ++j, ++t) {
+                const uint32_t rows = ring + slot * stage_bytes, next_rows = ring + next * stage_bytes;
+                if (j + 1 < n) {
+                    ok = mbar_wait_warp(full(next), next_phase, status, 4);
+                    tcgen05_fence_after();
+                    if (!ok) return false;
+                    if (elect_one()) {
+                        scores(t + 1, next_rows);
+                        if (DP_BUFFERS == 2) {
+                            grads(t + 1, next_rows);
+                            if (j + 2 == n) umma_commit(a_empty);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (KEYS) {
+                    ok = mbar_wait_warp(p_full(t & 1), (t >> 1) & 1u, status, 5);
+                    tcgen05_fence_after();
+                    if (!ok) return false;
+                    if (elect_one()) sums(ACC2, S + (t & 1) * 64, rows + QC * STEP_CHUNK, i_v, j != 0);
+                    __syncwarp();
+                }
+                ok = mbar_wait_warp(ds_full(t & 1), (t >> 1) & 1u, status, 6);
+                tcgen05_fence_after();
+                if (!ok) return false;
+                if (elect_one()) {
+                    const uint32_t f = DP + (DP_BUFFERS == 2 ? t & 1 : 0) * 64;
+                    sums(ACC1, f, rows, i_1, j != 0);
+                    if (!joined) sums(ACC1 + D, f, rows + plan.key_chunks * STEP_CHUNK, i_r, j != 0);
+                    umma_commit(empty(slot));
+                    if (DP_BUFFERS == 1 && j + 1 < n) {
+                        grads(t + 1, next_rows);
+                        if (j + 2 == n) umma_commit(a_empty);
+                    }
+                    if (j + 1 == n) umma_commit(done);
+                }
+                __syncwarp();
+                slot = next;
+                if (j + 1 < n) advance();
+            }
+            return true;
+        });
     } else {
         // ================= probabilities and their gradients =================
-        const int half = warp >> 2, quarter = warp & 3, row = r0 + quarter * 32 + lane;
+        const int half = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, cols = half * 32;
         const float by = a.scale * mamba::LOG2E;
         const rowio::f32x2 by2 = rowio::pair(by, by);
-        float lse = INFINITY, del = 0.0f;
-        if (!KEYS && row < seq.queries) {
-            lse = a.lse[stat_row + row];
-            del = delta[stat_row + row];
-        }
-        // columns (of all) that the row meets: first .. last - 1
-        long long first = 0, last = 0;
-        if (row < live) {
-            first = KEYS ? seq.query_begin(row) : 0;
-            last = KEYS ? seq.queries : row + seq.shift + 1;
-            if (!KEYS && last > seq.keys) last = seq.keys;
-        }
         bool ok = true;
         int slot = 0;
-        uint32_t phase = 0;
-        for (int j = 0; j < n; ++j) {
-            const int c0 = begin + j * STEP + cols, buf = j & 1, dbuf = DP_BUFFERS == 2 ? buf : 0;
-            const uint32_t dph = DP_BUFFERS == 2 ? (uint32_t)(j >> 1) & 1u : (uint32_t)j & 1u;
-            const float* st = stats_gen + slot * 2 * STEP + cols;
-            if (!(ok = mbar_wait_warp(s_full(buf), (uint32_t)(j >> 1) & 1u, status, 7))) break;
-            tcgen05_fence_after();
-            uint32_t s[32], w[16];
-            tmem_ld32(S + buf * 64 + lanes + cols, s);
-            tmem_ld_wait();
-            // what a bulk copy brought is visible to who has waited for it: a phase that the product's issuer has already seen
-            if (KEYS && !(ok = mbar_wait_warp(full(slot), phase, status, 8))) break;
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-                float4 l = make_float4(lse, lse, lse, lse);
-                if (KEYS) l = *reinterpret_cast<const float4*>(st + k);
-                const rowio::f32x2 x = rowio::fma2(rowio::pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), by2, rowio::pair(-l.x, -l.y));
-                const rowio::f32x2 y = rowio::fma2(rowio::pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), by2, rowio::pair(-l.z, -l.w));
-                s[k] = __float_as_uint(mamba::ex2(rowio::lo_of(x)));
-                s[k + 1] = __float_as_uint(mamba::ex2(rowio::hi_of(x)));
-                s[k + 2] = __float_as_uint(mamba::ex2(rowio::lo_of(y)));
-                s[k + 3] = __float_as_uint(mamba::ex2(rowio::hi_of(y)));
+        uint32_t phase = 0, t = 0, done_phase = 0;
+        each_item(items, [&](unsigned item) {
+            const Item it(a, item, tiles);
+            const int n = it.n, row = it.r0 + quarter * 32 + lane;
+            float lse = INFINITY, del = 0.0f;
+            if (!KEYS && row < it.seq.queries) {
+                lse = a.lse[it.stat_row(a) + row];
+                del = delta[it.stat_row(a) + row];
             }
-            const int lo = (int)(first - c0 < 0 ? 0 : first - c0 > 32 ? 32 : first - c0), hi = (int)(last - c0 < 0 ? 0 : last - c0 > 32 ? 32 : last - c0);
-            const bool partial = __any_sync(0xffffffffu, lo > 0 || hi < 32);
-            if (partial) {
-#pragma unroll
-                for (int k = 0; k < 32; ++k) s[k] = k >= lo && k < hi ? s[k] : 0u;
+            // columns (of all) that the row meets: first .. last - 1
+            long long first = 0, last = 0;
+            if (row < it.live) {
+                first = KEYS ? it.seq.query_begin(row) : 0;
+                last = KEYS ? it.seq.queries : row + it.seq.shift + 1;
+                if (!KEYS && last > it.seq.keys) last = it.seq.keys;
             }
-            if (KEYS) {
+            for (int j = 0; j < n; ++j, ++t) {
+                const int c0 = it.begin + j * STEP + cols, buf = t & 1, dbuf = DP_BUFFERS == 2 ? buf : 0;
+                const uint32_t dph = DP_BUFFERS == 2 ? (t >> 1) & 1u : t & 1u;
+                const float* st = stats_gen + slot * 2 * STEP + cols;
+                if (!(ok = mbar_wait_warp(s_full(buf), (t >> 1) & 1u, status, 7))) break;
+                tcgen05_fence_after();
+                uint32_t s[32], w[16];
+                tmem_ld32(S + buf * 64 + lanes + cols, s);
+                tmem_ld_wait();
+                // what a bulk copy brought is visible to who has waited for it: a phase that the product's issuer has already seen
+                if (KEYS && !(ok = mbar_wait_warp(full(slot), phase, status, 8))) break;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-                tmem_st16(S + buf * 64 + lanes + cols, w);
+                for (int k = 0; k < 32; k += 4) {
+                    float4 l = make_float4(lse, lse, lse, lse);
+                    if (KEYS) l = *reinterpret_cast<const float4*>(st + k);
+                    const rowio::f32x2 x = rowio::fma2(rowio::pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), by2, rowio::pair(-l.x, -l.y));
+                    const rowio::f32x2 y = rowio::fma2(rowio::pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), by2, rowio::pair(-l.z, -l.w));
+                    s[k] = __float_as_uint(mamba::ex2(rowio::lo_of(x)));
+                    s[k + 1] = __float_as_uint(mamba::ex2(rowio::hi_of(x)));
+                    s[k + 2] = __float_as_uint(mamba::ex2(rowio::lo_of(y)));
+                    s[k + 3] = __float_as_uint(mamba::ex2(rowio::hi_of(y)));
+                }
+                const int lo = (int)(first - c0 < 0 ? 0 : first - c0 > 32 ? 32 : first - c0), hi = (int)(last - c0 < 0 ? 0 : last - c0 > 32 ? 32 : last - c0);
+                const bool partial = __any_sync(0xffffffffu, lo > 0 || hi < 32);
+                if (partial) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) s[k] = k >= lo && k < hi ? s[k] : 0u;
+                }
+                if (KEYS) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+                    tmem_st16(S + buf * 64 + lanes + cols, w);
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full(buf));
+                }
+                if (!(ok = mbar_wait_warp(dp_full(dbuf), dph, status, 9))) break;
+                tcgen05_fence_after();
+                uint32_t g[32];
+                tmem_ld32(DP + dbuf * 64 + lanes + cols, g);
+                tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    float4 d = make_float4(del, del, del, del);
+                    if (KEYS) d = *reinterpret_cast<const float4*>(st + STEP + k);
+                    const rowio::f32x2 x = rowio::mul2(rowio::pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
+                                                       rowio::add2(rowio::pair(__uint_as_float(g[k]), __uint_as_float(g[k + 1])), rowio::pair(-d.x, -d.y)));
+                    const rowio::f32x2 y = rowio::mul2(rowio::pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])),
+                                                       rowio::add2(rowio::pair(__uint_as_float(g[k + 2]), __uint_as_float(g[k + 3])), rowio::pair(-d.z, -d.w)));
+                    g[k] = __float_as_uint(rowio::lo_of(x));
+                    g[k + 1] = __float_as_uint(rowio::hi_of(x));
+                    g[k + 2] = __float_as_uint(rowio::lo_of(y));
+                    g[k + 3] = __float_as_uint(rowio::hi_of(y));
+                }
+                if (partial) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) g[k] = k >= lo && k < hi ? g[k] : 0u;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(g[2 * k]), __uint_as_float(g[2 * k + 1]));
+                tmem_st16(DP + dbuf * 64 + lanes + cols, w);
                 tmem_st_wait();
                 tcgen05_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(buf));
+                if (lane == 0) mbar_arrive(ds_full(buf));
+                if (++slot == NS) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
             }
-            if (!(ok = mbar_wait_warp(dp_full(dbuf), dph, status, 9))) break;
+            if (ok && n > 0) {
+                ok = mbar_wait_warp(done, done_phase, status, 10);
+                done_phase ^= 1u;
+            }
+            if (!ok) return false;
             tcgen05_fence_after();
-            uint32_t g[32];
-            tmem_ld32(DP + dbuf * 64 + lanes + cols, g);
-            tmem_ld_wait();
+            // 32 columns at a time, the two halves of the threads in turn; four lanes share the stores of their four rows
+            const int first_row = row & ~3, piece = lane & 3;
+            auto put = [&](uint32_t acc, int width, float scale, T* to, long long pitch) {         // `to`: the first of the four rows
+                for (int c = half * 32; c < width; c += 64) {
+                    uint32_t o[32], w[16];
+                    if (n > 0) {
+                        tmem_ld32(acc + lanes + c, o);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-                float4 d = make_float4(del, del, del, del);
-                if (KEYS) d = *reinterpret_cast<const float4*>(st + STEP + k);
-                const rowio::f32x2 x = rowio::mul2(rowio::pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])),
-                                                   rowio::add2(rowio::pair(__uint_as_float(g[k]), __uint_as_float(g[k + 1])), rowio::pair(-d.x, -d.y)));
-                const rowio::f32x2 y = rowio::mul2(rowio::pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])),
-                                                   rowio::add2(rowio::pair(__uint_as_float(g[k + 2]), __uint_as_float(g[k + 3])), rowio::pair(-d.z, -d.w)));
-                g[k] = __float_as_uint(rowio::lo_of(x));
-                g[k + 1] = __float_as_uint(rowio::hi_of(x));
-                g[k + 2] = __float_as_uint(rowio::lo_of(y));
-                g[k + 3] = __float_as_uint(rowio::hi_of(y));
-            }
-            if (partial) {
+                    for (int k = 0; k < 16; ++k) w[k] = n > 0 && row < it.live ? pack_word<T>(__uint_as_float(o[2 * k]) * scale, __uint_as_float(o[2 * k + 1]) * scale) : 0u;
+                    transpose_rows(w);
+                    if (to && c + piece * 8 < width) {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) g[k] = k >= lo && k < hi ? g[k] : 0u;
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(g[2 * k]), __uint_as_float(g[2 * k + 1]));
-            tmem_st16(DP + dbuf * 64 + lanes + cols, w);
-            tmem_st_wait();
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(ds_full(buf));
-            if (++slot == NS) {
-                slot = 0;
-                phase ^= 1u;
-            }
-        }
-        if (ok && n > 0) ok = mbar_wait_warp(done, 0, status, 10);
-        tcgen05_fence_after();
-        if (ok) {
-            // 16 columns at a time, the two halves of the threads in turn
-            auto columns = [&](uint32_t acc, int c, float scale, float (&v)[16]) {
-                uint32_t o[16];
-                if (n > 0) {
-                    tmem_ld16(acc + lanes + c, o);
-                    tmem_ld_wait();
+                        for (int k = 0; k < 4; ++k)
+                            if (first_row + k < all) *reinterpret_cast<uint4*>(to + k * pitch + c + piece * 8) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                    }
+                    __syncwarp();
                 }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = n > 0 && row < live ? __uint_as_float(o[k]) * scale : 0.0f;
             };
-            auto put = [&](T* p, const float (&v)[16]) {
-                *reinterpret_cast<uint4*>(p) = make_uint4(pack_word<T>(v[0], v[1]), pack_word<T>(v[2], v[3]), pack_word<T>(v[4], v[5]), pack_word<T>(v[6], v[7]));
-                *reinterpret_cast<uint4*>(p + 8) = make_uint4(pack_word<T>(v[8], v[9]), pack_word<T>(v[10], v[11]), pack_word<T>(v[12], v[13]), pack_word<T>(v[14], v[15]));
-            };
-            const long long at_q = ((long long)b * a.length + row) * a.heads + h;
-            T* to = KEYS ? (a.dk ? static_cast<T*>(a.dk) + b * a.dk_stride_b + row * a.dk_stride_t + h * a.dk_stride_h : nullptr)
-                         : (a.dq ? static_cast<T*>(a.dq) + at_q * a.key_dim : nullptr);
-            float v[16];
-            for (int c = half * 16; c < a.key_dim; c += 32) {
-                columns(ACC1, c, a.scale, v);
-                if (row < all && to) put(to + c, v);
-            }
-            for (int c = half * 16; c < a.rot_dim; c += 32) {
-                columns(ACC1, a.key_dim + c, a.scale, v);
-                if (row < all && KEYS && rot_parts) {
-                    float4* p = reinterpret_cast<float4*>(rot_parts + (((long long)b * a.heads + h) * a.keys + row) * a.rot_dim + c);
+            if (KEYS) {
+                put(ACC1, a.key_dim, a.scale, a.dk ? static_cast<T*>(a.dk) + it.b * a.dk_stride_b + first_row * a.dk_stride_t + it.h * a.dk_stride_h : nullptr, a.dk_stride_t);
+                put(ACC2, a.value_dim, 1.0f, a.dv ? static_cast<T*>(a.dv) + it.b * a.dv_stride_b + first_row * a.dv_stride_t + it.h * a.dv_stride_h : nullptr, a.dv_stride_t);
+                float* to = rot_parts + (((long long)it.b * a.heads + it.h) * a.keys + first_row) * a.rot_dim + piece * 4;
+                for (int c = half * 16; c < a.rot_dim; c += 32) {
+                    uint32_t w[16];
+                    if (n > 0) {
+                        tmem_ld16(ACC1 + a.key_dim + lanes + c, w);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) p[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-                } else if (row < all && !KEYS && a.dq_rot) {
-                    put(static_cast<T*>(a.dq_rot) + at_q * a.rot_dim + c, v);
+                    for (int k = 0; k < 16; ++k) w[k] = n > 0 && row < it.live ? __float_as_uint(__uint_as_float(w[k]) * a.scale) : 0u;
+                    transpose_rows(w);
+                    if (rot_parts) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (first_row + k < all) *reinterpret_cast<uint4*>(to + (long long)k * a.rot_dim + c) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                    }
+                    __syncwarp();
                 }
+            } else {
+                const long long at = ((long long)it.b * a.length + first_row) * a.heads + it.h;
+                put(ACC1, a.key_dim, a.scale, a.dq ? static_cast<T*>(a.dq) + at * a.key_dim : nullptr, (long long)a.heads * a.key_dim);
+                put(ACC1 + a.key_dim, a.rot_dim, a.scale, a.dq_rot ? static_cast<T*>(a.dq_rot) + at * a.rot_dim : nullptr, (long long)a.heads * a.rot_dim);
             }
-            if (KEYS && a.dv) {
-                T* dv = static_cast<T*>(a.dv) + b * a.dv_stride_b + row * a.dv_stride_t + h * a.dv_stride_h;
-                for (int c = half * 16; c < a.value_dim; c += 32) {
-                    columns(ACC2, c, 1.0f, v);
-                    if (row < all) put(dv + c, v);
-                }
-            }
-        }
+            tcgen05_fence_before();                                  // the sums have been read: the next item's wait for these warps' factors
+            return true;
+        });
     }
     if (status != nullptr && *reinterpret_cast<volatile int32_t*>(status) != 0) {
         // a wait gave up somewhere: copies and products still in flight get time to land before their memory is released
@@ -379,7 +440,7 @@ Plan plan_of(const el_attention_t& a) {
 }
 int shared_bytes(const Plan& p) {
     const int chunks = p.key_chunks + p.rot_chunks + p.value_chunks;
-    return 1024 + chunks * HELD_CHUNK + p.stages * (chunks * STEP_CHUNK + 2 * STEP * 4) + 8 * (11 + 2 * MAX_STAGES) + 16;
+    return 1024 + chunks * HELD_CHUNK + p.stages * (chunks * STEP_CHUNK + 2 * STEP * 4) + 8 * (12 + 2 * MAX_STAGES) + 16;
 }
 
 template <typename T, bool KEYS>
@@ -392,7 +453,10 @@ int launch(const el_attention_t& a, const CUtensorMap* held, const CUtensorMap* 
         once.mark(dev);
     }
     const Plan plan = plan_of(a);
-    attention_backward_tc_kernel<T, KEYS><<<blocks_of(a, KEYS ? a.keys : a.length, HELD), THREADS, shared_bytes(plan), st>>>(
+    int sms = 148;
+    device_sm_count(&sms);
+    const unsigned items = blocks_of(a, KEYS ? a.keys : a.length, HELD);
+    attention_backward_tc_kernel<T, KEYS><<<items < (unsigned)sms ? items : sms, THREADS, shared_bytes(plan), st>>>(
         held[0], held[1], held[2], step[0], step[1], step[2], a, delta, rot_parts, plan);
     return check_launch();
 }

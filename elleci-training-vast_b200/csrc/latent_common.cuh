@@ -39,16 +39,25 @@ struct Sequence {
 constexpr int LSE_PAD = 128;          // the rows of a log-sum array are padded to a multiple of this
 __host__ __device__ inline long long lse_pitch(int length) { return ((long long)length + LSE_PAD - 1) / LSE_PAD * LSE_PAD; }
 
-// A block's tile, sequence and head: all heads of all sequences take their first tiles first.
+// A block's (or work item's) tile, sequence and head: all heads of all sequences take their first tiles first.
 struct Place {
     int tile, batch, head;
-    __device__ __forceinline__ Place(const el_attention_t& a) {
-        const unsigned pairs = (unsigned)a.batch * a.heads, t = blockIdx.x / pairs, bh = blockIdx.x - t * pairs;
+    __device__ __forceinline__ Place(const el_attention_t& a, unsigned item = blockIdx.x) {
+        const unsigned pairs = (unsigned)a.batch * a.heads, t = item / pairs, bh = item - t * pairs;
         tile = (int)t;
         batch = (int)(bh / a.heads);
         head = (int)(bh - (unsigned)batch * a.heads);
     }
 };
+// Work items in rounds of one for every block, forwards and backwards in turn: items come largest first, so a block that has a larger one of a round has a smaller
+// one of the next.  Calls f(item) until it returns false.
+template <typename F> __device__ __forceinline__ void each_item(unsigned items, F f) {
+    for (unsigned first = 0, back = 0; first < items; first += gridDim.x, back ^= 1u) {
+        const unsigned item = first + (back ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (item < items && !f(item)) return;
+        if (first + gridDim.x < first) return;
+    }
+}
 inline unsigned blocks_of(const el_attention_t& a, int rows, int tile) { return (unsigned)((rows + (long long)tile - 1) / tile * a.batch * a.heads); }
 
 // 2^x where x <= 0 or -inf (0 then)

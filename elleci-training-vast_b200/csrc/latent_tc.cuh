@@ -104,6 +104,31 @@ template <typename T> __device__ __forceinline__ uint32_t idesc_f16(int a_mn_maj
     constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
     return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn_major << 15) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// Four lanes that hold four neighbouring rows, 64 bytes of each (w), exchange them so that each lane has one 16-byte piece of all four: w[4 k ..] becomes
+// piece lane % 4 of row k.  A store of piece k then writes 64 neighbouring bytes of eight rows instead of 16 bytes of 32.
+__device__ __forceinline__ void transpose_rows(uint32_t (&w)[16]) {
+    const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+#pragma unroll
+    for (int u = 0; u < 4; u += 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t a = w[4 * u + e], b = w[4 * u + 4 + e], got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+            w[4 * u + e] = odd ? got : a;
+            w[4 * u + 4 + e] = odd ? b : got;
+        }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t a = w[4 * u + e], b = w[4 * u + 8 + e], got = __shfl_xor_sync(0xffffffffu, upper ? a : b, 2);
+            w[4 * u + e] = upper ? got : a;
+            w[4 * u + 8 + e] = upper ? b : got;
+        }
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+// The split of a block's registers among its groups of four warps; every warp of a group calls one of the two.
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // two values as a word of type T, the first in its low half
 template <typename T> __device__ __forceinline__ uint32_t pack_word(float lo, float hi) {
     return std::is_same<T, __half>::value ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
