@@ -91,6 +91,7 @@ SIGNATURES = {
     "el_rotary": [_vp, _vp],
     "el_latent_attention": [_vp, _vp],
     "el_latent_attention_lse_bytes": [_vp],
+    "el_latent_attention_workspace_bytes": [_vp],
     "el_latent_attention_backward": [_vp, _vp],
     "el_latent_attention_backward_workspace_bytes": [_vp],
     "el_latent_cache_write": [_vp, _vp],

@@ -88,6 +88,7 @@ int launch_block_norm_backward(const el_block_norm_t& a, cudaStream_t st);
 
 int launch_rotary(const el_rotary_t& a, cudaStream_t st);
 size_t attention_lse_bytes(const el_attention_t& a);
+size_t attention_workspace_bytes(const el_attention_t& a);
 size_t attention_backward_workspace_bytes(const el_attention_t& a);
 int launch_attention(const el_attention_t& a, cudaStream_t st);
 int launch_attention_backward(const el_attention_t& a, cudaStream_t st);
@@ -767,13 +768,14 @@ static int check_attention(const el_attention_t* a) {
     if (!float_dtype(a->dtype) || a->batch < 0 || a->length < 0 || a->keys < 0 || a->heads < 0 || a->key_dim < 0 || a->rot_dim < 0 || a->value_dim < 0)
         return EL_ERR_INVALID_ARG;
     if ((long long)a->key_dim + a->rot_dim > 256 || a->value_dim > 256) return EL_ERR_UNSUPPORTED_SHAPE;
-    // a block for every 64 rows of every head, counted in 31 bits
+    // a block for every 8 rows of every head, counted in 31 bits
     const long long rows = (a->length > a->keys ? a->length : a->keys) + 127LL;
-    if (a->length > 0x7FFFFF00 || a->keys > 0x7FFFFF00 || (double)(rows / 64 + 1) * a->batch * a->heads > 2147483647.0) return EL_ERR_TOO_LARGE;
+    if (a->length > 0x7FFFFF00 || a->keys > 0x7FFFFF00 || (double)(rows / 8 + 1) * a->batch * a->heads > 2147483647.0) return EL_ERR_TOO_LARGE;
     return EL_OK;
 }
 
 size_t el_latent_attention_lse_bytes(const el_attention_t* a) { return check_attention(a) == EL_OK ? attention_lse_bytes(*a) : 0; }
+size_t el_latent_attention_workspace_bytes(const el_attention_t* a) { return check_attention(a) == EL_OK ? attention_workspace_bytes(*a) : 0; }
 size_t el_latent_attention_backward_workspace_bytes(const el_attention_t* a) { return check_attention(a) == EL_OK ? attention_backward_workspace_bytes(*a) : 0; }
 
 int el_latent_attention(const el_attention_t* a, el_stream_t stream) {
@@ -784,6 +786,10 @@ int el_latent_attention(const el_attention_t* a, el_stream_t stream) {
     if (a->value_dim > 0 && !a->out) return EL_ERR_NULL_PTR;
     if ((a->key_dim > 0 && !a->q) || (a->rot_dim > 0 && !a->q_rot)) return EL_ERR_NULL_PTR;
     if (a->keys > 0 && ((a->key_dim > 0 && !a->k) || (a->value_dim > 0 && !a->v) || (a->rot_dim > 0 && !a->k_rot))) return EL_ERR_NULL_PTR;
+    const size_t need = attention_workspace_bytes(*a);
+    if (need > 0 && !a->workspace) return EL_ERR_NULL_PTR;
+    if (need > 0 && a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
     return launch_attention(*a, (cudaStream_t)stream);
 }
 

@@ -43,7 +43,7 @@ PyObject* g_check_status = nullptr;     // int2_tc_ops.check_device_status(devic
     X(el_selective_scan) X(el_selective_scan_checkpoint_bytes) X(el_selective_scan_workspace_bytes)                       \
     X(el_selective_scan_backward) X(el_selective_scan_backward_workspace_bytes) X(el_selective_scan_step)                 \
     X(el_block_norm) X(el_block_norm_backward) X(el_block_norm_backward_workspace_bytes)                                  \
-    X(el_rotary) X(el_latent_attention) X(el_latent_attention_lse_bytes) X(el_latent_attention_backward)                  \
+    X(el_rotary) X(el_latent_attention) X(el_latent_attention_lse_bytes) X(el_latent_attention_workspace_bytes) X(el_latent_attention_backward) \
     X(el_latent_attention_backward_workspace_bytes) X(el_latent_cache_write) X(el_latent_cache_read)                      \
     X(el_latent_attention_step) X(el_latent_attention_step_workspace_bytes)
 struct Library {
@@ -1202,6 +1202,9 @@ PyObject* latent_attention(PyObject* const* a) {
     if (int_arg(a[8])) lse = new_empty(k.q, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&k.c) / sizeof(float))}, at::kFloat);
     k.c.out = ptr(out);
     k.c.lse = ptr<float>(lse);
+    k.c.workspace_bytes = g_lib.el_latent_attention_workspace_bytes(&k.c);
+    Tensor ws = scratch(k.q, k.c.workspace_bytes);
+    k.c.workspace = ptr(ws);
     call("el_latent_attention", g_lib.el_latent_attention, &k.c, stream_on(k.q));
     maybe_check(k.q);
     return tuple_of(wrap(out), wrap_or_none(lse));

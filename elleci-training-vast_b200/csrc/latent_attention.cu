@@ -15,6 +15,7 @@ namespace el {
 int launch_attention_tc(const el_attention_t& a, cudaStream_t st);
 int launch_attention_backward_tc(const el_attention_t& a, const float* delta, float* rot_parts, cudaStream_t st);
 bool attention_tc_takes(const el_attention_t& a, bool backward);
+size_t attention_tc_workspace_bytes(const el_attention_t& a);
 
 using namespace latent;
 
@@ -144,22 +145,31 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const el_attent
     }
 }
 
-// delta[b,h,i] = dout[i] . out[i], zeros for padding.  A warp takes a row.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) attention_delta_kernel(const el_attention_t a, float* __restrict__ delta) {
-    const long long pitch = lse_pitch(a.length), row = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-    if (row >= a.batch * (long long)a.heads * pitch) return;
-    const long long i = row % pitch, bh = row / pitch;
-    const int b = (int)(bh / a.heads), h = (int)(bh - (long long)b * a.heads), lane = threadIdx.x & 31;
+// delta[b,h,i] = dout[i] . out[i], zeros for padding.  `lanes` threads (a power of two from 2 to 32) take a row, 8 values each (VEC: as vectors on 16 bytes), the
+// block the rows of one head: 128 is a multiple of its row count.  Bound: memory (4 x 1024 tokens, 32 heads of 128: 67 MB).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(THREADS) attention_delta_kernel(const el_attention_t a, float* __restrict__ delta, int lanes) {
+    const int rows = THREADS / lanes, part = threadIdx.x & (lanes - 1);
+    const unsigned per = (unsigned)(lse_pitch(a.length) / rows), bh = blockIdx.x / per, b = bh / a.heads, h = bh - b * a.heads;
+    const int i = (int)(blockIdx.x - bh * per) * rows + threadIdx.x / lanes;
     float s = 0.0f;
     if (i < length_of(a.lengths, b, a.length, a.length)) {
-        const T* o = static_cast<const T*>(a.out) + ((b * (long long)a.length + i) * a.heads + h) * a.value_dim;
+        const T* o = static_cast<const T*>(a.out) + (((long long)b * a.length + i) * a.heads + h) * a.value_dim;
         const T* g = static_cast<const T*>(a.dout) + b * a.dout_stride_b + i * a.dout_stride_t + h * a.dout_stride_h;
-        for (int c = lane; c < a.value_dim; c += 32) s = fmaf(to_float(o[c]), to_float(g[c]), s);
-    }
+        for (int c = part * 8; c < a.value_dim; c += lanes * 8) {
+            if constexpr (VEC) {
+                float x[8], y[8];
+                rowio::Io<T>::load8(o + c, x);
+                rowio::Io<T>::load8(g + c, y);
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    if (lane == 0) delta[row] = s;
+                for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
+            } else {
+                for (int k = c; k < c + 8 && k < a.value_dim; ++k) s = fmaf(to_float(o[k]), to_float(g[k]), s);
+            }
+        }
+    }
+    for (int w = lanes / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    if (part == 0) delta[bh * lse_pitch(a.length) + i] = s;
 }
 
 // KEYS: the block holds 64 keys, walks over the queries and forms dk and dv; otherwise it holds 64 queries, walks over the keys and forms dq.
@@ -302,17 +312,25 @@ __global__ void __launch_bounds__(THREADS) attention_backward_rows_kernel(const 
     }
 }
 
-// dk_rot[b,j,c] = sum over the heads of parts[b,h,j,c], in their order
-template <typename T>
+// dk_rot[b,j,c] = sum over the heads of parts[b,h,j,c], in their order.  VEC values a thread: 4 where a head's part is a multiple of 4, else one.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(THREADS) attention_rot_sum_kernel(const float* __restrict__ parts, T* __restrict__ out, int heads, long long per_head, long long n) {
-    const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
+    const long long i = ((long long)blockIdx.x * THREADS + threadIdx.x) * VEC;
     if (i >= n) return;
     const long long b = i / per_head, at = i - b * per_head;
     const float* p = parts + b * heads * per_head + at;
-    float s = 0.0f;
-#pragma unroll 4
-    for (int h = 0; h < heads; ++h) s += p[h * per_head];
-    out[i] = mamba::from_float<T>(s);
+    float s[VEC] = {};
+#pragma unroll 8
+    for (int h = 0; h < heads; ++h) {
+        if constexpr (VEC == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + h * per_head);
+            s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+        } else {
+            s[0] += p[h * per_head];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) out[i + k] = mamba::from_float<T>(s[k]);
 }
 
 template <typename F> int of_type(int dtype, F f) {
@@ -342,6 +360,7 @@ size_t delta_bytes(const el_attention_t& a) { return align16((size_t)a.batch * a
 }  // namespace
 
 size_t attention_lse_bytes(const el_attention_t& a) { return (size_t)a.batch * a.heads * lse_pitch(a.length) * 4; }
+size_t attention_workspace_bytes(const el_attention_t& a) { return attention_tc_takes(a, false) ? attention_tc_workspace_bytes(a) : 0; }
 size_t attention_backward_workspace_bytes(const el_attention_t& a) {
     return delta_bytes(a) + (a.dk_rot ? align16((size_t)a.batch * a.heads * a.keys * a.rot_dim * 4) : 0);
 }
@@ -365,8 +384,14 @@ int launch_attention_backward(const el_attention_t& a, cudaStream_t st) {
     return of_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         if (a.length > 0) {
-            const long long rows = (long long)a.batch * a.heads * lse_pitch(a.length);
-            attention_delta_kernel<T><<<(unsigned)((rows + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, st>>>(a, delta);
+            int lanes = 2;
+            while (lanes < 32 && lanes * 8 < a.value_dim) lanes *= 2;
+            const long long e = 16 / (int)sizeof(T);
+            const bool vec = a.value_dim % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && reinterpret_cast<uintptr_t>(a.dout) % 16 == 0 &&
+                             a.dout_stride_b % e == 0 && a.dout_stride_t % e == 0 && a.dout_stride_h % e == 0;
+            const unsigned grid = blocks_of(a, (int)lse_pitch(a.length), THREADS / lanes);
+            if (vec) attention_delta_kernel<T, true><<<grid, THREADS, 0, st>>>(a, delta, lanes);
+            else attention_delta_kernel<T, false><<<grid, THREADS, 0, st>>>(a, delta, lanes);
             int rc = check_launch();
             if (rc != EL_OK) return rc;
         }
@@ -392,7 +417,8 @@ int launch_attention_backward(const el_attention_t& a, cudaStream_t st) {
         }
         if (!a.dk_rot || a.keys == 0) return rc;
         const long long per_head = (long long)a.keys * a.rot_dim, n = a.batch * per_head;
-        attention_rot_sum_kernel<T><<<(unsigned)((n + THREADS - 1) / THREADS), THREADS, 0, st>>>(rot_parts, static_cast<T*>(a.dk_rot), a.heads, per_head, n);
+        if (per_head % 4 == 0) attention_rot_sum_kernel<T, 4><<<(unsigned)((n / 4 + THREADS - 1) / THREADS), THREADS, 0, st>>>(rot_parts, static_cast<T*>(a.dk_rot), a.heads, per_head, n);
+        else attention_rot_sum_kernel<T, 1><<<(unsigned)((n + THREADS - 1) / THREADS), THREADS, 0, st>>>(rot_parts, static_cast<T*>(a.dk_rot), a.heads, per_head, n);
         return check_launch();
     });
 }

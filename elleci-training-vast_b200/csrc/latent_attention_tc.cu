@@ -30,12 +30,21 @@ constexpr float GROWTH = 8.0f;                  // exponent of 2 by which a row'
 struct Plan {
     int key_chunks, rot_chunks, value_chunks;   // of 64 columns
     int slots;
+    int splits;                                 // items that share a pair of tiles, each a part of its keys
+};
+
+// What an item leaves where the keys are split: for every row its reference and sum, and the sums with values, not yet divided.
+struct Parts {
+    float *sums, *stats;
+    long long rows;                             // batch * heads * the padded length
+    __device__ __forceinline__ float* sum_of(int split, long long row, int width) const { return sums + (split * rows + row) * width; }
+    __device__ __forceinline__ float* stats_of(int split, long long row) const { return stats + (split * rows + row) * 2; }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQr, const __grid_constant__ CUtensorMap tmK,
-                    const __grid_constant__ CUtensorMap tmKr, const __grid_constant__ CUtensorMap tmV, const el_attention_t a, const Plan plan) {
+                    const __grid_constant__ CUtensorMap tmKr, const __grid_constant__ CUtensorMap tmV, const el_attention_t a, const Plan plan, const Parts parts) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
@@ -55,16 +64,27 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const uint32_t q_empty = slot_empty(MAX_SLOTS);             // two
     const int warp = warp_index(), lane = threadIdx.x & 31;
     const int pairs = (a.length + 2 * TILE - 1) / (2 * TILE);
-    const unsigned items = (unsigned)pairs * a.batch * a.heads;
+    const unsigned items = (unsigned)pairs * a.batch * a.heads * plan.splits;
     int32_t* status = a.dev_status;
-    // an item: its queries, and the key tiles of its two query tiles
+    // an item: its queries, its first key tile, and how many from there its two query tiles take
     struct Item {
-        int b, h, i0, n0, n1, n;
+        int b, h, i0, split, j0, n0, n1, n;
         Sequence seq;
-        __device__ __forceinline__ Item(const el_attention_t& a, unsigned item, int pairs) : Item(a, Place(a, item), pairs) {}
-        __device__ __forceinline__ Item(const el_attention_t& a, const Place& at, int pairs) : b(at.batch), h(at.head), i0((pairs - 1 - at.tile) * 2 * TILE), seq(a, at.batch) {
-            n0 = uniform(i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0);
-            n1 = uniform(i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0);
+        __device__ __forceinline__ Item(const el_attention_t& a, unsigned item, int pairs, int splits) : Item(a, Place(a, splits == 1 ? item : item / splits), pairs, splits, splits == 1 ? 0 : item % splits) {}
+        __device__ __forceinline__ Item(const el_attention_t& a, const Place& at, int pairs, int splits, int part)
+            : b(at.batch), h(at.head), i0((pairs - 1 - at.tile) * 2 * TILE), split(part), seq(a, at.batch) {
+            n0 = i0 < seq.queries ? (seq.key_end(i0 + TILE) + TILE - 1) / TILE : 0;
+            n1 = i0 + TILE < seq.queries ? (seq.key_end(i0 + 2 * TILE) + TILE - 1) / TILE : 0;
+            j0 = 0;
+            if (splits > 1) {
+                const int all = n0 > n1 ? n0 : n1, j1 = (int)((long long)all * (part + 1) / splits);
+                j0 = (int)((long long)all * part / splits);
+                n0 = max(min(n0, j1) - j0, 0);
+                n1 = max(min(n1, j1) - j0, 0);
+            }
+            j0 = uniform(j0);
+            n0 = uniform(n0);
+            n1 = uniform(n1);
             n = n0 > n1 ? n0 : n1;
         }
     };
@@ -106,7 +126,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         uint32_t ph = 0, land = 0, q_phase[2] = {1u, 1u};
         bool ok = true;
         each_item(items, [&](unsigned item) {
-            const Item it(a, item, pairs);
+            const Item it(a, item, pairs, plan.splits);
             for (int i = 0; i < 2 && ok; ++i) {
                 if ((i == 0 ? it.n0 : it.n1) == 0) continue;
                 if (!mbar_wait_warp(q_empty + 8u * i, q_phase[i], status, 1)) { ok = false; break; }
@@ -121,8 +141,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             for (int j = 0; j < it.n && ok; ++j) {
                 // values behind the sequence's end may be anything, and zero times anything is not always zero: those rows are cleared
-                const int live = it.seq.keys - j * TILE;
-                const bool clear = live < TILE && j * TILE + live < a.keys;
+                const int key = (it.j0 + j) * TILE, live = it.seq.keys - key;
+                const bool clear = live < TILE && key + live < a.keys;
                 int head = 0;
                 for (int c = 0; c < QC + VC; ++c) {
                     if (!mbar_wait_warp(slot_empty(s), ph ^ 1u, status, 1)) { ok = false; break; }
@@ -132,9 +152,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                         const uint32_t dst = ring + s * CHUNK, bar = late ? landed : slot_full(head);
                         if (late) mbar_expect_tx(bar, CHUNK);
                         else if (s == head) mbar_expect_tx(bar, (value ? VC : QC) * CHUNK);
-                        if (value) tma_load_3d(dst, &tmV, bar, (int)(it.h * a.v_stride_h) + (c - QC) * CHUNK_COLS, j * TILE, it.b);
-                        else if (c < plan.key_chunks) tma_load_3d(dst, &tmK, bar, (int)(it.h * a.k_stride_h) + c * CHUNK_COLS, j * TILE, it.b);
-                        else tma_load_3d(dst, &tmKr, bar, 0, j * TILE, it.b);
+                        if (value) tma_load_3d(dst, &tmV, bar, (int)(it.h * a.v_stride_h) + (c - QC) * CHUNK_COLS, key, it.b);
+                        else if (c < plan.key_chunks) tma_load_3d(dst, &tmK, bar, (int)(it.h * a.k_stride_h) + c * CHUNK_COLS, key, it.b);
+                        else tma_load_3d(dst, &tmKr, bar, 0, key, it.b);
                     }
                     __syncwarp();
                     if (late) {
@@ -195,7 +215,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         int place = 0;                                          // of the next tile of keys or values
         uint32_t q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};
         each_item(items, [&](unsigned item) {
-            const Item it(a, item, pairs);
+            const Item it(a, item, pairs, plan.splits);
             if (it.n == 0) return true;
             const int only = it.n0 == 0 ? 1 : 0;                // the tile that waits for what both need: the first that there is
             for (int i = 0; i < 2; ++i) {
@@ -259,7 +279,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         bool ok = true;
         uint32_t phase = 0;                                     // of this tile's s_full; o_full of the tile before has the other one
         each_item(items, [&](unsigned item) {
-            const Item it(a, item, pairs);
+            const Item it(a, item, pairs, plan.splits);
             const int mine = i == 0 ? it.n0 : it.n1, row = it.i0 + i * TILE + quarter * 32 + lane;
             // keys that this row sees: 0 .. sees - 1
             long long sees = row < it.seq.queries ? row + it.seq.shift + 1 : 0;
@@ -272,7 +292,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
                 tmem_ld_wait();
-                const int here = (int)sees - j * TILE;               // columns that the row sees
+                const int here = (int)sees - (it.j0 + j) * TILE;               // columns that the row sees
                 if (__any_sync(0xffffffffu, here < TILE)) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
@@ -333,13 +353,31 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
             const bool empty = ref == -INFINITY && !(sum != sum);    // sees nothing; a NaN is no such row
             const float inv = 1.0f / sum;
-            if (a.lse && row < lse_pitch(a.length))
-                a.lse[((long long)it.b * a.heads + it.h) * lse_pitch(a.length) + row] = empty ? INFINITY : ref + log2f(sum);
+            const long long stat_row = ((long long)it.b * a.heads + it.h) * lse_pitch(a.length) + row;
+            if (row < lse_pitch(a.length)) {
+                if (plan.splits > 1) *reinterpret_cast<float2*>(parts.stats_of(it.split, stat_row)) = make_float2(sum != sum ? sum : ref, sum);
+                else if (a.lse) a.lse[stat_row] = empty ? INFINITY : ref + log2f(sum);
+            }
             if (ok && mine > 0) ok = mbar_wait_warp(o_full(i), phase ^ 1u, status, 8);
             if (!ok) return false;
             tcgen05_fence_after();
             // four lanes share the stores of their four rows
             const int first = row & ~3;
+            if (plan.splits > 1) {                               // (without a tile there are no sums: such a part's are not read)
+                float* to = parts.sum_of(it.split, stat_row - (lane & 3), a.value_dim) + (lane & 3) * 4;
+                for (int c = 0; c < a.value_dim && mine > 0; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(o_addr + c, o);
+                    tmem_ld_wait();
+                    transpose_rows(o);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (first + k < lse_pitch(a.length)) *reinterpret_cast<uint4*>(to + (long long)k * a.value_dim + c) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    __syncwarp();
+                }
+                tcgen05_fence_before();
+                return true;
+            }
             T* out = static_cast<T*>(a.out) + (((long long)it.b * a.length + first) * a.heads + it.h) * a.value_dim + (lane & 3) * 8;
             for (int c = 0; c < a.value_dim; c += 32) {
                 uint32_t o[32], w[16];
@@ -376,6 +414,53 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
 }
 
+// out and lse from the parts of every row.  A warp takes a row; value_dim is a multiple of 16 up to 128, four values a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_kernel(const el_attention_t a, const Parts parts, int splits) {
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), pitch = lse_pitch(a.length);
+    if (row >= parts.rows) return;
+    const int lane = threadIdx.x & 31;
+    const unsigned bh = (unsigned)(row / pitch), b = bh / a.heads, h = bh - b * a.heads;
+    const int i = (int)(row - bh * pitch);
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = mamba::max_nan(top, parts.stats_of(s, row)[0]);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+        const float2 st = *reinterpret_cast<const float2*>(parts.stats_of(s, row));
+        if (st.x == -INFINITY) continue;
+        const float f = exp2_neg(st.x - top);
+        sum = fmaf(f, st.y, sum);
+        if (lane * 4 < a.value_dim) {
+            const float4 v = *reinterpret_cast<const float4*>(parts.sum_of(s, row, a.value_dim) + lane * 4);
+            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+        }
+    }
+    const bool empty = top == -INFINITY;
+    if (a.lse && lane == 0) a.lse[row] = empty ? INFINITY : top + log2f(sum);
+    if (i >= a.length || lane * 4 >= a.value_dim) return;
+    const float inv = empty ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (((long long)b * a.length + i) * a.heads + h) * a.value_dim + lane * 4) =
+        make_uint2(pack_word<T>(o.x * inv, o.y * inv), pack_word<T>(o.z * inv, o.w * inv));
+}
+
+// Items that share a pair of query tiles, where there are fewer pairs than SMs: what makes the rounds over the SMs times the tiles of an item least, an item's own
+// start and end counted as two tiles and a part's way through memory as one more.  2 x 250 queries, 3999 keys, 32 heads (64 pairs): 1 item 101 us, 2 items 62.
+int splits_of(const el_attention_t& a) {
+    int sms = 148, best = 1;
+    device_sm_count(&sms);
+    const long long items = blocks_of(a, a.length, 2 * TILE), n = ((long long)a.keys + TILE - 1) / TILE;
+    long long least = 0;
+    for (int s = 1; s <= 16 && s <= n && (s == 1 || items < sms); ++s) {
+        const long long cost = (items * s + sms - 1) / sms * ((n + s - 1) / s + 2 + (s > 1));
+        if (s == 1 || cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
+
 Plan plan_of(const el_attention_t& a) {
     Plan p;
     p.key_chunks = (a.key_dim + 63) / 64;
@@ -383,6 +468,7 @@ Plan plan_of(const el_attention_t& a) {
     p.value_chunks = (a.value_dim + 63) / 64;
     const int room = (227 * 1024 - 2048) / CHUNK - 2 * (p.key_chunks + p.rot_chunks);
     p.slots = room < MAX_SLOTS ? room : MAX_SLOTS;
+    p.splits = splits_of(a);
     return p;
 }
 int shared_bytes(const Plan& p) { return 1024 + (2 * (p.key_chunks + p.rot_chunks) + p.slots) * CHUNK + 8 * (11 + 2 * MAX_SLOTS) + 16; }
@@ -401,8 +487,14 @@ template <typename T> int launch(const el_attention_t& a, const Plan& plan, cons
     }
     int sms = 148;
     device_sm_count(&sms);
-    const unsigned items = blocks_of(a, a.length, 2 * TILE);
-    attention_tc_kernel<T><<<items < (unsigned)sms ? items : sms, THREADS, shared_bytes(plan), st>>>(m[0], m[1], m[2], m[3], m[4], a, plan);
+    const unsigned items = blocks_of(a, a.length, 2 * TILE) * plan.splits;
+    const long long rows = (long long)a.batch * a.heads * lse_pitch(a.length);
+    float* sums = static_cast<float*>(a.workspace);
+    const Parts parts{sums, plan.splits > 1 ? sums + plan.splits * rows * a.value_dim : nullptr, rows};
+    attention_tc_kernel<T><<<items < (unsigned)sms ? items : sms, THREADS, shared_bytes(plan), st>>>(m[0], m[1], m[2], m[3], m[4], a, plan, parts);
+    const int rc = check_launch();
+    if (rc != EL_OK || plan.splits == 1) return rc;
+    attention_join_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(a, parts, plan.splits);
     return check_launch();
 }
 
@@ -435,6 +527,11 @@ int attention_maps(const el_attention_t& a, CUtensorMap m[5], int query_rows, in
     if (rc == EL_OK && a.rot_dim) rc = make_map_tokens(&m[1], a.q_rot, (a.heads - 1) * a.q_rot_stride_h + a.rot_dim, a.length, a.q_rot_stride_t, a.batch, a.q_rot_stride_b, query_rows);
     if (rc == EL_OK && a.rot_dim) rc = make_map_tokens(&m[3], a.k_rot, a.rot_dim, a.keys, a.k_rot_stride_t, a.batch, a.k_rot_stride_b, key_rows);
     return rc;
+}
+
+size_t attention_tc_workspace_bytes(const el_attention_t& a) {
+    const int splits = splits_of(a);
+    return splits > 1 ? (size_t)splits * a.batch * a.heads * lse_pitch(a.length) * (a.value_dim + 2) * 4 : 0;
 }
 
 int launch_attention_tc(const el_attention_t& a, cudaStream_t st) {

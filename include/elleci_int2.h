@@ -592,11 +592,12 @@ typedef struct el_attention_t {
     void* dv;
     long long dv_stride_b, dv_stride_t, dv_stride_h;
     void* dk_rot;                       /* dense, as k_rot */
-    void* workspace;                    /* backward: el_latent_attention_backward_workspace_bytes, 16-byte aligned */
+    void* workspace;                    /* el_latent_attention_workspace_bytes (forward) / _backward_workspace_bytes, 16-byte aligned */
     size_t workspace_bytes;
     int32_t* dev_status;
 } el_attention_t;
 EL_API size_t el_latent_attention_lse_bytes(const el_attention_t* args);
+EL_API size_t el_latent_attention_workspace_bytes(const el_attention_t* args);
 EL_API int el_latent_attention(const el_attention_t* args, el_stream_t stream);
 EL_API size_t el_latent_attention_backward_workspace_bytes(const el_attention_t* args);
 EL_API int el_latent_attention_backward(const el_attention_t* args, el_stream_t stream);
