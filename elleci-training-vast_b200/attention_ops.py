@@ -18,12 +18,9 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from ._lib import host_ops
 from .int2_tc_ops import ACT_EPS, NORM_EPS, _require
-from .ssm_ops import _bits, _wants_grad
 
 
 def rotary_table(positions: int, dim: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
@@ -35,45 +32,12 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, device: Option
     return torch.cat([angle.cos(), angle.sin()], -1).float()
 
 
-class _Rotary(Function):
-    @staticmethod
-    def forward(ctx, x, table, positions, neighbours):
-        ctx.save_for_backward(table, positions)
-        ctx.neighbours = neighbours
-        return host_ops().rotary(x, table, positions, neighbours, 0)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        table, positions = ctx.saved_tensors
-        return host_ops().rotary(dy, table, positions, ctx.neighbours, 1), None, None, None
-
-
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: Optional[torch.Tensor] = None, neighbours: bool = False) -> torch.Tensor:
     """x [batch, length, heads, dim] or [batch, length, dim] with its pairs (x[i], x[i + dim/2]) (`neighbours`: (x[2i], x[2i+1])) turned by the angles of the
     token's position.  `table` as from `rotary_table`.  `positions` (int32 or int64): [batch] the position of each sequence's first token, or [batch,
     length], or None (token t is at t); positions outside the table are clamped to it.  Differentiable in x."""
     _require(not (isinstance(table, torch.Tensor) and table.requires_grad), "rotary has no gradient of its table")
-    if _wants_grad(x):
-        return _Rotary.apply(x, table, positions, int(neighbours))
     return host_ops().rotary(x, table, positions, int(neighbours), 0)
-
-
-class _LatentAttention(Function):
-    @staticmethod
-    def forward(ctx, q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths):
-        out, lse = host_ops().latent_attention(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, 1)
-        ctx.save_for_backward(q, kv, q_rot, k_rot, lengths, key_lengths, out, lse)
-        ctx.causal, ctx.scale = causal, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, kv, q_rot, k_rot, lengths, key_lengths, out, lse = ctx.saved_tensors
-        grads = host_ops().latent_attention_backward(q, kv, q_rot, k_rot, ctx.causal, ctx.scale, lengths, key_lengths, out, lse, dout,
-                                                     _bits(ctx.needs_input_grad[:4]))
-        return (*grads, None, None, None, None)
 
 
 def latent_attention(q: torch.Tensor, kv: torch.Tensor, q_rot: Optional[torch.Tensor] = None, k_rot: Optional[torch.Tensor] = None, causal: bool = True,
@@ -86,9 +50,7 @@ def latent_attention(q: torch.Tensor, kv: torch.Tensor, q_rot: Optional[torch.Te
     keys as queries, else all keys): a sequence's queries and keys, padding behind them.  A sequence's queries are its last tokens: with `causal`, query i of m
     sees the keys up to i + n - m of n.  A query that sees no key has the output 0.  Padding is not read (it may hold anything, NaN included), its
     outputs and gradients are zeros; an infinity or NaN in a token's own key or value reaches other queries of its tile too.  Differentiable in q, kv, q_rot, k_rot."""
-    if _wants_grad(q, kv, q_rot, k_rot):
-        return _LatentAttention.apply(q, kv, q_rot, k_rot, int(causal), scale, lengths, key_lengths)
-    return host_ops().latent_attention(q, kv, q_rot, k_rot, int(causal), scale, lengths, key_lengths, 0)[0]
+    return host_ops().latent_attention(q, kv, q_rot, k_rot, int(causal), scale, lengths, key_lengths)
 
 
 class LatentCache(NamedTuple):

@@ -15,12 +15,16 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <dlfcn.h>
 
 #include <cmath>
 #include <cstdlib>
+#include <optional>
 #include <vector>
 
 #include "../../include/elleci_int2.h"
@@ -1084,9 +1088,93 @@ Tensor table_arg(PyObject* o, const Tensor& x, int64_t dim) {
     return t.contiguous();
 }
 
+// ---- recorded calls -----------------------------------------------------------------------------------------------------
+// Autograd nodes of native code: where kernels are short the host's time counts, and a node in Python costs 10 us more a direction.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(PyObject* const* a, std::initializer_list<int> tensors) {
+    if (!c10::GradMode::is_enabled()) return false;
+    for (int i : tensors)
+        if (THPVariable_Check(a[i]) && THPVariable_Unpack(a[i]).requires_grad()) return true;
+    return false;
+}
+Tensor tensor_or_none(PyObject* o) { return is_none(o) ? Tensor() : tensor_arg(o, "an argument"); }
+
+using MaybeTensor = std::optional<Tensor>;          // a node's input that may be missing (an undefined tensor is not taken)
+MaybeTensor maybe_tensor(PyObject* o) { return is_none(o) ? MaybeTensor() : MaybeTensor(tensor_arg(o, "an argument")); }
+
+struct Objects {                        // arguments of an entry, owned
+    std::vector<PyObject*> all;
+    ~Objects() { for (PyObject* o : all) Py_XDECREF(o); }
+    Objects() = default;
+    Objects(const Objects&) = delete;
+    void add(PyObject* o) {
+        all.push_back(o);
+        if (o == nullptr) throw PyError();
+    }
+};
+// Runs f, an entry's call, in an engine thread: with the GIL, its exception carried to the thread that called backward.  A first-order derivative: where a
+// graph of the backward pass is recorded, its results end in a node that refuses.
+template <typename F> variable_list in_backward(const char* name, int results, variable_list saved, const variable_list& grads, F f) {
+    variable_list out(results);
+    {
+        struct Gil {
+            PyGILState_STATE state = PyGILState_Ensure();
+            ~Gil() { PyGILState_Release(state); }
+        } gil;
+        try {
+            const at::AutoGradMode off(false);
+            Objects made;
+            made.add(f());
+            PyObject* r = made.all[0];
+            for (int i = 0; i < results; ++i) {
+                PyObject* o = PyTuple_Check(r) ? PyTuple_GET_ITEM(r, i) : r;
+                if (!is_none(o)) out[i] = THPVariable_Unpack(o);
+            }
+        } catch (const PyError&) {
+            python_error e;
+            e.persist();
+            throw e;
+        }
+    }
+    if (c10::GradMode::is_enabled()) {
+        saved.insert(saved.end(), grads.begin(), grads.end());
+        const auto refuse = std::make_shared<torch::autograd::Error>(std::string(name) + " has derivatives of the first order only", torch::autograd::collect_next_edges(saved));
+        for (Tensor& t : out)
+            if (t.defined()) torch::autograd::set_history(t, refuse);
+    }
+    return out;
+}
+
+PyObject* rotary(PyObject* const* a);
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor&, PyObject* const* a) {
+        Objects made;
+        made.add(rotary(a));
+        ctx->save_for_backward({tensor_or_none(a[1]), tensor_or_none(a[2])});
+        ctx->saved_data["neighbours"] = (int64_t)int_arg(a[3]);
+        return THPVariable_Unpack(made.all[0]);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list r = in_backward("rotary", 1, saved, grads, [&] {
+            Objects o;
+            o.add(wrap(grads[0]));
+            for (const Tensor& t : saved) o.add(wrap_or_none(t));
+            o.add(PyLong_FromLongLong(ctx->saved_data["neighbours"].toInt()));
+            o.add(PyLong_FromLong(1));
+            return rotary(o.all.data());
+        });
+        r.resize(2);
+        return r;
+    }
+};
+
 // rotary(x, table, positions, neighbours, inverse) -> y
 PyObject* rotary(PyObject* const* a) {
     no_tangent("rotary", a, {0, 1});
+    if (wants_grad(a, {0})) return wrap(RotaryNode::apply(tensor_arg(a[0], "x"), a));
     const Tensor& x4 = cuda_arg(a[0], "x");
     EL_REQUIRE(float_type(x4.scalar_type()), "x must be float16, bfloat16 or float32");
     EL_REQUIRE(x4.dim() == 3 || x4.dim() == 4, "x must be [batch, length, (heads,) dim]");
@@ -1192,14 +1280,50 @@ void attention_call(AttentionCall& k, PyObject* const* a) {
     k.keep = {pair, qr, kr, lengths, key_lengths};
 }
 
-// latent_attention(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, log sums wanted) -> (out, log sums or None)
+PyObject* latent_attention_backward(PyObject* const* a);
+void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse);
+struct AttentionNode : torch::autograd::Function<AttentionNode> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& kv, const MaybeTensor& q_rot, const MaybeTensor& k_rot, PyObject* const* a) {
+        Tensor out, lse;
+        attention_forward(a, true, out, lse);
+        ctx->save_for_backward({q, kv, q_rot.value_or(Tensor()), k_rot.value_or(Tensor()), tensor_or_none(a[6]), tensor_or_none(a[7]), out, lse});
+        ctx->saved_data["causal"] = (int64_t)int_arg(a[4]);
+        if (!is_none(a[5])) ctx->saved_data["scale"] = float_arg(a[5]);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list r = in_backward("latent_attention", 4, saved, grads, [&] {
+            Objects o;
+            for (int i = 0; i < 4; ++i) o.add(wrap_or_none(saved[i]));
+            o.add(PyLong_FromLongLong(ctx->saved_data["causal"].toInt()));
+            o.add(ctx->saved_data.count("scale") ? PyFloat_FromDouble(ctx->saved_data["scale"].toDouble()) : none());
+            for (int i = 4; i < 8; ++i) o.add(wrap_or_none(saved[i]));
+            o.add(wrap(grads[0]));
+            long wanted = 0;
+            for (int i = 0; i < (saved[2].defined() ? 4 : 2); ++i) wanted |= (ctx->needs_input_grad(i) ? 1L : 0L) << i;
+            o.add(PyLong_FromLong(wanted));
+            return latent_attention_backward(o.all.data());
+        });
+        r.resize(5);
+        return r;
+    }
+};
+
+// latent_attention(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths) -> out
 PyObject* latent_attention(PyObject* const* a) {
     no_tangent("latent_attention", a, {0, 1, 2, 3});
+    if (wants_grad(a, {0, 1, 2, 3})) return wrap(AttentionNode::apply(tensor_arg(a[0], "q"), tensor_arg(a[1], "kv"), maybe_tensor(a[2]), maybe_tensor(a[3]), a));
+    Tensor out, lse;
+    attention_forward(a, false, out, lse);
+    return wrap(out);
+}
+void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse) {
     AttentionCall k;
     attention_call(k, a);
     const c10::cuda::CUDAGuard device(k.q.device());
-    Tensor out = new_empty(k.q, {k.B, k.T, k.H, k.V}, k.q.scalar_type()), lse;
-    if (int_arg(a[8])) lse = new_empty(k.q, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&k.c) / sizeof(float))}, at::kFloat);
+    out = new_empty(k.q, {k.B, k.T, k.H, k.V}, k.q.scalar_type());
+    if (sums) lse = new_empty(k.q, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&k.c) / sizeof(float))}, at::kFloat);
     k.c.out = ptr(out);
     k.c.lse = ptr<float>(lse);
     k.c.workspace_bytes = g_lib.el_latent_attention_workspace_bytes(&k.c);
@@ -1207,7 +1331,6 @@ PyObject* latent_attention(PyObject* const* a) {
     k.c.workspace = ptr(ws);
     call("el_latent_attention", g_lib.el_latent_attention, &k.c, stream_on(k.q));
     maybe_check(k.q);
-    return tuple_of(wrap(out), wrap_or_none(lse));
 }
 
 // latent_attention_backward(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, out, log sums, dout, wanted) -> (dq, dkv, dq_rot, dk_rot), `wanted`: bits
@@ -1501,7 +1624,7 @@ PyMethodDef methods[] = {
     EL_ENTRY(gemm_fwd, 7), EL_ENTRY(gemm_dx, 8), EL_ENTRY(dw_hysteresis, 11), EL_ENTRY(weight_update, 13), EL_ENTRY(linear_decode, 8), EL_ENTRY(set_hooks, 4),
     EL_ENTRY(causal_conv, 7), EL_ENTRY(causal_conv_backward, 9), EL_ENTRY(causal_conv_step, 6), EL_ENTRY(selective_scan, 13),
     EL_ENTRY(selective_scan_backward, 15), EL_ENTRY(selective_scan_step, 11), EL_ENTRY(block_norm, 8), EL_ENTRY(block_norm_backward, 11),
-    EL_ENTRY(rotary, 5), EL_ENTRY(latent_attention, 9), EL_ENTRY(latent_attention_backward, 12), EL_ENTRY(latent_cache_write, 13), EL_ENTRY(latent_cache_read, 8),
+    EL_ENTRY(rotary, 5), EL_ENTRY(latent_attention, 8), EL_ENTRY(latent_attention_backward, 12), EL_ENTRY(latent_cache_write, 13), EL_ENTRY(latent_cache_read, 8),
     EL_ENTRY(latent_attention_step, 13),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "elleci_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

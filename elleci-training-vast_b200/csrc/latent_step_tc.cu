@@ -117,11 +117,12 @@ __device__ __forceinline__ float reduce16max(const float (&v)[16]) {
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1)
 step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant__ CUtensorMap tmKeys, const el_latent_step_t a, const uint8_t* __restrict__ images,
-               const float* __restrict__ steps, const StepParts parts, int workers, const int box) {
+               const float* __restrict__ steps, const StepParts parts, int workers, const int box_bits) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const StepImage image(a);
+    const int box = box_bits ? 1 << box_bits : 0;                            // 8 to 32 tokens
     const int R = a.rank, P = a.rot_dim, HP = image.hp, N = 2 * HP, KC = image.chunks, key_steps = (R + 31) / 32, rot_steps = (P + 15) / 16;
     const int stage_bytes = (KC + (P ? 1 : 0)) * CHUNK;
     // two stages [rows][keys]; the query's image; p digits [tokens][128]
@@ -197,15 +198,15 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const int to = q * 32 + lane;
-                            const long long r = __shfl_sync(0xffffffffu, start, to / box);
-                            row[q] = r >= 0 && p + to < k.p1 ? r + to % box : -1;
+                            const long long r = __shfl_sync(0xffffffffu, start, to >> box_bits);
+                            row[q] = r >= 0 && p + to < k.p1 ? r + (to & (box - 1)) : -1;
                             sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
                         }
                         if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
                         const unsigned there = __ballot_sync(0xffffffffu, start >= 0);
                         if (elect_one()) mbar_expect_tx_only(full(mine), __popc(there) * box * 128 * (KC + (P ? 1 : 0)) + (i == 0 ? image.bytes() : 0));
                         __syncwarp();
-                        for (int x = 0; x < TOKENS / box; ++x) {
+                        for (int x = 0; x < TOKENS >> box_bits; ++x) {
                             const int r = __shfl_sync(0xffffffffu, (int)start, x);
                             if (r >= 0 && elect_one()) {
                                 for (int c = 0; c < KC; ++c) tma_load_2d(at + c * CHUNK + x * box * 128, &tmRows, full(mine), c * 128, r);
@@ -558,6 +559,8 @@ bool latent_step_tc_takes(const el_latent_step_t& a) {
 int launch_latent_step_tc(const el_latent_step_t& a, const uint8_t* images, const float* steps, const StepParts& parts, int workers, cudaStream_t st) {
     const StepImage image(a);
     const int box = box_of(a);
+    int box_bits = 0;
+    while (box > 1 << box_bits) ++box_bits;
     CUtensorMap rows = {}, keys = {};
     if (box) {
         const uint64_t tokens = (uint64_t)a.pages * a.page_size;
@@ -585,7 +588,7 @@ int launch_latent_step_tc(const el_latent_step_t& a, const uint8_t* images, cons
         cfg.stream = st;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        EL_CUDA_TRY(cudaLaunchKernelEx(&cfg, step_tc_kernel<T>, rows, keys, a, images, steps, parts, workers, box));
+        EL_CUDA_TRY(cudaLaunchKernelEx(&cfg, step_tc_kernel<T>, rows, keys, a, images, steps, parts, workers, box_bits));
         return check_launch();
     };
     return a.dtype == EL_F16 ? run(__half()) : run(__nv_bfloat16());

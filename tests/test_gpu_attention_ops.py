@@ -301,6 +301,32 @@ def test_cache_reads_values(ops, out):
     _close("values", values, want, (R.UNIT[out] + 4 * R.E) * want.abs() + R.TINY[out])
 
 
+@pytest.mark.parametrize("rank, rot, page", [(16, 2, 7), (48, 0, 64), (272, 64, 33), (512, 64, 64)])
+def test_cache_reads_many_tokens(ops, rank, rot, page):
+    """So many that a warp takes several; the last warp's are not all there."""
+    g = _gen(rank)
+    B, L = 5, 5003
+    per = -(-L // page)
+    latents, absmax, keys = _pool(g, 300, page, rank, rot, BF)
+    blocks = torch.randint(-2, 302, (B, per), generator=g, dtype=torch.int32)
+    starts, lengths = torch.tensor([0, 5, 0, 4000, 17]), torch.tensor([L, 1, 0, L, 2500])
+    at = torch.arange(L)[None] + starts[:, None]
+    page_of = torch.where(at < per * page, torch.gather(blocks.long(), 1, (at // page).clamp(max=per - 1)), -1)
+    there = (torch.arange(L)[None] < lengths[:, None]) & (page_of >= 0) & (page_of < 300)
+    row = torch.where(there, page_of * page + at % page, 0).flatten()
+    there = there.flatten()
+    want, want_max = latents.view(-1, rank)[row] * there[:, None], absmax.flatten()[row] * there
+    cache = ops.LatentCache(latents.to(DEV), absmax.to(DEV), keys.to(DEV) if rot else None)
+    rows, most, back = ops.latent_cache_read(cache, blocks.to(DEV), L, starts.to(DEV), lengths.to(DEV))
+    assert torch.equal(rows.cpu(), want.to(torch.int8)) and torch.equal(most.cpu(), want_max)
+    values, again = ops.latent_cache_read(cache, blocks.to(DEV), L, starts.to(DEV), lengths.to(DEV), BF)
+    true = want.double() * (want_max.double() / 127)[:, None]
+    _close("values", values.view(-1, rank), true, (R.UNIT[BF] + 4 * R.E) * true.abs() + R.TINY[BF])
+    if rot:
+        want_keys = keys.view(-1, rot)[row] * there[:, None]
+        assert torch.equal(back.cpu().view(-1, rot), want_keys) and torch.equal(again, back)
+
+
 def test_cache_drops_what_has_no_page(ops):
     cache = ops.LatentCache.new(4, 8, 64, 32, BF, DEV)
     blocks = torch.tensor([[1, -1], [4, 2]], dtype=torch.int32, device=DEV)
@@ -473,3 +499,82 @@ def test_refusals(ops):
     ]:
         with pytest.raises(RuntimeError, match=message):
             call()
+
+
+# ---- recorded calls -----------------------------------------------------------------------------------------------------
+
+def _leaves(rot=True):
+    g = _gen(77)
+    q, kv = _randn(g, 2, 70, 2, 64, dtype=BF).to(DEV), _randn(g, 2, 70, 2 * 128, dtype=BF).to(DEV)
+    qr, kr = (_randn(g, 2, 70, 2, 32, dtype=BF).to(DEV), _randn(g, 2, 70, 32, dtype=BF).to(DEV)) if rot else (None, None)
+    return [t.requires_grad_(True) for t in (q, kv, qr, kr) if t is not None]
+
+
+def test_second_derivatives_are_refused(ops):
+    leaves = _leaves()
+    table = ops.rotary_table(70, 32, device=DEV)
+    for out, leaf in ((ops.latent_attention(*leaves), leaves[0]), (ops.rotary(leaves[2], table), leaves[2])):
+        (d,) = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
+        assert d.requires_grad
+        with pytest.raises(RuntimeError, match="first order"):
+            torch.autograd.grad(d.float().sum(), leaf)
+
+
+def test_recorded_calls_keep_autograds_rules(ops):
+    from torch.utils.checkpoint import checkpoint
+    leaves = _leaves()
+    table = ops.rotary_table(70, 32, device=DEV)
+
+    def f(q, kv, qr, kr):
+        return ops.latent_attention(q, kv, ops.rotary(qr, table), ops.rotary(kr, table))
+
+    dout = torch.randn(2, 70, 2, 64, device=DEV).to(BF)
+    want = torch.autograd.grad(f(*leaves), leaves, dout)
+    for a, b in zip(want, torch.autograd.grad(checkpoint(f, *leaves, use_reentrant=False), leaves, dout)):
+        assert torch.equal(a, b)
+    # two graphs of the same leaves, walked twice and out of order; gradients that are views
+    one, two = f(*leaves), f(*leaves)
+    wide = torch.empty(2, 70, 2, 80, device=DEV, dtype=BF)
+    wide[..., 8:72] = dout
+    for out in (two, one):
+        for _ in range(2):
+            for a, b in zip(want, torch.autograd.grad(out, leaves, wide[..., 8:72], retain_graph=True)):
+                assert torch.equal(a, b)
+    # leaves without a gradient, and a graph without the rotated parts
+    q, kv = _leaves(False)
+    (only,) = torch.autograd.grad(ops.latent_attention(q.detach(), kv), [kv], dout)
+    both = torch.autograd.grad(ops.latent_attention(q, kv), [q, kv], dout)
+    assert torch.equal(only, both[1])
+    with torch.no_grad():
+        assert not ops.latent_attention(q, kv).requires_grad
+    # what a graph needs and has changed since
+    x = leaves[2].detach() * 1
+    out = ops.latent_attention(leaves[0], leaves[1], x, leaves[3])
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(dout)
+    out = ops.latent_attention(*leaves)
+    out.backward(dout)
+    with pytest.raises(RuntimeError, match="second time"):
+        out.backward(dout)
+
+
+def test_errors_of_a_backward_pass_reach_its_caller(ops):
+    leaves = _leaves()
+    out = ops.latent_attention(*leaves)
+
+    class Wrong(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, dy):
+            raise ValueError("from a node in front")
+
+    with pytest.raises(ValueError, match="in front"):
+        Wrong.apply(out).sum().backward()
+    with pytest.raises(RuntimeError):
+        ops.latent_attention(leaves[0], leaves[1][:, :, :100], *leaves[2:])
+    ops.latent_attention(*leaves).sum().backward()
+    assert all(t.grad is not None for t in leaves)
