@@ -11,7 +11,7 @@
 //
 // Warps 0-7: thread t of each half is token t of the tile and takes 16 heads' scores; then two of the four blocks of 128 latent channels, a thread a channel.
 // The sums of a tile are taken after the next tile's scores, so that the tensor core has work meanwhile.  Warp 8 issues the products.  Warps
-// 9 and 10 load, each every other tile: by tensor maps where pages are multiples of 8 tokens (a box lies in one page), otherwise by 16-byte
+// 9 and 10 load, each half of a tile's tokens: by tensor maps where pages are multiples of 8 tokens (a box lies in one page), otherwise by 16-byte
 // asynchronous copies of each token's row.
 // Bound: memory; a tile of 128 tokens of rank 512 and 64 rotated channels is 82 KB, 3400 cycles of an SM's share of the HBM, and 1100 of its tensor core.
 #include "latent_step.cuh"
@@ -150,7 +150,7 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
     int32_t* status = a.dev_status;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), 2);
             mbar_init(empty(s), 1);
             mbar_init(s_full(s), 1);
             mbar_init(half_at(s), 4);
@@ -180,54 +180,55 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
 
     if (warp >= WARP_LOAD) {
         // ================= loads =================
-        const int mine = warp - WARP_LOAD;                                            // every other tile
+        const int mine = warp - WARP_LOAD;                                            // half of every tile's tokens
         int g = 0, part = 0;
         bool ok = true;
         if (first < last) {
             for (Walk k(a, first, last); k.more() && ok; k.next(), ++part) {
                 const int count = k.tiles();
                 for (int i = 0; i < count && ok; ++i, ++g) {
-                    if ((g & 1) != mine) continue;
-                    const uint32_t at = base + mine * stage_bytes;
+                    const int s = g & 1;
+                    const uint32_t at = base + s * stage_bytes, gone = ((uint32_t)(g >> 1) & 1u) ^ 1u;
                     const int p = k.p0 + i * TOKENS;
-                    long long row[4];
-                    float sc[4];
+                    long long row[2];
+                    float sc[2];
                     if (box) {                                                  // lane l looks up box l
-                        const int pos = p + lane * box;
-                        const long long start = lane * box < TOKENS && pos < k.p1 ? step_row(a, k.b, pos) : -1;
+                        const int first_box = mine * 64 >> box_bits, pos = p + (first_box + lane) * box;
+                        const long long start = lane * box < 64 && pos < k.p1 ? step_row(a, k.b, pos) : -1;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
+                        for (int q = 0; q < 2; ++q) {
                             const int to = q * 32 + lane;
                             const long long r = __shfl_sync(0xffffffffu, start, to >> box_bits);
-                            row[q] = r >= 0 && p + to < k.p1 ? r + (to & (box - 1)) : -1;
+                            row[q] = r >= 0 && p + mine * 64 + to < k.p1 ? r + (to & (box - 1)) : -1;
                             sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
                         }
-                        if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
+                        if (!mbar_wait_warp(empty(s), gone, status, 1)) { ok = false; break; }
                         const unsigned there = __ballot_sync(0xffffffffu, start >= 0);
-                        if (elect_one()) mbar_expect_tx_only(full(mine), __popc(there) * box * 128 * (KC + (P ? 1 : 0)) + (i == 0 ? image.bytes() : 0));
+                        if (elect_one()) mbar_expect_tx_only(full(s), __popc(there) * box * 128 * (KC + (P ? 1 : 0)) + (i == 0 && mine == 0 ? image.bytes() : 0));
                         __syncwarp();
-                        for (int x = 0; x < TOKENS >> box_bits; ++x) {
+                        for (int x = 0; x < 64 >> box_bits; ++x) {
                             const int r = __shfl_sync(0xffffffffu, (int)start, x);
                             if (r >= 0 && elect_one()) {
-                                for (int c = 0; c < KC; ++c) tma_load_2d(at + c * CHUNK + x * box * 128, &tmRows, full(mine), c * 128, r);
-                                if (P) tma_load_2d(at + KC * CHUNK + x * box * 128, &tmKeys, full(mine), 0, r);
+                                const uint32_t to = at + ((first_box + x) << (box_bits + 7));
+                                for (int c = 0; c < KC; ++c) tma_load_2d(to + c * CHUNK, &tmRows, full(s), c * 128, r);
+                                if (P) tma_load_2d(to + KC * CHUNK, &tmKeys, full(s), 0, r);
                             }
                             __syncwarp();
                         }
                     } else {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int pos = p + q * 32 + lane;
+                        for (int q = 0; q < 2; ++q) {
+                            const int pos = p + mine * 64 + q * 32 + lane;
                             row[q] = pos < k.p1 ? step_row(a, k.b, pos) : -1;
                             sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
                         }
-                        if (!mbar_wait_warp(empty(mine), ((uint32_t)(g >> 1) & 1u) ^ 1u, status, 1)) { ok = false; break; }
+                        if (!mbar_wait_warp(empty(s), gone, status, 1)) { ok = false; break; }
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
+                        for (int q = 0; q < 2; ++q) {
 #pragma unroll 8
                             for (int t = 0; t < 32; ++t) {
                                 const long long r = __shfl_sync(0xffffffffu, row[q], t);
-                                const int to = q * 32 + t;
+                                const int to = mine * 64 + q * 32 + t;
                                 if (lane * 16 < R && r >= 0)
                                     copy16(at + (lane >> 3) * CHUNK + to * 128 + (((lane & 7) ^ (to & 7)) << 4), a.latents + r * R + lane * 16, true);
                             }
@@ -235,7 +236,7 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                                 const int pieces = (P + 15) / 16 * 2;                 // of 8 channels, zeros behind the last
 #pragma unroll 4
                                 for (int t = 0; t < 32; t += 4) {
-                                    const int tt = t + (lane >> 3), c = lane & 7, to = q * 32 + tt;
+                                    const int tt = t + (lane >> 3), c = lane & 7, to = mine * 64 + q * 32 + tt;
                                     const long long r = __shfl_sync(0xffffffffu, row[q], tt);
                                     if (c < pieces) {
                                         const bool there = r >= 0 && c * 8 < P;
@@ -246,18 +247,18 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                         }
                     }
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        scale_of[mine * 128 + q * 32 + lane] = __fdiv_rn(sc[q], 127.0f);
+                    for (int q = 0; q < 2; ++q) {
+                        scale_of[s * 128 + mine * 64 + q * 32 + lane] = __fdiv_rn(sc[q], 127.0f);
                         const uint32_t have = __ballot_sync(0xffffffffu, row[q] >= 0);
-                        if (lane == 0) seen[mine * 4 + q] = have;
+                        if (lane == 0) seen[s * 4 + mine * 2 + q] = have;
                     }
-                    if (i == 0) {                                                     // the part's query
+                    if (i == 0 && mine == 0) {                                        // the part's query
                         if (part > 0 && !mbar_wait_warp(q_empty, (uint32_t)(part - 1) & 1u, status, 2)) { ok = false; break; }
                         griddep_wait();                                               // the kernel in front made it
                         const long long bg = (long long)k.b * image.groups + group;
                         if (elect_one()) {
-                            if (!box) mbar_expect_tx_only(full(mine), image.bytes());
-                            bulk_load(q_at, images + bg * image.bytes(), image.bytes(), full(mine));
+                            if (!box) mbar_expect_tx_only(full(s), image.bytes());
+                            bulk_load(q_at, images + bg * image.bytes(), image.bytes(), full(s));
                         }
                         __syncwarp();
                         step_of[(part & 1) * 32 + lane] = lane < HP ? steps[bg * 32 + lane] : 0.0f;
@@ -265,7 +266,7 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(full(mine));
+                    if (lane == 0) mbar_arrive(full(s));
                 }
             }
         }
