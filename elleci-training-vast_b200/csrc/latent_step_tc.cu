@@ -50,6 +50,9 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
+}
 // bytes that a barrier's phase waits for, without an arrival
 __device__ __forceinline__ void mbar_expect_tx_only(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -202,19 +205,24 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
                             row[q] = r >= 0 && p + mine * 64 + to < k.p1 ? r + (to & (box - 1)) : -1;
                             sc[q] = row[q] >= 0 ? a.absmax[row[q]] : 0.0f;
                         }
+                        // the stage is taken for the time of most of a tile: the bytes come as far as the L2 meanwhile
+                        if (g >= 2 && start >= 0) {
+#pragma unroll 4
+                            for (int c = 0; c < KC; ++c) tma_prefetch_2d(&tmRows, c * 128, (int)start);
+                            if (P) tma_prefetch_2d(&tmKeys, 0, (int)start);
+                        }
+                        __syncwarp();
                         if (!mbar_wait_warp(empty(s), gone, status, 1)) { ok = false; break; }
                         const unsigned there = __ballot_sync(0xffffffffu, start >= 0);
                         if (elect_one()) mbar_expect_tx_only(full(s), __popc(there) * box * 128 * (KC + (P ? 1 : 0)) + (i == 0 && mine == 0 ? image.bytes() : 0));
                         __syncwarp();
-                        for (int x = 0; x < 64 >> box_bits; ++x) {
-                            const int r = __shfl_sync(0xffffffffu, (int)start, x);
-                            if (r >= 0 && elect_one()) {
-                                const uint32_t to = at + ((first_box + x) << (box_bits + 7));
-                                for (int c = 0; c < KC; ++c) tma_load_2d(to + c * CHUNK, &tmRows, full(s), c * 128, r);
-                                if (P) tma_load_2d(to + KC * CHUNK, &tmKeys, full(s), 0, r);
-                            }
-                            __syncwarp();
+                        if (start >= 0) {                                       // a lane loads its box
+                            const uint32_t to = at + ((first_box + lane) << (box_bits + 7));
+#pragma unroll 4
+                            for (int c = 0; c < KC; ++c) tma_load_2d(to + c * CHUNK, &tmRows, full(s), c * 128, (int)start);
+                            if (P) tma_load_2d(to + KC * CHUNK, &tmKeys, full(s), 0, (int)start);
                         }
+                        __syncwarp();
                     } else {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
