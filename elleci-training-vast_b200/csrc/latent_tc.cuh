@@ -61,6 +61,17 @@ __device__ __forceinline__ void umma_f16_chunk(uint32_t d_tmem, uint32_t a_low, 
 #pragma unroll 1
     for (int x = 1; x < steps; ++x) umma_f16(d_tmem, desc_of(a_low + 2 * x), desc_of(b_low + 2 * x), idesc, 1u);
 }
+// the same with the left operand in tensor memory, 8 columns a step
+__device__ __forceinline__ void umma_f16_ts_chunk(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate, int steps) {
+    umma_f16_ts(d_tmem, a_tmem, desc_of(b_low), idesc, accumulate);
+    if (steps == 4) {
+#pragma unroll
+        for (int x = 1; x < 4; ++x) umma_f16_ts(d_tmem, a_tmem + 8 * x, desc_of(b_low + 2 * x), idesc, 1u);
+        return;
+    }
+#pragma unroll 1
+    for (int x = 1; x < steps; ++x) umma_f16_ts(d_tmem, a_tmem + 8 * x, desc_of(b_low + 2 * x), idesc, 1u);
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
