@@ -789,7 +789,7 @@ int el_latent_attention(const el_attention_t* a, el_stream_t stream) {
     const size_t need = attention_workspace_bytes(*a);
     if (need > 0 && !a->workspace) return EL_ERR_NULL_PTR;
     if (need > 0 && a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
-    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(a->out_rest) % 16 != 0) return EL_ERR_ALIGNMENT;
     return launch_attention(*a, (cudaStream_t)stream);
 }
 
@@ -801,7 +801,7 @@ int el_latent_attention_backward(const el_attention_t* a, el_stream_t stream) {
     const size_t need = attention_backward_workspace_bytes(*a);
     if (need > 0 && !a->workspace) return EL_ERR_NULL_PTR;
     if (a->workspace_bytes < need) return EL_ERR_INVALID_ARG;
-    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return EL_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(a->out_rest) % 16 != 0) return EL_ERR_ALIGNMENT;
     if (a->length > 0 && (!a->lse || (a->value_dim > 0 && (!a->out || !a->dout)) || (a->key_dim > 0 && !a->q) || (a->rot_dim > 0 && !a->q_rot))) return EL_ERR_NULL_PTR;
     if (a->keys > 0 && ((a->key_dim > 0 && !a->k) || (a->value_dim > 0 && !a->v) || (a->rot_dim > 0 && !a->k_rot))) return EL_ERR_NULL_PTR;
     return launch_attention_backward(*a, (cudaStream_t)stream);

@@ -1281,12 +1281,12 @@ void attention_call(AttentionCall& k, PyObject* const* a) {
 }
 
 PyObject* latent_attention_backward(PyObject* const* a);
-void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse);
+void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse, Tensor& rest);
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& kv, const MaybeTensor& q_rot, const MaybeTensor& k_rot, PyObject* const* a) {
-        Tensor out, lse;
-        attention_forward(a, true, out, lse);
-        ctx->save_for_backward({q, kv, q_rot.value_or(Tensor()), k_rot.value_or(Tensor()), tensor_or_none(a[6]), tensor_or_none(a[7]), out, lse});
+        Tensor out, lse, rest;
+        attention_forward(a, true, out, lse, rest);
+        ctx->save_for_backward({q, kv, q_rot.value_or(Tensor()), k_rot.value_or(Tensor()), tensor_or_none(a[6]), tensor_or_none(a[7]), out, lse, rest});
         ctx->saved_data["causal"] = (int64_t)int_arg(a[4]);
         if (!is_none(a[5])) ctx->saved_data["scale"] = float_arg(a[5]);
         return out;
@@ -1298,7 +1298,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
             for (int i = 0; i < 4; ++i) o.add(wrap_or_none(saved[i]));
             o.add(PyLong_FromLongLong(ctx->saved_data["causal"].toInt()));
             o.add(ctx->saved_data.count("scale") ? PyFloat_FromDouble(ctx->saved_data["scale"].toDouble()) : none());
-            for (int i = 4; i < 8; ++i) o.add(wrap_or_none(saved[i]));
+            for (int i = 4; i < 9; ++i) o.add(wrap_or_none(saved[i]));
             o.add(wrap(grads[0]));
             long wanted = 0;
             for (int i = 0; i < (saved[2].defined() ? 4 : 2); ++i) wanted |= (ctx->needs_input_grad(i) ? 1L : 0L) << i;
@@ -1314,17 +1314,20 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
 PyObject* latent_attention(PyObject* const* a) {
     no_tangent("latent_attention", a, {0, 1, 2, 3});
     if (wants_grad(a, {0, 1, 2, 3})) return wrap(AttentionNode::apply(tensor_arg(a[0], "q"), tensor_arg(a[1], "kv"), maybe_tensor(a[2]), maybe_tensor(a[3]), a));
-    Tensor out, lse;
-    attention_forward(a, false, out, lse);
+    Tensor out, lse, rest;
+    attention_forward(a, false, out, lse, rest);
     return wrap(out);
 }
-void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse) {
+// `sums`: with what the backward pass needs
+void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse, Tensor& rest) {
     AttentionCall k;
     attention_call(k, a);
     const c10::cuda::CUDAGuard device(k.q.device());
     out = new_empty(k.q, {k.B, k.T, k.H, k.V}, k.q.scalar_type());
     if (sums) lse = new_empty(k.q, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&k.c) / sizeof(float))}, at::kFloat);
+    if (sums && out.element_size() == 2) rest = new_empty(k.q, out.sizes(), at::kChar);
     k.c.out = ptr(out);
+    k.c.out_rest = ptr<int8_t>(rest);
     k.c.lse = ptr<float>(lse);
     k.c.workspace_bytes = g_lib.el_latent_attention_workspace_bytes(&k.c);
     Tensor ws = scratch(k.q, k.c.workspace_bytes);
@@ -1333,10 +1336,10 @@ void attention_forward(PyObject* const* a, bool sums, Tensor& out, Tensor& lse) 
     maybe_check(k.q);
 }
 
-// latent_attention_backward(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, out, log sums, dout, wanted) -> (dq, dkv, dq_rot, dk_rot), `wanted`: bits
+// latent_attention_backward(q, kv, q_rot, k_rot, causal, scale, lengths, key_lengths, out, log sums, out's rest or None, dout, wanted) -> (dq, dkv, dq_rot, dk_rot), `wanted`: bits
 // 0 .. 3 in this order
 PyObject* latent_attention_backward(PyObject* const* a) {
-    no_tangent("latent_attention_backward", a, {0, 1, 2, 3, 8, 10});
+    no_tangent("latent_attention_backward", a, {0, 1, 2, 3, 8, 11});
     AttentionCall k;
     attention_call(k, a);
     const Tensor& q = k.q;
@@ -1344,8 +1347,9 @@ PyObject* latent_attention_backward(PyObject* const* a) {
     el_attention_t& c = k.c;
     Tensor out = dense_arg(a[8], "out", q, q.scalar_type(), {k.B, k.T, k.H, k.V});
     Tensor lse = dense_arg(a[9], "lse", q, at::kFloat, {(int64_t)(g_lib.el_latent_attention_lse_bytes(&c) / sizeof(float))});
-    Tensor dout = attention_arg(a[10], "dout", q, out.sizes());
-    const int want = (int)int_arg(a[11]);
+    Tensor rest = maybe_dense(a[10], "rest", q, at::kChar, out.sizes());
+    Tensor dout = attention_arg(a[11], "dout", q, out.sizes());
+    const int want = (int)int_arg(a[12]);
     const auto io = q.scalar_type();
     Tensor dq, dkv, dqr, dkr;
     if (want & 1) dq = new_empty(q, {k.B, k.T, k.H, k.D}, io);
@@ -1353,6 +1357,7 @@ PyObject* latent_attention_backward(PyObject* const* a) {
     if ((want & 4) && k.R) dqr = new_empty(q, {k.B, k.T, k.H, k.R}, io);
     if ((want & 8) && k.R) dkr = new_empty(q, {k.B, k.S, k.R}, io);
     c.out = ptr(out);
+    c.out_rest = ptr<int8_t>(rest);
     c.lse = ptr<float>(lse);
     c.dout = ptr(dout);
     c.dout_stride_b = stride_of(dout, 0);
@@ -1624,7 +1629,7 @@ PyMethodDef methods[] = {
     EL_ENTRY(gemm_fwd, 7), EL_ENTRY(gemm_dx, 8), EL_ENTRY(dw_hysteresis, 11), EL_ENTRY(weight_update, 13), EL_ENTRY(linear_decode, 8), EL_ENTRY(set_hooks, 4),
     EL_ENTRY(causal_conv, 7), EL_ENTRY(causal_conv_backward, 9), EL_ENTRY(causal_conv_step, 6), EL_ENTRY(selective_scan, 13),
     EL_ENTRY(selective_scan_backward, 15), EL_ENTRY(selective_scan_step, 11), EL_ENTRY(block_norm, 8), EL_ENTRY(block_norm_backward, 11),
-    EL_ENTRY(rotary, 5), EL_ENTRY(latent_attention, 8), EL_ENTRY(latent_attention_backward, 12), EL_ENTRY(latent_cache_write, 13), EL_ENTRY(latent_cache_read, 8),
+    EL_ENTRY(rotary, 5), EL_ENTRY(latent_attention, 8), EL_ENTRY(latent_attention_backward, 13), EL_ENTRY(latent_cache_write, 13), EL_ENTRY(latent_cache_read, 8),
     EL_ENTRY(latent_attention_step, 13),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "elleci_host_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

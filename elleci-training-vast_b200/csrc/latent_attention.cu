@@ -141,21 +141,26 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const el_attent
         T* out = static_cast<T*>(a.out) + (((long long)b * a.length + i) * a.heads + h) * V;
 #pragma unroll
         for (int c = 0; c < MOST_DIM / 16; ++c)
-            if (tx + 16 * c < V) out[tx + 16 * c] = mamba::from_float<T>(empty ? 0.0f : o[r][c] * inv);
+            if (tx + 16 * c < V) {
+                const float x = empty ? 0.0f : o[r][c] * inv;
+                out[tx + 16 * c] = mamba::from_float<T>(x);
+                if constexpr (sizeof(T) == 2)
+                    if (a.out_rest) a.out_rest[out - static_cast<T*>(a.out) + tx + 16 * c] = (int8_t)(rest_of<T>(x, to_float(mamba::from_float<T>(x))) >> 8);
+            }
     }
 }
 
-// delta[b,h,i] = dout[i] . out[i], zeros for padding.  A block takes 8 tokens of up to 32 heads, whose values lie side by side (15.5 us; rows of one head, 256 bytes
+// delta[b,h,i] = dout[i] . out[i] (with what rounding took from out, where it is kept: an error of delta goes to all of a row's ds alike), zeros for padding.  A block takes 8 tokens of up to 32 heads, whose values lie side by side (15.5 us; rows of one head, 256 bytes
 // of every 8 KB, took 26), and writes 8 tokens of a head at a time.  `lanes` threads (a power of two from 2 to 32, 8 values each) take a row, and 4 rows
 // are on their way at once.  VEC: 8 values are vectors on 16 bytes.  Bound: memory (4 x 1024 tokens, 32 heads of 128: 67 MB).
 constexpr int DELTA_TOKENS = 8, DELTA_HEADS = 32;
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool REST>
 __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const el_attention_t a, float* __restrict__ delta, int lanes, int head_bits) {
     __shared__ float sums[DELTA_TOKENS * DELTA_HEADS];
     const int groups = THREADS / lanes, part = threadIdx.x & (lanes - 1), heads = 1 << head_bits, rows = DELTA_TOKENS << head_bits, c = part * 8, V = a.value_dim;
     const long long pitch = lse_pitch(a.length);
-    const unsigned per = (unsigned)(pitch / DELTA_TOKENS), b = blockIdx.x / per;
-    const int t0 = (int)(blockIdx.x - b * per) * DELTA_TOKENS, h0 = blockIdx.y * heads, live = length_of(a.lengths, b, a.length, a.length);
+    const unsigned per = (unsigned)(pitch / DELTA_TOKENS), groups_of_heads = (a.heads + heads - 1) >> head_bits, tile = blockIdx.x / groups_of_heads, b = tile / per;
+    const int t0 = (int)(tile - b * per) * DELTA_TOKENS, h0 = (int)(blockIdx.x - tile * groups_of_heads) * heads, live = length_of(a.lengths, b, a.length, a.length);
     const T *out0 = static_cast<const T*>(a.out), *dout0 = static_cast<const T*>(a.dout);
     const T *out = out0 + ((long long)b * a.length + t0) * a.heads * V, *dout = dout0 + b * a.dout_stride_b + t0 * a.dout_stride_t;
     if (V == 0 || t0 >= live) {
@@ -164,35 +169,53 @@ __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const el_atten
         return;
     }
     for (int r0 = threadIdx.x / lanes; r0 - (int)threadIdx.x / lanes < rows; r0 += 4 * groups) {
-        float x[4][8], y[4][8], s[4];
-        bool live_row[4];
+        float s[4];
+        bool there[4];
+        const T *o[4], *g[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 4; ++k) {                                  // (a row that is not there reads the first one)
             const int r = r0 + k * groups, t = r >> head_bits, h = h0 + (r & (heads - 1));
-            const bool there = r < rows && t0 + t < live && h < a.heads && c < V;
-            live_row[k] = there;
-            const T* o = there ? out + ((long long)t * a.heads + h) * V + c : out0;                   // (a row that is not there reads the first one)
-            const T* g = there ? dout + t * a.dout_stride_t + h * a.dout_stride_h + c : dout0;
-            if constexpr (VEC) {
-                rowio::Io<T>::load8(o, x[k]);
-                rowio::Io<T>::load8(g, y[k]);
-            } else {
+            there[k] = r < rows && t0 + t < live && h < a.heads && c < V;
+            o[k] = there[k] ? out + (t * a.heads + h) * V + c : out0;
+            g[k] = there[k] ? dout + t * a.dout_stride_t + h * a.dout_stride_h + c : dout0;
+        }
+        if constexpr (VEC) {
+            constexpr int WORDS = sizeof(T) * 8 / 16;
+            uint4 x[4][WORDS], y[4][WORDS];
+            uint2 z[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) {
+                    x[k][w] = reinterpret_cast<const uint4*>(o[k])[w];
+                    y[k][w] = reinterpret_cast<const uint4*>(g[k])[w];
+                }
+                if constexpr (REST) z[k] = *reinterpret_cast<const uint2*>(a.out_rest + (o[k] - out0));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const T *xs = reinterpret_cast<const T*>(x[k]), *ys = reinterpret_cast<const T*>(y[k]);
+                s[k] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int at = c + e < V ? e : 0;
-                    x[k][e] = there && c + e < V ? to_float(o[at]) : 0.0f;
-                    y[k][e] = to_float(g[at]);
+                    float v = to_float(xs[e]);
+                    if constexpr (REST) v = with_rest<T>(v, e < 4 ? z[k].x : z[k].y, e & 3);
+                    s[k] = fmaf(v, to_float(ys[e]), s[k]);
+                }
+            }
+        } else {
+            for (int k = 0; k < 4; ++k) {
+                s[k] = 0.0f;
+                for (int e = 0; e < 8 && c + e < V; ++e) {
+                    float v = to_float(o[k][e]);
+                    if constexpr (REST) v = with_rest<T>(v, (uint8_t)a.out_rest[o[k] - out0 + e], 0);
+                    s[k] = fmaf(v, to_float(g[k][e]), s[k]);
                 }
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            s[k] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (VEC || c + e < V) s[k] = fmaf(x[k][e], y[k][e], s[k]);
-            if (!live_row[k]) s[k] = 0.0f;
-        }
+        for (int k = 0; k < 4; ++k)
+            if (!there[k]) s[k] = 0.0f;
         for (int w = lanes / 2; w > 0; w >>= 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], w);
@@ -421,9 +444,13 @@ int launch_attention_backward(const el_attention_t& a, cudaStream_t st) {
                              a.dout_stride_b % e == 0 && a.dout_stride_t % e == 0 && a.dout_stride_h % e == 0;
             int head_bits = 0;
             while (1 << head_bits < a.heads && 1 << head_bits < DELTA_HEADS) ++head_bits;
-            const dim3 grid((unsigned)(a.batch * (lse_pitch(a.length) / DELTA_TOKENS)), (unsigned)((a.heads + (1 << head_bits) - 1) >> head_bits));
-            if (vec) attention_delta_kernel<T, true><<<grid, THREADS, 0, st>>>(a, delta, lanes, head_bits);
-            else attention_delta_kernel<T, false><<<grid, THREADS, 0, st>>>(a, delta, lanes, head_bits);
+            const unsigned grid = (unsigned)(a.batch * (lse_pitch(a.length) / DELTA_TOKENS) * ((a.heads + (1 << head_bits) - 1) >> head_bits));
+            auto run = [&](auto v, auto rest) {
+                attention_delta_kernel<T, decltype(v)::value, decltype(rest)::value><<<grid, THREADS, 0, st>>>(a, delta, lanes, head_bits);
+            };
+            auto form = [&](auto rest) { vec ? run(std::true_type(), rest) : run(std::false_type(), rest); };
+            if constexpr (sizeof(T) == 2) a.out_rest ? form(std::true_type()) : form(std::false_type());
+            else form(std::false_type());
             int rc = check_launch();
             if (rc != EL_OK) return rc;
         }

@@ -386,8 +386,18 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     tmem_ld_wait();
                 }
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    w[k] = mine == 0 || empty ? 0u : pack_word<T>(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
+                for (int k = 0; k < 32; ++k) o[k] = mine == 0 || empty ? 0u : __float_as_uint(__uint_as_float(o[k]) * inv);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) w[k] = pack_word<T>(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1]));
+                if (a.out_rest && row < a.length) {
+                    uint4* rest = reinterpret_cast<uint4*>(a.out_rest + (((long long)it.b * a.length + row) * a.heads + it.h) * a.value_dim + c);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        auto four = [&](int x) { return rest_word<T>(w[2 * x], w[2 * x + 1], __uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3])); };
+                        const uint4 r = make_uint4(four(4 * k), four(4 * k + 1), four(4 * k + 2), four(4 * k + 3));
+                        if (c + 16 * k < a.value_dim) rest[k] = r;
+                    }
+                }
                 transpose_rows(w);
                 if (c + (lane & 3) * 8 < a.value_dim) {
 #pragma unroll
@@ -440,8 +450,11 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const el_attention_
     if (a.lse && lane == 0) a.lse[row] = empty ? INFINITY : top + log2f(sum);
     if (i >= a.length || lane * 4 >= a.value_dim) return;
     const float inv = empty ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (((long long)b * a.length + i) * a.heads + h) * a.value_dim + lane * 4) =
-        make_uint2(pack_word<T>(o.x * inv, o.y * inv), pack_word<T>(o.z * inv, o.w * inv));
+    const long long at = (((long long)b * a.length + i) * a.heads + h) * a.value_dim + lane * 4;
+    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    const uint2 w = make_uint2(pack_word<T>(o.x, o.y), pack_word<T>(o.z, o.w));
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) = w;
+    if (a.out_rest) *reinterpret_cast<uint32_t*>(a.out_rest + at) = rest_word<T>(w.x, w.y, o.x, o.y, o.z, o.w);
 }
 
 // Items that share a pair of query tiles, where there are fewer pairs than SMs: what makes the rounds over the SMs times the tiles of an item least, an item's own

@@ -60,6 +60,19 @@ template <typename F> __device__ __forceinline__ void each_item(unsigned items, 
 }
 inline unsigned blocks_of(const el_attention_t& a, int rows, int tile) { return (unsigned)((rows + (long long)tile - 1) / tile * a.batch * a.heads); }
 
+// What rounding to a 16-bit type took from a float, as a signed byte: 256ths of a step of the type, which are 2^8 (bfloat16) or 2^5 (float16) steps of a
+// float32.  Floats of one sign are ordered as their bits are, so it is a difference of bits, across powers of two as well.  (A tie that went down has
+// 128 of them: 127 are kept.  Below float16's normal range a step holds more: the byte is clamped and next to nothing comes back.)
+template <typename T> __device__ __forceinline__ uint32_t rest_of(float v, float hi) {               // in bits 8 .. 15
+    const int d = __float_as_int(v) - __float_as_int(hi);
+    return std::is_same<T, __half>::value ? (uint32_t)max(min(d, 4095), -4096) << 3 : (uint32_t)min(d, 32767);
+}
+// the float of `hi` and byte `at` of `rests`, in the middle of what the byte stands for
+template <typename T> __device__ __forceinline__ float with_rest(float hi, uint32_t rests, int at) {
+    const int d = (int)prmt(rests, 0x80u, at == 0 ? 0x8804u : at == 1 ? 0x9914u : at == 2 ? 0xaa24u : 0xbb34u);
+    return __int_as_float(__float_as_int(hi) + (std::is_same<T, __half>::value ? d >> 3 : d));
+}
+
 // 2^x where x <= 0 or -inf (0 then)
 __device__ __forceinline__ float exp2_neg(float x) { return mamba::ex2(x); }
 

@@ -144,6 +144,19 @@ template <int N> __device__ __forceinline__ void fewer_registers() { asm volatil
 template <typename T> __device__ __forceinline__ uint32_t pack_word(float lo, float hi) {
     return std::is_same<T, __half>::value ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
 }
+// the rests of four values whose rounded ones are two words
+template <typename T> __device__ __forceinline__ uint32_t rest_word(uint32_t w0, uint32_t w1, float x0, float x1, float x2, float x3) {
+    float2 a, b;
+    if constexpr (std::is_same<T, __half>::value) {
+        a = __half22float2(*reinterpret_cast<const __half2*>(&w0));
+        b = __half22float2(*reinterpret_cast<const __half2*>(&w1));
+    } else {
+        a = make_float2(__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u));
+        b = make_float2(__uint_as_float(w1 << 16), __uint_as_float(w1 & 0xffff0000u));
+    }
+    using latent::rest_of;
+    return prmt(prmt(rest_of<T>(x0, a.x), rest_of<T>(x1, a.y), 0x0051u), prmt(rest_of<T>(x2, b.x), rest_of<T>(x3, b.y), 0x0051u), 0x5410u);
+}
 
 // host: a map of [batch, tokens, inner] 16-bit values for boxes of 64 columns and `rows` tokens; out-of-range reads give zeros
 int make_map_tokens(CUtensorMap* m, const void* base, uint64_t inner, uint64_t tokens, uint64_t stride_t, uint64_t batch, uint64_t stride_b, uint32_t rows);

@@ -562,6 +562,8 @@ EL_API int el_rotary(const el_rotary_t* args, el_stream_t stream);
  * over the keys that query i sees: of a sequence with m = lengths[b] queries and n = key_lengths[b] keys those below n and, with `causal`, up to
  * i + n - m (its queries are its last tokens).  A query that sees no key, and padding, has the output 0.  key_dim + rot_dim and value_dim up to
  * 256; rot_dim 0 for none.  lse (el_latent_attention_lse_bytes; NULL when no gradient is wanted) is what the backward pass needs beside the inputs and out.
+ * out_rest (written by the forward pass, read by the backward pass; may be NULL in either) lets dout . out be formed of out as it was before its rounding,
+ * which would otherwise be a third of what the products' own roundings cost dq and dk.
  * el_latent_attention_backward writes dq, dq_rot, dk, dv, dk_rot (each may be NULL) from dout; all sums have a fixed order.  dk and dv have strides of
  * their own, so that they can be parts of one tensor.  16-bit types whose three head sizes are multiples of 16 up to 128, 64 and 128 with strides and bases on
  * 16 bytes run on the tensor cores, which take probabilities and their gradients rounded to the type (float32 sums); the others run in float32.
@@ -582,6 +584,7 @@ typedef struct el_attention_t {
     const int32_t* lengths;             /* [batch] or NULL: all `length` */
     const int32_t* key_lengths;         /* [batch] or NULL: all `keys` */
     void* out;                          /* [batch, length, heads, value_dim] */
+    int8_t* out_rest;                   /* as out, 16-byte aligned, or NULL: what rounding took from out, in 256ths of a step (16-bit types) */
     float* lse;
     const void* dout;
     long long dout_stride_b, dout_stride_t, dout_stride_h;
