@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(THREADS) attention_delta_kernel(const el_atten
         for (int k = 0; k < 4; ++k) {                                  // (a row that is not there reads the first one)
             const int r = r0 + k * groups, t = r >> head_bits, h = h0 + (r & (heads - 1));
             there[k] = r < rows && t0 + t < live && h < a.heads && c < V;
-            o[k] = there[k] ? out + (t * a.heads + h) * V + c : out0;
+            o[k] = there[k] ? out + ((long long)t * a.heads + h) * V + c : out0;
             g[k] = there[k] ? dout + t * a.dout_stride_t + h * a.dout_stride_h + c : dout0;
         }
         if constexpr (VEC) {

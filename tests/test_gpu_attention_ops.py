@@ -576,6 +576,13 @@ def test_errors_of_a_backward_pass_reach_its_caller(ops):
         Wrong.apply(out).sum().backward()
     with pytest.raises(RuntimeError):
         ops.latent_attention(leaves[0], leaves[1][:, :, :100], *leaves[2:])
+    # an error of the call itself, in the engine's thread: what was kept comes back with another dtype
+    table = ops.rotary_table(70, 32, device=DEV)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.half() if t.is_floating_point() else t):
+        attended, turned = ops.latent_attention(*leaves), ops.rotary(leaves[2], table)
+    for out, message in ((attended, "lse must be Float"), (turned, "table must be Float")):
+        with pytest.raises(RuntimeError, match=message):
+            out.sum().backward()
     ops.latent_attention(*leaves).sum().backward()
     assert all(t.grad is not None for t in leaves)
 
