@@ -337,7 +337,7 @@ template <typename T, int BLOCKS> constexpr int JOIN_BYTES = JOIN_WARPS * (MOST_
 
 template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent_step_t a, const StepParts parts, int workers) {
-    constexpr int COLS = MOST_RANK / BLOCKS, WORDS = MOST_RANK / 16 / (BLOCKS == 1 ? 1 : 2);
+    constexpr int COLS = MOST_RANK / BLOCKS, WORDS = MOST_RANK / 16 / (BLOCKS == 1 ? 1 : 2), AT_ONCE = BLOCKS == 1 ? 4 : 10;
     extern __shared__ float4 join_smem[];
     float* o = reinterpret_cast<float*>(join_smem);                                            // [16 warps][COLS]
     __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(o + JOIN_WARPS * COLS);            // [terms][16 sequences][JOIN_PITCH]
@@ -384,15 +384,41 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
             w1 = step_worker(before + here - 1, active, tiles);
         }
     }
+    for (int i = threadIdx.x; i < JOIN_TERMS<T> * (JOIN_ROWS - nb) * (JOIN_PITCH / 2); i += JOIN_THREADS) {      // rows of no sequence
+        const int t = i / ((JOIN_ROWS - nb) * (JOIN_PITCH / 2));
+        reinterpret_cast<uint32_t*>(terms + (t * JOIN_ROWS + nb) * JOIN_PITCH)[i - t * (JOIN_ROWS - nb) * (JOIN_PITCH / 2)] = 0u;
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (w0 <= w1) {
+        // A load here takes some 1000 cycles (other SMs have just written what it reads), so all loads that a warp's first parts need are on their way at once.
+        float4 y[AT_ONCE][COLS / 128];
+        float own;                                   // lane l: the maximum of the l-th of them
+        auto fetch = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int p = w0 + share + (i0 + i) * shares;
+                const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + b) + (long long)h * R + c0) + lane;
+#pragma unroll
+                for (int c = 0; c < COLS / 128; ++c) y[i][c] = p <= w1 && (c * 32 + lane) * 4 < cols ? v[c * 32] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            const int p = w0 + share + (i0 + lane) * shares;
+            own = lane < AT_ONCE && p <= w1 ? parts.stats((long long)p + b)[2 * h] : -INFINITY;
+        };
+        fetch(0);
         float top = -INFINITY, sum = 0.0f;
-#pragma unroll 5
-        for (int p = w0 + lane; p <= w1; p += 32) {
-            const float2 st = *reinterpret_cast<const float2*>(parts.stats((long long)p + b) + 2 * h);
-            const float m = mamba::max_nan(top, st.x), from = m == -INFINITY ? 0.0f : m;
-            sum = fmaf(sum, exp2_neg(top - from), exp2_neg(st.x - from) * st.y);
-            top = m;
+        for (int p0 = w0; p0 <= w1; p0 += 160) {
+            float2 st[5];
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                const int p = p0 + lane + 32 * k;
+                st[k] = p <= w1 ? *reinterpret_cast<const float2*>(parts.stats((long long)p + b) + 2 * h) : make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                const float m = mamba::max_nan(top, st[k].x), from = m == -INFINITY ? 0.0f : m;
+                sum = fmaf(sum, exp2_neg(top - from), exp2_neg(st[k].x - from) * st[k].y);
+                top = m;
+            }
         }
         float all = top;
 #pragma unroll
@@ -402,23 +428,18 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         const float by = all == -INFINITY ? 0.0f : a.gamma / sum;
-        // 32 of this warp's parts at a time: lane l has the factor of the l-th
-        for (int p = w0 + share; p <= w1; p += 32 * shares) {
-            const int own = p + lane * shares, count = min(32, (w1 - p) / shares + 1);
-            const float f = own <= w1 ? exp2_neg(parts.stats((long long)own + b)[2 * h] - from) * by : 0.0f;
-            const float4* v = reinterpret_cast<const float4*>(parts.vectors((long long)p + b) + (long long)h * R + c0) + lane;
-            const long long step = (long long)shares * a.heads * (R / 4);
-#pragma unroll (BLOCKS == 1 ? 4 : 8)
-            for (int i = 0; i < count; ++i) {
+        for (int i0 = 0; w0 + share + i0 * shares <= w1; i0 += AT_ONCE) {
+            if (i0 > 0) fetch(i0);
+            const float f = exp2_neg(own - from) * by;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
                 const float x = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
                 for (int c = 0; c < COLS / 128; ++c) {
-                    if ((c * 32 + lane) * 4 >= cols) continue;
-                    const float4 y = v[i * step + c * 32];
-                    acc[4 * c] = fmaf(x, y.x, acc[4 * c]);
-                    acc[4 * c + 1] = fmaf(x, y.y, acc[4 * c + 1]);
-                    acc[4 * c + 2] = fmaf(x, y.z, acc[4 * c + 2]);
-                    acc[4 * c + 3] = fmaf(x, y.w, acc[4 * c + 3]);
+                    acc[4 * c] = fmaf(x, y[i][c].x, acc[4 * c]);
+                    acc[4 * c + 1] = fmaf(x, y[i][c].y, acc[4 * c + 1]);
+                    acc[4 * c + 2] = fmaf(x, y[i][c].z, acc[4 * c + 2]);
+                    acc[4 * c + 3] = fmaf(x, y[i][c].w, acc[4 * c + 3]);
                 }
             }
         }
@@ -435,16 +456,17 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
         }
     };
     meet();                                          // the other blocks have begun, too: their shared memory may be written
-    for (int i = threadIdx.x; i < JOIN_ROWS * COLS / 2; i += JOIN_THREADS) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < nb * COLS / 2; i += JOIN_THREADS) {
         const int n = i / (COLS / 2), c = i % (COLS / 2) * 2;
         if (c >= cols) continue;
         float2 v = make_float2(0.0f, 0.0f);
-        if (n < nb)
-            for (int s = 0; s < shares; ++s) {
-                const float2 x = *reinterpret_cast<const float2*>(o + (s * spread + n) * COLS + c);
-                v.x += x.x;
-                v.y += x.y;
-            }
+#pragma unroll 4
+        for (int s = 0; s < shares; ++s) {
+            const float2 x = *reinterpret_cast<const float2*>(o + (s * spread + n) * COLS + c);
+            v.x += x.x;
+            v.y += x.y;
+        }
 #pragma unroll
         for (int t = 0; t < JOIN_TERMS<T>; ++t) {
             const uint32_t x = pack_bf16x2(v.x, v.y);
@@ -461,21 +483,29 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
     }
     meet();
     for (int v0 = (warp % groups) * 8;; v0 += 128) {                                           // (more than 128 value rows: one block, depth 1)
-        float d[4] = {};
+        // eight words in a row of code: the kernel is short and its code is not in the instruction cache when it begins
+        float d[4] = {}, e[4] = {};
+#pragma unroll 1
+        for (int k0 = 0; first + k0 * depth < words; k0 += 8) {
 #pragma unroll
-        for (int k = 0; k < WORDS; ++k) {
-            const int word = first + k * depth;
-            if (word >= words) break;
-            const uint32_t x = w[k] >> (2 * k2);
-            const uint32_t x0 = weight_pair<__nv_bfloat16>(x & 3u, (x >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((x >> 16) & 3u, (x >> 18) & 3u);
+            for (int k = 0; k < 8; ++k) {
+                const int word = first + (k0 + k) * depth;
+                if (word >= words) break;
+                const uint32_t x = w[k] >> (2 * k2);
+                const uint32_t x0 = weight_pair<__nv_bfloat16>(x & 3u, (x >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((x >> 16) & 3u, (x >> 18) & 3u);
 #pragma unroll
-            for (int t = JOIN_TERMS<T> - 1; t >= 0; --t) {
-                const __nv_bfloat16* p = terms + (t * JOIN_ROWS + r) * JOIN_PITCH + word * 16 + k2;
-                const uint32_t y[4] = {*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH), *reinterpret_cast<const uint32_t*>(p + 8),
-                                       *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH + 8)};
-                warp_mma<__nv_bfloat16>(d, y, x0, x1);
+                for (int t = JOIN_TERMS<T> - 1; t >= 0; --t) {
+                    const __nv_bfloat16* p = terms + (t * JOIN_ROWS + r) * JOIN_PITCH + word * 16 + k2;
+                    const uint32_t y[4] = {*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH), *reinterpret_cast<const uint32_t*>(p + 8),
+                                           *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH + 8)};
+                    warp_mma<__nv_bfloat16>(t == 0 ? d : e, y, x0, x1);
+                }
             }
+#pragma unroll
+            for (int k = 0; k + 8 < WORDS; ++k) w[k] = w[k + 8];
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] += e[i];
         if (depth > 1) {                             // the warps' shares of the reduction: [warp][16 sequences][8 rows]
             *reinterpret_cast<float2*>(o + warp * 128 + r * 8 + k2) = make_float2(d[0], d[1]);
             *reinterpret_cast<float2*>(o + warp * 128 + (r + 8) * 8 + k2) = make_float2(d[2], d[3]);
