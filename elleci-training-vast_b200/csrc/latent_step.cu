@@ -113,33 +113,64 @@ __global__ void __launch_bounds__(THREADS) step_query_kernel(const el_latent_ste
 // u and w for the tensor cores: of one head, 128 columns of u for 16 sequences, into the images of latent_step.cuh.  u = gamma scale log2(e) q W is held in
 // two 8-bit digits of 1 / 32512 of gamma scale log2(e) sum |q|, which it cannot exceed whatever the weights are: no block has to know another's columns.
 // (For weights of random signs that is 3 to 4 times the largest u, 14 bits of it.)  steps [batch, groups, 32].  A warp takes 16 columns, which are one
-// word of every row of the weights.
+// word of every row of the weights (32: 94 us for the whole step of 64 sequences instead of 87).  Operands go from memory to the threads' registers as the products take them (a lane has 8 neighbouring channels of
+// every 32, in the query and in the weights, whatever the order of a product's own reduction), 64 channels at a time: shared memory in between, and its
+// barriers, made the kernel 13000 cycles long where there are 64 sequences of 32 heads of 128 channels.
 constexpr int QUERY_ROWS = 16, QUERY_COLS = 128;
 template <typename T>
-__global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_latent_step_t a, uint8_t* __restrict__ images, float* __restrict__ steps, const bool vectors) {
-    __shared__ __align__(16) T q[QUERY_ROWS][256 + 8];
-    __shared__ uint32_t W[256][WARPS + 1];
-    __shared__ float most[QUERY_ROWS];
+__global__ void __launch_bounds__(THREADS, 4) step_query_digits_kernel(const el_latent_step_t a, uint8_t* __restrict__ images, float* __restrict__ steps, const bool vectors) {
     const StepImage image(a);
     asm volatile("griddepcontrol.launch_dependents;");
     const int h = blockIdx.x, c0 = blockIdx.y * QUERY_COLS, b0 = blockIdx.z * QUERY_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int nb = min(QUERY_ROWS, a.batch - b0), D = h < a.heads ? a.key_dim : 0, DP = (D + 15) / 16 * 16, words = a.rank / 16, rp = (a.rank + 31) / 32 * 32;
-    const int group = h / 32, hg = h % 32;
+    const int nb = min(QUERY_ROWS, a.batch - b0), D = h < a.heads ? a.key_dim : 0, words = a.rank / 16, rp = (a.rank + 31) / 32 * 32;
+    const int group = h / 32, hg = h % 32, r = lane >> 2, own = (lane & 3) * 8, word = c0 / 16 + warp;
     const float by = a.gamma * a.scale * mamba::LOG2E;
-    for (int i = threadIdx.x; i < DP * WARPS; i += THREADS) {
-        const int d = i / WARPS, w = i % WARPS;
-        W[d][w] = d < D && c0 / 16 + w < words ? reinterpret_cast<const uint32_t*>(a.W_packed)[((long long)h * D + d) * words + c0 / 16 + w] : 0x55555555u;
-    }
-    const int rows = (nb + 15) / 16 * 16;
-    if (vectors) {                                   // rows of 8 values on 16 bytes
-        const int per = DP / 8;
-        for (int n = threadIdx.x / 32; n < rows; n += WARPS)
-            if (lane < per)
-                *reinterpret_cast<uint4*>(&q[n][lane * 8]) = n < nb && lane * 8 < D ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (b0 + n) * a.q_stride_b + h * a.q_stride_h + lane * 8)
-                                                                                    : make_uint4(0u, 0u, 0u, 0u);
-    } else {
-        for (int n = threadIdx.x / 32; n < rows; n += WARPS)
-            for (int d = lane; d < DP; d += 32) q[n][d] = n < nb && d < D ? static_cast<const T*>(a.q)[(b0 + n) * a.q_stride_b + h * a.q_stride_h + d] : mamba::from_float<T>(0.0f);
+    const uint32_t* weights = reinterpret_cast<const uint32_t*>(a.W_packed) + (long long)h * a.key_dim * words + word;
+    float sum[2][4] = {}, total[2] = {};             // of columns t * 8 ..; of |q| of rows r, r + 8
+#pragma unroll 1
+    for (int k0 = 0; k0 < D; k0 += 64) {
+        uint32_t q[2][2][4], w[2][8];                // [32 channels][row][pairs of 8], [32 channels][8]
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int d0 = k0 + 32 * x + own;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) w[x][d] = d0 + d < D && word < words ? weights[(long long)(d0 + d) * words] : 0x55555555u;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int n = r + 8 * m;
+                const T* from = static_cast<const T*>(a.q) + (b0 + n) * a.q_stride_b + h * a.q_stride_h + d0;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (vectors) {                       // rows of 8 values on 16 bytes
+                    if (n < nb && d0 < D) v = *reinterpret_cast<const uint4*>(from);
+                } else {
+                    T one[8];
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) one[d] = n < nb && d0 + d < D ? from[d] : mamba::from_float<T>(0.0f);
+                    memcpy(&v, one, 16);
+                }
+                q[x][m][0] = v.x; q[x][m][1] = v.y; q[x][m][2] = v.z; q[x][m][3] = v.w;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                T one[8];
+                memcpy(one, q[x][m], 16);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) total[m] += fabsf(to_float(one[d]));
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {            // 16 channels: four of each lane's eight
+                const uint32_t f[4] = {q[x][0][2 * y], q[x][1][2 * y], q[x][0][2 * y + 1], q[x][1][2 * y + 1]};
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int at = 2 * (t * 8 + r);
+                    warp_mma<T>(sum[t], f, weight_pair<T>((w[x][4 * y] >> at) & 3u, (w[x][4 * y + 1] >> at) & 3u),
+                                weight_pair<T>((w[x][4 * y + 2] >> at) & 3u, (w[x][4 * y + 3] >> at) & 3u));
+                }
+            }
+        }
     }
     if (a.rot_dim) {                                 // the column blocks share the rows
         const int pairs = 32;                        // of the 64 places of w; those behind rot_dim are zeros
@@ -153,60 +184,30 @@ __global__ void __launch_bounds__(THREADS) step_query_digits_kernel(const el_lat
                 for (int x = c; x < a.rot_dim; x += pairs) put(x, 0.0f);
         }
     }
-    __syncthreads();
-    for (int n = warp; n < nb; n += WARPS) {
-        float s = 0.0f;
-        for (int d = lane; d < D; d += 32) s += fabsf(to_float(q[n][d]));
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        if (lane == 0) {
-            most[n] = s > 0.0f ? STEPS / s : 0.0f;
-            if (c0 == 0) steps[((long long)(b0 + n) * image.groups + group) * 32 + hg] = by * s * (1.0f / STEPS);      // a NaN or infinity makes the scores NaN
-        }
-    }
-    float sum[QUERY_ROWS / 16][2][4] = {};
-    const int r = lane >> 2, k2 = (lane & 3) * 2;
-    for (int k = 0; k < DP; k += 16) {
-        const uint32_t w0 = W[k + k2][warp], w1 = W[k + k2 + 1][warp], w2 = W[k + k2 + 8][warp], w3 = W[k + k2 + 9][warp];
-        uint32_t b[2][2];
+    for (int m = 0; m < 2; ++m) {
+        const int n = r + 8 * m;
+        float s = total[m];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if (n >= nb) continue;
+        if (c0 == 0 && warp == 0 && (lane & 3) == 0) steps[((long long)(b0 + n) * image.groups + group) * 32 + hg] = by * s * (1.0f / STEPS);      // a NaN or infinity makes the scores NaN
+        const float inv = s > 0.0f ? STEPS / s : 0.0f;
+        uint8_t* out = images + ((long long)(b0 + n) * image.groups + group) * image.bytes();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int at = 2 * (t * 8 + r);
-            b[t][0] = weight_pair<T>((w0 >> at) & 3u, (w1 >> at) & 3u);
-            b[t][1] = weight_pair<T>((w2 >> at) & 3u, (w3 >> at) & 3u);
-        }
+            const int c = c0 + warp * 16 + t * 8 + (lane & 3) * 2;
+            if (c >= rp) continue;
+            int v[2], hi[2];
 #pragma unroll
-        for (int m = 0; m < QUERY_ROWS / 16; ++m) {
-            if (m * 16 >= nb) break;
-            const uint32_t x[4] = {*reinterpret_cast<const uint32_t*>(&q[m * 16 + r][k + k2]), *reinterpret_cast<const uint32_t*>(&q[m * 16 + r + 8][k + k2]),
-                                   *reinterpret_cast<const uint32_t*>(&q[m * 16 + r][k + k2 + 8]), *reinterpret_cast<const uint32_t*>(&q[m * 16 + r + 8][k + k2 + 8])};
-            warp_mma<T>(sum[m][0], x, b[0][0], b[0][1]);
-            warp_mma<T>(sum[m][1], x, b[1][0], b[1][1]);
+            for (int e = 0; e < 2; ++e) {
+                v[e] = min(max(__float2int_rn(sum[t][2 * m + e] * inv), -(int)STEPS), (int)STEPS);
+                hi[e] = (v[e] + 128) >> 8;
+            }
+            *reinterpret_cast<char2*>(out + image.digit(c, 0, hg)) = make_char2((signed char)hi[0], (signed char)hi[1]);
+            *reinterpret_cast<char2*>(out + image.digit(c, 1, hg)) = make_char2((signed char)(v[0] - hi[0] * 256), (signed char)(v[1] - hi[1] * 256));
         }
     }
-    __syncthreads();
-#pragma unroll
-    for (int m = 0; m < QUERY_ROWS / 16; ++m)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int n = m * 16 + r + 8 * i;
-            if (n >= nb) continue;
-            const float inv = most[n];
-            uint8_t* out = images + ((long long)(b0 + n) * image.groups + group) * image.bytes();
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int c = c0 + warp * 16 + t * 8 + k2;
-                if (c >= rp) continue;
-                int v[2], hi[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    v[e] = min(max(__float2int_rn(sum[m][t][2 * i + e] * inv), -(int)STEPS), (int)STEPS);
-                    hi[e] = (v[e] + 128) >> 8;
-                }
-                *reinterpret_cast<char2*>(out + image.digit(c, 0, hg)) = make_char2((signed char)hi[0], (signed char)hi[1]);
-                *reinterpret_cast<char2*>(out + image.digit(c, 1, hg)) = make_char2((signed char)(v[0] - hi[0] * 256), (signed char)(v[1] - hi[1] * 256));
-            }
-        }
 }
 
 // A block takes 32 heads of a worker's tokens, 32 at a time; a warp takes 4 heads: a lane is a token for the scores, a column in every 32 for the sums.
