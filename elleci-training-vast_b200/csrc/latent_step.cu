@@ -334,33 +334,38 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, int rank, uint32_t 
 // with four; 64 sequences: 17.5 and 27.
 constexpr int JOIN_THREADS = 512, JOIN_WARPS = 16, JOIN_ROWS = 16, JOIN_PITCH = MOST_RANK + 8;
 template <typename T> constexpr int JOIN_TERMS = sizeof(T) == 4 ? 3 : 2;
-template <typename T, int BLOCKS> constexpr int JOIN_BYTES = JOIN_WARPS * (MOST_RANK / BLOCKS) * 4 + JOIN_TERMS<T> * JOIN_ROWS * JOIN_PITCH * 2;
+template <int BLOCKS> constexpr int JOIN_FLOATS = JOIN_WARPS * (MOST_RANK / BLOCKS > 256 ? MOST_RANK / BLOCKS : 256);          // sums by warp; of 16 x 16 results by warp
+template <typename T, int BLOCKS> constexpr int JOIN_BYTES = JOIN_FLOATS<BLOCKS> * 4 + JOIN_TERMS<T> * JOIN_ROWS * JOIN_PITCH * 2;
 
 template <typename T, int BLOCKS>
 __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent_step_t a, const StepParts parts, int workers) {
-    constexpr int COLS = MOST_RANK / BLOCKS, WORDS = MOST_RANK / 16 / (BLOCKS == 1 ? 1 : 2), AT_ONCE = BLOCKS == 1 ? 4 : 10;
+    constexpr int COLS = MOST_RANK / BLOCKS, WORDS = BLOCKS == 1 ? 16 : 8, AT_ONCE = BLOCKS == 1 ? 4 : 10;
     extern __shared__ float4 join_smem[];
     float* o = reinterpret_cast<float*>(join_smem);                                            // [16 warps][COLS]
-    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(o + JOIN_WARPS * COLS);            // [terms][16 sequences][JOIN_PITCH]
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(o + JOIN_FLOATS<BLOCKS>);            // [terms][16 sequences][JOIN_PITCH]
     const int h = blockIdx.x / BLOCKS, quarter = blockIdx.x % BLOCKS, b0 = blockIdx.y * JOIN_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.rank;
     const int nb = min(JOIN_ROWS, a.batch - b0);
     int spread = 1;                                  // sequences side by side, a power of two; 16 / spread warps share one
     while (spread < nb) spread *= 2;
     const int shares = JOIN_WARPS / spread, share = warp / spread, b = b0 + warp % spread;
     const int c0 = quarter * COLS, cols = min(COLS, R - c0);                                   // this block's channels (none: 0 or less)
-    // the value rows of this block, eight for a warp at a time; warps that have the same ones take every `depth`-th word (16 channels) of them
+    // the value rows of this block, 16 for a warp at a time (its operand of the sequences serves both eights); warps that have the same ones take every
+    // `depth`-th word (16 channels) of them
     const int words = R / 16, r = lane >> 2, k2 = (lane & 3) * 2, per = (a.value_dim + 8 * BLOCKS - 1) / (8 * BLOCKS) * 8, v_begin = quarter * per;
-    int groups = 1;                                  // of eight rows, a power of two and 16 at most
-    while (groups * 8 < per && groups < JOIN_WARPS) groups *= 2;
-    const int depth = JOIN_WARPS / groups, first = warp / groups;
-    uint32_t w[WORDS];                               // (four blocks have 64 value rows at most: depth is 2 or more)
+    int groups = 1;                                  // of 16 rows, a power of two and 8 at most: depth is 2 or more, with four blocks (64 rows) 4 or more
+    while (groups * 16 < per && groups < JOIN_WARPS / 2) groups *= 2;
+    const int depth = JOIN_WARPS / groups, first = warp / groups, mine = (warp % groups) * 16;
+    uint32_t w[2][WORDS];
     auto load_weights = [&](int v0) {
-        const int row = v_begin + v0 + r;
-        const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim + row) * words;
 #pragma unroll
-        for (int k = 0; k < WORDS; ++k) w[k] = v0 < per && row < a.value_dim && first + k * depth < words ? W[first + k * depth] : 0x55555555u;
+        for (int e = 0; e < 2; ++e) {
+            const int v = v0 + mine + 8 * e + r, row = v_begin + v;
+            const uint32_t* W = reinterpret_cast<const uint32_t*>(a.W_packed) + ((long long)a.heads * a.key_dim + (long long)h * a.value_dim + row) * words;
+#pragma unroll
+            for (int k = 0; k < WORDS; ++k) w[e][k] = v < per && row < a.value_dim && first + k * depth < words ? W[first + k * depth] : 0x55555555u;
+        }
     };
-    load_weights((warp % groups) * 8);               // before anything that the kernels before leave is there
+    load_weights(0);                                 // before anything that the kernels before leave is there
     float acc[COLS / 32] = {};
     int w0 = 0, w1 = -1;
     if (warp % spread < nb) {
@@ -483,52 +488,58 @@ __global__ void __launch_bounds__(JOIN_THREADS) step_join_kernel(const el_latent
         }
     }
     meet();
-    for (int v0 = (warp % groups) * 8;; v0 += 128) {                                           // (more than 128 value rows: one block, depth 1)
-        // eight words in a row of code: the kernel is short and its code is not in the instruction cache when it begins
-        float d[4] = {}, e[4] = {};
+    for (int v0 = 0; v0 < per; v0 += groups * 16) {
+        if (v0 > 0) {
+            __syncthreads();                         // the results before have been read
+            load_weights(v0);
+        }
+        // four words in a row of code: the kernel is short and its code is not in the instruction cache when it begins
+        float d[2][4] = {}, low[2][4] = {};
 #pragma unroll 1
-        for (int k0 = 0; first + k0 * depth < words; k0 += 8) {
+        for (int k0 = 0; first + k0 * depth < words; k0 += 4) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < 4; ++k) {
                 const int word = first + (k0 + k) * depth;
                 if (word >= words) break;
-                const uint32_t x = w[k] >> (2 * k2);
-                const uint32_t x0 = weight_pair<__nv_bfloat16>(x & 3u, (x >> 2) & 3u), x1 = weight_pair<__nv_bfloat16>((x >> 16) & 3u, (x >> 18) & 3u);
+                uint32_t x[2][2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t y = w[e][k] >> (2 * k2);
+                    x[e][0] = weight_pair<__nv_bfloat16>(y & 3u, (y >> 2) & 3u);
+                    x[e][1] = weight_pair<__nv_bfloat16>((y >> 16) & 3u, (y >> 18) & 3u);
+                }
 #pragma unroll
                 for (int t = JOIN_TERMS<T> - 1; t >= 0; --t) {
                     const __nv_bfloat16* p = terms + (t * JOIN_ROWS + r) * JOIN_PITCH + word * 16 + k2;
                     const uint32_t y[4] = {*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH), *reinterpret_cast<const uint32_t*>(p + 8),
                                            *reinterpret_cast<const uint32_t*>(p + 8 * JOIN_PITCH + 8)};
-                    warp_mma<__nv_bfloat16>(t == 0 ? d : e, y, x0, x1);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) warp_mma<__nv_bfloat16>(t == 0 ? d[e] : low[e], y, x[e][0], x[e][1]);
                 }
             }
 #pragma unroll
-            for (int k = 0; k + 8 < WORDS; ++k) w[k] = w[k + 8];
+            for (int k = 0; k + 4 < WORDS; ++k) {
+                w[0][k] = w[0][k + 4];
+                w[1][k] = w[1][k + 4];
+            }
         }
+        // the warps' shares of the reduction: [warp][16 sequences][16 rows]
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] += e[i];
-        if (depth > 1) {                             // the warps' shares of the reduction: [warp][16 sequences][8 rows]
-            *reinterpret_cast<float2*>(o + warp * 128 + r * 8 + k2) = make_float2(d[0], d[1]);
-            *reinterpret_cast<float2*>(o + warp * 128 + (r + 8) * 8 + k2) = make_float2(d[2], d[3]);
-            break;
+        for (int e = 0; e < 2; ++e) {
+            float* to = o + warp * 256 + r * 16 + 8 * e + k2;
+            *reinterpret_cast<float2*>(to) = make_float2(d[e][0] + low[e][0], d[e][1] + low[e][1]);
+            *reinterpret_cast<float2*>(to + 128) = make_float2(d[e][2] + low[e][2], d[e][3] + low[e][3]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = r + 8 * (i >> 1), v = v0 + k2 + (i & 1);
-            if (n < nb && v < per && v_begin + v < a.value_dim)
-                static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v_begin + v] = mamba::from_float<T>(d[i]);
+        __syncthreads();
+        const int here = min(groups * 16, per - v0);
+        for (int i = threadIdx.x; i < nb * here; i += JOIN_THREADS) {
+            const int n = i / here, v = i - n * here;
+            if (v_begin + v0 + v >= a.value_dim) continue;
+            float x = 0.0f;
+#pragma unroll 2
+            for (int s = 0; s < depth; ++s) x += o[(s * groups + v / 16) * 256 + n * 16 + v % 16];
+            static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v_begin + v0 + v] = mamba::from_float<T>(x);
         }
-        if (v0 + 128 >= per) break;
-        load_weights(v0 + 128);
-    }
-    if (depth == 1) return;
-    __syncthreads();
-    for (int i = threadIdx.x; i < nb * per; i += JOIN_THREADS) {
-        const int n = i / per, v = i - n * per;
-        if (v_begin + v >= a.value_dim) continue;
-        float x = 0.0f;
-        for (int s = 0; s < depth; ++s) x += o[(s * groups + v / 8) * 128 + n * 8 + v % 8];
-        static_cast<T*>(a.out)[((long long)(b0 + n) * a.heads + h) * a.value_dim + v_begin + v] = mamba::from_float<T>(x);
     }
 }
 
