@@ -542,6 +542,9 @@ step_tc_kernel(const __grid_constant__ CUtensorMap tmRows, const __grid_constant
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000) { }
     }
+    // No block ends before the kernel in front has, also one that had no use for the query: what is launched behind the join waits for the join, and by that for
+    // both, and may then be given their workspace.
+    if (warp == WARP_LOAD) griddep_wait();
     tcgen05_fence_before();
     __syncthreads();
     if (warp == WARP_MMA) {
